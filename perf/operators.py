@@ -247,7 +247,7 @@ def _own(s):
     op = s["op"]
     if op == "layer8":
         x, conn, raw = (s[k].detach().requires_grad_() for k in ("x", "conn", "raw"))
-        y = torch.ops.silogic_hip.fc_layer8(x, s["cand"], conn, raw, KINDS[s["node"]], s["inv_tau"])[0]
+        y = sl.ops.fc_layer8(x, s["cand"], conn, raw, KINDS[s["node"]], s["inv_tau"])
         gx, gconn, graw = torch.autograd.grad(y, [x, conn, raw], s["gy"])
         return {"y": y, "gx": gx, "gconn": gconn, "graw": graw}
     if op == "rows8":
