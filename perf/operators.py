@@ -157,8 +157,9 @@ def _rows8(x):
     """Codes, offset and step of every row (module docstring)."""
     lo = x.amin(1, keepdim=True)
     span = x.amax(1, keepdim=True) - lo
-    inv = torch.where(span > 0, 255 / span, torch.zeros_like(span))
-    return torch.round((x - lo) * inv), lo, span / 255
+    most = torch.full_like(span, 255.0)   # quotients of tensors: a number's would be a product with a reciprocal
+    inv = torch.where(span > 0, most / span, torch.zeros_like(span))
+    return torch.round((x - lo) * inv), lo, span / most
 
 
 def _node(node, a, b, p, inv_tau):
