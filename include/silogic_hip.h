@@ -265,6 +265,60 @@ int slg_learned_thermo_bwd(const float* x, int64_t B, int64_t F, int32_t T, cons
                            float scale, const float* g, float* gx, float* gt, float* workspace,
                            int64_t workspace_floats, slg_stream_t stream);
 
+/* Token encoder (no counterpart in the reference, whose encoders take numbers):
+ * a learned row of D soft bits per token id. table [V,D] (dtype 0: fp32, 1:
+ * bf16, 2: fp16), ids [N] of id_bytes 4 or 8 (signed). A token with id pad, or
+ * outside 0..V-1, is absent: values and bits 0, no gradient (pad < 0: every id
+ * of the table counts).
+ *   slg_token_encode       y [N,D] fp32 = sigmoid(scale * table[id]); ste: 1
+ *                          where table[id] > 0, else 0
+ *   slg_token_encode_bwd   gtable [V,D] (the table's type, all of it written) =
+ *                          scale * sigmoid'(scale * table) * (gy [N,D] summed
+ *                          over each id's tokens, in ascending order of n: the
+ *                          same bits on every call). workspace: that many
+ *                          4-byte words, at a multiple of 16 bytes
+ *   slg_token_bits         bits [V, ceil(D/64)] = table > 0, bit d % 64 of word
+ *                          d / 64: the table of slg_token_encode_hard, made
+ *                          once per set of weights
+ *   slg_token_encode_hard  ids [B,L] -> bits of feature l*D + d: layout 0
+ *                          packed [L*D, nw], 1 packed word-major [nw, L*D], 2
+ *                          uint8 [B, L*D] */
+int slg_token_encode(const void* ids, int32_t id_bytes, int64_t N, int64_t V, int64_t D, int64_t pad,
+                     const void* table, int32_t dtype, float scale, int32_t ste, float* y,
+                     slg_stream_t stream);
+int64_t slg_token_encode_bwd_workspace(int64_t N, int64_t V, int64_t D);
+int slg_token_encode_bwd(const void* ids, int32_t id_bytes, int64_t N, int64_t V, int64_t D,
+                         int64_t pad, const void* table, int32_t dtype, float scale,
+                         const float* gy, void* gtable, int32_t* workspace,
+                         int64_t workspace_words, slg_stream_t stream);
+int slg_token_bits(const void* table, int32_t dtype, int64_t V, int64_t D, uint64_t* bits,
+                   slg_stream_t stream);
+int slg_token_encode_hard(const void* ids, int32_t id_bytes, int64_t B, int64_t L, int64_t V,
+                          int64_t D, int64_t pad, const uint64_t* bits, int32_t layout, void* out,
+                          slg_stream_t stream);
+
+/* Activations kept in 8 bits between a layer's forward and its backward (no
+ * counterpart in the reference). x [B,D] fp32 -> codes [ceil(B/4)][ld][4] uint8
+ * (at a multiple of 16 bytes), ld = slg_rows8_ld(D), byte v of (t, i) the code
+ * of sample 4t + v, input i, 0 past B and D; rows [B][2] fp32: a sample's
+ * lo = min x and step = (max x - lo) / 255;
+ *   code = rint((x - lo) * (255 / (max x - lo))), standing for lo + code * step
+ * in fp32 (a row whose 255 / span is not finite: codes and step 0). A row with
+ * an infinity or a NaN, or whose span overflows, has lo = NaN. */
+int64_t slg_rows8_ld(int64_t D);
+int slg_rows8_pack(const float* x, int64_t B, int64_t D, uint8_t* codes, float* rows,
+                   slg_stream_t stream);
+int slg_rows8_unpack(const uint8_t* codes, const float* rows, int64_t B, int64_t D, float* x,
+                     slg_stream_t stream);
+/* slg_fc_soft_bwd at the values that x's codes stand for. Workspace of
+ * slg_fc_soft_bwd8_workspace floats at a multiple of 16 bytes (-1: shape not
+ * taken: rows of more than 40960 inputs, K past 16; unpack those). */
+int64_t slg_fc_soft_bwd8_workspace(int64_t B, int64_t IN, int64_t OUT, int32_t K);
+int slg_fc_soft_bwd8(const uint8_t* codes, const float* rows, int64_t B, int64_t IN, int64_t OUT,
+                     int32_t K, const int32_t* cand, const float* w, int32_t node_kind,
+                     const float* node_param, float inv_tau, const float* gy, float* gx, float* gw,
+                     float* gnp, float* workspace, int64_t workspace_floats, slg_stream_t stream);
+
 /* GroupSum.forward (silogic/heads.py:34-39): x [B,W] -> logits [B,C] =
  * sum over class block of (ste ? (x > 0.5) : x), divided by tau. */
 int slg_groupsum_soft(const float* x, int64_t B, int64_t W, int32_t C, float tau,

@@ -31,7 +31,8 @@ from .heads import GroupSum, build_decoder
 from .layers import (LogicLayer, WARPLayer, WARPLayerN, LUTkLayer, LUTNodeLayer, ConvLogicTree,
                      ConvLogicLayer, OrPool)
 from .models import LogicNet, WARPNet, WARPNetN, LUTkNet, LUTNodeNet, LogicConvNet, LogicTreeNet
-from .encoders import LearnedThermometerEncoder
+from .encoders import LearnedThermometerEncoder, TokenEncoder
+from .activations import pack_rows8, unpack_rows8, save_activations
 from .data import (binarize, binarize_spatial, binarize_packed, edge_bits, MNIST_THRESH,
                    SEVEN_THRESH, FOUR_THRESH, FIVE_THRESH, CIFAR3_THRESH, EDGE_THRESH)
 from . import derived, kernels, library, ops
@@ -43,6 +44,7 @@ __all__ = [
     "LogicLayer", "WARPLayer", "WARPLayerN", "LUTkLayer", "LUTNodeLayer", "ConvLogicTree",
     "ConvLogicLayer", "OrPool", "LogicNet", "WARPNet", "WARPNetN", "LUTkNet", "LUTNodeNet",
     "LogicConvNet", "LogicTreeNet", "kernels", "ops",
-    "LearnedThermometerEncoder", "binarize", "binarize_spatial", "binarize_packed", "edge_bits",
+    "LearnedThermometerEncoder", "TokenEncoder", "pack_rows8", "unpack_rows8", "save_activations",
+    "binarize", "binarize_spatial", "binarize_packed", "edge_bits",
     "MNIST_THRESH", "SEVEN_THRESH", "FOUR_THRESH", "FIVE_THRESH", "CIFAR3_THRESH", "EDGE_THRESH",
 ]

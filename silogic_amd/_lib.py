@@ -52,6 +52,18 @@ SIGNATURES = {
     "slg_fc_soft_bwd_workspace": (C.c_int64, [_I64, _I64, _I64, _I32]),
     "slg_fc_soft_bwd": (C.c_int, [_P, _I64, _I64, _I64, _I32, _P, _P, _I32, _P, _F32, _P, _P, _P, _P,
                                   _P, _I64, _P]),
+    "slg_rows8_ld": (_I64, [_I64]),
+    "slg_rows8_pack": (C.c_int, [_P, _I64, _I64, _P, _P, _P]),
+    "slg_rows8_unpack": (C.c_int, [_P, _P, _I64, _I64, _P, _P]),
+    "slg_fc_soft_bwd8_workspace": (_I64, [_I64, _I64, _I64, _I32]),
+    "slg_fc_soft_bwd8": (C.c_int, [_P, _P, _I64, _I64, _I64, _I32, _P, _P, _I32, _P, _F32, _P, _P, _P,
+                                   _P, _P, _I64, _P]),
+    "slg_token_encode": (C.c_int, [_P, _I32, _I64, _I64, _I64, _I64, _P, _I32, _F32, _I32, _P, _P]),
+    "slg_token_encode_bwd_workspace": (_I64, [_I64, _I64, _I64]),
+    "slg_token_encode_bwd": (C.c_int, [_P, _I32, _I64, _I64, _I64, _I64, _P, _I32, _F32, _P, _P, _P,
+                                       _I64, _P]),
+    "slg_token_bits": (C.c_int, [_P, _I32, _I64, _I64, _P, _P]),
+    "slg_token_encode_hard": (C.c_int, [_P, _I32, _I64, _I64, _I64, _I64, _I64, _P, _I32, _P, _P]),
     "slg_conv_soft_bwd_workspace": (C.c_int64, [_I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32,
                                                 _I32, _I32, _I32]),
     "slg_conv_soft_bwd": (C.c_int, [_P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _P,

@@ -1,0 +1,267 @@
+// FC soft backward from an input kept in 8 bits (rows8.h): the gradients of
+// slg_fc_soft_bwd at xq[b][i] = lo[b] + step[b] * q[b][i].
+//
+//   A[b,o]    = sum_k w_a xq[b, ca]   = lo W_a + step * sum_k w_a q[b, ca],   W_a = sum_k w_a
+//   gw_a[o,k] = sum_b ga xq[b, ca]    = sum_b ga lo + sum_b (ga step) q[b, ca]
+//
+// so the gathers read codes and the offsets and steps stay scalars of a
+// sample. Operands, operand gradients and every sum are fp32.
+//
+// A 32-bit word of the codes holds an input's four samples: one LDS read
+// gathers what takes a 16-byte one in fp32, the tile is a quarter of the
+// LDS and a copy of a row of the codes (no transpose), and the 2K gathered
+// words stay in registers from the operands to the weight gradients, where
+// the fp32 kernel gathers twice.
+#include <algorithm>
+
+#include "fc_bwd_input.h"
+#include "fc_bwd_weights.h"
+#include "rows8.h"
+
+namespace slg {
+
+template <int KC>
+constexpr int bwd8_threads() { return KC > 0 ? 1024 : 512; }
+
+// The four codes of a word as floats (v_cvt_f32_ubyte0..3).
+__device__ inline float code_of(uint32_t w, int v) { return (float)((w >> (8 * v)) & 255u); }
+
+// One output per thread over a range of 4-sample tiles: part and gbr as
+// fc_soft_bwd_w_kernel writes them.
+template <int NODE, int KC>
+__global__ void __launch_bounds__((bwd8_threads<KC>()))
+fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ rows, int B, int IN, int ld,
+                 int OUT, int Kr, ParamView pv, float inv_tau, const float* __restrict__ gy, int n_orange,
+                 int n_range, int tiles_per_range, float* __restrict__ part, float* __restrict__ gbr) {
+  constexpr int S = kRows8Tile, KM = KC > 0 ? KC : 16;
+  extern __shared__ __align__(16) unsigned char smem[];
+  uint32_t* xs = reinterpret_cast<uint32_t*>(smem);
+  const int K = KC > 0 ? KC : Kr;
+  // the output ranges of one sample range on one XCD: they stage the same codes
+  const uint32_t lid = xcd_logical_id(blockIdx.x, gridDim.x);
+  const int r_o = (int)(lid % (uint32_t)n_orange);
+  const int r_b = (int)(lid / (uint32_t)n_orange);
+  if (r_b >= n_range) return;  // the grid is padded to a multiple of 8
+  const int o = r_o * blockDim.x + threadIdx.x;
+  const bool valid = o < OUT;
+  FcParams<KM> P;
+  load_params<KC, KM, true>(P, min(o, OUT - 1), K, pv);
+  uint32_t pk[KM];  // index pairs (inputs below 65536)
+  float Wa = 0.0f, Wb = 0.0f;
+#pragma unroll
+  for (int k = 0; k < KM; ++k) {
+    pk[k] = (uint32_t)P.ia[k] | ((uint32_t)P.ib[k] << 16);
+    Wa += P.fa[k];
+    Wb += P.fb[k];
+  }
+  float swa[KM], swb[KM], sp[4] = {0.f, 0.f, 0.f, 0.f}, sla = 0.0f, slb = 0.0f;
+#pragma unroll
+  for (int k = 0; k < KM; ++k) swa[k] = swb[k] = 0.0f;
+  const int n_tiles = (B + S - 1) / S;
+  const int t0 = r_b * tiles_per_range, t_end = min(n_tiles, t0 + tiles_per_range);
+  const int vo = valid ? o * 4 : 0x7ffffffc;
+  for (int t = t0; t < t_end; ++t) {
+    const int b0 = t * S;
+    __syncthreads();  // the previous tile's reads are done
+    const uint4* src = reinterpret_cast<const uint4*>(codes + (int64_t)t * ld);
+    for (int q = threadIdx.x; q < (ld >> 2); q += blockDim.x) reinterpret_cast<uint4*>(xs)[q] = src[q];
+    float g[S], lo[S], step[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int b = min(b0 + s, B - 1);
+      const auto gr = uniform_rsrc(gy + (int64_t)b * OUT, b0 + s < B ? OUT * 4 : 0);
+      g[s] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(gr, vo, 0, 0));
+      lo[s] = b0 + s < B ? rows[2 * (int64_t)b] : 0.0f;
+      step[s] = b0 + s < B ? rows[2 * (int64_t)b + 1] : 0.0f;
+    }
+    __syncthreads();
+    uint32_t qa[KM], qb[KM];
+#pragma unroll
+    for (int k = 0; k < KM; ++k) {
+      if (KC > 0 || k < K) {
+        qa[k] = xs[pk[k] & 0xffffu];
+        qb[k] = xs[pk[k] >> 16];
+      }
+    }
+    float A[S] = {0.f, 0.f, 0.f, 0.f}, Bv[S] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KM; ++k) {
+      if (KC > 0 || k < K) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          A[s] = fmaf(P.fa[k], code_of(qa[k], s), A[s]);
+          Bv[s] = fmaf(P.fb[k], code_of(qb[k], s), Bv[s]);
+        }
+      }
+    }
+    float ga[S], gb[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      float gp[4];
+      node_grad<NODE>(fmaf(step[s], A[s], lo[s] * Wa), fmaf(step[s], Bv[s], lo[s] * Wb), g[s], P.p,
+                      inv_tau, ga[s], gb[s], gp);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sp[q] += gp[q];
+    }
+    if (gbr != nullptr) {  // sample rows of 2*OUT; outputs past OUT are not stored
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const auto gr = uniform_rsrc(gbr + (int64_t)(b0 + s) * (2 * OUT), OUT * 8);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(ga[s]), gr, vo, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(gb[s]), gr, valid ? vo + OUT * 4 : vo, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      sla = fmaf(ga[s], lo[s], sla);
+      slb = fmaf(gb[s], lo[s], slb);
+      ga[s] *= step[s];
+      gb[s] *= step[s];
+    }
+#pragma unroll
+    for (int k = 0; k < KM; ++k) {
+      if (KC > 0 || k < K) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          swa[k] = fmaf(ga[s], code_of(qa[k], s), swa[k]);
+          swb[k] = fmaf(gb[s], code_of(qb[k], s), swb[k]);
+        }
+      }
+    }
+  }
+  if (part != nullptr && valid) {
+    float* base = part + (int64_t)r_b * (2 * K + 4) * OUT + o;
+#pragma unroll
+    for (int k = 0; k < KM; ++k) {
+      if (KC > 0 || k < K) {
+        base[(int64_t)k * OUT] = swa[k] + sla;
+        base[(int64_t)(K + k) * OUT] = swb[k] + slb;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) base[(int64_t)(2 * K + q) * OUT] = sp[q];
+  }
+}
+
+// Workspace (in 4-byte words): records | partials | operand gradients | input-gradient part.
+struct Bwd8Plan {
+  int threads, n_orange, NR, tiles_per_range;
+  int64_t rec, part, gbr, in_ws;
+  int64_t total() const { return rec + part + gbr + in_ws; }
+};
+
+static int64_t bwd8_lds_cap() { return std::min<int64_t>(device_lds_bytes(), 160 * 1024); }
+
+static bool bwd8_takes(int64_t B, int64_t IN, int64_t OUT, int K) {
+  return B >= 0 && B < (1LL << 31) - 8 && IN > 0 && OUT > 0 && OUT < (1LL << 28) && K >= 1 && K <= 16 &&
+         2 * OUT * K < (1LL << 31) && rows8_ld(IN) * 4 <= bwd8_lds_cap() && B * IN < (1LL << 40);
+}
+
+static Bwd8Plan bwd8_plan(int64_t B, int64_t IN, int64_t OUT, int K) {
+  Bwd8Plan p{};
+  p.threads = K == 8 || K == 4 ? 1024 : 512;
+  p.n_orange = (int)cdiv(OUT, p.threads);
+  const int64_t n_tiles = cdiv(std::max<int64_t>(B, 1), kRows8Tile);
+  // one round of workgroups: as many sample ranges as resident slots allow
+  const int64_t per_cu = std::max<int64_t>(1, std::min<int64_t>(1024 / p.threads, 160 * 1024 / (rows8_ld(IN) * 4)));
+  const int64_t slots = per_cu * device_cus();
+  p.NR = (int)std::max<int64_t>(1, std::min<int64_t>(n_tiles, slots / p.n_orange));
+  p.tiles_per_range = (int)cdiv(n_tiles, p.NR);
+  p.NR = (int)cdiv(n_tiles, p.tiles_per_range);
+  auto round4 = [](int64_t n) { return (n + 3) & ~int64_t(3); };
+  p.rec = fc_bwd_record_words(OUT, K);
+  p.part = round4((int64_t)p.NR * (2 * K + 4) * OUT);
+  p.gbr = round4(2 * OUT * n_tiles * kRows8Tile);  // the last tile's rows whole
+  p.in_ws = fc_input_grad_floats(B, IN, OUT, 2, K);
+  return p;
+}
+
+struct Bwd8Args {
+  const uint32_t* codes;
+  const float* rows;
+  int64_t B, IN, OUT;
+  int K;
+  const float* rec;
+  float inv_tau;
+  const float* gy;
+  float *part, *gbr;
+};
+
+template <int NODE, int KC>
+static int launch_bwd8(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
+  auto kern = fc_bwd8_w_kernel<NODE, KC>;
+  const size_t lds = (size_t)rows8_ld(a.IN) * 4;
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)lds);
+    SLG_REQUIRE(e == hipSuccess, (int)e, "fc_soft_bwd8: LDS %zu: %s", lds, hipGetErrorString(e));
+  }
+  ParamView pv{};
+  pv.rec = a.rec;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(cdiv((int64_t)p.n_orange * p.NR, 8) * 8)), dim3(bwd8_threads<KC>()),
+                     lds, st, a.codes, a.rows, (int)a.B, (int)a.IN, (int)rows8_ld(a.IN), (int)a.OUT, a.K, pv,
+                     a.inv_tau, a.gy, p.n_orange, p.NR, p.tiles_per_range, a.part, a.gbr);
+  SLG_LAUNCH_CHECK("fc_soft_bwd8");
+  return 0;
+}
+
+template <int NODE>
+static int launch_bwd8_k(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
+  if (a.K == 8) return launch_bwd8<NODE, 8>(a, p, st);
+  if (a.K == 4) return launch_bwd8<NODE, 4>(a, p, st);
+  return launch_bwd8<NODE, 0>(a, p, st);
+}
+
+}  // namespace slg
+
+using namespace slg;
+
+extern "C" {
+
+int64_t slg_fc_soft_bwd8_workspace(int64_t B, int64_t IN, int64_t OUT, int32_t K) {
+  return bwd8_takes(B, IN, OUT, K) ? bwd8_plan(B, IN, OUT, K).total() : -1;
+}
+
+int slg_fc_soft_bwd8(const uint8_t* codes, const float* rows, int64_t B, int64_t IN, int64_t OUT, int32_t K,
+                     const int32_t* cand, const float* w, int32_t node_kind, const float* node_param,
+                     float inv_tau, const float* gy, float* gx, float* gw, float* gnp, float* workspace,
+                     int64_t workspace_floats, slg_stream_t stream) {
+  SLG_REQUIRE(cand && w && node_param && workspace && ((codes && rows && gy) || B == 0), SLG_E_ARG,
+              "fc_soft_bwd8: null pointer");
+  SLG_REQUIRE(node_kind == SLG_NODE_GATE16 || node_kind == SLG_NODE_WALSH ||
+                  node_kind == SLG_NODE_MULTILINEAR2,
+              SLG_E_ARG, "fc_soft_bwd8: node_kind %d", node_kind);
+  SLG_REQUIRE(bwd8_takes(B, IN, OUT, K), SLG_E_SHAPE, "fc_soft_bwd8: B %lld, IN %lld, OUT %lld, K %d",
+              (long long)B, (long long)IN, (long long)OUT, K);
+  SLG_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)workspace % 16 == 0, SLG_E_ARG,
+              "fc_soft_bwd8: codes or workspace not at a multiple of 16 bytes");
+  const Bwd8Plan p = bwd8_plan(B, IN, OUT, K);
+  SLG_REQUIRE(workspace_floats >= p.total(), SLG_E_ARG, "fc_soft_bwd8: workspace of %lld floats, %lld needed",
+              (long long)workspace_floats, (long long)p.total());
+  hipStream_t st = as_stream(stream);
+  float* part = workspace + p.rec;
+  float* gbr = part + p.part;
+  float* in_ws = gbr + p.gbr;
+  const bool want_w = gw || gnp, want_x = gx != nullptr && B > 0;
+  if (B > 0 && (want_w || want_x)) {
+    fc_bwd_pack_records(cand, w, node_param, OUT, K, IN, reinterpret_cast<uint32_t*>(workspace), st);
+    SLG_LAUNCH_CHECK("fc_soft_bwd8 records");
+    const Bwd8Args a{reinterpret_cast<const uint32_t*>(codes), rows, B, IN, OUT, K, workspace, inv_tau, gy,
+                     want_w ? part : nullptr, want_x ? gbr : nullptr};
+    const int rc = node_kind == SLG_NODE_GATE16  ? launch_bwd8_k<SLG_NODE_GATE16>(a, p, st)
+                   : node_kind == SLG_NODE_WALSH ? launch_bwd8_k<SLG_NODE_WALSH>(a, p, st)
+                                                 : launch_bwd8_k<SLG_NODE_MULTILINEAR2>(a, p, st);
+    if (rc) return rc;
+  }
+  if (want_x) {
+    const int rc = fc_input_grad(gbr, B, IN, OUT, 2, K, cand, w, in_ws, gx, st);
+    if (rc) return rc;
+  }
+  if (want_w) {
+    fc_bwd_reduce(part, B > 0 ? p.NR : 0, OUT, K, gw, gnp, st);  // no samples: zero gradients
+    SLG_LAUNCH_CHECK("fc_soft_bwd8 sums");
+  }
+  return 0;
+}
+
+}  // extern "C"

@@ -20,39 +20,10 @@
 //     ascending order.
 //   * the input gradient is a gather over a table of each input's references
 //     (fc_bwd_input.hip).
-#include "fc_soft_common.h"
 #include "fc_bwd_input.h"
+#include "fc_bwd_weights.h"
 
 namespace slg {
-
-// dL/da, dL/db and dL/dparam of one node at operands (a, b), given dL/dy = g.
-template <int NODE>
-__device__ inline void node_grad(float a, float b, float g, const float4& p, float inv_tau,
-                                 float& ga, float& gb, float (&gp)[4]) {
-  if constexpr (NODE == SLG_NODE_MULTILINEAR2) {
-    // y = (1-a)(1-b) s0 + a(1-b) s1 + (1-a) b s2 + a b s3 (nodes.py:174-178)
-    const float ua = 1.0f - a, ub = 1.0f - b;
-    gp[0] = g * (ua * ub);
-    gp[1] = g * (a * ub);
-    gp[2] = g * (ua * b);
-    gp[3] = g * (a * b);
-    ga = g * (ub * (p.y - p.x) + b * (p.w - p.z));
-    gb = g * (ua * (p.z - p.x) + a * (p.w - p.y));
-  } else {
-    float gz = g;
-    if constexpr (NODE == SLG_NODE_WALSH) {
-      // y = sigmoid(z * inv_tau), z = c0 + c1 a + c2 b + c3 ab (warp.py:14-31)
-      const float y = sigmoid_hw(bilinear(a, b, p) * inv_tau);
-      gz = g * (y * (1.0f - y)) * inv_tau;
-    }
-    gp[0] = gz;
-    gp[1] = gz * a;
-    gp[2] = gz * b;
-    gp[3] = gz * (a * b);
-    ga = gz * (p.y + p.w * b);
-    gb = gz * (p.z + p.w * a);
-  }
-}
 
 // Records from separate arrays: cand [OUT,2,K] int32 (clamped to IN),
 // w [OUT,2,K], np [OUT,4] -> the chunk-major records of fc_soft_kernel
@@ -333,6 +304,17 @@ fc_soft_bwd_reduce_kernel(const float* __restrict__ part, int NR, int OUT, int K
 // ---------------------------------------------------------------------------
 // launch helpers
 // ---------------------------------------------------------------------------
+void fc_bwd_pack_records(const int* cand, const float* w, const float* np, int64_t OUT, int K, int64_t IN,
+                         uint32_t* rec, hipStream_t st) {
+  hipLaunchKernelGGL(fc_soft_pack_records_kernel, dim3((unsigned)cdiv(fc_bwd_record_words(OUT, K), 256)),
+                     dim3(256), 0, st, cand, w, np, (int)OUT, K, (int)IN, rec);
+}
+
+void fc_bwd_reduce(const float* part, int NR, int64_t OUT, int K, float* gw, float* gnp, hipStream_t st) {
+  hipLaunchKernelGGL(fc_soft_bwd_reduce_kernel, dim3((unsigned)cdiv((2 * K + 4) * OUT, kSumCols)),
+                     dim3(kSumThreads), 0, st, part, NR, (int)OUT, K, gw, gnp);
+}
+
 static int bwd_tile(int64_t IN, int64_t per_float_bytes_per_sample) {
   const int64_t cap = std::min<int64_t>(device_lds_bytes(), 160 * 1024);
   for (int s : {4, 2, 1})
@@ -371,7 +353,7 @@ static BwdPlan bwd_plan(int64_t B, int64_t IN, int64_t OUT, int K) {
   p.NR = (int)std::max<int64_t>(1, std::min<int64_t>(n_tiles, slots / p.n_orange));
   p.tiles_per_range = (int)cdiv(n_tiles, p.NR);
   p.NR = (int)cdiv(n_tiles, p.tiles_per_range);
-  p.rec_floats = p.SL ? 0 : cdiv(OUT, 64) * 64 * (int64_t)rec_quads(K) * 4;
+  p.rec_floats = p.SL ? 0 : fc_bwd_record_words(OUT, K);
   p.part_floats = round4((int64_t)p.NR * (2 * K + 4) * OUT);
   p.gbr_floats = round4(2 * OUT * n_tiles * p.Sw);  // the last tile's rows whole
   p.in_floats = fc_input_grad_floats(B, IN, OUT, 2, K);
@@ -468,9 +450,7 @@ int slg_fc_soft_bwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t 
   float* gbr = part + p.part_floats;
   float* in_ws = gbr + p.gbr_floats;
   if (!p.SL) {
-    hipLaunchKernelGGL(fc_soft_pack_records_kernel, dim3((unsigned)cdiv(p.rec_floats, 256)),
-                       dim3(256), 0, st, cand, w, node_param, (int)OUT, K, (int)IN,
-                       reinterpret_cast<uint32_t*>(rec));
+    fc_bwd_pack_records(cand, w, node_param, OUT, K, IN, reinterpret_cast<uint32_t*>(rec), st);
     SLG_LAUNCH_CHECK("fc_soft_pack_records");
   }
   const bool want_w = gw || gnp;
@@ -508,11 +488,7 @@ int slg_fc_soft_bwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t 
     if (rc) return rc;
   }
   if (want_w) {
-    const int NR = B > 0 ? p.NR : 0;  // no samples: zero gradients
-    const int64_t n = (int64_t)(2 * K + 4) * OUT;
-    hipLaunchKernelGGL(fc_soft_bwd_reduce_kernel, dim3((unsigned)cdiv(n, kSumCols)),
-                       dim3(kSumThreads), 0, st, part, NR, (int)OUT, K, gw,
-                       gnp);
+    fc_bwd_reduce(part, B > 0 ? p.NR : 0, OUT, K, gw, gnp, st);  // no samples: zero gradients
     SLG_LAUNCH_CHECK("fc_soft_bwd_reduce");
   }
   return 0;

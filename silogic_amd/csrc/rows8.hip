@@ -1,0 +1,203 @@
+// Rows of activations in 8 bits and back (rows8.h has the layout):
+//   lo = min_i x_i, step = (max_i x_i - lo) / 255,
+//   code_i = rint((x_i - lo) * (255 / (max - lo))),
+// in fp32 with IEEE division, so the codes are defined to the bit. A row of
+// equal values (or one so narrow that 255 / span overflows) has codes 0 and
+// step 0, exact to within its span. Soft activations of a sample share one
+// range; a sample's own lo and step use all 256 codes of it (deep layers
+// crowd around 1/2), and rows of bits {0, 1} come back exactly. A value off by
+// at most half a step: (max - min) / 510. A row that holds an infinity or a
+// NaN, or whose span overflows, has lo = NaN: it comes back as NaN everywhere
+// rather than as finite values that were not there.
+#include <algorithm>
+
+#include "rows8.h"
+
+namespace slg {
+
+constexpr int64_t kRows8Grid = 1 << 20;  // workgroups at most; the rest in turn
+
+struct Rows8Range {
+  float lo, hi;
+  bool bad;
+};
+
+__device__ inline void rows8_take(Rows8Range& r, float v) {
+  r.lo = fminf(r.lo, v);
+  r.hi = fmaxf(r.hi, v);
+  r.bad |= !(fabsf(v) <= 3.402823466e38f);
+}
+
+// Offset, step and reciprocal step of a row from its range.
+__device__ inline void rows8_scale(float lo, float hi, bool bad, float& lo_out, float& step, float& inv) {
+  const float span = hi - lo;
+  bad |= !(span <= 3.402823466e38f);
+  inv = 255.0f / span;
+  step = span / 255.0f;
+  if (!(span > 0.0f) || !(inv <= 3.402823466e38f)) inv = step = 0.0f;
+  lo_out = lo;
+  if (bad) {
+    lo_out = __int_as_float(0x7fc00000);
+    inv = step = 0.0f;
+  }
+}
+
+__device__ inline uint32_t rows8_code(float x, float lo, float inv) {
+  // inv = 0: a constant or not finite row, code 0 (a NaN lo would reach the cast)
+  return inv > 0.0f ? (uint32_t)fminf(rintf((x - lo) * inv), 255.0f) : 0u;
+}
+
+// One workgroup per tile of 4 samples. NU > 0: the tile's values stay in
+// registers between the range and the codes (NU inputs of each row a thread,
+// D <= NU * blockDim); NU = 0: they are read again.
+template <int NU, int T>
+__global__ void __launch_bounds__(T)
+rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_t* __restrict__ codes,
+                  float* __restrict__ rows) {
+  __shared__ Rows8Range part[T / 64][kRows8Tile];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int64_t t = blockIdx.x; t * kRows8Tile < B; t += gridDim.x) {
+    const int64_t b0 = t * kRows8Tile;
+    const int nb = (int)min((int64_t)kRows8Tile, B - b0);
+    const float* p[kRows8Tile];
+#pragma unroll
+    for (int v = 0; v < kRows8Tile; ++v) p[v] = x + (b0 + min(v, nb - 1)) * D;  // past the batch: its last row
+    Rows8Range r[kRows8Tile];
+#pragma unroll
+    for (int v = 0; v < kRows8Tile; ++v) r[v] = {INFINITY, -INFINITY, false};
+    float keep[NU > 0 ? NU : 1][kRows8Tile];
+    if constexpr (NU > 0) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const int i = min(tid + u * T, D - 1);  // past the row: its last value
+#pragma unroll
+        for (int v = 0; v < kRows8Tile; ++v) keep[u][v] = p[v][i];
+      }
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int v = 0; v < kRows8Tile; ++v) rows8_take(r[v], keep[u][v]);
+    } else {
+      for (int i = tid; i < D; i += T)
+#pragma unroll
+        for (int v = 0; v < kRows8Tile; ++v) rows8_take(r[v], p[v][i]);
+    }
+#pragma unroll
+    for (int v = 0; v < kRows8Tile; ++v) {
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        r[v].lo = fminf(r[v].lo, __shfl_xor(r[v].lo, d, 64));
+        r[v].hi = fmaxf(r[v].hi, __shfl_xor(r[v].hi, d, 64));
+      }
+      r[v].bad = __any(r[v].bad);
+      if (lane == 0) part[wave][v] = r[v];
+    }
+    __syncthreads();
+    float lo[kRows8Tile], inv[kRows8Tile];
+#pragma unroll
+    for (int v = 0; v < kRows8Tile; ++v) {
+      Rows8Range a = part[0][v];
+#pragma unroll
+      for (int w = 1; w < T / 64; ++w) {
+        a.lo = fminf(a.lo, part[w][v].lo);
+        a.hi = fmaxf(a.hi, part[w][v].hi);
+        a.bad |= part[w][v].bad;
+      }
+      float step;
+      rows8_scale(a.lo, a.hi, a.bad, lo[v], step, inv[v]);
+      if (tid == 0 && v < nb) {
+        rows[2 * (b0 + v)] = lo[v];
+        rows[2 * (b0 + v) + 1] = step;
+      }
+      if (v >= nb) inv[v] = 0.0f;  // codes 0 past the batch
+    }
+    uint32_t* c = codes + t * ld;
+    auto word = [&](const float (&e)[kRows8Tile]) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int v = 0; v < kRows8Tile; ++v) w |= rows8_code(e[v], lo[v], inv[v]) << (8 * v);
+      return w;
+    };
+    if constexpr (NU > 0) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const int i = tid + u * T;
+        if (i < D) c[i] = word(keep[u]);
+      }
+    } else {
+      for (int i = tid; i < D; i += T) {
+        float e[kRows8Tile];
+#pragma unroll
+        for (int v = 0; v < kRows8Tile; ++v) e[v] = p[v][i];
+        c[i] = word(e);
+      }
+    }
+    if (tid < ld - D) c[D + tid] = 0u;
+    __syncthreads();  // part is written again
+  }
+}
+
+// Values that the codes stand for: one thread per word, four rows written.
+__global__ void __launch_bounds__(256)
+rows8_unpack_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ rows, int64_t B, int D,
+                    int ld, int per_tile, int64_t blocks, float* __restrict__ x) {
+  for (int64_t k = blockIdx.x; k < blocks; k += gridDim.x) {
+    const int64_t t = k / per_tile;
+    const int i = (int)(k - t * per_tile) * 256 + threadIdx.x;
+    if (i >= D) continue;
+    const uint32_t w = codes[t * ld + i];
+#pragma unroll
+    for (int v = 0; v < kRows8Tile; ++v) {
+      const int64_t b = t * kRows8Tile + v;
+      if (b < B) x[b * D + i] = fmaf((float)((w >> (8 * v)) & 255u), rows[2 * b + 1], rows[2 * b]);
+    }
+  }
+}
+
+template <int NU, int T>
+static void launch_pack(const float* x, int64_t B, int64_t D, uint32_t* codes, float* rows, hipStream_t st) {
+  hipLaunchKernelGGL((rows8_pack_kernel<NU, T>), dim3((unsigned)std::min<int64_t>(cdiv(B, kRows8Tile), kRows8Grid)), dim3(T), 0, st, x, B,
+                     (int)D, (int)rows8_ld(D), codes, rows);
+}
+
+}  // namespace slg
+
+using namespace slg;
+
+extern "C" {
+
+int64_t slg_rows8_ld(int64_t D) { return rows8_ld(D); }
+
+int slg_rows8_pack(const float* x, int64_t B, int64_t D, uint8_t* codes, float* rows, slg_stream_t stream) {
+  SLG_REQUIRE((x && codes && rows) || B == 0, SLG_E_ARG, "rows8_pack: null pointer");
+  SLG_REQUIRE(B >= 0 && D > 0 && D < (1LL << 28) && B < (1LL << 31) && B * D < (1LL << 40), SLG_E_SHAPE,
+              "rows8_pack: B %lld, D %lld", (long long)B, (long long)D);
+  SLG_REQUIRE((uintptr_t)codes % 16 == 0, SLG_E_ARG, "rows8_pack: codes not at a multiple of 16 bytes");
+  if (B == 0) return 0;
+  hipStream_t st = as_stream(stream);
+  uint32_t* c = reinterpret_cast<uint32_t*>(codes);
+  if (D <= 256) launch_pack<1, 256>(x, B, D, c, rows, st);
+  else if (D <= 1024) launch_pack<4, 256>(x, B, D, c, rows, st);
+  else if (D <= 4096) launch_pack<4, 1024>(x, B, D, c, rows, st);
+  else if (D <= 8192) launch_pack<8, 1024>(x, B, D, c, rows, st);
+  else if (D <= 16384) launch_pack<16, 1024>(x, B, D, c, rows, st);
+  else launch_pack<0, 1024>(x, B, D, c, rows, st);
+  SLG_LAUNCH_CHECK("rows8_pack");
+  return 0;
+}
+
+int slg_rows8_unpack(const uint8_t* codes, const float* rows, int64_t B, int64_t D, float* x,
+                     slg_stream_t stream) {
+  SLG_REQUIRE((x && codes && rows) || B == 0, SLG_E_ARG, "rows8_unpack: null pointer");
+  SLG_REQUIRE(B >= 0 && D > 0 && D < (1LL << 28) && B < (1LL << 31) && B * D < (1LL << 40), SLG_E_SHAPE,
+              "rows8_unpack: B %lld, D %lld", (long long)B, (long long)D);
+  SLG_REQUIRE((uintptr_t)codes % 16 == 0, SLG_E_ARG, "rows8_unpack: codes not at a multiple of 16 bytes");
+  if (B == 0) return 0;
+  const int64_t per = cdiv(D, 256), blocks = cdiv(B, kRows8Tile) * per;
+  hipLaunchKernelGGL(rows8_unpack_kernel, dim3((unsigned)std::min(blocks, kRows8Grid)), dim3(256), 0, as_stream(stream),
+                     reinterpret_cast<const uint32_t*>(codes), rows, B, (int)D, (int)rows8_ld(D), (int)per, blocks, x);
+  SLG_LAUNCH_CHECK("rows8_unpack");
+  return 0;
+}
+
+}  // extern "C"

@@ -1,8 +1,9 @@
-"""Learnable thermometer encoder (silogic/encoders.py:12-49) on the GPU."""
+"""Learnable encoders on the GPU: the thermometer of numbers
+(silogic/encoders.py:12-49) and the bits of tokens."""
 import torch
 import torch.nn as nn
 
-from . import _lib, ops
+from . import _lib, derived, ops
 from .data import _encode
 
 
@@ -64,3 +65,116 @@ class LearnedThermometerEncoder(nn.Module):
         ops.require_gpu(x)
         return _encode(ops._as_f32(x), ops._c(self.thresholds.detach(), torch.float32), True,
                        1 if word_major else 0, self.bits)
+
+
+class _TokenFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale, ste, pad):
+        ctx.save_for_backward(ids, table)
+        ctx.meta = (scale, pad)
+        return ops.token_encode(ids, table.detach(), scale, ste, pad)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        ids, table = ctx.saved_tensors
+        return None, ops.token_encode_bwd(ids, table.detach(), *ctx.meta, gy), None, None, None
+
+
+class TokenEncoder(nn.Module):
+    """Learned bits of discrete tokens (no counterpart in the reference, whose
+    encoders take numbers): ids ``[B]`` or ``[B, L]`` (int32 or int64) ->
+    ``[B, L*bits]``, feature ``l*bits + d`` of token ``l``.
+
+    The soft forward is ``sigmoid(scale * weight[id])`` in fp32, with ``ste``
+    the hard bits ``weight[id] > 0`` under the same gradient (straight
+    through); :meth:`forward_hard` and :meth:`forward_packed` are the hard
+    bits. A token with id ``padding_idx``, or outside the table, is absent: its
+    features are 0 and it adds to no gradient. ``weight [num_tokens, bits]``
+    may be fp32, bf16 or fp16; its gradient sums each id's tokens in fp32 in
+    one order (the same bits on every call)."""
+
+    def __init__(self, num_tokens, bits, scale=1.0, ste=False, padding_idx=None):
+        super().__init__()
+        self._settle(torch.randn(num_tokens, bits), scale, ste, padding_idx)
+
+    @classmethod
+    def from_weight(cls, weight, scale=1.0, ste=False, padding_idx=None):
+        """An encoder on ``weight [num_tokens, bits]`` itself (not a copy)."""
+        enc = cls.__new__(cls)
+        nn.Module.__init__(enc)
+        enc._settle(weight, scale, ste, padding_idx)
+        return enc
+
+    def _settle(self, weight, scale, ste, padding_idx):
+        if weight.dim() != 2 or 0 in weight.shape:
+            raise ValueError(f"TokenEncoder: weight {tuple(weight.shape)}, [num_tokens, bits] expected")
+        if weight.dtype not in ops.TABLE_DTYPES:
+            raise TypeError(f"TokenEncoder: weight of {weight.dtype} (fp32, bf16 or fp16)")
+        self.num_tokens, self.bits = weight.shape
+        if padding_idx is not None:
+            if not -self.num_tokens <= padding_idx < self.num_tokens:
+                raise ValueError(f"TokenEncoder: padding_idx {padding_idx} for {self.num_tokens} tokens")
+            padding_idx %= self.num_tokens
+        self.scale, self.ste, self.padding_idx = float(scale), bool(ste), padding_idx
+        self.weight = weight if isinstance(weight, nn.Parameter) else nn.Parameter(weight)
+
+    def extra_repr(self):
+        return (f"{self.num_tokens}, {self.bits}, scale={self.scale}, ste={self.ste}, "
+                f"padding_idx={self.padding_idx}")
+
+    @property
+    def _pad(self):
+        return -1 if self.padding_idx is None else self.padding_idx
+
+    def _ids(self, ids):
+        if ids.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"TokenEncoder: ids of {ids.dtype} (int32 or int64)")
+        if ids.dim() not in (1, 2):
+            raise ValueError(f"TokenEncoder: ids {tuple(ids.shape)}, [B] or [B, L] expected")
+        if self.weight.dtype not in ops.TABLE_DTYPES:
+            raise TypeError(f"TokenEncoder: weight of {self.weight.dtype} (fp32, bf16 or fp16)")
+        ops.require_gpu(ids, self.weight)
+        ops.same_device("TokenEncoder", ids, self.weight)
+        return ops._c(ids if ids.dim() == 2 else ids.unsqueeze(1))
+
+    def forward(self, ids):
+        ids = self._ids(ids)
+        if torch.compiler.is_compiling():
+            return torch.ops.silogic_hip.token_encode(ids, self.weight, self.scale, self.ste, self._pad)
+        return _TokenFn.apply(ids, ops._c(self.weight), self.scale, self.ste, self._pad)
+
+    def _bit_table(self):
+        """Bit words of the weight, made once per version of it. Another stream
+        than the one that made them waits for them; a captured call that finds
+        none of its own stream makes them inside the graph."""
+        w, here = self.weight.detach(), torch.cuda.current_stream(self.weight.device)
+        if torch.cuda.is_current_stream_capturing():
+            slot = self.__dict__.get("_derived_bits")
+            if slot is not None and slot[0] == derived.state_key(self) and slot[1][2] == here:
+                return slot[1][1]
+            return ops.token_bits(ops._c(w))
+
+        def build():
+            bits = ops.token_bits(ops._c(w))
+            return w, bits, here, here.record_event()   # w: its address stays taken while the key holds it
+
+        _, bits, there, done = derived.cached(self, "_derived_bits", derived.state_key(self), build)
+        if there != here:
+            here.wait_event(done)
+            bits.record_stream(here)
+        return bits
+
+    @torch.no_grad()
+    def forward_hard(self, ids):
+        """uint8 bits ``[B, L*bits]``."""
+        ids = self._ids(ids)
+        return ops.token_encode_hard(ids, self._bit_table(), self.bits, self._pad, 2)
+
+    @torch.no_grad()
+    def forward_packed(self, ids, word_major=False):
+        """The bits of :meth:`forward_hard` packed 64 samples per word:
+        ``[L*bits, nw]`` (``word_major``: ``[nw, L*bits]``), the input of
+        ``LogicNet.forward_hard_packed``."""
+        ids = self._ids(ids)
+        return ops.token_encode_hard(ids, self._bit_table(), self.bits, self._pad, int(word_major))

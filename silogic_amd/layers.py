@@ -44,6 +44,8 @@ class LogicLayer(nn.Module):
     / fixed wiring. ``use_triton`` is accepted for API compatibility and
     ignored (the HIP kernels always run)."""
 
+    saved_bits = 32   # of the input, kept for the backward (activations.save_activations)
+
     def __init__(self, in_dim, out_dim, node="gate16", connectome="topk", arity=2,
                  k=8, gate_eval="basis", residual_p=0.0, seed=None,
                  window=0, tau=1.0, degree=None, gate_select="softmax",
@@ -144,6 +146,10 @@ class LogicLayer(nn.Module):
                 and conn.candidates_i32().numel() < 1 << 31
                 and ops.param_levels_ok(getattr(conn, "conn", None), [raw], conn.k))
 
+    def takes_rows8(self):
+        """Whether the layer can keep its input in 8 bits for the backward."""
+        return self.arity == 2 and not self.is_lut and self._conn.k <= 16
+
     def records_ok(self):
         """Whether the forward without gradients runs on per-output records:
         a plain softmax selection over inputs below 65536 (records hold 16-bit
@@ -196,8 +202,8 @@ class LogicLayer(nn.Module):
                                     self.node.corner_z(), False)
             else:
                 self._check_supported()
-                z = ops.fc_soft(x, conn.candidates_i32(), conn.weights(), self.node.coef(),
-                                ops.GATE16, 1.0)
+                fc = ops.fc_soft8 if self.saved_bits == 8 and _needs_grad(self, x) else ops.fc_soft
+                z = fc(x, conn.candidates_i32(), conn.weights(), self.node.coef(), ops.GATE16, 1.0)
             return self.node.gumbel_sigmoid(z)
         if self.is_lut:
             conn = self._conn
@@ -217,6 +223,9 @@ class LogicLayer(nn.Module):
         grad = _needs_grad(self, x)
         if grad and self._params_op(self.node.raw()):
             conn = self._conn
+            if self.saved_bits == 8:
+                return ops.fc_layer8(x, conn.candidates_i32(), getattr(conn, "conn", None),
+                                     self.node.raw(), self.node.kind, self._inv_tau())
             return torch.ops.silogic_hip.fc_layer(
                 x, conn.candidates_i32(), getattr(conn, "conn", None), self.node.raw(),
                 self.node.kind, float(self._inv_tau()))[0]
@@ -227,6 +236,8 @@ class LogicLayer(nn.Module):
             return ops.fc_soft_rec(x, rec, self.in_dim, self.out_dim, K, self.node.kind,
                                    self._inv_tau())
         cand, w, npar = self.soft_params(grad)
+        if grad and self.saved_bits == 8:
+            return ops.fc_soft8(x, cand, w, npar, self.node.kind, self._inv_tau())
         return ops.fc_soft(x, cand, w, npar, self.node.kind, self._inv_tau())
 
     def hard_spec(self):

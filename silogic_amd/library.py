@@ -346,6 +346,154 @@ fc_lut_layer.register_autograd(_fc_lut_layer_backward, setup_context=_fc_lut_lay
 
 
 # ---------------------------------------------------------------------------
+# Gate layers that keep their input in 8 bits for the backward: what
+# torch.compile traces (eager calls take ops.fc_layer8 / ops.fc_soft8, whose
+# autograd functions cost less on the host)
+# ---------------------------------------------------------------------------
+def _rows8_outputs(x):
+    B, D = x.shape
+    return (x.new_empty(((B + 3) // 4, (D + 3) // 4 * 4, 4), dtype=torch.uint8),
+            x.new_empty((B, 2), dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{_NS}::fc_layer8", mutates_args=())
+def fc_layer8(x: Tensor, cand: Tensor, conn: Optional[Tensor], raw: Tensor, node_kind: int,
+              inv_tau: float) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """``(y, codes, rows, w, kept)`` of :func:`ops.fc_layer8`."""
+    return ops.fc_layer8_fwd(x, cand, conn, raw, node_kind, inv_tau)
+
+
+@fc_layer8.register_fake
+def _(x, cand, conn, raw, node_kind, inv_tau):
+    y, w, kept = _layer_outputs(x, (x.shape[0], cand.shape[0]), cand.shape,
+                                (cand.shape[0] * (5 if node_kind == ops.GATE16 else 1), 4))
+    return (y, *_rows8_outputs(x), w, kept)
+
+
+@torch.library.custom_op(f"{_NS}::fc_layer8_bwd", mutates_args=())
+def fc_layer8_bwd(codes: Tensor, rows: Tensor, cand: Tensor, w: Tensor, kept: Tensor, in_dim: int,
+                  node_kind: int, inv_tau: float, gy: Tensor, need_x: bool, need_conn: bool,
+                  need_raw: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """``(gx, gconn, graw)`` of fc_layer8; unneeded ones are empty."""
+    got = ops.fc_layer8_bwd(codes, rows, cand, w, kept, in_dim, node_kind, inv_tau, gy, need_x,
+                            need_conn, need_raw)
+    return tuple(g if g is not None else _empty(rows) for g in got)
+
+
+@fc_layer8_bwd.register_fake
+def _(codes, rows, cand, w, kept, in_dim, node_kind, inv_tau, gy, need_x, need_conn, need_raw):
+    raw = (cand.shape[0], 16 if node_kind == ops.GATE16 else 4)
+    return _gradients(rows, ((rows.shape[0], in_dim), need_x), (w.shape, need_conn), (raw, need_raw))
+
+
+def _fc_layer8_setup(ctx, inputs, output):
+    x, cand, conn, raw, node_kind, inv_tau = inputs
+    ctx.mark_non_differentiable(*output[1:])
+    ctx.set_materialize_grads(False)   # no zero tensors in their place
+    ctx.y_shape = output[0].shape
+    ctx.save_for_backward(*output[1:3], cand, *output[3:])
+    ctx.meta = (x.shape[1], node_kind, inv_tau)
+
+
+def _fc_layer8_backward(ctx, gy, *_):
+    need, saved = ctx.needs_input_grad, ctx.saved_tensors
+    gy = _output_gradient(ctx, saved[1], gy)
+    gx, gc, gr = fc_layer8_bwd(*saved, *ctx.meta, gy, need[0], need[2], need[3])
+    return _none(gx, need[0]), None, _none(gc, need[2]), _none(gr, need[3]), None, None
+
+
+fc_layer8.register_autograd(_fc_layer8_backward, setup_context=_fc_layer8_setup)
+
+
+@torch.library.custom_op(f"{_NS}::fc_soft8", mutates_args=())
+def fc_soft8(x: Tensor, cand: Tensor, w: Tensor, npar: Tensor, node_kind: int,
+             inv_tau: float) -> Tuple[Tensor, Tensor, Tensor]:
+    """``(y, codes, rows)`` of :func:`ops.fc_soft8`."""
+    ops.require_gpu(x, cand, w, npar)
+    ops.check_layer8(x, cand, w=(w, cand.shape), npar=(npar, (cand.shape[0], 4)))
+    return ops.fc_soft8_fwd(ops._as_f32(x), ops._c(cand, torch.int32), ops._c(w, torch.float32),
+                            ops._c(npar, torch.float32), node_kind, inv_tau)
+
+
+@fc_soft8.register_fake
+def _(x, cand, w, npar, node_kind, inv_tau):
+    return (x.new_empty((x.shape[0], cand.shape[0]), dtype=torch.float32), *_rows8_outputs(x))
+
+
+@torch.library.custom_op(f"{_NS}::fc_soft8_bwd", mutates_args=())
+def fc_soft8_bwd(codes: Tensor, rows: Tensor, cand: Tensor, w: Tensor, npar: Tensor, in_dim: int,
+                 node_kind: int, inv_tau: float, gy: Tensor, need_x: bool, need_w: bool,
+                 need_np: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """``(gx, gw, gnp)`` of fc_soft8; unneeded ones are empty."""
+    got = ops.fc_soft_bwd8(codes, rows, in_dim, cand, w, npar, node_kind, inv_tau, gy, need_x, need_w,
+                           need_np)
+    return tuple(g if g is not None else _empty(rows) for g in got)
+
+
+@fc_soft8_bwd.register_fake
+def _(codes, rows, cand, w, npar, in_dim, node_kind, inv_tau, gy, need_x, need_w, need_np):
+    return _gradients(rows, ((rows.shape[0], in_dim), need_x), (w.shape, need_w), (npar.shape, need_np))
+
+
+def _fc_soft8_setup(ctx, inputs, output):
+    x, cand, w, npar, node_kind, inv_tau = inputs
+    ctx.mark_non_differentiable(*output[1:])
+    ctx.set_materialize_grads(False)
+    ctx.y_shape = output[0].shape
+    ctx.save_for_backward(*output[1:], cand, w, npar)
+    ctx.meta = (x.shape[1], node_kind, inv_tau)
+
+
+def _fc_soft8_backward(ctx, gy, *_):
+    need, saved = ctx.needs_input_grad, ctx.saved_tensors
+    gy = _output_gradient(ctx, saved[1], gy)
+    gx, gw, gn = fc_soft8_bwd(*saved, *ctx.meta, gy, need[0], need[2], need[3])
+    return _none(gx, need[0]), None, _none(gw, need[2]), _none(gn, need[3]), None, None
+
+
+fc_soft8.register_autograd(_fc_soft8_backward, setup_context=_fc_soft8_setup)
+
+
+# ---------------------------------------------------------------------------
+# Token encoder: what torch.compile traces
+# ---------------------------------------------------------------------------
+@torch.library.custom_op(f"{_NS}::token_encode", mutates_args=())
+def token_encode(ids: Tensor, table: Tensor, scale: float, ste: bool, pad: int) -> Tensor:
+    """``ids [B,L]``, ``table [V,D]`` -> ``[B, L*D]`` fp32."""
+    ops.require_gpu(ids, table)
+    return ops.token_encode(ops._c(ids), ops._c(table), scale, ste, pad)
+
+
+@token_encode.register_fake
+def _(ids, table, scale, ste, pad):
+    return table.new_empty((ids.shape[0], ids.shape[1] * table.shape[1]), dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_NS}::token_encode_bwd", mutates_args=())
+def token_encode_bwd(ids: Tensor, table: Tensor, scale: float, pad: int, gy: Tensor) -> Tensor:
+    return ops.token_encode_bwd(ops._c(ids), ops._c(table), scale, pad, gy)
+
+
+@token_encode_bwd.register_fake
+def _(ids, table, scale, pad, gy):
+    return table.new_empty(table.shape)
+
+
+def _token_setup(ctx, inputs, output):
+    ids, table, scale, ste, pad = inputs
+    ctx.save_for_backward(ids, table)
+    ctx.meta = (scale, pad)
+
+
+def _token_backward(ctx, gy):
+    g = token_encode_bwd(*ctx.saved_tensors, *ctx.meta, gy) if ctx.needs_input_grad[1] else None
+    return None, g, None, None, None
+
+
+token_encode.register_autograd(_token_backward, setup_context=_token_setup)
+
+
+# ---------------------------------------------------------------------------
 # LUT FC layer (multilinear_logic)
 # ---------------------------------------------------------------------------
 @torch.library.custom_op(f"{_NS}::fc_lut_soft", mutates_args=())

@@ -70,6 +70,69 @@ def _as_f32(x):
     return x.contiguous()
 
 
+def call_on(t, name, *args):
+    """Entry point ``name`` with ``args`` and the current stream of ``t``'s
+    device, launched from that device."""
+    if t.get_device() == torch.cuda.current_device():
+        _lib.call(name, *args, _stream(t))
+    else:
+        with torch.cuda.device(t.device):
+            _lib.call(name, *args, _stream(t))
+
+
+def same_device(what, *ts):
+    """Raise unless all of ``ts`` (None apart) are on one device."""
+    ds = {t.device for t in ts if t is not None}
+    if len(ds) > 1:
+        raise ValueError(f"{what}: tensors on {', '.join(sorted(map(str, ds)))}")
+
+
+# ---------------------------------------------------------------------------
+# activations in 8 bits
+# ---------------------------------------------------------------------------
+def rows8_pack(x):
+    """``x [B, D]`` fp32 -> ``(codes [ceil(B/4), ld, 4] uint8, rows [B, 2])``
+    (``slg_rows8_pack``)."""
+    B, D = x.shape
+    codes = torch.empty((-(-B // 4), (D + 3) // 4 * 4, 4), device=x.device, dtype=torch.uint8)
+    rows = torch.empty((B, 2), device=x.device, dtype=torch.float32)
+    call_on(x, "slg_rows8_pack", _p(x), B, D, _p(codes), _p(rows))
+    return codes, rows
+
+
+def rows8_unpack(codes, rows, D):
+    """The values that the codes stand for, ``[B, D]`` fp32."""
+    B = rows.shape[0]
+    x = torch.empty((B, D), device=codes.device, dtype=torch.float32)
+    call_on(codes, "slg_rows8_unpack", _p(codes), _p(rows), B, D, _p(x))
+    return x
+
+
+def fc_soft_bwd8(codes, rows, in_dim, cand, w, npar, node_kind, inv_tau, gy, need_x=True,
+                 need_w=True, need_np=True):
+    """:func:`fc_soft_bwd` of an input kept as ``codes`` and ``rows``. Rows too
+    wide for the kernel on codes are unpacked for the one on fp32."""
+    require_gpu(codes, rows, cand, w, npar, gy)
+    same_device("fc_soft_bwd8", codes, rows, cand, w, npar, gy)
+    cand, w, npar = _c(cand, torch.int32), _c(w, torch.float32), _c(npar, torch.float32)
+    gy = _c(gy, torch.float32)
+    B, (OUT, _, K) = rows.shape[0], cand.shape
+    if gy.shape != (B, OUT):
+        raise ValueError(f"fc_soft_bwd8: gradient {tuple(gy.shape)} for {(B, OUT)}")
+    ws = _lib.lib().slg_fc_soft_bwd8_workspace(B, in_dim, OUT, K)
+    if ws < 0:
+        x = rows8_unpack(codes, rows, in_dim)
+        return fc_soft_bwd(x, cand, w, npar, node_kind, inv_tau, gy, need_x, need_w, need_np)
+    dev, f32 = codes.device, torch.float32
+    gx = torch.empty((B, in_dim), device=dev, dtype=f32) if need_x else None
+    gw = torch.empty((OUT, 2, K), device=dev, dtype=f32) if need_w else None
+    gn = torch.empty((OUT, 4), device=dev, dtype=f32) if need_np else None
+    work = torch.empty(max(ws, 1), device=dev, dtype=f32)
+    call_on(codes, "slg_fc_soft_bwd8", _p(codes), _p(rows), B, in_dim, OUT, K, _p(cand), _p(w),
+            node_kind, _p(npar), float(inv_tau), _p(gy), _p(gx), _p(gw), _p(gn), _p(work), ws)
+    return gx, gw, gn
+
+
 # ---------------------------------------------------------------------------
 # FC soft
 # ---------------------------------------------------------------------------
@@ -256,6 +319,165 @@ def layer_params_bwd(w, gw, kept, nodes, kind, arity, scale, gnp, need_conn, nee
               None if kind == WALSH else ctypes.c_void_p(kept.data_ptr() + 4 * skip), _p(gnp),
               _p(gconn), _ptrs(graw), _stream(w))
     return gconn, graw
+
+
+# ---------------------------------------------------------------------------
+# gate layers whose input is kept in 8 bits for the backward
+# ---------------------------------------------------------------------------
+def check_layer8(x, cand, **shapes):
+    """Raise for sizes that the 8-bit backward does not take."""
+    if cand.dim() != 3 or cand.shape[1] != 2 or not 1 <= cand.shape[2] <= 16 or cand.shape[0] < 1:
+        raise NotImplementedError(f"8-bit activations: candidates {tuple(cand.shape)} "
+                                  "(gate layers [OUT, 2, K] of 1 to 16 candidates)")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"8-bit activations: input {tuple(x.shape)}, [B, IN] expected")
+    for name, (t, shape) in shapes.items():
+        if t is not None and tuple(t.shape) != tuple(shape):
+            raise ValueError(f"8-bit activations: {name} {tuple(t.shape)}, {tuple(shape)} expected")
+
+
+def fc_soft8_fwd(x, cand, w, npar, node_kind, inv_tau):
+    """``(y, codes, rows)``: the soft gate layer and its input in 8 bits."""
+    y = _fc_soft_launch(x, cand, w, npar, node_kind, inv_tau)
+    return (y, *rows8_pack(x))
+
+
+def fc_layer8_fwd(x, cand, conn, raw, node_kind, inv_tau):
+    """``(y, codes, rows, w, kept)`` of a gate layer from its own parameters
+    (``w``, ``kept`` as :func:`layer_params` returns them)."""
+    require_gpu(x, cand, conn, raw)
+    same_device("fc_layer8", x, cand, conn, raw)
+    check_layer8(x, cand, conn=(conn, cand.shape),
+                 raw=(raw, (cand.shape[0], 16 if node_kind == GATE16 else 4)))
+    x, cand = _as_f32(x), _c(cand, torch.int32)
+    w, kept = layer_params(conn, tuple(cand.shape), [raw], node_kind, 2)
+    npar = kept[:cand.shape[0]] if node_kind == GATE16 else kept
+    return (*fc_soft8_fwd(x, cand, w, npar, node_kind, inv_tau), w, kept)
+
+
+def fc_layer8_bwd(codes, rows, cand, w, kept, in_dim, node_kind, inv_tau, gy, need_x, need_conn,
+                  need_raw):
+    """``(gx, gconn, graw)`` of :func:`fc_layer8`; None where not needed."""
+    gx, gw, gn = fc_soft_bwd8(codes, rows, in_dim, cand, w, kept[:cand.shape[0]], node_kind, inv_tau,
+                              gy, need_x, need_conn, need_raw)
+    gconn, (graw,) = layer_params_bwd(w, gw, kept, [1], node_kind, 2, 1.0, gn, need_conn, [need_raw],
+                                      4 * w.shape[0] if node_kind == GATE16 else 0)
+    return gx, gconn, None if graw is None else graw.squeeze(1)
+
+
+class _FcLayer8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, cand, conn, raw, node_kind, inv_tau):
+        y, *saved = fc_layer8_fwd(x.detach(), cand, None if conn is None else conn.detach(),
+                                  raw.detach(), node_kind, inv_tau)
+        ctx.save_for_backward(cand, *saved)
+        ctx.meta = (x.shape[1], node_kind, inv_tau)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        cand, codes, rows, w, kept = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        gx, gc, gr = fc_layer8_bwd(codes, rows, cand, w, kept, *ctx.meta, gy, need[0], need[2], need[3])
+        return gx, None, gc, gr, None, None
+
+
+class _FcSoft8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, cand, w, npar, node_kind, inv_tau):
+        require_gpu(x, cand, w, npar)
+        same_device("fc_soft8", x, cand, w, npar)
+        check_layer8(x, cand, w=(w, cand.shape), npar=(npar, (cand.shape[0], 4)))
+        cand, w, npar = _c(cand, torch.int32), _c(w.detach(), torch.float32), _c(npar.detach(), torch.float32)
+        y, codes, rows = fc_soft8_fwd(_as_f32(x.detach()), cand, w, npar, node_kind, inv_tau)
+        ctx.save_for_backward(codes, rows, cand, w, npar)
+        ctx.meta = (x.shape[1], node_kind, inv_tau)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        codes, rows, cand, w, npar = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        IN, node_kind, inv_tau = ctx.meta
+        gx, gw, gn = fc_soft_bwd8(codes, rows, IN, cand, w, npar, node_kind, inv_tau, gy, need[0], need[2],
+                                  need[3])
+        return gx, None, gw, gn, None, None
+
+
+def fc_layer8(x, cand, conn, raw, node_kind, inv_tau=1.0):
+    """A gate layer from its own parameters, ``x [B,IN] -> [B,OUT]``, that keeps
+    ``x`` in 8 bits for the backward: ``cand [OUT,2,K]``, ``conn`` the same shape
+    (None: fixed wiring), ``raw [OUT,16]`` (gate16) or ``[OUT,4]``. The output is
+    :func:`fc_soft`'s; the gradients are taken at the values that the codes
+    stand for (``activations.pack_rows8``)."""
+    if torch.compiler.is_compiling():
+        return torch.ops.silogic_hip.fc_layer8(x, cand, conn, raw, node_kind, float(inv_tau))[0]
+    if not _grad_path(x, conn, raw):   # nothing to keep
+        w, npar = fc_soft_prep(conn, raw, node_kind, *cand.shape[::2])
+        return fc_soft(x, cand, w, npar, node_kind, inv_tau)
+    return _FcLayer8.apply(x, cand, conn, raw, node_kind, float(inv_tau))
+
+
+def fc_soft8(x, cand, w, npar, node_kind, inv_tau=1.0):
+    """:func:`fc_soft` that keeps ``x`` in 8 bits for the backward."""
+    if torch.compiler.is_compiling():
+        return torch.ops.silogic_hip.fc_soft8(x, cand, w, npar, node_kind, float(inv_tau))[0]
+    if not _grad_path(x, w, npar):
+        return fc_soft(x, cand, w, npar, node_kind, inv_tau)
+    return _FcSoft8.apply(x, cand, w, npar, node_kind, float(inv_tau))
+
+
+# ---------------------------------------------------------------------------
+# token encoder
+# ---------------------------------------------------------------------------
+TABLE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def token_encode(ids, table, scale, ste, pad):
+    """``ids [B, L]`` int32 / int64, ``table [V, D]`` -> ``[B, L * D]`` fp32
+    (``slg_token_encode``)."""
+    (B, L), (V, D) = ids.shape, table.shape
+    y = torch.empty((B, L * D), device=table.device, dtype=torch.float32)
+    call_on(table, "slg_token_encode", _p(ids), ids.element_size(), B * L, V, D, pad, _p(table),
+            TABLE_DTYPES[table.dtype], float(scale), int(ste), _p(y))
+    return y
+
+
+def token_encode_bwd(ids, table, scale, pad, gy):
+    """The table's gradient, in the table's type."""
+    (B, L), (V, D) = ids.shape, table.shape
+    if gy.shape != (B, L * D):
+        raise ValueError(f"token_encode_bwd: gradient {tuple(gy.shape)} for {(B, L * D)}")
+    g = torch.empty_like(table)
+    ws = _lib.lib().slg_token_encode_bwd_workspace(B * L, V, D)
+    work = torch.empty(max(ws, 1), device=table.device, dtype=torch.int32)
+    call_on(table, "slg_token_encode_bwd", _p(ids), ids.element_size(), B * L, V, D, pad, _p(table),
+            TABLE_DTYPES[table.dtype], float(scale), _p(_c(gy, torch.float32)), _p(g), _p(work), ws)
+    return g
+
+
+def token_bits(table):
+    """Bit words ``[V, ceil(D / 64)]`` of ``table > 0``."""
+    V, D = table.shape
+    bits = torch.empty((V, -(-D // 64)), device=table.device, dtype=torch.int64)
+    call_on(table, "slg_token_bits", _p(table), TABLE_DTYPES[table.dtype], V, D, _p(bits))
+    return bits
+
+
+def token_encode_hard(ids, bits, D, pad, layout):
+    """Bits of ``ids [B, L]``'s tokens: layout 0 ``[L*D, nw]``, 1 ``[nw, L*D]``,
+    2 uint8 ``[B, L*D]``."""
+    B, L = ids.shape
+    if layout == 2:
+        out = torch.empty((B, L * D), device=bits.device, dtype=torch.uint8)
+    else:
+        nw = n_words(B)
+        out = torch.empty((nw, L * D) if layout else (L * D, nw), device=bits.device, dtype=torch.int64)
+    call_on(bits, "slg_token_encode_hard", _p(ids), ids.element_size(), B, L, bits.shape[0], D, pad,
+            _p(bits), layout, _p(out))
+    return out
 
 
 # ---------------------------------------------------------------------------
