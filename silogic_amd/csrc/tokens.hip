@@ -15,7 +15,7 @@
 
 #include <algorithm>
 
-#include "slg_common.h"
+#include "radix_sort.h"
 
 namespace slg {
 
@@ -51,9 +51,11 @@ __device__ inline int tok_row(const IdT* __restrict__ ids, int64_t n, int V, int
   return (t >= 0 && t < V && t != pad) ? (int)t : V;
 }
 
-__device__ inline float tok_value(float e, float scale, bool ste) {
+// sigmoid(z) of a table's entry, from t = -z log2 e: 1 / (1 + 2^t) with the
+// hardware exp2 and reciprocal (about an ulp each).
+__device__ inline float tok_value(float e, float nlog2, bool ste) {
   if (ste) return e > 0.0f ? 1.0f : 0.0f;
-  return 1.0f / (1.0f + expf(-scale * e));
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(e * nlog2));
 }
 
 // scale * sigmoid'(scale e), from exp(-|z|): no difference of values near 1.
@@ -62,217 +64,220 @@ __device__ inline float tok_slope(float e, float scale) {
   return scale * (t / (u * u));
 }
 
-// One thread per unit of VU values of one token (D a multiple of VU).
-template <int DT, typename IdT, int VU>
-__global__ void __launch_bounds__(256)
-tok_encode_kernel(const IdT* __restrict__ ids, int64_t units, int upr, int V, int64_t pad,
-                  const typename TabType<DT>::t* __restrict__ tab, float scale, int ste, float* __restrict__ y) {
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < units; u += (int64_t)gridDim.x * 256) {
-    const int64_t n = u / upr;
-    const int c = (int)(u - n * upr);
-    const int r = tok_row(ids, n, V, pad);
+typedef float f32x4t __attribute__((ext_vector_type(4)));
+
+// VU values of a table's row, or of a gradient's.
+template <int DT, int VU>
+__device__ inline void tab_load(const typename TabType<DT>::t* __restrict__ p, float (&v)[VU]) {
+  using T = typename TabType<DT>::t;
+  typedef T Vt __attribute__((ext_vector_type(VU)));
+  const Vt r = *reinterpret_cast<const Vt*>(p);
 #pragma unroll
-    for (int j = 0; j < VU; ++j) {
-      const float e = r < V ? tab_get<DT>(tab[((int64_t)r * upr + c) * VU + j]) : 0.0f;
-      y[u * VU + j] = r < V ? tok_value(e, scale, ste != 0) : 0.0f;
+  for (int j = 0; j < VU; ++j) v[j] = tab_get<DT>(VU == 1 ? ((const T*)&r)[0] : r[j]);
+}
+template <int DT, int VU>
+__device__ inline void tab_store(typename TabType<DT>::t* __restrict__ p, const float (&v)[VU]) {
+  using T = typename TabType<DT>::t;
+  typedef T Vt __attribute__((ext_vector_type(VU)));
+  Vt r;
+#pragma unroll
+  for (int j = 0; j < VU; ++j) r[j] = tab_put<DT>(v[j]);
+  *reinterpret_cast<Vt*>(p) = r;
+}
+
+// A thread takes kEncUnits units of VU values of one token (D a multiple of
+// VU), a workgroup's units next to each other. upr: units per row. Idx: the
+// type that counts units.
+constexpr int kEncUnits = 4;
+template <int DT, typename IdT, int VU, typename Idx>
+__global__ void __launch_bounds__(256)
+tok_encode_kernel(const IdT* __restrict__ ids, Idx units, Idx upr, int V, int64_t pad,
+                  const typename TabType<DT>::t* __restrict__ tab, float nlog2, int ste, float* __restrict__ y) {
+  for (Idx u0 = (Idx)blockIdx.x * (256 * kEncUnits) + threadIdx.x; u0 < units;
+       u0 += (Idx)gridDim.x * (256 * kEncUnits)) {
+    int r[kEncUnits];
+    Idx c[kEncUnits];
+    float e[kEncUnits][VU];
+#pragma unroll
+    for (int k = 0; k < kEncUnits; ++k) {
+      const Idx u = min(u0 + k * 256, units - 1), n = u / upr;
+      c[k] = u - n * upr;
+      r[k] = tok_row(ids, (int64_t)n, V, pad);
+    }
+#pragma unroll
+    for (int k = 0; k < kEncUnits; ++k)  // an absent token reads row 0
+      tab_load<DT, VU>(tab + ((int64_t)(r[k] < V ? r[k] : 0) * upr + c[k]) * VU, e[k]);
+#pragma unroll
+    for (int k = 0; k < kEncUnits; ++k) {
+      if (u0 + k * 256 < units) {
+        float v[VU];
+#pragma unroll
+        for (int j = 0; j < VU; ++j) v[j] = r[k] < V ? tok_value(e[k][j], nlog2, ste != 0) : 0.0f;
+        tab_store<kTabF32, VU>(y + (int64_t)(u0 + k * 256) * VU, v);
+      }
     }
   }
 }
 
 // ---------------------------------------------------------------------------
-// Sorting tokens: entries (row, token) in ascending rows, tokens of one row in
-// ascending order (a stable least-significant-digit radix sort), so that every
-// sum has one order. Absent tokens (row V) come last.
+// Gradient of the table: tokens sorted by row (radix_sort.h; absent ones, of
+// row V, come last), then summed in that order.
 // ---------------------------------------------------------------------------
-constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int kSortBlocks = 128;      // workgroups at most: each reads every one's counts
-constexpr int kSortMinTile = 4096;    // entries a workgroup at least
-constexpr int kSortMaxBits = 9;       // digits of at most 512 values: 32 KB of counts in LDS
-
-struct SortArgs {
-  int64_t N;
-  int64_t tile;        // entries a workgroup (a multiple of 1024)
+template <typename IdT>
+struct TokenKeys {
+  const IdT* ids;
   int V;
   int64_t pad;
-  int shift, bits;
+  __device__ int key(int64_t i) const { return tok_row(ids, i, V, pad); }
 };
-
-template <typename IdT>
-__device__ inline int2 sort_entry(const IdT* ids, const int2* in, int64_t i, const SortArgs& a) {
-  return in ? in[i] : make_int2(tok_row(ids, i, a.V, a.pad), (int)i);
-}
-
-// Lanes of this wave with the same digit (among valid lanes).
-__device__ inline uint64_t same_digit(int d, int bits, bool valid) {
-  uint64_t m = __ballot(valid);
-  for (int b = 0; b < bits; ++b) {
-    const uint64_t on = __ballot((d >> b) & 1);
-    m &= (d >> b) & 1 ? on : ~on;
-  }
-  return m;
-}
-
-// Digit counts of each workgroup's entries: hist [workgroup][1 << bits].
-template <typename IdT>
-__global__ void __launch_bounds__(kSortThreads)
-tok_hist_kernel(SortArgs a, const IdT* __restrict__ ids, const int2* __restrict__ in, int* __restrict__ hist) {
-  __shared__ int cnt[1 << kSortMaxBits];
-  const int R = 1 << a.bits;
-  for (int d = threadIdx.x; d < R; d += kSortThreads) cnt[d] = 0;
-  __syncthreads();
-  const int64_t i0 = blockIdx.x * a.tile, i1 = min(a.N, i0 + a.tile);
-  for (int64_t i = i0 + threadIdx.x; i < i1; i += kSortThreads)
-    atomicAdd(&cnt[(sort_entry(ids, in, i, a).x >> a.shift) & (R - 1)], 1);
-  __syncthreads();
-  for (int d = threadIdx.x; d < R; d += kSortThreads) hist[(int64_t)blockIdx.x * R + d] = cnt[d];
-}
-
-// One pass: each workgroup's entries to their places. A wave takes a
-// contiguous part of the tile in order, 64 entries at a time.
-template <typename IdT>
-__global__ void __launch_bounds__(kSortThreads)
-tok_scatter_kernel(SortArgs a, const IdT* __restrict__ ids, const int2* __restrict__ in,
-                   const int* __restrict__ hist, int2* __restrict__ out) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  const int R = 1 << a.bits;
-  volatile int* cnt = reinterpret_cast<int*>(smem);  // [waves][R]
-  __shared__ int scan[kSortWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int d = tid; d < kSortWaves * R; d += kSortThreads) cnt[d] = 0;
-  __syncthreads();
-  const int64_t i0 = blockIdx.x * a.tile, i1 = min(a.N, i0 + a.tile);
-  const int64_t w0 = i0 + wave * (a.tile / kSortWaves), w1 = min(i1, w0 + a.tile / kSortWaves);
-  volatile int* mine = cnt + wave * R;
-  const uint64_t below = (1ull << lane) - 1;
-  for (int64_t i = w0; i < w1; i += 64) {  // this wave's counts
-    const bool valid = i + lane < w1;
-    const int d = valid ? (sort_entry(ids, in, i + lane, a).x >> a.shift) & (R - 1) : 0;
-    const uint64_t m = same_digit(d, a.bits, valid);
-    if (valid && (m & below) == 0) mine[d] += __popcll(m);
-  }
-  __syncthreads();
-  // digit d's first place: all smaller digits, then earlier workgroups'
-  // entries of d, then earlier waves'
-  int total = 0, before = 0;
-  if (tid < R) {
-    for (int g = 0; g < (int)gridDim.x; ++g) {
-      const int c = hist[(int64_t)g * R + tid];
-      total += c;
-      before += g < (int)blockIdx.x ? c : 0;
-    }
-  }
-  int x = total;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
-  if (lane == 63) scan[wave] = x;
-  __syncthreads();
-  int base = x - total + before;
-  for (int w = 0; w < wave; ++w) base += scan[w];
-  if (tid < R) {
-    for (int w = 0; w < kSortWaves; ++w) {
-      const int c = cnt[w * R + tid];
-      cnt[w * R + tid] = base;
-      base += c;
-    }
-  }
-  __syncthreads();
-  for (int64_t i = w0; i < w1; i += 64) {
-    const bool valid = i + lane < w1;
-    const int2 e = valid ? sort_entry(ids, in, i + lane, a) : make_int2(0, 0);
-    const int d = (e.x >> a.shift) & (R - 1);
-    const uint64_t m = same_digit(d, a.bits, valid);
-    int at = 0;
-    if (valid) {
-      at = mine[d] + __popcll(m & below);
-      out[at] = e;
-    }
-    __builtin_amdgcn_wave_barrier();
-    if (valid && (m & below) == 0) mine[d] = at + __popcll(m);
-    __builtin_amdgcn_wave_barrier();
-  }
-}
-
-// ---------------------------------------------------------------------------
-// Sums of the sorted tokens' gradients
-// ---------------------------------------------------------------------------
-constexpr int kSegChunk = 32;  // entries a group of lanes sums in order
 
 struct SegArgs {
   int64_t N, chunks;
-  int V, D;
+  int V, D, C, G;  // C entries a chunk, G lanes a row
   float scale;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(256) tok_zero_kernel(T* __restrict__ p, int64_t n) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = (T)0;
-}
-
-template <int DT>
-__device__ inline void seg_write(const SegArgs& a, int v, int d, float sum,
+template <int DT, int VU>
+__device__ inline void seg_write(const SegArgs& a, int v, int d, const float (&sum)[VU],
                                  const typename TabType<DT>::t* __restrict__ tab,
                                  typename TabType<DT>::t* __restrict__ gtab) {
   const int64_t at = (int64_t)v * a.D + d;
-  gtab[at] = tab_put<DT>(sum * tok_slope(tab_get<DT>(tab[at]), a.scale));
+  float e[VU], g[VU];
+  tab_load<DT, VU>(tab + at, e);
+#pragma unroll
+  for (int j = 0; j < VU; ++j) g[j] = sum[j] * tok_slope(e[j], a.scale);
+  tab_store<DT, VU>(gtab + at, g);
 }
 
-// A group of G lanes sums a chunk of kSegChunk entries over G columns. A run
-// of one row that lies inside the chunk is written; a run that the chunk
-// before it began goes to edge[0][chunk], one that begins here and goes on to
-// edge[1][chunk], for tok_join_kernel.
-template <int DT>
+// G lanes sum a chunk of C entries, VU columns each, kSegAhead rows of the
+// gradient in flight. A run of one row inside the chunk is written; one that
+// the chunk before it began goes to edge[0][chunk], one that begins here and
+// goes on to edge[1][chunk] and on the list of tok_join_kernel (whose order
+// does not matter: every run is summed by itself).
+constexpr int kSegAhead = 8;
+template <int DT, int VU>
 __global__ void __launch_bounds__(256)
-tok_segment_kernel(SegArgs a, int G, const int2* __restrict__ ent, const float* __restrict__ gy,
+tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict__ gy,
                    const typename TabType<DT>::t* __restrict__ tab,
-                   typename TabType<DT>::t* __restrict__ gtab, float* __restrict__ edge) {
-  const int per = 256 / G;
-  const int64_t c = (int64_t)blockIdx.x * per + threadIdx.x / G;
+                   typename TabType<DT>::t* __restrict__ gtab, float* __restrict__ edge,
+                   int* __restrict__ list, int* __restrict__ listed) {
+  const int per = 256 / a.G, l = threadIdx.x % a.G;
+  const int64_t c = (int64_t)blockIdx.x * per + threadIdx.x / a.G;
   if (c >= a.chunks) return;
-  const int64_t i0 = c * kSegChunk, i1 = min(a.N, i0 + kSegChunk);
-  for (int d = threadIdx.x % G; d < a.D; d += G) {
-    int row = ent[i0].x;
-    bool from_before = i0 > 0 && ent[i0 - 1].x == row;
-    float sum = 0.0f;
-    for (int64_t i = i0; i < i1; ++i) {
-      const int2 e = ent[i];
-      if (e.x != row) {
-        if (from_before) edge[c * a.D + d] = sum;
-        else if (row < a.V) seg_write<DT>(a, row, d, sum, tab, gtab);
-        row = e.x;
-        from_before = false;
-        sum = 0.0f;
+  const int64_t i0 = c * a.C, i1 = min(a.N, i0 + a.C);
+  const int first = ent[i0].x;
+  if (first >= a.V) return;  // absent tokens to the end
+  const bool begun = i0 > 0 && ent[i0 - 1].x == first;
+  const int after = i1 < a.N ? ent[i1].x : -1;
+  for (int d = l * VU; d < a.D; d += a.G * VU) {
+    int row = first;
+    bool from_before = begun;
+    float sum[VU];
+#pragma unroll
+    for (int j = 0; j < VU; ++j) sum[j] = 0.0f;
+    for (int64_t i = i0; i < i1 && row < a.V; i += kSegAhead) {
+      int2 e[kSegAhead];
+      float g[kSegAhead][VU];
+#pragma unroll
+      for (int u = 0; u < kSegAhead; ++u) e[u] = ent[min(i + u, i1 - 1)];
+#pragma unroll
+      for (int u = 0; u < kSegAhead; ++u) tab_load<kTabF32, VU>(gy + (int64_t)(uint32_t)e[u].y * a.D + d, g[u]);
+#pragma unroll
+      for (int u = 0; u < kSegAhead; ++u) {
+        if (i + u >= i1) break;
+        if (e[u].x != row) {
+          if (from_before) tab_store<kTabF32, VU>(edge + c * a.D + d, sum);
+          else if (row < a.V) seg_write<DT, VU>(a, row, d, sum, tab, gtab);
+          row = e[u].x;
+          from_before = false;
+#pragma unroll
+          for (int j = 0; j < VU; ++j) sum[j] = 0.0f;
+        }
+        if (row < a.V) {
+#pragma unroll
+          for (int j = 0; j < VU; ++j) sum[j] += g[u][j];
+        }
       }
-      if (row >= a.V) break;
-      sum += gy[(int64_t)(uint32_t)e.y * a.D + d];
     }
     if (row >= a.V) continue;
-    const bool goes_on = i1 < a.N && ent[i1].x == row;
-    if (from_before) edge[c * a.D + d] = sum;
-    else if (goes_on) edge[(a.chunks + c) * a.D + d] = sum;
-    else seg_write<DT>(a, row, d, sum, tab, gtab);
+    if (from_before) {
+      tab_store<kTabF32, VU>(edge + c * a.D + d, sum);
+    } else if (after == row) {
+      tab_store<kTabF32, VU>(edge + (a.chunks + c) * a.D + d, sum);
+      if (d == 0) list[atomicAdd(listed, 1)] = (int)c;
+    } else {
+      seg_write<DT, VU>(a, row, d, sum, tab, gtab);
+    }
   }
 }
 
-// The runs that cross chunks: the workgroup of the chunk where one begins
-// adds the chunks' parts in order.
-template <int DT>
-__global__ void __launch_bounds__(256)
+// The runs that cross chunks, a workgroup each: G lanes a row, the chunks'
+// parts dealt to kJoinThreads / G groups (each in ascending order), whose sums
+// are added in order.
+constexpr int kJoinThreads = 512;
+template <int DT, int VU>
+__global__ void __launch_bounds__(kJoinThreads)
 tok_join_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict__ edge,
                 const typename TabType<DT>::t* __restrict__ tab,
-                typename TabType<DT>::t* __restrict__ gtab) {
-  const int64_t c = blockIdx.x, i0 = c * kSegChunk, i1 = min(a.N, i0 + kSegChunk);
-  const int row = ent[i1 - 1].x;
-  if (row >= a.V || i1 >= a.N || ent[i1].x != row) return;      // nothing goes on
-  if (i0 > 0 && ent[i0].x == row && ent[i0 - 1].x == row) return;  // begun before this chunk
-  int64_t last = c + 1;  // the run's last chunk
-  while (last + 1 < a.chunks && ent[(last + 1) * kSegChunk].x == row) ++last;
-  for (int d = threadIdx.x; d < a.D; d += 256) {
-    float sum = edge[(a.chunks + c) * a.D + d];
-    for (int64_t k = c + 1; k <= last; ++k) sum += edge[k * a.D + d];
-    seg_write<DT>(a, row, d, sum, tab, gtab);
+                typename TabType<DT>::t* __restrict__ gtab, const int* __restrict__ list,
+                const int* __restrict__ listed) {
+  __shared__ float red[kJoinThreads * VU];
+  __shared__ int end[kJoinThreads / 64];
+  const int tid = threadIdx.x, wave = tid >> 6;
+  const int P = kJoinThreads / a.G, part = tid / a.G, l = tid % a.G;
+  const int n = *listed;
+  for (int k = blockIdx.x; k < n; k += gridDim.x) {
+    const int64_t c = list[k];
+    const int row = ent[min(a.N, (c + 1) * a.C) - 1].x;
+    // chunks past c that begin with the row: the first that does not ends it
+    int64_t last = c;
+    for (;;) {
+      const int64_t q = last + 1 + tid;
+      const uint64_t off = __ballot(!(q < a.chunks && ent[q * a.C].x == row));
+      if ((tid & 63) == 0) end[wave] = off ? __ffsll((unsigned long long)off) - 1 : 64;
+      __syncthreads();
+      int m = 0;
+      bool more = true;
+#pragma unroll
+      for (int w = 0; w < kJoinThreads / 64; ++w) {
+        m += more ? end[w] : 0;
+        more &= end[w] == 64;
+      }
+      __syncthreads();
+      last += m;
+      if (!more) break;
+    }
+    for (int d0 = 0; d0 < a.D; d0 += a.G * VU) {
+      const int d = d0 + l * VU;
+      float sum[VU];
+#pragma unroll
+      for (int j = 0; j < VU; ++j) sum[j] = 0.0f;
+      if (d < a.D) {
+        constexpr int U = 8;
+        for (int64_t q = c + 1 + part; q <= last; q += (int64_t)U * P) {
+          float g[U][VU];
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            tab_load<kTabF32, VU>(edge + min(q + (int64_t)u * P, last) * a.D + d, g[u]);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < VU; ++j) sum[j] += q + (int64_t)u * P <= last ? g[u][j] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < VU; ++j) red[(part * a.G + l) * VU + j] = sum[j];
+      __syncthreads();
+      if (part == 0 && d < a.D) {
+        float s[VU];
+        tab_load<kTabF32, VU>(edge + (a.chunks + c) * a.D + d, s);
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int j = 0; j < VU; ++j) s[j] += red[(p * a.G + l) * VU + j];
+        seg_write<DT, VU>(a, row, d, s, tab, gtab);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -293,44 +298,74 @@ tok_bits_kernel(const typename TabType<DT>::t* __restrict__ tab, int64_t words, 
   }
 }
 
-// Bits as uint8 [N, D].
-template <typename IdT>
+// Bits as uint8 [N, D], VU of a token a thread (D a multiple of VU).
+template <typename IdT, int VU>
 __global__ void __launch_bounds__(256)
-tok_bytes_kernel(const IdT* __restrict__ ids, int64_t N, int V, int64_t pad, int D, int DW,
+tok_bytes_kernel(const IdT* __restrict__ ids, int64_t units, int upr, int V, int64_t pad, int DW,
                  const uint64_t* __restrict__ bits, uint8_t* __restrict__ out) {
-  const int64_t n_all = N * D;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n_all; i += (int64_t)gridDim.x * 256) {
-    const int64_t n = i / D;
-    const int d = (int)(i - n * D), r = tok_row(ids, n, V, pad);
-    out[i] = r < V ? (uint8_t)((bits[(int64_t)r * DW + (d >> 6)] >> (d & 63)) & 1u) : 0;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < units; i += (int64_t)gridDim.x * 256) {
+    const int64_t n = i / upr;
+    const int d = (int)(i - n * upr) * VU, r = tok_row(ids, n, V, pad);
+    const uint32_t b = r < V ? (uint32_t)(bits[(int64_t)r * DW + (d >> 6)] >> (d & 63)) : 0u;
+    if constexpr (VU == 4)
+      reinterpret_cast<uint32_t*>(out)[i] = ((b & 15u) * 0x00204081u) & 0x01010101u;  // bit j to byte j
+    else
+      out[i] = (uint8_t)(b & 1u);
   }
 }
 
-// Bits packed 64 samples a word: a wave takes 64 samples' word dw of token l
-// and writes the transpose, word j = bit j of the 64 samples.
-template <typename IdT, bool WM>
-__global__ void __launch_bounds__(256)
+// The wave's 64 x 64 bits transposed: lane j's word becomes bit j of every
+// lane's word (six exchanges of halves; a ballot per bit took 5 times the
+// instructions).
+__device__ inline uint64_t wave_transpose(uint64_t m) {
+  const int lane = threadIdx.x & 63;
+  uint32_t lo = (uint32_t)m, hi = (uint32_t)(m >> 32);
+  const uint32_t got = (uint32_t)__shfl_xor((int)(lane & 32 ? lo : hi), 32, 64);
+  if (lane & 32) lo = got; else hi = got;
+  auto halves = [&](int s, uint32_t keep) {
+    const uint32_t ylo = (uint32_t)__shfl_xor((int)lo, s, 64), yhi = (uint32_t)__shfl_xor((int)hi, s, 64);
+    if (lane & s) {
+      lo = (lo & ~keep) | ((ylo >> s) & keep);
+      hi = (hi & ~keep) | ((yhi >> s) & keep);
+    } else {
+      lo = (lo & keep) | ((ylo & keep) << s);
+      hi = (hi & keep) | ((yhi & keep) << s);
+    }
+  };
+  halves(16, 0x0000ffffu);
+  halves(8, 0x00ff00ffu);
+  halves(4, 0x0f0f0f0fu);
+  halves(2, 0x33333333u);
+  halves(1, 0x55555555u);
+  return (uint64_t)hi << 32 | lo;
+}
+
+// Bits packed 64 samples a word. A wave takes 64 samples' word dw of token l
+// and transposes it: lane j then holds feature j's word. Word-major rows of
+// features are written as they are; for the rows [F][nw] a workgroup's waves
+// take TW neighbouring words, which leave through LDS in runs of TW.
+template <typename IdT, bool WM, int TW>
+__global__ void __launch_bounds__(64 * TW)
 tok_packed_kernel(const IdT* __restrict__ ids, int64_t B, int64_t L, int V, int64_t pad, int D, int DW,
                   int64_t nw, const uint64_t* __restrict__ bits, uint64_t* __restrict__ out) {
-  const int lane = threadIdx.x & 63;
-  const int64_t F = L * D, jobs = nw * L * DW;
-  for (int64_t k = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); k < jobs; k += (int64_t)gridDim.x * 4) {
-    const int64_t w = k / (L * DW);
-    const int64_t r = k - w * (L * DW);
-    const int64_t l = r / DW;
+  __shared__ uint64_t tile[WM ? 1 : 64][WM ? 1 : TW + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t F = L * D, wt = (nw + TW - 1) / TW, jobs = wt * L * DW;
+  for (int64_t k = blockIdx.x; k < jobs; k += gridDim.x) {
+    const int64_t t = k / (L * DW), r = k - t * (L * DW), l = r / DW;
     const int dw = (int)(r - l * DW);
-    const int64_t b = w * 64 + lane;
+    const int64_t w = t * TW + wave, b = w * 64 + lane;
     const int row = b < B ? tok_row(ids, b * L + l, V, pad) : V;
-    const uint64_t m = row < V ? bits[(int64_t)row * DW + dw] : 0ull;
-    uint64_t mine = 0;
-    for (int j = 0; j < 64; ++j) {
-      const uint64_t t = __ballot((m >> j) & 1);
-      if (lane == j) mine = t;
-    }
+    const uint64_t m = wave_transpose(row < V ? bits[(int64_t)row * DW + dw] : 0ull);
     const int d = dw * 64 + lane;
-    if (d < D) {
-      const int64_t f = l * D + d;
-      out[WM ? w * F + f : f * nw + w] = mine;
+    if constexpr (WM) {
+      if (w < nw && d < D) out[w * F + l * D + d] = m;
+    } else {
+      tile[lane][wave] = m;
+      __syncthreads();
+      const int j = threadIdx.x / TW, i = threadIdx.x % TW;
+      if (t * TW + i < nw && dw * 64 + j < D) out[(l * D + dw * 64 + j) * nw + t * TW + i] = tile[j][i];
+      __syncthreads();
     }
   }
 }
@@ -354,26 +389,33 @@ static void tok_dispatch(int dtype, int id_bytes, F&& f) {
   else ids(std::integral_constant<int, kTabF16>{});
 }
 
+// f(values a lane takes) by the width and the alignment of every row.
+template <typename F>
+static void tok_vector(int64_t D, bool aligned, F&& f) {
+  if (D % 4 == 0 && aligned) f(std::integral_constant<int, 4>{});
+  else f(std::integral_constant<int, 1>{});
+}
+
 struct TokBwdPlan {
-  int64_t blocks, tile, chunks;
-  int passes, bits;
-  int64_t ent, hist, edge;  // 4-byte words of one entry array, the counts, the edges
-  int64_t total() const { return 2 * ent + hist + edge; }
+  RadixPlan sort;
+  int64_t chunks, edge, list;
+  int C, G, VU;
+  int64_t total() const { return sort.words() + edge + list; }
 };
 
+// Lanes a row: a power of two up to the wave. Chunks: 64 entries, fewer where
+// that leaves less than about 8 waves a CU.
 static TokBwdPlan tok_bwd_plan(int64_t N, int64_t V, int64_t D) {
   TokBwdPlan p{};
-  auto round4 = [](int64_t n) { return (n + 3) & ~int64_t(3); };
-  p.tile = std::max<int64_t>(kSortMinTile, cdiv(cdiv(N, kSortBlocks), 1024) * 1024);
-  p.blocks = std::max<int64_t>(1, cdiv(N, p.tile));
-  int key = 1;  // bits of the largest key, V
-  while (key < 31 && (V >> key) != 0) ++key;
-  p.passes = (key + kSortMaxBits - 1) / kSortMaxBits;
-  p.bits = (key + p.passes - 1) / p.passes;
-  p.chunks = cdiv(N, kSegChunk);
-  p.ent = round4(2 * N);
-  p.hist = round4(p.blocks << p.bits);
-  p.edge = round4(2 * p.chunks * D);
+  p.sort = radix_plan(N, V + 1);
+  p.VU = D % 4 == 0 ? 4 : 1;
+  p.G = 1;
+  while (p.G < 64 && p.G * p.VU < D) p.G *= 2;
+  p.C = 64;
+  while (p.C > 16 && cdiv(N, p.C) * p.G < 131072) p.C /= 2;
+  p.chunks = cdiv(N, p.C);
+  p.edge = (2 * p.chunks * D + 3) & ~int64_t(3);
+  p.list = p.chunks + 1;
   return p;
 }
 
@@ -396,12 +438,24 @@ int slg_token_encode(const void* ids, int32_t id_bytes, int64_t N, int64_t V, in
   TOK_CHECK("token_encode");
   if (N == 0) return 0;
   hipStream_t st = as_stream(stream);
+  const float nlog2 = (float)(-1.4426950408889634 * (double)scale);
   tok_dispatch(dtype, id_bytes, [&](auto dt, auto it) {
+    constexpr int DT = decltype(dt)::value;
     using Id = decltype(it);
-    using T = typename TabType<decltype(dt)::value>::t;
-    hipLaunchKernelGGL((tok_encode_kernel<decltype(dt)::value, Id, 1>), dim3(grid_of(cdiv(N * D, 256))),
-                       dim3(256), 0, st, static_cast<const Id*>(ids), N * D, (int)D, (int)V, pad,
-                       static_cast<const T*>(table), scale, ste, y);
+    using T = typename TabType<DT>::t;
+    tok_vector(D, (uintptr_t)table % (4 * sizeof(T)) == 0 && (uintptr_t)y % 16 == 0, [&](auto vu) {
+      constexpr int VU = decltype(vu)::value;
+      const int64_t units = N * D / VU;
+      auto go = [&](auto kern, auto idx) {
+        using Idx = decltype(idx);
+        hipLaunchKernelGGL(kern, dim3(grid_of(cdiv(units, 256 * kEncUnits))), dim3(256), 0, st,
+                           static_cast<const Id*>(ids), (Idx)units, (Idx)(D / VU), (int)V, pad,
+                           static_cast<const T*>(table), nlog2, ste, y);
+      };
+      // a round of the grid past the last unit still counts within 32 bits
+      if (units < (1LL << 31)) go(tok_encode_kernel<DT, Id, VU, uint32_t>, uint32_t(0));
+      else go(tok_encode_kernel<DT, Id, VU, int64_t>, int64_t(0));
+    });
   });
   SLG_LAUNCH_CHECK("token_encode");
   return 0;
@@ -422,36 +476,32 @@ int slg_token_encode_bwd(const void* ids, int32_t id_bytes, int64_t N, int64_t V
               "token_encode_bwd: workspace of %lld words, %lld at a multiple of 16 bytes needed",
               (long long)workspace_words, (long long)p.total());
   hipStream_t st = as_stream(stream);
-  int2* ent[2] = {reinterpret_cast<int2*>(workspace), reinterpret_cast<int2*>(workspace + p.ent)};
-  int* hist = workspace + 2 * p.ent;
-  float* edge = reinterpret_cast<float*>(hist + p.hist);
-  const size_t lds = sizeof(int) * kSortWaves << p.bits;
-  int rc = 0;
+  SLG_REQUIRE((uintptr_t)gtable % 16 == 0, SLG_E_ARG, "token_encode_bwd: gtable not at a multiple of 16 bytes");
+  float* edge = reinterpret_cast<float*>(workspace + p.sort.words());
+  int* listed = workspace + p.sort.words() + p.edge;
   tok_dispatch(dtype, id_bytes, [&](auto dt, auto it) {
     using Id = decltype(it);
     constexpr int DT = decltype(dt)::value;
     using T = typename TabType<DT>::t;
-    hipLaunchKernelGGL((tok_zero_kernel<T>), dim3(grid_of(cdiv(V * D, 256))), dim3(256), 0, st,
-                       static_cast<T*>(gtable), V * D);
-    if (N == 0) return;
-    SortArgs a{N, p.tile, (int)V, pad, 0, p.bits};
-    const int2* in = nullptr;
-    for (int k = 0; k < p.passes; ++k, a.shift += p.bits) {
-      hipLaunchKernelGGL((tok_hist_kernel<Id>), dim3((unsigned)p.blocks), dim3(kSortThreads), 0, st, a,
-                         static_cast<const Id*>(ids), in, hist);
-      hipLaunchKernelGGL((tok_scatter_kernel<Id>), dim3((unsigned)p.blocks), dim3(kSortThreads), lds, st, a,
-                         static_cast<const Id*>(ids), in, hist, ent[k & 1]);
-      in = ent[k & 1];
+    const RadixClear clear{gtable, V * D * (int64_t)sizeof(T), N > 0 ? listed : nullptr};
+    if (N == 0) {
+      hipLaunchKernelGGL(radix_clear_kernel, dim3(grid_of(cdiv(clear.bytes, 16 * kRadixThreads))),
+                         dim3(kRadixThreads), 0, st, clear);
+      return;
     }
-    const SegArgs s{N, p.chunks, (int)V, (int)D, scale};
-    int G = 16;
-    while (G < 64 && G < D) G *= 2;
-    hipLaunchKernelGGL((tok_segment_kernel<DT>), dim3((unsigned)cdiv(p.chunks, 256 / G)), dim3(256), 0, st, s, G,
-                       in, gy, static_cast<const T*>(table), static_cast<T*>(gtable), edge);
-    hipLaunchKernelGGL((tok_join_kernel<DT>), dim3((unsigned)p.chunks), dim3(256), 0, st, s, in, edge,
-                       static_cast<const T*>(table), static_cast<T*>(gtable));
+    const int2* ent = radix_sort(TokenKeys<Id>{static_cast<const Id*>(ids), (int)V, pad}, p.sort, workspace, clear, st);
+    const bool aligned = (uintptr_t)table % (4 * sizeof(T)) == 0 && (uintptr_t)gy % 16 == 0;
+    tok_vector(D, aligned, [&](auto vu) {
+      constexpr int VU = decltype(vu)::value;
+      const SegArgs s{N, p.chunks, (int)V, (int)D, p.C, p.G, scale};
+      hipLaunchKernelGGL((tok_segment_kernel<DT, VU>), dim3((unsigned)cdiv(p.chunks, 256 / p.G)), dim3(256), 0, st,
+                         s, ent, gy, static_cast<const T*>(table), static_cast<T*>(gtable), edge, listed + 1,
+                         listed);
+      hipLaunchKernelGGL((tok_join_kernel<DT, VU>), dim3((unsigned)std::min<int64_t>(p.chunks, 512)),
+                         dim3(kJoinThreads), 0, st, s, ent, edge, static_cast<const T*>(table),
+                         static_cast<T*>(gtable), listed + 1, listed);
+    });
   });
-  if (rc) return rc;
   SLG_LAUNCH_CHECK("token_encode_bwd");
   return 0;
 }
@@ -486,17 +536,21 @@ int slg_token_encode_hard(const void* ids, int32_t id_bytes, int64_t B, int64_t 
     using Id = decltype(it);
     const Id* id = static_cast<const Id*>(ids);
     if (layout == 2) {
-      hipLaunchKernelGGL((tok_bytes_kernel<Id>), dim3(grid_of(cdiv(N * D, 256))), dim3(256), 0, st, id, N, (int)V,
-                         pad, (int)D, (int)DW, bits, static_cast<uint8_t*>(out));
+      tok_vector(D, (uintptr_t)out % 4 == 0, [&](auto vu) {
+        constexpr int VU = decltype(vu)::value;
+        hipLaunchKernelGGL((tok_bytes_kernel<Id, VU>), dim3(grid_of(cdiv(N * D / VU, 256))), dim3(256), 0, st, id,
+                           N * D / VU, (int)(D / VU), (int)V, pad, (int)DW, bits, static_cast<uint8_t*>(out));
+      });
       return;
     }
-    const dim3 grid(grid_of(cdiv(nw * L * DW, 4)));
-    if (layout == 1)
-      hipLaunchKernelGGL((tok_packed_kernel<Id, true>), grid, dim3(256), 0, st, id, B, L, (int)V, pad, (int)D,
-                         (int)DW, nw, bits, static_cast<uint64_t*>(out));
-    else
-      hipLaunchKernelGGL((tok_packed_kernel<Id, false>), grid, dim3(256), 0, st, id, B, L, (int)V, pad, (int)D,
-                         (int)DW, nw, bits, static_cast<uint64_t*>(out));
+    auto go = [&](auto kern, int tw) {
+      hipLaunchKernelGGL(kern, dim3(grid_of(cdiv(nw, tw) * L * DW)), dim3(64 * tw), 0, st, id, B, L, (int)V, pad,
+                         (int)D, (int)DW, nw, bits, static_cast<uint64_t*>(out));
+    };
+    if (layout == 1) go(tok_packed_kernel<Id, true, 4>, 4);
+    else if (nw == 1) go(tok_packed_kernel<Id, false, 1>, 1);
+    else if (nw <= 4) go(tok_packed_kernel<Id, false, 4>, 4);
+    else go(tok_packed_kernel<Id, false, 8>, 8);
   });
   SLG_LAUNCH_CHECK("token_encode_hard");
   return 0;

@@ -57,8 +57,10 @@ def _check(B, L, V, D, how="zipf", dtype=torch.float32, ste=False, pad=None, sca
     (gt,) = torch.autograd.grad(y, [enc.weight], gy.to(DEV))
     yw, bits, gw, spread, size = _oracle(ids, table, scale, ste, enc.padding_idx, gy)
     z = (scale * table.to(F64).abs()).max()
-    # exp of a rounded argument (z 2^-24), its own two units, the sum and the quotient
-    orc.close(y, yw, (z + 8) * orc.EPS * yw.abs(), "values")
+    # 1 / (1 + 2^t), t = e * (scale log2 e): the factor and the product each rounded once shift t ln 2 = z by
+    # at most 2 z 2^-24, which y follows by no more than that relative to it; the exponential and the
+    # reciprocal are off by an ulp (2 units) each, the sum by one
+    orc.close(y, yw, (2 * z + 8) * orc.EPS * yw.abs(), "values")
     assert gt.dtype == dtype and gt.shape == table.shape
     # n - 1 sums of n terms: off by at most n 2^-24 of the terms' sizes; the slope as above; the type's rounding
     # (with fp16, values under its normal range go by its smallest step, 2^-25 at most)
@@ -108,7 +110,7 @@ def test_large_values_and_scales():
     yw, _, gw, spread, size = _oracle(ids, table, 1.0, False, None, gy)
     z = table.to(F64).abs().clamp_max(104)   # past it exp is 0 in fp32
     zy = z[ids].reshape(3, 8)
-    orc.close(y, yw, (zy + 8) * orc.EPS * yw + 2.0 ** -126, "values")
+    orc.close(y, yw, (2 * zy + 8) * orc.EPS * yw + 2.0 ** -126, "values")
     orc.close(gt, gw, orc.EPS * spread + (2 * z + 16) * orc.EPS * size + 2.0 ** -126, "gradient")
 
 
