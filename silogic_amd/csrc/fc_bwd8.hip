@@ -27,15 +27,17 @@ constexpr int bwd8_threads() { return KC > 0 ? 1024 : 512; }
 __device__ inline float code_of(uint32_t w, int v) { return (float)((w >> (8 * v)) & 255u); }
 
 // One output per thread over a range of 4-sample tiles: part and gbr as
-// fc_soft_bwd_w_kernel writes them.
-template <int NODE, int KC>
+// fc_soft_bwd_w_kernel writes them. AHEAD: two tiles in LDS, the next one's
+// codes on their way in registers (up to kBwd8Quads quads a thread) while this
+// one computes, one barrier a tile; else one tile and two barriers.
+constexpr int kBwd8Quads = 3;
+template <int NODE, int KC, bool AHEAD>
 __global__ void __launch_bounds__((bwd8_threads<KC>()))
 fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ rows, int B, int IN, int ld,
                  int OUT, int Kr, ParamView pv, float inv_tau, const float* __restrict__ gy, int n_orange,
                  int n_range, int tiles_per_range, float* __restrict__ part, float* __restrict__ gbr) {
   constexpr int S = kRows8Tile, KM = KC > 0 ? KC : 16;
   extern __shared__ __align__(16) unsigned char smem[];
-  uint32_t* xs = reinterpret_cast<uint32_t*>(smem);
   const int K = KC > 0 ? KC : Kr;
   // the output ranges of one sample range on one XCD: they stage the same codes
   const uint32_t lid = xcd_logical_id(blockIdx.x, gridDim.x);
@@ -59,22 +61,60 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
   for (int k = 0; k < KM; ++k) swa[k] = swb[k] = 0.0f;
   const int n_tiles = (B + S - 1) / S;
   const int t0 = r_b * tiles_per_range, t_end = min(n_tiles, t0 + tiles_per_range);
-  const int vo = valid ? o * 4 : 0x7ffffffc;
+  const int vo = valid ? o * 4 : 0x7ffffffc, n4 = ld >> 2, T = blockDim.x;
+  uint4 pf[AHEAD ? kBwd8Quads : 1];
+  auto issue = [&](int t) {
+    const auto r = uniform_rsrc(codes + (int64_t)t * ld, ld * 4);
+#pragma unroll
+    for (int u = 0; u < kBwd8Quads; ++u)  // zeros past the row
+      pf[u] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, (threadIdx.x + u * T) * 16, 0, 0));
+  };
+  auto place = [&](int t) {
+    uint4* dst = reinterpret_cast<uint4*>(smem) + (t & 1) * n4;
+#pragma unroll
+    for (int u = 0; u < kBwd8Quads; ++u) {
+      const int q = threadIdx.x + u * T;
+      if (q < n4) dst[q] = pf[u];
+    }
+  };
+  auto load_g = [&](int t, float (&g)[S]) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int b = t * S + s;
+      const auto gr = uniform_rsrc(gy + (int64_t)min(b, B - 1) * OUT, b < B ? OUT * 4 : 0);
+      g[s] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(gr, vo, 0, 0));
+    }
+  };
+  float gn[S];
+  if (t0 < t_end) {
+    load_g(t0, gn);
+    if constexpr (AHEAD) {
+      issue(t0);
+      place(t0);
+      __syncthreads();
+    }
+  }
   for (int t = t0; t < t_end; ++t) {
     const int b0 = t * S;
-    __syncthreads();  // the previous tile's reads are done
-    const uint4* src = reinterpret_cast<const uint4*>(codes + (int64_t)t * ld);
-    for (int q = threadIdx.x; q < (ld >> 2); q += blockDim.x) reinterpret_cast<uint4*>(xs)[q] = src[q];
     float g[S], lo[S], step[S];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const int b = min(b0 + s, B - 1);
-      const auto gr = uniform_rsrc(gy + (int64_t)b * OUT, b0 + s < B ? OUT * 4 : 0);
-      g[s] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(gr, vo, 0, 0));
-      lo[s] = b0 + s < B ? rows[2 * (int64_t)b] : 0.0f;
-      step[s] = b0 + s < B ? rows[2 * (int64_t)b + 1] : 0.0f;
+      const int64_t b = min(b0 + s, B - 1);
+      g[s] = gn[s];
+      lo[s] = b0 + s < B ? rows[2 * b] : 0.0f;
+      step[s] = b0 + s < B ? rows[2 * b + 1] : 0.0f;
     }
-    __syncthreads();
+    const uint32_t* xs = reinterpret_cast<const uint32_t*>(smem) + (AHEAD ? (t & 1) * ld : 0);
+    if constexpr (!AHEAD) {
+      __syncthreads();  // the previous tile's reads are done
+      const uint4* src = reinterpret_cast<const uint4*>(codes + (int64_t)t * ld);
+      for (int q = threadIdx.x; q < n4; q += T) reinterpret_cast<uint4*>(smem)[q] = src[q];
+      __syncthreads();
+    }
+    if (t + 1 < t_end) {
+      if constexpr (AHEAD) issue(t + 1);
+      load_g(t + 1, gn);
+    }
     uint32_t qa[KM], qb[KM];
 #pragma unroll
     for (int k = 0; k < KM; ++k) {
@@ -94,6 +134,9 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
         }
       }
     }
+    // converted again for the weight gradients: 64 floats kept would spill
+#pragma unroll
+    for (int k = 0; k < KM; ++k) asm volatile("" : "+v"(qa[k]), "+v"(qb[k]));
     float ga[S], gb[S];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
@@ -127,6 +170,10 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
           swb[k] = fmaf(gb[s], code_of(qb[k], s), swb[k]);
         }
       }
+    }
+    if constexpr (AHEAD) {  // the other tile's reads ended at the last barrier
+      if (t + 1 < t_end) place(t + 1);
+      __syncthreads();
     }
   }
   if (part != nullptr && valid) {
@@ -189,8 +236,10 @@ struct Bwd8Args {
 
 template <int NODE, int KC>
 static int launch_bwd8(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
-  auto kern = fc_bwd8_w_kernel<NODE, KC>;
-  const size_t lds = (size_t)rows8_ld(a.IN) * 4;
+  const int64_t ld = rows8_ld(a.IN);
+  const bool ahead = p.tiles_per_range > 1 && ld <= kBwd8Quads * 4 * bwd8_threads<KC>();
+  auto kern = ahead ? fc_bwd8_w_kernel<NODE, KC, true> : fc_bwd8_w_kernel<NODE, KC, false>;
+  const size_t lds = (size_t)ld * 4 * (ahead ? 2 : 1);
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)lds);
@@ -199,7 +248,7 @@ static int launch_bwd8(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
   ParamView pv{};
   pv.rec = a.rec;
   hipLaunchKernelGGL(kern, dim3((unsigned)(cdiv((int64_t)p.n_orange * p.NR, 8) * 8)), dim3(bwd8_threads<KC>()),
-                     lds, st, a.codes, a.rows, (int)a.B, (int)a.IN, (int)rows8_ld(a.IN), (int)a.OUT, a.K, pv,
+                     lds, st, a.codes, a.rows, (int)a.B, (int)a.IN, (int)ld, (int)a.OUT, a.K, pv,
                      a.inv_tau, a.gy, p.n_orange, p.NR, p.tiles_per_range, a.part, a.gbr);
   SLG_LAUNCH_CHECK("fc_soft_bwd8");
   return 0;

@@ -122,6 +122,12 @@ def test_layer(kind, B, IN, OUT, K):
     _check_layer(KINDS[kind], B, IN, OUT, K, 0.5 if kind == "walsh" else 1.0)
 
 
+@pytest.mark.parametrize("B,IN,OUT,K", [(1, 2, 169, 11), (5, 1, 900, 16), (3, 3, 5000, 8)])
+def test_few_inputs_under_many_outputs(B, IN, OUT, K):
+    """Lists of hundreds to tens of thousands of references to one input."""
+    _check_layer(orc.MULTILINEAR, B, IN, OUT, K, 1.0)
+
+
 @pytest.mark.parametrize("IN", [16400, 40960, 40964, 66000])
 def test_wide_rows(IN):
     """Rows up to the LDS's 40960 words on the codes, wider ones unpacked."""
