@@ -47,10 +47,22 @@ __device__ inline uint32_t rows8_code(float x, float lo, float inv) {
   return inv > 0.0f ? (uint32_t)fminf(rintf((x - lo) * inv), 255.0f) : 0u;
 }
 
+// VU neighbouring values or words as one access.
+template <int VU>
+__device__ inline void rows8_load(const float* __restrict__ p, float (&v)[VU]) {
+  if constexpr (VU == 4) {
+    const float4 r = *reinterpret_cast<const float4*>(p);
+    v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
+  } else {
+    v[0] = *p;
+  }
+}
+
 // One workgroup per tile of 4 samples. NU > 0: the tile's values stay in
-// registers between the range and the codes (NU inputs of each row a thread,
-// D <= NU * blockDim); NU = 0: they are read again.
-template <int NU, int T>
+// registers between the range and the codes (NU runs of VU inputs of each row
+// a thread, D <= NU * VU * T); NU = 0: they are read again. VU = 4: D a
+// multiple of 4 and x at one of 16 bytes.
+template <int NU, int VU, int T>
 __global__ void __launch_bounds__(T)
 rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_t* __restrict__ codes,
                   float* __restrict__ rows) {
@@ -65,22 +77,28 @@ rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_
     Rows8Range r[kRows8Tile];
 #pragma unroll
     for (int v = 0; v < kRows8Tile; ++v) r[v] = {INFINITY, -INFINITY, false};
-    float keep[NU > 0 ? NU : 1][kRows8Tile];
+    float keep[NU > 0 ? NU : 1][kRows8Tile][VU];
     if constexpr (NU > 0) {
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        const int i = min(tid + u * T, D - 1);  // past the row: its last value
+        const int i = min((tid + u * T) * VU, D - VU);  // past the row: its last values
 #pragma unroll
-        for (int v = 0; v < kRows8Tile; ++v) keep[u][v] = p[v][i];
+        for (int v = 0; v < kRows8Tile; ++v) rows8_load<VU>(p[v] + i, keep[u][v]);
       }
 #pragma unroll
       for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int v = 0; v < kRows8Tile; ++v) rows8_take(r[v], keep[u][v]);
-    } else {
-      for (int i = tid; i < D; i += T)
+        for (int v = 0; v < kRows8Tile; ++v)
 #pragma unroll
-        for (int v = 0; v < kRows8Tile; ++v) rows8_take(r[v], p[v][i]);
+          for (int j = 0; j < VU; ++j) rows8_take(r[v], keep[u][v][j]);
+    } else {
+      for (int i = tid * VU; i < D; i += T * VU)
+#pragma unroll
+        for (int v = 0; v < kRows8Tile; ++v) {
+          rows8_load<VU>(p[v] + i, keep[0][v]);
+#pragma unroll
+          for (int j = 0; j < VU; ++j) rows8_take(r[v], keep[0][v][j]);
+        }
     }
 #pragma unroll
     for (int v = 0; v < kRows8Tile; ++v) {
@@ -112,24 +130,28 @@ rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_
       if (v >= nb) inv[v] = 0.0f;  // codes 0 past the batch
     }
     uint32_t* c = codes + t * ld;
-    auto word = [&](const float (&e)[kRows8Tile]) {
-      uint32_t w = 0;
+    auto put = [&](int i, const float (&e)[kRows8Tile][VU]) {
+      uint32_t w[VU];
 #pragma unroll
-      for (int v = 0; v < kRows8Tile; ++v) w |= rows8_code(e[v], lo[v], inv[v]) << (8 * v);
-      return w;
+      for (int j = 0; j < VU; ++j) {
+        w[j] = 0;
+#pragma unroll
+        for (int v = 0; v < kRows8Tile; ++v) w[j] |= rows8_code(e[v][j], lo[v], inv[v]) << (8 * v);
+      }
+      if constexpr (VU == 4) *reinterpret_cast<uint4*>(c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+      else c[i] = w[0];
     };
     if constexpr (NU > 0) {
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        const int i = tid + u * T;
-        if (i < D) c[i] = word(keep[u]);
+        const int i = (tid + u * T) * VU;
+        if (i < D) put(i, keep[u]);
       }
     } else {
-      for (int i = tid; i < D; i += T) {
-        float e[kRows8Tile];
+      for (int i = tid * VU; i < D; i += T * VU) {
 #pragma unroll
-        for (int v = 0; v < kRows8Tile; ++v) e[v] = p[v][i];
-        c[i] = word(e);
+        for (int v = 0; v < kRows8Tile; ++v) rows8_load<VU>(p[v] + i, keep[0][v]);
+        put(i, keep[0]);
       }
     }
     if (tid < ld - D) c[D + tid] = 0u;
@@ -137,28 +159,58 @@ rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_
   }
 }
 
-// Values that the codes stand for: one thread per word, four rows written.
+// Values that the codes stand for: a thread takes VU neighbouring words and
+// writes four rows of them (VU = 4: as above).
+template <int VU>
 __global__ void __launch_bounds__(256)
 rows8_unpack_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ rows, int64_t B, int D,
                     int ld, int per_tile, int64_t blocks, float* __restrict__ x) {
   for (int64_t k = blockIdx.x; k < blocks; k += gridDim.x) {
     const int64_t t = k / per_tile;
-    const int i = (int)(k - t * per_tile) * 256 + threadIdx.x;
+    const int i = ((int)(k - t * per_tile) * 256 + threadIdx.x) * VU;
     if (i >= D) continue;
-    const uint32_t w = codes[t * ld + i];
+    uint32_t w[VU];
+    if constexpr (VU == 4) {
+      const uint4 r = *reinterpret_cast<const uint4*>(codes + t * ld + i);
+      w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
+    } else {
+      w[0] = codes[t * ld + i];
+    }
 #pragma unroll
     for (int v = 0; v < kRows8Tile; ++v) {
       const int64_t b = t * kRows8Tile + v;
-      if (b < B) x[b * D + i] = fmaf((float)((w >> (8 * v)) & 255u), rows[2 * b + 1], rows[2 * b]);
+      if (b >= B) break;
+      const float lo = rows[2 * b], step = rows[2 * b + 1];
+      float e[VU];
+#pragma unroll
+      for (int j = 0; j < VU; ++j) e[j] = fmaf((float)((w[j] >> (8 * v)) & 255u), step, lo);
+      if constexpr (VU == 4) *reinterpret_cast<float4*>(x + b * D + i) = make_float4(e[0], e[1], e[2], e[3]);
+      else x[b * D + i] = e[0];
     }
   }
 }
 
-template <int NU, int T>
+template <int NU, int VU, int T>
 static void launch_pack(const float* x, int64_t B, int64_t D, uint32_t* codes, float* rows, hipStream_t st) {
-  hipLaunchKernelGGL((rows8_pack_kernel<NU, T>), dim3((unsigned)std::min<int64_t>(cdiv(B, kRows8Tile), kRows8Grid)), dim3(T), 0, st, x, B,
+  hipLaunchKernelGGL((rows8_pack_kernel<NU, VU, T>),
+                     dim3((unsigned)std::min<int64_t>(cdiv(B, kRows8Tile), kRows8Grid)), dim3(T), 0, st, x, B,
                      (int)D, (int)rows8_ld(D), codes, rows);
 }
+
+// Workgroups that hold a tile in registers: 16 values of each row a thread at
+// most.
+template <int VU>
+static void launch_pack_v(const float* x, int64_t B, int64_t D, uint32_t* codes, float* rows, hipStream_t st) {
+  constexpr int Q = 4 / VU;  // runs that make 4 values
+  if (D <= 256 * VU) launch_pack<1, VU, 256>(x, B, D, codes, rows, st);
+  else if (D <= 4096 && Q * VU * 256 >= D) launch_pack<Q, VU, 256>(x, B, D, codes, rows, st);
+  else if (D <= 4096) launch_pack<Q, VU, 1024>(x, B, D, codes, rows, st);
+  else if (D <= 8192) launch_pack<2 * Q, VU, 1024>(x, B, D, codes, rows, st);
+  else if (D <= 16384) launch_pack<4 * Q, VU, 1024>(x, B, D, codes, rows, st);
+  else launch_pack<0, VU, 1024>(x, B, D, codes, rows, st);
+}
+
+static bool rows8_vector(const float* x, int64_t D) { return D % 4 == 0 && (uintptr_t)x % 16 == 0; }
 
 }  // namespace slg
 
@@ -176,12 +228,8 @@ int slg_rows8_pack(const float* x, int64_t B, int64_t D, uint8_t* codes, float* 
   if (B == 0) return 0;
   hipStream_t st = as_stream(stream);
   uint32_t* c = reinterpret_cast<uint32_t*>(codes);
-  if (D <= 256) launch_pack<1, 256>(x, B, D, c, rows, st);
-  else if (D <= 1024) launch_pack<4, 256>(x, B, D, c, rows, st);
-  else if (D <= 4096) launch_pack<4, 1024>(x, B, D, c, rows, st);
-  else if (D <= 8192) launch_pack<8, 1024>(x, B, D, c, rows, st);
-  else if (D <= 16384) launch_pack<16, 1024>(x, B, D, c, rows, st);
-  else launch_pack<0, 1024>(x, B, D, c, rows, st);
+  if (rows8_vector(x, D)) launch_pack_v<4>(x, B, D, c, rows, st);
+  else launch_pack_v<1>(x, B, D, c, rows, st);
   SLG_LAUNCH_CHECK("rows8_pack");
   return 0;
 }
@@ -193,9 +241,12 @@ int slg_rows8_unpack(const uint8_t* codes, const float* rows, int64_t B, int64_t
               "rows8_unpack: B %lld, D %lld", (long long)B, (long long)D);
   SLG_REQUIRE((uintptr_t)codes % 16 == 0, SLG_E_ARG, "rows8_unpack: codes not at a multiple of 16 bytes");
   if (B == 0) return 0;
-  const int64_t per = cdiv(D, 256), blocks = cdiv(B, kRows8Tile) * per;
-  hipLaunchKernelGGL(rows8_unpack_kernel, dim3((unsigned)std::min(blocks, kRows8Grid)), dim3(256), 0, as_stream(stream),
-                     reinterpret_cast<const uint32_t*>(codes), rows, B, (int)D, (int)rows8_ld(D), (int)per, blocks, x);
+  const bool vec = rows8_vector(x, D);
+  const int64_t per = cdiv(D, vec ? 1024 : 256), blocks = cdiv(B, kRows8Tile) * per;
+  hipLaunchKernelGGL(vec ? rows8_unpack_kernel<4> : rows8_unpack_kernel<1>,
+                     dim3((unsigned)std::min(blocks, kRows8Grid)), dim3(256), 0, as_stream(stream),
+                     reinterpret_cast<const uint32_t*>(codes), rows, B, (int)D, (int)rows8_ld(D), (int)per, blocks,
+                     x);
   SLG_LAUNCH_CHECK("rows8_unpack");
   return 0;
 }
