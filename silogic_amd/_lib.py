@@ -55,6 +55,7 @@ SIGNATURES = {
     "slg_rows8_ld": (_I64, [_I64]),
     "slg_rows8_pack": (C.c_int, [_P, _I64, _I64, _P, _P, _P]),
     "slg_rows8_unpack": (C.c_int, [_P, _P, _I64, _I64, _P, _P]),
+    "slg_fc_soft_fwd8": (C.c_int, [_P, _I64, _I64, _I64, _I32, _P, _P, _I32, _P, _F32, _P, _P, _P, _P]),
     "slg_fc_soft_bwd8_workspace": (_I64, [_I64, _I64, _I64, _I32]),
     "slg_fc_soft_bwd8": (C.c_int, [_P, _P, _I64, _I64, _I64, _I32, _P, _P, _I32, _P, _F32, _P, _P, _P,
                                    _P, _P, _I64, _P]),

@@ -27,6 +27,7 @@
 // pass (heavy inputs: lane by lane, then over the lanes).
 #include "fc_bwd_input.h"
 #include "fc_soft_common.h"
+#include "radix_sort.h"
 #include "ref_table.h"
 
 namespace slg {
@@ -57,15 +58,16 @@ __host__ __device__ inline int ig_slack(int IB) {
 }
 
 // group = pass * NB + block; key = group * IB + input within the block
-__global__ void __launch_bounds__(256) ig_keys_kernel(IgArgs a, const int* __restrict__ cand,
-                                                      int* __restrict__ keys) {
-  const int r = blockIdx.x * 256 + threadIdx.x;
-  if (r >= a.R) return;
-  const int i = min(max(cand[r], 0), a.IN - 1);
-  const int SK = a.NS * a.K, o = r / SK, side = (r - o * SK) / a.K;
-  const int q = i / a.IB;
-  keys[r] = ((side * a.OUT + o) / a.RB * a.NB + q) * a.IB + (i - q * a.IB);
-}
+struct IgKeys {
+  IgArgs a;
+  const int* cand;
+  __device__ int key(int64_t r) const {
+    const int i = min(max(cand[r], 0), a.IN - 1);
+    const int SK = a.NS * a.K, o = (int)r / SK, side = ((int)r - o * SK) / a.K;
+    const int q = i / a.IB;
+    return ((side * a.OUT + o) / a.RB * a.NB + q) * a.IB + (i - q * a.IB);
+  }
+};
 
 // One workgroup per group: its inputs in descending order of their counts
 // (by a counting sort; the place among equal counts does not matter to any
@@ -143,8 +145,7 @@ __global__ void __launch_bounds__(1024) ig_slots_kernel(IgArgs a, const int* __r
 
 // Entries (LDS byte offset of the row within its pass, weight) of each
 // reference: a chunk's lists [step][lane], heavy inputs' lists as they lie.
-__global__ void __launch_bounds__(256) ig_entries_kernel(IgArgs a, const int* __restrict__ sorted,
-                                                         const int* __restrict__ keys,
+__global__ void __launch_bounds__(256) ig_entries_kernel(IgArgs a, const int2* __restrict__ sorted,
                                                          const int* __restrict__ start,
                                                          const int* __restrict__ slot,
                                                          const int* __restrict__ off,
@@ -153,7 +154,7 @@ __global__ void __launch_bounds__(256) ig_entries_kernel(IgArgs a, const int* __
                                                          int2* __restrict__ ent_heavy) {
   const int j = blockIdx.x * 256 + threadIdx.x;
   if (j >= a.R) return;
-  const int r = sorted[j], key = keys[r];
+  const int key = sorted[j].x, r = sorted[j].y;
   const int SK = a.NS * a.K, o = r / SK, side = (r - o * SK) / a.K;
   const int row = side * a.OUT + o;
   const int2 e = make_int2((row - row / a.RB * a.RB) * 16, __float_as_int(w[r]));
@@ -424,19 +425,19 @@ ig_gather_kernel(IgArgs a, const float* __restrict__ gbr, const int* __restrict_
 // with few references to spread that over; here a reference costs the same at
 // any width.
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) iw_keys_kernel(const int* __restrict__ cand, int R,
-                                                               int IN, int* __restrict__ keys) {
-  const int r = blockIdx.x * blockDim.x + threadIdx.x;
-  if (r < R) keys[r] = min(max(cand[r], 0), IN - 1);
-}
+struct IwKeys {
+  const int* cand;
+  int IN;
+  __device__ int key(int64_t r) const { return min(max(cand[r], 0), IN - 1); }
+};
 
-__global__ void __launch_bounds__(256) iw_entries_kernel(const int* __restrict__ sorted,
+__global__ void __launch_bounds__(256) iw_entries_kernel(const int2* __restrict__ sorted,
                                                                   int R, int OUT, int NS, int K,
                                                                   const float* __restrict__ w,
                                                                   int2* __restrict__ ent) {
   const int j = blockIdx.x * blockDim.x + threadIdx.x;
   if (j >= R) return;
-  const int r = sorted[j], SK = NS * K;  // r = (o * NS + side) * K + k
+  const int r = sorted[j].y, SK = NS * K;  // r = (o * NS + side) * K + k
   const int o = r / SK, side = (r - o * SK) / K;
   ent[j] = make_int2(side * OUT + o, __float_as_int(w[r]));
 }
@@ -576,7 +577,7 @@ static inline int64_t ig_round(int64_t n) { return (n + 3) & ~int64_t(3); }
 
 struct IgPlan {
   IgArgs a;
-  int64_t keys, table, perm, slot, off, heavy, ent, ent_heavy, total;  // offsets, 4-byte words
+  int64_t start, sort, perm, slot, off, heavy, ent, ent_heavy, total;  // offsets, 4-byte words
   int64_t groups, nkeys, tiles;
 };
 
@@ -605,8 +606,8 @@ static IgPlan ig_plan(int64_t B, int64_t IN, int64_t OUT, int nsides, int K) {
     o += ig_round(n);
     return at;
   };
-  p.keys = take(a.R);
-  p.table = take(ref_table_ints(a.R, p.nkeys));
+  p.start = take(p.nkeys + 1);
+  p.sort = take(radix_plan(a.R, p.nkeys).words());
   p.perm = take(p.nkeys);
   p.slot = take(p.nkeys);
   p.off = take(p.groups * cdiv(a.IB, 64));
@@ -617,15 +618,15 @@ static IgPlan ig_plan(int64_t B, int64_t IN, int64_t OUT, int nsides, int K) {
   return p;
 }
 
-// Workspace of the wide way: gab [R2][LB] | keys | table | entries.
+// Workspace of the wide way: gab [R2][LB] | starts | sort | entries.
 constexpr int kIwV = 4;              // samples per lane in the gather
 constexpr int kIwIW = 8;             // inputs per wave
 constexpr int kIwSamples = 64 * kIwV;
 constexpr int kIwInputs = 4 * kIwIW;
 
 struct IwPlan {
-  int64_t LB, R, R2, gab, keys, table, ent;
-  int64_t total() const { return gab + keys + table + ent; }
+  int64_t LB, R, R2, gab, start, sort, ent;
+  int64_t total() const { return gab + start + sort + ent; }
 };
 
 static IwPlan iw_plan(int64_t B, int64_t IN, int64_t OUT, int nsides, int K) {
@@ -634,8 +635,8 @@ static IwPlan iw_plan(int64_t B, int64_t IN, int64_t OUT, int nsides, int K) {
   q.R2 = nsides * OUT;
   q.R = q.R2 * K;
   q.gab = q.R2 * q.LB;
-  q.keys = ig_round(q.R);
-  q.table = ref_table_ints(q.R, IN);
+  q.start = ig_round(IN + 1);
+  q.sort = radix_plan(q.R, IN).words();
   q.ent = 2 * q.R;
   return q;
 }
@@ -643,7 +644,7 @@ static IwPlan iw_plan(int64_t B, int64_t IN, int64_t OUT, int nsides, int K) {
 // Whether the wide way is the shorter, by the nanoseconds that the two differ in
 // (fitted to 700 random layers of 100-400000 inputs and outputs, 1-4096 samples,
 // K 1-16; the choice is within 3% of the better way for nineteen in twenty and 1%
-// slower than it on average). From LDS: the key scan by one workgroup, keys per
+// slower than it on average). From LDS: the key scan, keys per
 // (pass, input), then per round of workgroups the passes, the staging of every
 // row and the block's references. Wide: the transpose and the gather over 256
 // samples at a time, and the list of one input, which is walked alone. FC
@@ -679,22 +680,19 @@ static int fc_input_grad_wide(const float* gbr, int64_t B, int64_t IN, int64_t O
   SLG_REQUIRE(q.R < (1LL << 31) && n_tr < (1LL << 31) && n_blocks < (1LL << 31) - 8, SLG_E_SHAPE,
               "fc input gradient: too many references");
   float* gab = ws;
-  int* keys = reinterpret_cast<int*>(gab + q.gab);
-  int* table = keys + q.keys;
-  int2* ent = reinterpret_cast<int2*>(table + q.table);  // offsets are multiples of 4
+  int* start = reinterpret_cast<int*>(gab + q.gab);
+  int* sort = start + q.start;
+  int2* ent = reinterpret_cast<int2*>(sort + q.sort);  // offsets are multiples of 4
   const int R = (int)q.R, R2 = (int)q.R2;
-  hipLaunchKernelGGL(iw_keys_kernel, dim3((unsigned)cdiv(R, 256)), dim3(256), 0, st, cand, R, (int)IN,
-                     keys);
-  RefTable tb{};
-  const int rc = build_ref_table(keys, R, IN, table, st, &tb);
-  if (rc) return rc;
-  hipLaunchKernelGGL(iw_entries_kernel, dim3((unsigned)cdiv(R, 256)), dim3(256), 0, st, tb.sorted, R,
+  const int2* sorted = radix_sort(IwKeys{cand, (int)IN}, radix_plan(R, IN), sort, RadixClear{}, st);
+  ref_starts(sorted, R, IN, start, nullptr, st);
+  hipLaunchKernelGGL(iw_entries_kernel, dim3((unsigned)cdiv(R, 256)), dim3(256), 0, st, sorted, R,
                      (int)OUT, nsides, K, w, ent);
   hipLaunchKernelGGL(iw_transpose_kernel, dim3((unsigned)n_tr), dim3(256), 0, st, gbr, (int)B, R2, q.LB,
                      (int)n_rtiles, gab);
   // a multiple of 8 workgroups for the XCD order
   hipLaunchKernelGGL((iw_gather_kernel<kIwV, kIwIW>), dim3((unsigned)(cdiv(n_blocks, 8) * 8)), dim3(256),
-                     0, st, gab, q.LB, (int)B, (int)IN, tb.start, ent, (int)n_itiles, (int)n_blocks, gx);
+                     0, st, gab, q.LB, (int)B, (int)IN, start, ent, (int)n_itiles, (int)n_blocks, gx);
   SLG_LAUNCH_CHECK("fc input gradient (wide)");
   return 0;
 }
@@ -721,13 +719,11 @@ int fc_input_grad(const float* gbr, int64_t B, int64_t IN, int64_t OUT, int nsid
   if (ig_wide(p)) return fc_input_grad_wide(gbr, B, IN, OUT, nsides, K, cand, w, ws, gx, st);
   const IgArgs& a = p.a;
   int* iw = reinterpret_cast<int*>(ws);
-  int *keys = iw + p.keys, *perm = iw + p.perm, *slot = iw + p.slot, *off = iw + p.off,
+  int *start = iw + p.start, *perm = iw + p.perm, *slot = iw + p.slot, *off = iw + p.off,
       *heavy = iw + p.heavy;
   int2* ent = reinterpret_cast<int2*>(iw + p.ent);
   int2* ent_heavy = reinterpret_cast<int2*>(iw + p.ent_heavy);
-  RefTable tb{};
   if (ig_small(a)) {
-    tb.start = iw + p.table;
     const size_t lds = ig_small_lds(a);
     if (lds > 65536 - 8192) {
       const hipError_t e = hipFuncSetAttribute((const void*)ig_table_kernel,
@@ -735,16 +731,15 @@ int fc_input_grad(const float* gbr, int64_t B, int64_t IN, int64_t OUT, int nsid
       SLG_REQUIRE(e == hipSuccess, (int)e, "fc input gradient: LDS %zu: %s", lds,
                   hipGetErrorString(e));
     }
-    hipLaunchKernelGGL(ig_table_kernel, dim3((unsigned)a.NB), dim3(1024), lds, st, a, cand, w, tb.start,
+    hipLaunchKernelGGL(ig_table_kernel, dim3((unsigned)a.NB), dim3(1024), lds, st, a, cand, w, start,
                        perm, slot, off, heavy, ent, ent_heavy);
   } else {
     const unsigned rb = (unsigned)cdiv(a.R, 256);
-    hipLaunchKernelGGL(ig_keys_kernel, dim3(rb), dim3(256), 0, st, a, cand, keys);
-    const int rc = build_ref_table(keys, a.R, p.nkeys, iw + p.table, st, &tb);
-    if (rc) return rc;
-    hipLaunchKernelGGL(ig_slots_kernel, dim3((unsigned)p.groups), dim3(1024), 0, st, a, tb.start, perm,
+    const int2* sorted = radix_sort(IgKeys{a, cand}, radix_plan(a.R, p.nkeys), iw + p.sort, RadixClear{}, st);
+    ref_starts(sorted, a.R, p.nkeys, start, nullptr, st);
+    hipLaunchKernelGGL(ig_slots_kernel, dim3((unsigned)p.groups), dim3(1024), 0, st, a, start, perm,
                        slot, off, heavy);
-    hipLaunchKernelGGL(ig_entries_kernel, dim3(rb), dim3(256), 0, st, a, tb.sorted, keys, tb.start,
+    hipLaunchKernelGGL(ig_entries_kernel, dim3(rb), dim3(256), 0, st, a, sorted, start,
                        slot, off, w, ent, ent_heavy);
   }
   SLG_LAUNCH_CHECK("fc input gradient table");
@@ -755,7 +750,7 @@ int fc_input_grad(const float* gbr, int64_t B, int64_t IN, int64_t OUT, int nsid
     SLG_REQUIRE(e == hipSuccess, (int)e, "fc input gradient: LDS %zu: %s", lds, hipGetErrorString(e));
   }
   hipLaunchKernelGGL(ig_gather_kernel, dim3((unsigned)(p.tiles * a.NB)), dim3(kIgThreads), lds, st, a,
-                     gbr, tb.start, perm, off, heavy, ent, ent_heavy, gx);
+                     gbr, start, perm, off, heavy, ent, ent_heavy, gx);
   SLG_LAUNCH_CHECK("fc input gradient gather");
   return 0;
 }

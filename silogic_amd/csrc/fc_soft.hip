@@ -20,6 +20,7 @@
 //   * The tile/chunk index is remapped so chunks of one tile run on the same
 //     XCD and share its L2 copy of the input rows.
 #include "fc_soft_common.h"
+#include "rows8.h"
 
 namespace slg {
 
@@ -37,10 +38,14 @@ struct HeadArgs {
 template <int KC, int S>
 constexpr int soft_max_threads() { return (KC == 0 || S >= 8) ? 512 : 1024; }
 
-template <int NODE, int KC, int S, bool HEAD, bool REC>
+// PACK: the input also in 8 bits (rows8.h), from the staged tile: what a
+// training layer keeps of it, without reading it again (10000 -> 10000, K = 8,
+// B = 4096: %PACK%).
+template <int NODE, int KC, int S, bool HEAD, bool REC, bool PACK = false>
 __global__ void __launch_bounds__((soft_max_threads<KC, S>()))
 fc_soft_kernel(const float* __restrict__ x, int B, int IN, int OUT, int Kr, ParamView pv,
-               float inv_tau, float* __restrict__ y, int n_chunks, int chunk, HeadArgs hd) {
+               float inv_tau, float* __restrict__ y, int n_chunks, int chunk, HeadArgs hd,
+               Rows8Out po) {
   constexpr int V = S >= 4 ? 4 : S;
   constexpr int G = S / V;
   constexpr int KM = KC > 0 ? KC : 16;
@@ -65,6 +70,10 @@ fc_soft_kernel(const float* __restrict__ x, int B, int IN, int OUT, int Kr, Para
   // of input i.
   for (int g = 0; g < G; ++g) stage_rows<V, true>(lds + g * IN, x, B, IN, b0 + g * V);
   __syncthreads();
+  if constexpr (PACK) {
+    if (ch == 0)  // one of the tile's output chunks
+      rows8_pack_tile<S>(lds, IN, b0, B, reinterpret_cast<float*>(lds + G * IN), po);
+  }
 
   const uint32_t lim = (uint32_t)IN - 1u;
   const int lane = threadIdx.x & 63;
@@ -866,6 +875,7 @@ struct SoftArgs {
   float inv_tau; float* y;
   int S, threads;
   HeadArgs hd;  // hd.logits != nullptr: fused GroupSum, y unused
+  Rows8Out po{};  // po.codes != nullptr: the input in 8 bits too (no head, no records)
 };
 
 // Output chunks per sample tile: enough workgroups to fill the chip twice
@@ -900,7 +910,13 @@ static int launch_soft_s(const SoftArgs& a, hipStream_t st) {
               (long long)a.OUT);
   auto kern = fc_soft_kernel<NODE, KC, S, HEAD, REC>;
   const int threads = std::min(a.threads, soft_max_threads<KC, S>());
-  const size_t lds = (size_t)a.IN * S * sizeof(float) + (HEAD ? (size_t)S * a.hd.C * 4 : 0);
+  size_t lds = (size_t)a.IN * S * sizeof(float) + (HEAD ? (size_t)S * a.hd.C * 4 : 0);
+  if constexpr (!HEAD && !REC && S >= 4) {
+    if (a.po.codes) {
+      kern = fc_soft_kernel<NODE, KC, S, HEAD, REC, true>;
+      lds += sizeof(float) * rows8_scratch(S, threads / 64);
+    }
+  }
   if constexpr (REC && (KC == 4 || KC == 8)) {
     auto rk = fc_soft_rec_kernel<NODE, KC, S, HEAD>;
     SLG_REQUIRE(lds <= (size_t)device_lds_bytes(), SLG_E_SHAPE, "fc_soft: %zu B LDS needed", lds);
@@ -936,7 +952,7 @@ static int launch_soft_s(const SoftArgs& a, hipStream_t st) {
   }
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(threads), lds, st, a.x, (int)a.B,
                      (int)a.IN, (int)a.OUT, a.K, a.pv, a.inv_tau, a.y, (int)n_chunks, (int)chunk,
-                     a.hd);
+                     a.hd, a.po);
   SLG_LAUNCH_CHECK("fc_soft");
   return 0;
 }
@@ -1073,11 +1089,16 @@ static int fc_soft_dispatch(SoftArgs a, int node_kind, hipStream_t st) {
   if (a.S == 0 && pick_tile(a.IN, 0) == 0) {  // rows wider than LDS: slab staging
     SLG_REQUIRE(!head, SLG_E_UNSUPPORTED, "fc_soft: the fused GroupSum needs IN <= %lld",
                 (long long)(device_lds_bytes() / 4));
+    if (a.po.codes) rows8_pack(a.x, a.B, a.IN, a.po.codes, a.po.rows, st);
     return fc_soft_wide(a, node_kind, st);
   }
   a.S = pick_tile(a.IN, a.S, a.B);
   SLG_REQUIRE(a.S > 0 && (int64_t)a.IN * a.S * 4 <= device_lds_bytes(), SLG_E_SHAPE,
               "fc_soft: IN=%lld does not fit LDS", (long long)a.IN);
+  if (a.po.codes && a.S < 4) {  // the codes' words are tiles of 4 samples
+    rows8_pack(a.x, a.B, a.IN, a.po.codes, a.po.rows, st);
+    a.po.codes = nullptr;
+  }
   a.threads = pick_threads(a.IN, a.S, a.threads);
   SLG_REQUIRE(a.threads % 64 == 0 && a.threads <= 1024, SLG_E_ARG, "fc_soft: threads=%d", a.threads);
   if (head) {
@@ -1360,6 +1381,18 @@ int slg_fc_soft_fwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t 
   SLG_REQUIRE(cand && w, SLG_E_ARG, "fc_soft_fwd: null cand/w");
   SoftArgs a{x, B, IN, OUT, K, arrays_view(cand, cand + K, 2 * K, w, w + K, 2 * K, node_param),
              inv_tau, out, tile_samples, threads, HeadArgs{nullptr, 0, 0, 1.0f}};
+  return fc_soft_dispatch(a, node_kind, as_stream(stream));
+}
+
+int slg_fc_soft_fwd8(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t K,
+                     const int32_t* cand, const float* w, int32_t node_kind,
+                     const float* node_param, float inv_tau, float* out, uint8_t* codes, float* rows,
+                     slg_stream_t stream) {
+  SLG_REQUIRE(cand && w && ((codes && rows) || B == 0), SLG_E_ARG, "fc_soft_fwd8: null pointer");
+  SLG_REQUIRE((uintptr_t)codes % 16 == 0, SLG_E_ARG, "fc_soft_fwd8: codes not at a multiple of 16 bytes");
+  SoftArgs a{x, B, IN, OUT, K, arrays_view(cand, cand + K, 2 * K, w, w + K, 2 * K, node_param),
+             inv_tau, out, 0, 0, HeadArgs{nullptr, 0, 0, 1.0f},
+             Rows8Out{reinterpret_cast<uint32_t*>(codes), rows, (int)rows8_ld(IN)}};
   return fc_soft_dispatch(a, node_kind, as_stream(stream));
 }
 

@@ -1,7 +1,7 @@
 // Stable radix sort of (key, index) pairs, the order in which sums over
 // references or tokens run: entries in ascending keys, indices of one key
 // ascending, the same on every call. Least significant digits first, at most
-// 9 bits a pass; a pass is a count of every workgroup's digits and a scatter.
+// 10 bits a pass; a pass is a count of every workgroup's digits and a scatter.
 //
 // A wave ranks 64 entries at a time: ballots over the digit's bits give each
 // lane the lanes that share its digit, the first of them adds their number to
@@ -23,15 +23,15 @@
 namespace slg {
 
 constexpr int kRadixThreads = 512, kRadixWaves = kRadixThreads / 64;
-constexpr int kRadixMaxBits = 9;
-constexpr int kRadixSmall = 8 * kRadixThreads;  // entries of the one-launch sort, at most
+constexpr int kRadixBits = 10, kRadixSmallBits = 9;  // of a digit, at most (the small sort's LDS holds entries too)
+constexpr int kRadixSmall = 8 * kRadixThreads;       // entries of the one-launch sort, at most
 
 // A range of 4-byte words that the first launch clears beside its own work,
 // and up to one more word.
 struct RadixClear {
-  void* p;
-  int64_t bytes;
-  int* word;
+  void* p = nullptr;
+  int64_t bytes = 0;
+  int* word = nullptr;
 };
 
 struct RadixPlan {
@@ -51,7 +51,8 @@ inline RadixPlan radix_plan(int64_t N, int64_t nkeys) {
   p.N = N;
   int key = 1;
   while (key < 31 && ((nkeys - 1) >> key) != 0) ++key;
-  p.passes = (key + kRadixMaxBits - 1) / kRadixMaxBits;
+  const int most = N <= kRadixSmall ? kRadixSmallBits : kRadixBits;
+  p.passes = (key + most - 1) / most;
   p.bits = (key + p.passes - 1) / p.passes;
   // short rounds spread few entries over more CUs; past 64 workgroups longer
   // ones keep the counts that every workgroup reads few
@@ -134,7 +135,7 @@ template <typename Src>
 __global__ void __launch_bounds__(kRadixThreads)
 radix_small_kernel(Src src, int N, int passes, int bits, int2* __restrict__ out, RadixClear clear) {
   constexpr int I = kRadixSmall / kRadixThreads;
-  __shared__ int cnt[kRadixWaves << kRadixMaxBits];
+  __shared__ int cnt[kRadixWaves << kRadixSmallBits];
   __shared__ int2 ent[kRadixSmall];
   __shared__ int part[kRadixWaves];
   if (gridDim.x == 1 || blockIdx.x > 0)
@@ -186,7 +187,7 @@ template <typename Src>
 __global__ void __launch_bounds__(kRadixThreads)
 radix_count_kernel(Src src, const int2* __restrict__ in, RadixPlan p, int shift, int* __restrict__ hist,
                    RadixClear clear) {
-  __shared__ int cnt[1 << kRadixMaxBits];
+  __shared__ int cnt[1 << kRadixBits];
   if ((int)blockIdx.x >= p.blocks) {
     radix_clear(clear, blockIdx.x - p.blocks, gridDim.x - p.blocks);
     return;
@@ -215,46 +216,54 @@ template <typename Src, int I>
 __global__ void __launch_bounds__(kRadixThreads)
 radix_scatter_kernel(Src src, const int2* __restrict__ in, RadixPlan p, int shift,
                      const int* __restrict__ hist, int2* __restrict__ out) {
-  __shared__ int cnt[kRadixWaves << kRadixMaxBits];
-  __shared__ int tot[1 << kRadixMaxBits], base[1 << kRadixMaxBits], part[kRadixWaves];
+  __shared__ int cnt[kRadixWaves << kRadixBits];
+  __shared__ int tot[1 << kRadixBits], base[1 << kRadixBits], part[kRadixWaves];
   const int R = 1 << p.bits, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int mine = blockIdx.x;
   {  // P neighbouring threads to a digit
-    const int P = min(kRadixThreads >> p.bits, 64), d = tid / P, q = tid - d * P, nq = p.nbp >> 2;
-    int total = 0, before = 0;
-    if (d < R) {
-      const int4* h = reinterpret_cast<const int4*>(hist + (int64_t)d * p.nbp);
-      constexpr int U = 8;
-      for (int j0 = q; j0 < nq; j0 += U * P) {
-        int4 c[U];
+    const int P = max(1, min(kRadixThreads >> p.bits, 64)), q = tid % P, nq = p.nbp >> 2;
+    for (int d0 = 0; d0 < R; d0 += kRadixThreads / P) {  // every lane takes part in the sums
+      const int d = d0 + tid / P;
+      int total = 0, before = 0;
+      if (d < R) {
+        const int4* h = reinterpret_cast<const int4*>(hist + (int64_t)d * p.nbp);
+        constexpr int U = 8;
+        for (int j0 = q; j0 < nq; j0 += U * P) {
+          int4 c[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) c[u] = h[min(j0 + u * P, nq - 1)];
+          for (int u = 0; u < U; ++u) c[u] = h[min(j0 + u * P, nq - 1)];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int j = j0 + u * P;
-          if (j < nq) {
-            const int b = 4 * j;
-            total += c[u].x + c[u].y + c[u].z + c[u].w;
-            before += (b < mine ? c[u].x : 0) + (b + 1 < mine ? c[u].y : 0) + (b + 2 < mine ? c[u].z : 0) +
-                      (b + 3 < mine ? c[u].w : 0);
+          for (int u = 0; u < U; ++u) {
+            const int j = j0 + u * P;
+            if (j < nq) {
+              const int b = 4 * j;
+              total += c[u].x + c[u].y + c[u].z + c[u].w;
+              before += (b < mine ? c[u].x : 0) + (b + 1 < mine ? c[u].y : 0) + (b + 2 < mine ? c[u].z : 0) +
+                        (b + 3 < mine ? c[u].w : 0);
+            }
           }
         }
       }
-    }
-    for (int s = 1; s < P; s <<= 1) {
-      total += __shfl_xor(total, s, 64);
-      before += __shfl_xor(before, s, 64);
-    }
-    if (d < R && q == 0) {
-      tot[d] = total;
-      base[d] = before;
+      for (int s = 1; s < P; s <<= 1) {
+        total += __shfl_xor(total, s, 64);
+        before += __shfl_xor(before, s, 64);
+      }
+      if (d < R && q == 0) {
+        tot[d] = total;
+        base[d] = before;
+      }
     }
   }
   __syncthreads();
-  {
-    const int t = tid < R ? tot[tid] : 0;
-    const int x = radix_scan(t, part) - t;
-    if (tid < R) base[tid] += x;
+  {  // a thread's neighbouring digits
+    const int per = max(1, R / kRadixThreads), d0 = min(tid * per, R), d1 = min(d0 + per, R);
+    int t = 0;
+    for (int d = d0; d < d1; ++d) t += tot[d];
+    int x = radix_scan(t, part) - t;
+    for (int d = d0; d < d1; ++d) {
+      base[d] += x;
+      x += tot[d];
+    }
   }
   const int64_t i0 = mine * p.tile, i1 = min(p.N, i0 + p.tile);
   for (int64_t r0 = i0; r0 < i1; r0 += I * kRadixThreads) {
@@ -273,15 +282,15 @@ radix_scatter_kernel(Src src, const int2* __restrict__ in, RadixPlan p, int shif
     __syncthreads();
     radix_rank<I>(d, valid, p.bits, cnt + wave * R, rank);
     __syncthreads();
-    if (tid < R) {
-      int run = base[tid];
+    for (int b = tid; b < R; b += kRadixThreads) {
+      int run = base[b];
 #pragma unroll
       for (int w = 0; w < kRadixWaves; ++w) {
-        const int c = cnt[w * R + tid];
-        cnt[w * R + tid] = run;
+        const int c = cnt[w * R + b];
+        cnt[w * R + b] = run;
         run += c;
       }
-      base[tid] = run;
+      base[b] = run;
     }
     __syncthreads();
 #pragma unroll
@@ -306,7 +315,7 @@ inline const int2* radix_sort(const Src& src, const RadixPlan& p, int* ws, const
   }
   const int2* in = nullptr;
   for (int k = 0, shift = 0; k < p.passes; ++k, shift += p.bits) {
-    const RadixClear c = k == 0 ? clear : RadixClear{nullptr, 0, nullptr};
+    const RadixClear c = k == 0 ? clear : RadixClear{};
     hipLaunchKernelGGL((radix_count_kernel<Src>), dim3(p.blocks + (k == 0 ? std::max(extra, clear.word ? 1 : 0) : 0)),
                        dim3(kRadixThreads), 0, st, src, in, p, shift, hist, c);
     if (p.items == 4)

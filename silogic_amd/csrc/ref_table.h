@@ -21,4 +21,8 @@ int64_t ref_table_ints(int64_t R, int64_t nkeys);
 int build_ref_table(const int* keys, int64_t R, int64_t nkeys, int* ws, hipStream_t st,
                     RefTable* out);
 
+// start[k] = how many of R entries sorted by key (x) lie below key k, k in
+// [0, nkeys]; with sorted, also their references (y) alone.
+void ref_starts(const int2* ent, int64_t R, int64_t nkeys, int* start, int* sorted, hipStream_t st);
+
 }  // namespace slg

@@ -39,6 +39,12 @@ __global__ void __launch_bounds__(256) ref_start_kernel(const int2* __restrict__
 
 static inline int64_t round4i(int64_t n) { return (n + 3) & ~int64_t(3); }
 
+void ref_starts(const int2* ent, int64_t R, int64_t nkeys, int* start, int* sorted, hipStream_t st) {
+  const int64_t sb = cdiv(nkeys + 1, 256);
+  hipLaunchKernelGGL(ref_start_kernel, dim3((unsigned)(sb + (sorted ? cdiv(R, 256) : 0))), dim3(256), 0, st, ent,
+                     (int)R, (int)nkeys, (int)sb, start, sorted);
+}
+
 int64_t ref_table_ints(int64_t R, int64_t nkeys) {
   return round4i(nkeys + 1) + round4i(R) + radix_plan(R, nkeys).words();
 }
@@ -53,10 +59,8 @@ int build_ref_table(const int* keys, int64_t R, int64_t nkeys, int* ws, hipStrea
   int* sort_ws = sorted + round4i(R);
   const int2* ent = reinterpret_cast<const int2*>(sort_ws);
   if (R > 0)
-    ent = radix_sort(RefKeys{keys}, radix_plan(R, nkeys), sort_ws, RadixClear{nullptr, 0, nullptr}, st);
-  const int64_t sb = cdiv(nkeys + 1, 256);
-  hipLaunchKernelGGL(ref_start_kernel, dim3((unsigned)(sb + cdiv(R, 256))), dim3(256), 0, st, ent, (int)R,
-                     (int)nkeys, (int)sb, start, sorted);
+    ent = radix_sort(RefKeys{keys}, radix_plan(R, nkeys), sort_ws, RadixClear{}, st);
+  ref_starts(ent, R, nkeys, start, sorted, st);
   SLG_LAUNCH_CHECK("reference table");
   out->start = start;
   out->sorted = sorted;

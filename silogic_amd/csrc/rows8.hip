@@ -17,36 +17,6 @@ namespace slg {
 
 constexpr int64_t kRows8Grid = 1 << 20;  // workgroups at most; the rest in turn
 
-struct Rows8Range {
-  float lo, hi;
-  bool bad;
-};
-
-__device__ inline void rows8_take(Rows8Range& r, float v) {
-  r.lo = fminf(r.lo, v);
-  r.hi = fmaxf(r.hi, v);
-  r.bad |= !(fabsf(v) <= 3.402823466e38f);
-}
-
-// Offset, step and reciprocal step of a row from its range.
-__device__ inline void rows8_scale(float lo, float hi, bool bad, float& lo_out, float& step, float& inv) {
-  const float span = hi - lo;
-  bad |= !(span <= 3.402823466e38f);
-  inv = 255.0f / span;
-  step = span / 255.0f;
-  if (!(span > 0.0f) || !(inv <= 3.402823466e38f)) inv = step = 0.0f;
-  lo_out = lo;
-  if (bad) {
-    lo_out = __int_as_float(0x7fc00000);
-    inv = step = 0.0f;
-  }
-}
-
-__device__ inline uint32_t rows8_code(float x, float lo, float inv) {
-  // inv = 0: a constant or not finite row, code 0 (a NaN lo would reach the cast)
-  return inv > 0.0f ? (uint32_t)fminf(rintf((x - lo) * inv), 255.0f) : 0u;
-}
-
 // VU neighbouring values or words as one access.
 template <int VU>
 __device__ inline void rows8_load(const float* __restrict__ p, float (&v)[VU]) {
@@ -66,7 +36,8 @@ template <int NU, int VU, int T>
 __global__ void __launch_bounds__(T)
 rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_t* __restrict__ codes,
                   float* __restrict__ rows) {
-  __shared__ Rows8Range part[T / 64][kRows8Tile];
+  struct Ends { float lo, hi; };
+  __shared__ Ends part[T / 64][kRows8Tile];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int64_t t = blockIdx.x; t * kRows8Tile < B; t += gridDim.x) {
     const int64_t b0 = t * kRows8Tile;
@@ -75,8 +46,6 @@ rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_
 #pragma unroll
     for (int v = 0; v < kRows8Tile; ++v) p[v] = x + (b0 + min(v, nb - 1)) * D;  // past the batch: its last row
     Rows8Range r[kRows8Tile];
-#pragma unroll
-    for (int v = 0; v < kRows8Tile; ++v) r[v] = {INFINITY, -INFINITY, false};
     float keep[NU > 0 ? NU : 1][kRows8Tile][VU];
     if constexpr (NU > 0) {
 #pragma unroll
@@ -90,39 +59,33 @@ rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_
 #pragma unroll
         for (int v = 0; v < kRows8Tile; ++v)
 #pragma unroll
-          for (int j = 0; j < VU; ++j) rows8_take(r[v], keep[u][v][j]);
+          for (int j = 0; j < VU; ++j) r[v].take(keep[u][v][j]);
     } else {
       for (int i = tid * VU; i < D; i += T * VU)
 #pragma unroll
         for (int v = 0; v < kRows8Tile; ++v) {
           rows8_load<VU>(p[v] + i, keep[0][v]);
 #pragma unroll
-          for (int j = 0; j < VU; ++j) rows8_take(r[v], keep[0][v][j]);
+          for (int j = 0; j < VU; ++j) r[v].take(keep[0][v][j]);
         }
     }
 #pragma unroll
     for (int v = 0; v < kRows8Tile; ++v) {
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        r[v].lo = fminf(r[v].lo, __shfl_xor(r[v].lo, d, 64));
-        r[v].hi = fmaxf(r[v].hi, __shfl_xor(r[v].hi, d, 64));
-      }
-      r[v].bad = __any(r[v].bad);
-      if (lane == 0) part[wave][v] = r[v];
+      r[v].wave();
+      if (lane == 0) part[wave][v] = {r[v].lo, r[v].hi};
     }
     __syncthreads();
     float lo[kRows8Tile], inv[kRows8Tile];
 #pragma unroll
     for (int v = 0; v < kRows8Tile; ++v) {
-      Rows8Range a = part[0][v];
+      Ends a = part[0][v];
 #pragma unroll
       for (int w = 1; w < T / 64; ++w) {
         a.lo = fminf(a.lo, part[w][v].lo);
         a.hi = fmaxf(a.hi, part[w][v].hi);
-        a.bad |= part[w][v].bad;
       }
       float step;
-      rows8_scale(a.lo, a.hi, a.bad, lo[v], step, inv[v]);
+      rows8_scale(a.lo, a.hi, lo[v], step, inv[v]);
       if (tid == 0 && v < nb) {
         rows[2 * (b0 + v)] = lo[v];
         rows[2 * (b0 + v) + 1] = step;
@@ -136,7 +99,7 @@ rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_
       for (int j = 0; j < VU; ++j) {
         w[j] = 0;
 #pragma unroll
-        for (int v = 0; v < kRows8Tile; ++v) w[j] |= rows8_code(e[v][j], lo[v], inv[v]) << (8 * v);
+        for (int v = 0; v < kRows8Tile; ++v) w[j] = rows8_code(w[j], v, e[v][j], lo[v], inv[v]);
       }
       if constexpr (VU == 4) *reinterpret_cast<uint4*>(c + i) = make_uint4(w[0], w[1], w[2], w[3]);
       else c[i] = w[0];
@@ -212,6 +175,11 @@ static void launch_pack_v(const float* x, int64_t B, int64_t D, uint32_t* codes,
 
 static bool rows8_vector(const float* x, int64_t D) { return D % 4 == 0 && (uintptr_t)x % 16 == 0; }
 
+void rows8_pack(const float* x, int64_t B, int64_t D, uint32_t* codes, float* rows, hipStream_t st) {
+  if (rows8_vector(x, D)) launch_pack_v<4>(x, B, D, codes, rows, st);
+  else launch_pack_v<1>(x, B, D, codes, rows, st);
+}
+
 }  // namespace slg
 
 using namespace slg;
@@ -226,10 +194,7 @@ int slg_rows8_pack(const float* x, int64_t B, int64_t D, uint8_t* codes, float* 
               "rows8_pack: B %lld, D %lld", (long long)B, (long long)D);
   SLG_REQUIRE((uintptr_t)codes % 16 == 0, SLG_E_ARG, "rows8_pack: codes not at a multiple of 16 bytes");
   if (B == 0) return 0;
-  hipStream_t st = as_stream(stream);
-  uint32_t* c = reinterpret_cast<uint32_t*>(codes);
-  if (rows8_vector(x, D)) launch_pack_v<4>(x, B, D, c, rows, st);
-  else launch_pack_v<1>(x, B, D, c, rows, st);
+  rows8_pack(x, B, D, reinterpret_cast<uint32_t*>(codes), rows, as_stream(stream));
   SLG_LAUNCH_CHECK("rows8_pack");
   return 0;
 }

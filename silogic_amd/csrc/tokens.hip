@@ -156,7 +156,7 @@ __device__ inline void seg_write(const SegArgs& a, int v, int d, const float (&s
 // does not matter: every run is summed by itself).
 constexpr int kSegAhead = 8;
 template <int DT, int VU>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict__ gy,
                    const typename TabType<DT>::t* __restrict__ tab,
                    typename TabType<DT>::t* __restrict__ gtab, float* __restrict__ edge,
@@ -175,13 +175,19 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
     float sum[VU];
 #pragma unroll
     for (int j = 0; j < VU; ++j) sum[j] = 0.0f;
+    int2 next[kSegAhead];  // the next rows' entries, a batch ahead of their gradients
+#pragma unroll
+    for (int u = 0; u < kSegAhead; ++u) next[u] = ent[min(i0 + u, i1 - 1)];
     for (int64_t i = i0; i < i1 && row < a.V; i += kSegAhead) {
       int2 e[kSegAhead];
       float g[kSegAhead][VU];
 #pragma unroll
-      for (int u = 0; u < kSegAhead; ++u) e[u] = ent[min(i + u, i1 - 1)];
+      for (int u = 0; u < kSegAhead; ++u) {
+        e[u] = next[u];
+        tab_load<kTabF32, VU>(gy + (int64_t)(uint32_t)e[u].y * a.D + d, g[u]);
+      }
 #pragma unroll
-      for (int u = 0; u < kSegAhead; ++u) tab_load<kTabF32, VU>(gy + (int64_t)(uint32_t)e[u].y * a.D + d, g[u]);
+      for (int u = 0; u < kSegAhead; ++u) next[u] = ent[min(i + kSegAhead + u, i1 - 1)];
 #pragma unroll
       for (int u = 0; u < kSegAhead; ++u) {
         if (i + u >= i1) break;
@@ -214,7 +220,7 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
 // The runs that cross chunks, a workgroup each: G lanes a row, the chunks'
 // parts dealt to kJoinThreads / G groups (each in ascending order), whose sums
 // are added in order.
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 256;
 template <int DT, int VU>
 __global__ void __launch_bounds__(kJoinThreads)
 tok_join_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict__ edge,
@@ -497,7 +503,7 @@ int slg_token_encode_bwd(const void* ids, int32_t id_bytes, int64_t N, int64_t V
       hipLaunchKernelGGL((tok_segment_kernel<DT, VU>), dim3((unsigned)cdiv(p.chunks, 256 / p.G)), dim3(256), 0, st,
                          s, ent, gy, static_cast<const T*>(table), static_cast<T*>(gtable), edge, listed + 1,
                          listed);
-      hipLaunchKernelGGL((tok_join_kernel<DT, VU>), dim3((unsigned)std::min<int64_t>(p.chunks, 512)),
+      hipLaunchKernelGGL((tok_join_kernel<DT, VU>), dim3((unsigned)std::min<int64_t>(p.chunks, 2048)),
                          dim3(kJoinThreads), 0, st, s, ent, edge, static_cast<const T*>(table),
                          static_cast<T*>(gtable), listed + 1, listed);
     });

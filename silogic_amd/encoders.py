@@ -142,7 +142,10 @@ class TokenEncoder(nn.Module):
         ids = self._ids(ids)
         if torch.compiler.is_compiling():
             return torch.ops.silogic_hip.token_encode(ids, self.weight, self.scale, self.ste, self._pad)
-        return _TokenFn.apply(ids, ops._c(self.weight), self.scale, self.ste, self._pad)
+        w = ops._c(self.weight)
+        if not ops._grad_path(w):
+            return ops.token_encode(ids, w, self.scale, self.ste, self._pad)
+        return _TokenFn.apply(ids, w, self.scale, self.ste, self._pad)
 
     def _bit_table(self):
         """Bit words of the weight, made once per version of it. Another stream

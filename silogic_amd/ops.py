@@ -82,20 +82,27 @@ def call_on(t, name, *args):
 
 def same_device(what, *ts):
     """Raise unless all of ``ts`` (None apart) are on one device."""
-    ds = {t.device for t in ts if t is not None}
-    if len(ds) > 1:
-        raise ValueError(f"{what}: tensors on {', '.join(sorted(map(str, ds)))}")
+    ts = [t for t in ts if t is not None]
+    d = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != d:
+            raise ValueError(f"{what}: tensors on {', '.join(sorted({str(t.device) for t in ts}))}")
 
 
 # ---------------------------------------------------------------------------
 # activations in 8 bits
 # ---------------------------------------------------------------------------
+def _rows8_empty(x):
+    B, D = x.shape
+    return (torch.empty((-(-B // 4), (D + 3) // 4 * 4, 4), device=x.device, dtype=torch.uint8),
+            torch.empty((B, 2), device=x.device, dtype=torch.float32))
+
+
 def rows8_pack(x):
     """``x [B, D]`` fp32 -> ``(codes [ceil(B/4), ld, 4] uint8, rows [B, 2])``
     (``slg_rows8_pack``)."""
     B, D = x.shape
-    codes = torch.empty((-(-B // 4), (D + 3) // 4 * 4, 4), device=x.device, dtype=torch.uint8)
-    rows = torch.empty((B, 2), device=x.device, dtype=torch.float32)
+    codes, rows = _rows8_empty(x)
     call_on(x, "slg_rows8_pack", _p(x), B, D, _p(codes), _p(rows))
     return codes, rows
 
@@ -338,8 +345,12 @@ def check_layer8(x, cand, **shapes):
 
 def fc_soft8_fwd(x, cand, w, npar, node_kind, inv_tau):
     """``(y, codes, rows)``: the soft gate layer and its input in 8 bits."""
-    y = _fc_soft_launch(x, cand, w, npar, node_kind, inv_tau)
-    return (y, *rows8_pack(x))
+    (B, IN), (OUT, _, K) = x.shape, cand.shape
+    codes, rows = _rows8_empty(x)
+    y = torch.empty((B, OUT), device=x.device, dtype=torch.float32)
+    call_on(x, "slg_fc_soft_fwd8", _p(x), B, IN, OUT, K, _p(cand), _p(w), node_kind, _p(npar),
+            float(inv_tau), _p(y), _p(codes), _p(rows))
+    return y, codes, rows
 
 
 def fc_layer8_fwd(x, cand, conn, raw, node_kind, inv_tau):

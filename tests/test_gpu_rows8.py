@@ -134,6 +134,24 @@ def test_wide_rows(IN):
     _check_layer(orc.GATE16, 6, IN, 150, 8, 1.0)
 
 
+@pytest.mark.parametrize("B,IN,OUT,K", [(1, 1, 1, 1), (5, 64, 70, 8), (9, 1280, 700, 4), (130, 1281, 40, 8),
+                                        (4100, 1300, 64, 4), (4099, 4099, 65, 3), (33, 10000, 129, 8),
+                                        (7, 10177, 30, 8), (6, 16380, 200, 4), (5, 30001, 40, 2), (3, 41000, 50, 8)])
+def test_forward_writes_what_pack_writes(B, IN, OUT, K):
+    """The codes that a layer's forward makes from its staged tiles (4 and 8 samples, several output chunks a
+    tile) or beside them (narrower tiles), and its output, are those of the separate calls."""
+    x, cand, conn, raw, _ = _problem(orc.GATE16, B, IN, OUT, K, x=_rows(B, IN))
+    if B > 2:
+        x[2, IN // 2] = float("nan")
+    x, cand, conn, raw = (t.to(DEV) for t in (x, cand, conn, raw))
+    y, codes, rows, w, kept = ops.fc_layer8_fwd(x, cand, conn, raw, orc.GATE16, 1.0)
+    want = ops.rows8_pack(x)
+    assert torch.equal(codes, want[0]) and torch.equal(rows.isnan(), want[1].isnan())
+    assert torch.equal(rows.nan_to_num(7.0), want[1].nan_to_num(7.0))
+    yw = ops._fc_soft_launch(x, cand, w, kept[:OUT], orc.GATE16, 1.0)
+    assert torch.equal(y.nan_to_num(7.0), yw.nan_to_num(7.0))
+
+
 @pytest.mark.parametrize("kind", list(KINDS))
 def test_layer_of_rows_with_ranges_of_their_own(kind):
     x = _rows(37, 90)
