@@ -324,6 +324,22 @@ int slg_fc_soft_bwd8(const uint8_t* codes, const float* rows, int64_t B, int64_t
                      const float* node_param, float inv_tau, const float* gy, float* gx, float* gw,
                      float* gnp, float* workspace, int64_t workspace_floats, slg_stream_t stream);
 
+/* A gate layer's training step from its own parameters, its input kept in 8
+ * bits: slg_layer_params and slg_fc_soft_fwd8 one way (w [OUT,2,K] and kept as
+ * the former gives them: kept [OUT,4], gate16: followed by its probabilities
+ * [OUT,16]), slg_fc_soft_bwd8 and slg_layer_params_bwd the other (any of gx,
+ * gconn, graw may be NULL). conn NULL: fixed wiring. raw and kept at multiples
+ * of 16 bytes. */
+int slg_fc_layer8_fwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t K,
+                      const int32_t* cand, const float* conn, const float* raw, int32_t node_kind,
+                      float inv_tau, float* y, uint8_t* codes, float* rows, float* w, float* kept,
+                      slg_stream_t stream);
+int64_t slg_fc_layer8_bwd_workspace(int64_t B, int64_t IN, int64_t OUT, int32_t K);
+int slg_fc_layer8_bwd(const uint8_t* codes, const float* rows, int64_t B, int64_t IN, int64_t OUT,
+                      int32_t K, const int32_t* cand, const float* w, const float* kept,
+                      int32_t node_kind, float inv_tau, const float* gy, float* gx, float* gconn,
+                      float* graw, float* workspace, int64_t workspace_floats, slg_stream_t stream);
+
 /* GroupSum.forward (silogic/heads.py:34-39): x [B,W] -> logits [B,C] =
  * sum over class block of (ste ? (x > 0.5) : x), divided by tau. */
 int slg_groupsum_soft(const float* x, int64_t B, int64_t W, int32_t C, float tau,

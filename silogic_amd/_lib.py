@@ -59,6 +59,11 @@ SIGNATURES = {
     "slg_fc_soft_bwd8_workspace": (_I64, [_I64, _I64, _I64, _I32]),
     "slg_fc_soft_bwd8": (C.c_int, [_P, _P, _I64, _I64, _I64, _I32, _P, _P, _I32, _P, _F32, _P, _P, _P,
                                    _P, _P, _I64, _P]),
+    "slg_fc_layer8_fwd": (C.c_int, [_P, _I64, _I64, _I64, _I32, _P, _P, _P, _I32, _F32, _P, _P, _P, _P,
+                                    _P, _P]),
+    "slg_fc_layer8_bwd_workspace": (_I64, [_I64, _I64, _I64, _I32]),
+    "slg_fc_layer8_bwd": (C.c_int, [_P, _P, _I64, _I64, _I64, _I32, _P, _P, _P, _I32, _F32, _P, _P, _P,
+                                    _P, _P, _I64, _P]),
     "slg_token_encode": (C.c_int, [_P, _I32, _I64, _I64, _I64, _I64, _P, _I32, _F32, _I32, _P, _P]),
     "slg_token_encode_bwd_workspace": (_I64, [_I64, _I64, _I64]),
     "slg_token_encode_bwd": (C.c_int, [_P, _I32, _I64, _I64, _I64, _I64, _P, _I32, _F32, _P, _P, _P,

@@ -20,8 +20,8 @@ def pack_rows8(x):
     ops.require_gpu(x)
     if x.dim() != 2 or x.shape[1] < 1 or not x.dtype.is_floating_point:
         raise ValueError(f"pack_rows8: {x.dtype} {tuple(x.shape)}, floating [B, D] expected")
-    codes, rows = ops.rows8_pack(ops._as_f32(x.detach()))
-    return codes[:, :x.shape[1]], rows
+    codes, rows = ops.rows8_pack(ops._as_f32(x))
+    return codes if codes.shape[1] == x.shape[1] else codes[:, :x.shape[1]], rows
 
 
 def unpack_rows8(codes, rows):

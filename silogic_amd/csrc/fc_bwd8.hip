@@ -313,4 +313,45 @@ int slg_fc_soft_bwd8(const uint8_t* codes, const float* rows, int64_t B, int64_t
   return 0;
 }
 
+int slg_fc_layer8_fwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t K, const int32_t* cand,
+                      const float* conn, const float* raw, int32_t node_kind, float inv_tau, float* y,
+                      uint8_t* codes, float* rows, float* w, float* kept, slg_stream_t stream) {
+  SLG_REQUIRE(cand && raw && w && kept, SLG_E_ARG, "fc_layer8_fwd: null pointer");
+  SLG_REQUIRE(node_kind == SLG_NODE_GATE16 || node_kind == SLG_NODE_WALSH ||
+                  node_kind == SLG_NODE_MULTILINEAR2,
+              SLG_E_ARG, "fc_layer8_fwd: node_kind %d", node_kind);
+  SLG_REQUIRE(K >= 1 && K <= 16 && OUT > 0 && OUT < (1LL << 28) && 2 * OUT * K < (1LL << 31), SLG_E_SHAPE,
+              "fc_layer8_fwd: OUT %lld, K %d", (long long)OUT, K);
+  const int32_t one = 1;
+  const int rc = slg_layer_params(conn, 2 * OUT, K, 1, &raw, &one, OUT, node_kind, 2, 1.0f, w, kept,
+                                  node_kind == SLG_NODE_GATE16 ? kept + 4 * OUT : nullptr, stream);
+  return rc ? rc : slg_fc_soft_fwd8(x, B, IN, OUT, K, cand, w, node_kind, kept, inv_tau, y, codes, rows, stream);
+}
+
+int64_t slg_fc_layer8_bwd_workspace(int64_t B, int64_t IN, int64_t OUT, int32_t K) {
+  const int64_t n = slg_fc_soft_bwd8_workspace(B, IN, OUT, K);
+  return n < 0 ? n : n + ((2 * OUT * K + 3) & ~int64_t(3)) + 4 * OUT;
+}
+
+int slg_fc_layer8_bwd(const uint8_t* codes, const float* rows, int64_t B, int64_t IN, int64_t OUT, int32_t K,
+                      const int32_t* cand, const float* w, const float* kept, int32_t node_kind, float inv_tau,
+                      const float* gy, float* gx, float* gconn, float* graw, float* workspace,
+                      int64_t workspace_floats, slg_stream_t stream) {
+  SLG_REQUIRE(kept && workspace, SLG_E_ARG, "fc_layer8_bwd: null pointer");
+  SLG_REQUIRE(bwd8_takes(B, IN, OUT, K), SLG_E_SHAPE, "fc_layer8_bwd: B %lld, IN %lld, OUT %lld, K %d",
+              (long long)B, (long long)IN, (long long)OUT, K);
+  const int64_t own = ((2 * OUT * K + 3) & ~int64_t(3)) + 4 * OUT;  // the weights' and node parameters' gradients
+  float* gn = workspace;
+  float* gw = gn + 4 * OUT;
+  int rc = slg_fc_soft_bwd8(codes, rows, B, IN, OUT, K, cand, w, node_kind, kept, inv_tau, gy, gx,
+                            gconn ? gw : nullptr, graw ? gn : nullptr, workspace + own, workspace_floats - own,
+                            stream);
+  if (rc || (!gconn && !graw)) return rc;
+  const int32_t one = 1;
+  // gate16 kept its probabilities behind the coefficients; walsh needs neither
+  const float* from = node_kind == SLG_NODE_GATE16 ? kept + 4 * OUT : node_kind == SLG_NODE_WALSH ? nullptr : kept;
+  return slg_layer_params_bwd(w, gconn ? gw : nullptr, 2 * OUT, K, 1, &one, OUT, node_kind, 2, 1.0f, from,
+                              graw ? gn : nullptr, gconn, &graw, stream);
+}
+
 }  // extern "C"

@@ -1070,6 +1070,26 @@ static int fc_soft_wide(const SoftArgs& a, int node_kind, hipStream_t st) {
   return SLG_E_ARG;
 }
 
+static int fc_soft_dispatch(SoftArgs a, int node_kind, hipStream_t st);
+
+// The layer and its input in 8 bits: from the staged tiles where they hold the
+// codes' 4 samples or more. Narrower tiles would write them in bytes or
+// halves from two workgroups (16380 -> 16380, K = 4, B = 1024: 72 us and a
+// backward 20 us longer, against 51 + 25 us with the pack by itself); then
+// the pack comes second, so that the backward finds the codes in the caches.
+static int fc_soft_dispatch8(const SoftArgs& a, int node_kind, hipStream_t st) {
+  const Rows8Out po = a.po;
+  SoftArgs b = a;
+  const bool beside = pick_tile(a.IN, 0, a.B) < 4;
+  if (beside) b.po = Rows8Out{};
+  const int rc = fc_soft_dispatch(b, node_kind, st);
+  if (rc == 0 && beside && a.B > 0) {
+    rows8_pack(a.x, a.B, a.IN, po.codes, po.rows, st);
+    SLG_LAUNCH_CHECK("fc_soft_fwd8 pack");
+  }
+  return rc;
+}
+
 static int fc_soft_dispatch(SoftArgs a, int node_kind, hipStream_t st) {
   const ParamView& v = a.pv;
   const bool head = a.hd.logits != nullptr;
@@ -1089,16 +1109,11 @@ static int fc_soft_dispatch(SoftArgs a, int node_kind, hipStream_t st) {
   if (a.S == 0 && pick_tile(a.IN, 0) == 0) {  // rows wider than LDS: slab staging
     SLG_REQUIRE(!head, SLG_E_UNSUPPORTED, "fc_soft: the fused GroupSum needs IN <= %lld",
                 (long long)(device_lds_bytes() / 4));
-    if (a.po.codes) rows8_pack(a.x, a.B, a.IN, a.po.codes, a.po.rows, st);
     return fc_soft_wide(a, node_kind, st);
   }
   a.S = pick_tile(a.IN, a.S, a.B);
   SLG_REQUIRE(a.S > 0 && (int64_t)a.IN * a.S * 4 <= device_lds_bytes(), SLG_E_SHAPE,
               "fc_soft: IN=%lld does not fit LDS", (long long)a.IN);
-  if (a.po.codes && a.S < 4) {  // the codes' words are tiles of 4 samples
-    rows8_pack(a.x, a.B, a.IN, a.po.codes, a.po.rows, st);
-    a.po.codes = nullptr;
-  }
   a.threads = pick_threads(a.IN, a.S, a.threads);
   SLG_REQUIRE(a.threads % 64 == 0 && a.threads <= 1024, SLG_E_ARG, "fc_soft: threads=%d", a.threads);
   if (head) {
@@ -1393,7 +1408,7 @@ int slg_fc_soft_fwd8(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t
   SoftArgs a{x, B, IN, OUT, K, arrays_view(cand, cand + K, 2 * K, w, w + K, 2 * K, node_param),
              inv_tau, out, 0, 0, HeadArgs{nullptr, 0, 0, 1.0f},
              Rows8Out{reinterpret_cast<uint32_t*>(codes), rows, (int)rows8_ld(IN)}};
-  return fc_soft_dispatch(a, node_kind, as_stream(stream));
+  return fc_soft_dispatch8(a, node_kind, as_stream(stream));
 }
 
 int slg_dense_logic_fwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t K,

@@ -54,9 +54,9 @@ inline RadixPlan radix_plan(int64_t N, int64_t nkeys) {
   const int most = N <= kRadixSmall ? kRadixSmallBits : kRadixBits;
   p.passes = (key + most - 1) / most;
   p.bits = (key + p.passes - 1) / p.passes;
-  // short rounds spread few entries over more CUs; past 64 workgroups longer
+  // short rounds spread few entries over more CUs; past 256 workgroups longer
   // ones keep the counts that every workgroup reads few
-  p.items = N <= 64 * 4 * kRadixThreads ? 4 : 8;
+  p.items = N <= 256 * 4 * kRadixThreads ? 4 : 8;
   const int64_t round = (int64_t)p.items * kRadixThreads;
   p.tile = std::max<int64_t>(1, cdiv(N, 256 * round)) * round;
   p.blocks = (int)std::max<int64_t>(1, cdiv(N, p.tile));
@@ -196,14 +196,21 @@ radix_count_kernel(Src src, const int2* __restrict__ in, RadixPlan p, int shift,
   for (int d = threadIdx.x; d < R; d += kRadixThreads) cnt[d] = 0;
   __syncthreads();
   const int64_t i0 = blockIdx.x * p.tile, i1 = min(p.N, i0 + p.tile);
-  for (int64_t i = i0 + threadIdx.x; i < i1; i += 4 * kRadixThreads) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t i = i0 + threadIdx.x - lane; i < i1; i += 4 * kRadixThreads) {  // whole waves
     int k[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      k[u] = i + u * kRadixThreads < i1 ? radix_entry(src, in, i + u * kRadixThreads).x : -1;
+    for (int u = 0; u < 4; ++u) {
+      const int64_t at = i + u * kRadixThreads + lane;
+      k[u] = at < i1 ? radix_entry(src, in, at).x : -1;
+    }
+    // peers count once: after the first pass neighbours share their digits
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (k[u] >= 0) atomicAdd(&cnt[(k[u] >> shift) & (R - 1)], 1);
+    for (int u = 0; u < 4; ++u) {
+      const int d = (k[u] >> shift) & (R - 1);
+      const uint64_t m = radix_peers(d, p.bits, k[u] >= 0);
+      if (k[u] >= 0 && __ffsll((unsigned long long)m) - 1 == lane) atomicAdd(&cnt[d], __popcll(m));
+    }
   }
   __syncthreads();
   for (int d = threadIdx.x; d < R; d += kRadixThreads) hist[(int64_t)d * p.nbp + blockIdx.x] = cnt[d];

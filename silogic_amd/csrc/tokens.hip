@@ -58,13 +58,13 @@ __device__ inline float tok_value(float e, float nlog2, bool ste) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(e * nlog2));
 }
 
-// scale * sigmoid'(scale e), from exp(-|z|): no difference of values near 1.
+// scale * sigmoid'(scale e) = scale t / (1 + t)^2, t = exp(-|scale e|): no
+// difference of values near 1; exp2 and reciprocal as above (with expf and a
+// division the writes of short runs took as long as their loads).
 __device__ inline float tok_slope(float e, float scale) {
-  const float t = expf(-fabsf(scale * e)), u = 1.0f + t;
-  return scale * (t / (u * u));
+  const float t = __builtin_amdgcn_exp2f(-fabsf(e * (scale * 1.44269504f))), r = __builtin_amdgcn_rcpf(1.0f + t);
+  return scale * (t * r) * r;
 }
-
-typedef float f32x4t __attribute__((ext_vector_type(4)));
 
 // VU values of a table's row, or of a gradient's.
 template <int DT, int VU>
@@ -75,18 +75,21 @@ __device__ inline void tab_load(const typename TabType<DT>::t* __restrict__ p, f
 #pragma unroll
   for (int j = 0; j < VU; ++j) v[j] = tab_get<DT>(VU == 1 ? ((const T*)&r)[0] : r[j]);
 }
-template <int DT, int VU>
+template <int DT, int VU, bool NT = false>
 __device__ inline void tab_store(typename TabType<DT>::t* __restrict__ p, const float (&v)[VU]) {
   using T = typename TabType<DT>::t;
   typedef T Vt __attribute__((ext_vector_type(VU)));
   Vt r;
 #pragma unroll
   for (int j = 0; j < VU; ++j) r[j] = tab_put<DT>(v[j]);
-  *reinterpret_cast<Vt*>(p) = r;
+  if constexpr (NT) __builtin_nontemporal_store(r, reinterpret_cast<Vt*>(p));
+  else *reinterpret_cast<Vt*>(p) = r;
 }
 
 // A thread takes kEncUnits units of VU values of one token (D a multiple of
-// VU), a workgroup's units next to each other. upr: units per row. Idx: the
+// VU), a workgroup's units next to each other. The values stream past the
+// caches, which are left to the table's rows (524288 tokens of 128 values, 25.6
+// MB of table: 55 against 68 us). upr: units per row. Idx: the
 // type that counts units.
 constexpr int kEncUnits = 4;
 template <int DT, typename IdT, int VU, typename Idx>
@@ -113,7 +116,7 @@ tok_encode_kernel(const IdT* __restrict__ ids, Idx units, Idx upr, int V, int64_
         float v[VU];
 #pragma unroll
         for (int j = 0; j < VU; ++j) v[j] = r[k] < V ? tok_value(e[k][j], nlog2, ste != 0) : 0.0f;
-        tab_store<kTabF32, VU>(y + (int64_t)(u0 + k * 256) * VU, v);
+        tab_store<kTabF32, VU, true>(y + (int64_t)(u0 + k * 256) * VU, v);
       }
     }
   }
@@ -138,39 +141,40 @@ struct SegArgs {
 };
 
 template <int DT, int VU>
-__device__ inline void seg_write(const SegArgs& a, int v, int d, const float (&sum)[VU],
-                                 const typename TabType<DT>::t* __restrict__ tab,
+__device__ inline void seg_write(const SegArgs& a, int v, int d, const float (&sum)[VU], const float (&e)[VU],
                                  typename TabType<DT>::t* __restrict__ gtab) {
-  const int64_t at = (int64_t)v * a.D + d;
-  float e[VU], g[VU];
-  tab_load<DT, VU>(tab + at, e);
+  float g[VU];
 #pragma unroll
   for (int j = 0; j < VU; ++j) g[j] = sum[j] * tok_slope(e[j], a.scale);
-  tab_store<DT, VU>(gtab + at, g);
+  tab_store<DT, VU>(gtab + (int64_t)v * a.D + d, g);
 }
 
 // G lanes sum a chunk of C entries, VU columns each, kSegAhead rows of the
-// gradient in flight. A run of one row inside the chunk is written; one that
-// the chunk before it began goes to edge[0][chunk], one that begins here and
-// goes on to edge[1][chunk] and on the list of tok_join_kernel (whose order
-// does not matter: every run is summed by itself).
-constexpr int kSegAhead = 8;
+// gradient in flight together with the table's rows that the runs ending among
+// them are multiplied by. A run of one row inside the chunk is written; one
+// that the chunk before it began goes to edge[0][chunk], one that begins here
+// and goes on to edge[1][chunk] and on the list of tok_join_kernel (whose
+// order does not matter: every run is summed by itself), to which a workgroup
+// adds its runs at once (one atomic a run on one address took most of the
+// kernel: 17 us at 65536 tokens of 64 values).
+constexpr int kSegAhead = 4;
 template <int DT, int VU>
-__global__ void __launch_bounds__(256, 4)
+__global__ void __launch_bounds__(256)
 tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict__ gy,
                    const typename TabType<DT>::t* __restrict__ tab,
                    typename TabType<DT>::t* __restrict__ gtab, float* __restrict__ edge,
                    int* __restrict__ list, int* __restrict__ listed) {
+  __shared__ int runs[256], n_runs, at_list;
+  if (threadIdx.x == 0) n_runs = 0;
+  __syncthreads();
   const int per = 256 / a.G, l = threadIdx.x % a.G;
   const int64_t c = (int64_t)blockIdx.x * per + threadIdx.x / a.G;
-  if (c >= a.chunks) return;
-  const int64_t i0 = c * a.C, i1 = min(a.N, i0 + a.C);
+  const int64_t i0 = min(c * a.C, a.N - 1), i1 = min(a.N, c * a.C + a.C);
   const int first = ent[i0].x;
-  if (first >= a.V) return;  // absent tokens to the end
   const bool begun = i0 > 0 && ent[i0 - 1].x == first;
   const int after = i1 < a.N ? ent[i1].x : -1;
-  for (int d = l * VU; d < a.D; d += a.G * VU) {
-    int row = first;
+  // absent tokens from the chunk's start to the end: nothing
+  for (int d = c < a.chunks && first < a.V ? l * VU : a.D; d < a.D; d += a.G * VU) {
     bool from_before = begun;
     float sum[VU];
 #pragma unroll
@@ -178,9 +182,10 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
     int2 next[kSegAhead];  // the next rows' entries, a batch ahead of their gradients
 #pragma unroll
     for (int u = 0; u < kSegAhead; ++u) next[u] = ent[min(i0 + u, i1 - 1)];
-    for (int64_t i = i0; i < i1 && row < a.V; i += kSegAhead) {
+    for (int64_t i = i0; i < i1; i += kSegAhead) {
       int2 e[kSegAhead];
-      float g[kSegAhead][VU];
+      float g[kSegAhead][VU], t[kSegAhead][VU];
+      bool ends[kSegAhead];
 #pragma unroll
       for (int u = 0; u < kSegAhead; ++u) {
         e[u] = next[u];
@@ -190,31 +195,40 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
       for (int u = 0; u < kSegAhead; ++u) next[u] = ent[min(i + kSegAhead + u, i1 - 1)];
 #pragma unroll
       for (int u = 0; u < kSegAhead; ++u) {
-        if (i + u >= i1) break;
-        if (e[u].x != row) {
+        const int64_t at = i + u + 1;
+        const int then = at < i1 ? (u + 1 < kSegAhead ? e[(u + 1) % kSegAhead].x : next[0].x) : after;
+        ends[u] = i + u < i1 && e[u].x < a.V && e[u].x != then;
+        if (ends[u]) tab_load<DT, VU>(tab + (int64_t)e[u].x * a.D + d, t[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kSegAhead; ++u) {
+        if (i + u >= i1 || e[u].x >= a.V) break;
+#pragma unroll
+        for (int j = 0; j < VU; ++j) sum[j] += g[u][j];
+        if (ends[u]) {
           if (from_before) tab_store<kTabF32, VU>(edge + c * a.D + d, sum);
-          else if (row < a.V) seg_write<DT, VU>(a, row, d, sum, tab, gtab);
-          row = e[u].x;
+          else seg_write<DT, VU>(a, e[u].x, d, sum, t[u], gtab);
           from_before = false;
 #pragma unroll
           for (int j = 0; j < VU; ++j) sum[j] = 0.0f;
         }
-        if (row < a.V) {
-#pragma unroll
-          for (int j = 0; j < VU; ++j) sum[j] += g[u][j];
-        }
+      }
+      if (e[kSegAhead - 1].x >= a.V) break;
+    }
+    const int row = ent[i1 - 1].x;
+    if (row < a.V && after == row) {  // the last run goes on
+      if (from_before) {
+        tab_store<kTabF32, VU>(edge + c * a.D + d, sum);
+      } else {
+        tab_store<kTabF32, VU>(edge + (a.chunks + c) * a.D + d, sum);
+        if (d == 0) runs[atomicAdd(&n_runs, 1)] = (int)c;
       }
     }
-    if (row >= a.V) continue;
-    if (from_before) {
-      tab_store<kTabF32, VU>(edge + c * a.D + d, sum);
-    } else if (after == row) {
-      tab_store<kTabF32, VU>(edge + (a.chunks + c) * a.D + d, sum);
-      if (d == 0) list[atomicAdd(listed, 1)] = (int)c;
-    } else {
-      seg_write<DT, VU>(a, row, d, sum, tab, gtab);
-    }
   }
+  __syncthreads();
+  if (threadIdx.x == 0) at_list = n_runs ? atomicAdd(listed, n_runs) : 0;
+  __syncthreads();
+  for (int k = threadIdx.x; k < n_runs; k += 256) list[at_list + k] = runs[k];
 }
 
 // The runs that cross chunks, a workgroup each: G lanes a row, the chunks'
@@ -275,12 +289,13 @@ tok_join_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict
       for (int j = 0; j < VU; ++j) red[(part * a.G + l) * VU + j] = sum[j];
       __syncthreads();
       if (part == 0 && d < a.D) {
-        float s[VU];
+        float s[VU], e[VU];
         tab_load<kTabF32, VU>(edge + (a.chunks + c) * a.D + d, s);
+        tab_load<DT, VU>(tab + (int64_t)row * a.D + d, e);
         for (int p = 0; p < P; ++p)
 #pragma unroll
           for (int j = 0; j < VU; ++j) s[j] += red[(p * a.G + l) * VU + j];
-        seg_write<DT, VU>(a, row, d, s, tab, gtab);
+        seg_write<DT, VU>(a, row, d, s, e, gtab);
       }
       __syncthreads();
     }
@@ -346,31 +361,47 @@ __device__ inline uint64_t wave_transpose(uint64_t m) {
   return (uint64_t)hi << 32 | lo;
 }
 
-// Bits packed 64 samples a word. A wave takes 64 samples' word dw of token l
-// and transposes it: lane j then holds feature j's word. Word-major rows of
-// features are written as they are; for the rows [F][nw] a workgroup's waves
-// take TW neighbouring words, which leave through LDS in runs of TW.
+// Bits packed 64 samples a word. A wave takes 64 samples' word dw of kPackTokens
+// neighbouring tokens (whose ids share memory lines) and transposes each: lane
+// j then holds feature j's word. Word-major rows of features are written as
+// they are; for the rows [F][nw] a workgroup's waves take TW neighbouring
+// words, which leave through LDS in runs of TW.
+constexpr int kPackTokens = 4;
 template <typename IdT, bool WM, int TW>
 __global__ void __launch_bounds__(64 * TW)
 tok_packed_kernel(const IdT* __restrict__ ids, int64_t B, int64_t L, int V, int64_t pad, int D, int DW,
                   int64_t nw, const uint64_t* __restrict__ bits, uint64_t* __restrict__ out) {
-  __shared__ uint64_t tile[WM ? 1 : 64][WM ? 1 : TW + 1];
+  __shared__ uint64_t tile[WM ? 1 : kPackTokens][WM ? 1 : 64][WM ? 1 : TW + 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t F = L * D, wt = (nw + TW - 1) / TW, jobs = wt * L * DW;
+  const int64_t F = L * D, wt = (nw + TW - 1) / TW, lt = (L + kPackTokens - 1) / kPackTokens, jobs = wt * lt * DW;
   for (int64_t k = blockIdx.x; k < jobs; k += gridDim.x) {
-    const int64_t t = k / (L * DW), r = k - t * (L * DW), l = r / DW;
-    const int dw = (int)(r - l * DW);
+    const int64_t t = k / (lt * DW), r = k - t * (lt * DW), l0 = r / DW * kPackTokens;
+    const int dw = (int)(r % DW);
     const int64_t w = t * TW + wave, b = w * 64 + lane;
-    const int row = b < B ? tok_row(ids, b * L + l, V, pad) : V;
-    const uint64_t m = wave_transpose(row < V ? bits[(int64_t)row * DW + dw] : 0ull);
+    int row[kPackTokens];
+    uint64_t m[kPackTokens];
+#pragma unroll
+    for (int u = 0; u < kPackTokens; ++u)
+      row[u] = b < B && l0 + u < L ? tok_row(ids, b * L + l0 + u, V, pad) : V;
+#pragma unroll
+    for (int u = 0; u < kPackTokens; ++u) m[u] = row[u] < V ? bits[(int64_t)row[u] * DW + dw] : 0ull;
     const int d = dw * 64 + lane;
-    if constexpr (WM) {
-      if (w < nw && d < D) out[w * F + l * D + d] = m;
-    } else {
-      tile[lane][wave] = m;
+#pragma unroll
+    for (int u = 0; u < kPackTokens; ++u) {
+      const uint64_t v = wave_transpose(m[u]);
+      if constexpr (WM) {
+        if (w < nw && d < D && l0 + u < L) out[w * F + (l0 + u) * D + d] = v;
+      } else {
+        tile[u][lane][wave] = v;
+      }
+    }
+    if constexpr (!WM) {
       __syncthreads();
       const int j = threadIdx.x / TW, i = threadIdx.x % TW;
-      if (t * TW + i < nw && dw * 64 + j < D) out[(l * D + dw * 64 + j) * nw + t * TW + i] = tile[j][i];
+      if (t * TW + i < nw && dw * 64 + j < D)
+#pragma unroll
+        for (int u = 0; u < kPackTokens; ++u)
+          if (l0 + u < L) out[((l0 + u) * D + dw * 64 + j) * nw + t * TW + i] = tile[u][j][i];
       __syncthreads();
     }
   }
@@ -418,7 +449,7 @@ static TokBwdPlan tok_bwd_plan(int64_t N, int64_t V, int64_t D) {
   p.G = 1;
   while (p.G < 64 && p.G * p.VU < D) p.G *= 2;
   p.C = 64;
-  while (p.C > 16 && cdiv(N, p.C) * p.G < 131072) p.C /= 2;
+  while (p.C > 8 && cdiv(N, p.C) * p.G < 131072) p.C /= 2;
   p.chunks = cdiv(N, p.C);
   p.edge = (2 * p.chunks * D + 3) & ~int64_t(3);
   p.list = p.chunks + 1;
@@ -550,7 +581,7 @@ int slg_token_encode_hard(const void* ids, int32_t id_bytes, int64_t B, int64_t 
       return;
     }
     auto go = [&](auto kern, int tw) {
-      hipLaunchKernelGGL(kern, dim3(grid_of(cdiv(nw, tw) * L * DW)), dim3(64 * tw), 0, st, id, B, L, (int)V, pad,
+      hipLaunchKernelGGL(kern, dim3(grid_of(cdiv(nw, tw) * cdiv(L, kPackTokens) * DW)), dim3(64 * tw), 0, st, id, B, L, (int)V, pad,
                          (int)D, (int)DW, nw, bits, static_cast<uint64_t*>(out));
     };
     if (layout == 1) go(tok_packed_kernel<Id, true, 4>, 4);

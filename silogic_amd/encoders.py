@@ -3,7 +3,7 @@
 import torch
 import torch.nn as nn
 
-from . import _lib, derived, ops
+from . import _lib, ops
 from .data import _encode
 
 
@@ -72,13 +72,13 @@ class _TokenFn(torch.autograd.Function):
     def forward(ctx, ids, table, scale, ste, pad):
         ctx.save_for_backward(ids, table)
         ctx.meta = (scale, pad)
-        return ops.token_encode(ids, table.detach(), scale, ste, pad)
+        return ops.token_encode(ids, table, scale, ste, pad)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
         ids, table = ctx.saved_tensors
-        return None, ops.token_encode_bwd(ids, table.detach(), *ctx.meta, gy), None, None, None
+        return None, ops.token_encode_bwd(ids, table, *ctx.meta, gy), None, None, None
 
 
 class TokenEncoder(nn.Module):
@@ -127,57 +127,65 @@ class TokenEncoder(nn.Module):
     def _pad(self):
         return -1 if self.padding_idx is None else self.padding_idx
 
-    def _ids(self, ids):
+    def _ids(self, ids, weight):
+        """``ids`` as ``[B, L]``, checked against ``weight``."""
         if ids.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"TokenEncoder: ids of {ids.dtype} (int32 or int64)")
         if ids.dim() not in (1, 2):
             raise ValueError(f"TokenEncoder: ids {tuple(ids.shape)}, [B] or [B, L] expected")
-        if self.weight.dtype not in ops.TABLE_DTYPES:
-            raise TypeError(f"TokenEncoder: weight of {self.weight.dtype} (fp32, bf16 or fp16)")
-        ops.require_gpu(ids, self.weight)
-        ops.same_device("TokenEncoder", ids, self.weight)
+        if weight.dtype not in ops.TABLE_DTYPES:
+            raise TypeError(f"TokenEncoder: weight of {weight.dtype} (fp32, bf16 or fp16)")
+        ops.require_gpu(ids, weight)
+        ops.same_device("TokenEncoder", ids, weight)
         return ops._c(ids if ids.dim() == 2 else ids.unsqueeze(1))
 
     def forward(self, ids):
-        ids = self._ids(ids)
+        w = self.weight
+        ids = self._ids(ids, w)
         if torch.compiler.is_compiling():
-            return torch.ops.silogic_hip.token_encode(ids, self.weight, self.scale, self.ste, self._pad)
-        w = ops._c(self.weight)
+            return torch.ops.silogic_hip.token_encode(ids, w, self.scale, self.ste, self._pad)
+        w = ops._c(w)
         if not ops._grad_path(w):
             return ops.token_encode(ids, w, self.scale, self.ste, self._pad)
         return _TokenFn.apply(ids, w, self.scale, self.ste, self._pad)
 
-    def _bit_table(self):
-        """Bit words of the weight, made once per version of it. Another stream
-        than the one that made them waits for them; a captured call that finds
-        none of its own stream makes them inside the graph."""
-        w, here = self.weight.detach(), torch.cuda.current_stream(self.weight.device)
+    def _bit_table(self, weight):
+        """Bit words of the weight, made once per version of it (its storage and
+        version counter, as ``derived`` keys tables; ``derived.clear`` drops
+        them). Another stream than the one that made them waits for them; a
+        captured call that finds none of its own stream makes them inside the
+        graph, so that a replay reads the weight afresh."""
+        here = ops._stream(weight).value
+        slot = self.__dict__.get("_derived_bits")
+        if slot is not None and slot[0] == (weight.data_ptr(), weight._version):
+            if slot[1] == here:
+                return slot[2]
+        else:
+            slot = None
+        w = weight.detach()
         if torch.cuda.is_current_stream_capturing():
-            slot = self.__dict__.get("_derived_bits")
-            if slot is not None and slot[0] == derived.state_key(self) and slot[1][2] == here:
-                return slot[1][1]
             return ops.token_bits(ops._c(w))
-
-        def build():
+        stream = torch.cuda.current_stream(w.device)
+        if slot is None:
             bits = ops.token_bits(ops._c(w))
-            return w, bits, here, here.record_event()   # w: its address stays taken while the key holds it
+            # w itself: its address stays taken while the key holds it
+            self._derived_bits = ((w.data_ptr(), w._version), here, bits, stream.record_event(), w)
+            return bits
+        stream.wait_event(slot[3])
+        slot[2].record_stream(stream)
+        return slot[2]
 
-        _, bits, there, done = derived.cached(self, "_derived_bits", derived.state_key(self), build)
-        if there != here:
-            here.wait_event(done)
-            bits.record_stream(here)
-        return bits
+    def _hard(self, ids, layout):
+        w = self.weight
+        ids = self._ids(ids, w)
+        return ops.token_encode_hard(ids, self._bit_table(w), self.bits, self._pad, layout)
 
-    @torch.no_grad()
     def forward_hard(self, ids):
         """uint8 bits ``[B, L*bits]``."""
-        ids = self._ids(ids)
-        return ops.token_encode_hard(ids, self._bit_table(), self.bits, self._pad, 2)
+        return self._hard(ids, 2)
 
-    @torch.no_grad()
     def forward_packed(self, ids, word_major=False):
         """The bits of :meth:`forward_hard` packed 64 samples per word:
         ``[L*bits, nw]`` (``word_major``: ``[nw, L*bits]``), the input of
         ``LogicNet.forward_hard_packed``."""
-        ids = self._ids(ids)
-        return ops.token_encode_hard(ids, self._bit_table(), self.bits, self._pad, int(word_major))
+        return self._hard(ids, 1 if word_major else 0)

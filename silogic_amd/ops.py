@@ -94,8 +94,7 @@ def same_device(what, *ts):
 # ---------------------------------------------------------------------------
 def _rows8_empty(x):
     B, D = x.shape
-    return (torch.empty((-(-B // 4), (D + 3) // 4 * 4, 4), device=x.device, dtype=torch.uint8),
-            torch.empty((B, 2), device=x.device, dtype=torch.float32))
+    return x.new_empty(((B + 3) // 4, (D + 3) // 4 * 4, 4), dtype=torch.uint8), x.new_empty((B, 2))
 
 
 def rows8_pack(x):
@@ -110,7 +109,7 @@ def rows8_pack(x):
 def rows8_unpack(codes, rows, D):
     """The values that the codes stand for, ``[B, D]`` fp32."""
     B = rows.shape[0]
-    x = torch.empty((B, D), device=codes.device, dtype=torch.float32)
+    x = rows.new_empty((B, D))
     call_on(codes, "slg_rows8_unpack", _p(codes), _p(rows), B, D, _p(x))
     return x
 
@@ -353,17 +352,26 @@ def fc_soft8_fwd(x, cand, w, npar, node_kind, inv_tau):
     return y, codes, rows
 
 
-def fc_layer8_fwd(x, cand, conn, raw, node_kind, inv_tau):
-    """``(y, codes, rows, w, kept)`` of a gate layer from its own parameters
-    (``w``, ``kept`` as :func:`layer_params` returns them)."""
+def _layer8_args(x, cand, conn, raw, node_kind):
+    """The arguments as the kernels read them, and ``(B, IN, OUT, K)``."""
     require_gpu(x, cand, conn, raw)
     same_device("fc_layer8", x, cand, conn, raw)
     check_layer8(x, cand, conn=(conn, cand.shape),
                  raw=(raw, (cand.shape[0], 16 if node_kind == GATE16 else 4)))
-    x, cand = _as_f32(x), _c(cand, torch.int32)
-    w, kept = layer_params(conn, tuple(cand.shape), [raw], node_kind, 2)
-    npar = kept[:cand.shape[0]] if node_kind == GATE16 else kept
-    return (*fc_soft8_fwd(x, cand, w, npar, node_kind, inv_tau), w, kept)
+    return (_as_f32(x), _c(cand, torch.int32), _c(conn, torch.float32), _quads(_c(raw, torch.float32)),
+            (*x.shape, cand.shape[0], cand.shape[2]))
+
+
+def fc_layer8_fwd(x, cand, conn, raw, node_kind, inv_tau):
+    """``(y, codes, rows, w, kept)`` of a gate layer from its own parameters
+    (``w``, ``kept`` as :func:`layer_params` returns them)."""
+    x, cand, conn, raw, (B, IN, OUT, K) = _layer8_args(x, cand, conn, raw, node_kind)
+    codes, rows = _rows8_empty(x)
+    y, w = x.new_empty((B, OUT)), x.new_empty(cand.shape)
+    kept = x.new_empty((OUT * (5 if node_kind == GATE16 else 1), 4))
+    call_on(x, "slg_fc_layer8_fwd", _p(x), B, IN, OUT, K, _p(cand), _p(conn), _p(raw), node_kind,
+            float(inv_tau), _p(y), _p(codes), _p(rows), _p(w), _p(kept))
+    return y, codes, rows, w, kept
 
 
 def fc_layer8_bwd(codes, rows, cand, w, kept, in_dim, node_kind, inv_tau, gy, need_x, need_conn,
@@ -377,21 +385,53 @@ def fc_layer8_bwd(codes, rows, cand, w, kept, in_dim, node_kind, inv_tau, gy, ne
 
 
 class _FcLayer8(torch.autograd.Function):
+    """What the backward reads lies in one buffer (codes | rows | w | kept, each
+    at a multiple of 16 bytes): a call's host time is mostly allocations and
+    launches."""
+
     @staticmethod
     def forward(ctx, x, cand, conn, raw, node_kind, inv_tau):
-        y, *saved = fc_layer8_fwd(x.detach(), cand, None if conn is None else conn.detach(),
-                                  raw.detach(), node_kind, inv_tau)
-        ctx.save_for_backward(cand, *saved)
-        ctx.meta = (x.shape[1], node_kind, inv_tau)
+        x, cand, conn, raw, (B, IN, OUT, K) = _layer8_args(x, cand, conn, raw, node_kind)
+        ld, tiles = (IN + 3) // 4 * 4, (B + 3) // 4
+        at = [4 * tiles * ld]                        # rows
+        at.append(at[0] + (8 * B + 15) // 16 * 16)   # w
+        at.append(at[1] + (8 * OUT * K + 15) // 16 * 16)   # kept
+        y = x.new_empty((B, OUT))
+        saved = x.new_empty(at[2] + 16 * OUT * (5 if node_kind == GATE16 else 1), dtype=torch.uint8)
+        p = saved.data_ptr()
+        call_on(x, "slg_fc_layer8_fwd", x.data_ptr(), B, IN, OUT, K, cand.data_ptr(), _p(conn),
+                raw.data_ptr(), node_kind, inv_tau, y.data_ptr(), p, p + at[0], p + at[1], p + at[2])
+        ctx.save_for_backward(cand, saved)
+        ctx.meta = (B, IN, OUT, K, node_kind, inv_tau, at)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
-        cand, codes, rows, w, kept = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        gx, gc, gr = fc_layer8_bwd(codes, rows, cand, w, kept, *ctx.meta, gy, need[0], need[2], need[3])
-        return gx, None, gc, gr, None, None
+        cand, saved = ctx.saved_tensors
+        need_x, _, need_conn, need_raw = ctx.needs_input_grad[:4]
+        B, IN, OUT, K, node_kind, inv_tau, at = ctx.meta
+        P = 16 if node_kind == GATE16 else 4
+        ws = _lib.lib().slg_fc_layer8_bwd_workspace(B, IN, OUT, K)
+        if ws < 0:   # rows too wide for the kernel on codes
+            def part(a, b, dtype, shape):
+                return saved[a:b].view(dtype)[:shape.numel()].view(shape)
+            f32, size = torch.float32, torch.Size
+            gx, gconn, graw = fc_layer8_bwd(
+                part(0, at[0], torch.uint8, size(((B + 3) // 4, (IN + 3) // 4 * 4, 4))),
+                part(at[0], at[1], f32, size((B, 2))), cand, part(at[1], at[2], f32, cand.shape),
+                part(at[2], None, f32, size((OUT * (5 if P == 16 else 1), 4))), IN, node_kind, inv_tau, gy,
+                need_x, need_conn, need_raw)
+            return gx, None, gconn, graw, None, None
+        gy = _c(gy, torch.float32)
+        gx = gy.new_empty((B, IN)) if need_x else None
+        gconn = gy.new_empty((OUT, 2, K)) if need_conn else None
+        graw = gy.new_empty((OUT, P)) if need_raw else None
+        work, p = gy.new_empty(ws), saved.data_ptr()
+        call_on(saved, "slg_fc_layer8_bwd", p, p + at[0], B, IN, OUT, K, cand.data_ptr(), p + at[1],
+                p + at[2], node_kind, inv_tau, gy.data_ptr(), _p(gx), _p(gconn), _p(graw),
+                work.data_ptr(), ws)
+        return gx, None, gconn, graw, None, None
 
 
 class _FcSoft8(torch.autograd.Function):
@@ -450,9 +490,9 @@ def token_encode(ids, table, scale, ste, pad):
     """``ids [B, L]`` int32 / int64, ``table [V, D]`` -> ``[B, L * D]`` fp32
     (``slg_token_encode``)."""
     (B, L), (V, D) = ids.shape, table.shape
-    y = torch.empty((B, L * D), device=table.device, dtype=torch.float32)
-    call_on(table, "slg_token_encode", _p(ids), ids.element_size(), B * L, V, D, pad, _p(table),
-            TABLE_DTYPES[table.dtype], float(scale), int(ste), _p(y))
+    y = table.new_empty((B, L * D), dtype=torch.float32)
+    call_on(table, "slg_token_encode", ids.data_ptr(), ids.element_size(), B * L, V, D, pad,
+            table.data_ptr(), TABLE_DTYPES[table.dtype], scale, ste, y.data_ptr())
     return y
 
 
@@ -461,11 +501,12 @@ def token_encode_bwd(ids, table, scale, pad, gy):
     (B, L), (V, D) = ids.shape, table.shape
     if gy.shape != (B, L * D):
         raise ValueError(f"token_encode_bwd: gradient {tuple(gy.shape)} for {(B, L * D)}")
-    g = torch.empty_like(table)
+    g, gy = torch.empty_like(table), _c(gy, torch.float32)
     ws = _lib.lib().slg_token_encode_bwd_workspace(B * L, V, D)
-    work = torch.empty(max(ws, 1), device=table.device, dtype=torch.int32)
-    call_on(table, "slg_token_encode_bwd", _p(ids), ids.element_size(), B * L, V, D, pad, _p(table),
-            TABLE_DTYPES[table.dtype], float(scale), _p(_c(gy, torch.float32)), _p(g), _p(work), ws)
+    work = table.new_empty(max(ws, 1), dtype=torch.int32)
+    call_on(table, "slg_token_encode_bwd", ids.data_ptr(), ids.element_size(), B * L, V, D, pad,
+            table.data_ptr(), TABLE_DTYPES[table.dtype], scale, gy.data_ptr(), g.data_ptr(),
+            work.data_ptr(), ws)
     return g
 
 
@@ -481,13 +522,13 @@ def token_encode_hard(ids, bits, D, pad, layout):
     """Bits of ``ids [B, L]``'s tokens: layout 0 ``[L*D, nw]``, 1 ``[nw, L*D]``,
     2 uint8 ``[B, L*D]``."""
     B, L = ids.shape
+    nw = n_words(B)
     if layout == 2:
-        out = torch.empty((B, L * D), device=bits.device, dtype=torch.uint8)
+        out = bits.new_empty((B, L * D), dtype=torch.uint8)
     else:
-        nw = n_words(B)
-        out = torch.empty((nw, L * D) if layout else (L * D, nw), device=bits.device, dtype=torch.int64)
-    call_on(bits, "slg_token_encode_hard", _p(ids), ids.element_size(), B, L, bits.shape[0], D, pad,
-            _p(bits), layout, _p(out))
+        out = bits.new_empty((nw, L * D) if layout else (L * D, nw))
+    call_on(bits, "slg_token_encode_hard", ids.data_ptr(), ids.element_size(), B, L, bits.shape[0], D,
+            pad, bits.data_ptr(), layout, out.data_ptr())
     return out
 
 

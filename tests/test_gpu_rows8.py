@@ -285,7 +285,10 @@ def test_network_keeps_bytes_and_its_outputs(node):
         y8 = net(x)
     assert torch.equal(y8, y32)
     assert not any(t.dtype == torch.float32 and t.shape[0] == 30 and t.numel() > 60 for t in saved), "an fp32 input is kept"
-    assert sum(t.numel() for t in saved if t.dtype == torch.uint8) == 8 * 4 * (52 + 60)
+    # codes of whole tiles and quads, an offset and a step a sample, weights and node parameters
+    kept = 5 if node == "gate16" else 1
+    assert sum(t.numel() for t in saved if t.dtype == torch.uint8) == sum(
+        8 * 4 * ld + 8 * 30 + 8 * out * 4 + 16 * out * kept for ld, out in ((52, 60), (60, 40)))
     for a, b in zip(torch.autograd.grad(y8, list(net.parameters()), gy), g32):
         # inputs off by at most span / 510, twice through softmaxes' slopes: a hundredth of the norm
         assert (a - b).norm() < 0.01 * b.norm() + 1e-6
