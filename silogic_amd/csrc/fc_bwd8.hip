@@ -28,15 +28,16 @@ __device__ inline float code_of(uint32_t w, int v) { return (float)((w >> (8 * v
 
 // One output per thread over a range of 4-sample tiles: part and gbr as
 // fc_soft_bwd_w_kernel writes them. AHEAD: two tiles in LDS, the next one's
-// codes on their way in registers (up to kBwd8Quads quads a thread) while this
+// codes on their way in registers (up to bwd8_quads quads a thread) while this
 // one computes, one barrier a tile; else one tile and two barriers.
-constexpr int kBwd8Quads = 3;
+template <int KC>
+constexpr int bwd8_quads() { return KC == 8 ? 3 : KC == 4 ? 5 : 8; }
 template <int NODE, int KC, bool AHEAD>
 __global__ void __launch_bounds__((bwd8_threads<KC>()))
 fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ rows, int B, int IN, int ld,
                  int OUT, int Kr, ParamView pv, float inv_tau, const float* __restrict__ gy, int n_orange,
                  int n_range, int tiles_per_range, float* __restrict__ part, float* __restrict__ gbr) {
-  constexpr int S = kRows8Tile, KM = KC > 0 ? KC : 16;
+  constexpr int S = kRows8Tile, KM = KC > 0 ? KC : 16, NQ = bwd8_quads<KC>();
   extern __shared__ __align__(16) unsigned char smem[];
   const int K = KC > 0 ? KC : Kr;
   // the output ranges of one sample range on one XCD: they stage the same codes
@@ -62,17 +63,17 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
   const int n_tiles = (B + S - 1) / S;
   const int t0 = r_b * tiles_per_range, t_end = min(n_tiles, t0 + tiles_per_range);
   const int vo = valid ? o * 4 : 0x7ffffffc, n4 = ld >> 2, T = blockDim.x;
-  uint4 pf[AHEAD ? kBwd8Quads : 1];
+  uint4 pf[AHEAD ? NQ : 1];
   auto issue = [&](int t) {
     const auto r = uniform_rsrc(codes + (int64_t)t * ld, ld * 4);
 #pragma unroll
-    for (int u = 0; u < kBwd8Quads; ++u)  // zeros past the row
+    for (int u = 0; u < NQ; ++u)  // zeros past the row
       pf[u] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, (threadIdx.x + u * T) * 16, 0, 0));
   };
   auto place = [&](int t) {
     uint4* dst = reinterpret_cast<uint4*>(smem) + (t & 1) * n4;
 #pragma unroll
-    for (int u = 0; u < kBwd8Quads; ++u) {
+    for (int u = 0; u < NQ; ++u) {
       const int q = threadIdx.x + u * T;
       if (q < n4) dst[q] = pf[u];
     }
@@ -85,10 +86,8 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
       g[s] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(gr, vo, 0, 0));
     }
   };
-  float gn[S];
-  if (t0 < t_end) {
-    load_g(t0, gn);
-    if constexpr (AHEAD) {
+  if constexpr (AHEAD) {
+    if (t0 < t_end) {
       issue(t0);
       place(t0);
       __syncthreads();
@@ -100,7 +99,6 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       const int64_t b = min(b0 + s, B - 1);
-      g[s] = gn[s];
       lo[s] = b0 + s < B ? rows[2 * b] : 0.0f;
       step[s] = b0 + s < B ? rows[2 * b + 1] : 0.0f;
     }
@@ -111,9 +109,9 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
       for (int q = threadIdx.x; q < n4; q += T) reinterpret_cast<uint4*>(smem)[q] = src[q];
       __syncthreads();
     }
-    if (t + 1 < t_end) {
-      if constexpr (AHEAD) issue(t + 1);
-      load_g(t + 1, gn);
+    load_g(t, g);  // back by the time the operands are there
+    if constexpr (AHEAD) {
+      if (t + 1 < t_end) issue(t + 1);
     }
     uint32_t qa[KM], qb[KM];
 #pragma unroll
@@ -237,7 +235,8 @@ struct Bwd8Args {
 template <int NODE, int KC>
 static int launch_bwd8(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
   const int64_t ld = rows8_ld(a.IN);
-  const bool ahead = p.tiles_per_range > 1 && ld <= kBwd8Quads * 4 * bwd8_threads<KC>();
+  const bool ahead = p.tiles_per_range > 1 && ld <= bwd8_quads<KC>() * 4 * bwd8_threads<KC>() &&
+                     ld * 8 <= bwd8_lds_cap();
   auto kern = ahead ? fc_bwd8_w_kernel<NODE, KC, true> : fc_bwd8_w_kernel<NODE, KC, false>;
   const size_t lds = (size_t)ld * 4 * (ahead ? 2 : 1);
   if (lds > 65536) {
