@@ -316,8 +316,9 @@ int slg_fc_soft_fwd8(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t
                      const float* node_param, float inv_tau, float* out, uint8_t* codes, float* rows,
                      slg_stream_t stream);
 /* slg_fc_soft_bwd at the values that x's codes stand for. Workspace of
- * slg_fc_soft_bwd8_workspace floats at a multiple of 16 bytes (-1: shape not
- * taken: rows of more than 40960 inputs, K past 16; unpack those). */
+ * slg_fc_soft_bwd8_workspace floats (-1: shape not taken: rows of more than
+ * 40960 inputs, K past 16; unpack those). codes, cand, w, node_param and
+ * workspace at multiples of 16 bytes. */
 int64_t slg_fc_soft_bwd8_workspace(int64_t B, int64_t IN, int64_t OUT, int32_t K);
 int slg_fc_soft_bwd8(const uint8_t* codes, const float* rows, int64_t B, int64_t IN, int64_t OUT,
                      int32_t K, const int32_t* cand, const float* w, int32_t node_kind,

@@ -48,12 +48,13 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
   const int o = r_o * blockDim.x + threadIdx.x;
   const bool valid = o < OUT;
   FcParams<KM> P;
-  load_params<KC, KM, true>(P, min(o, OUT - 1), K, pv);
-  uint32_t pk[KM];  // index pairs (inputs below 65536)
+  load_params<KC, KM, false>(P, min(o, OUT - 1), K, pv);
+  const uint32_t lim = (uint32_t)IN - 1u;
+  uint32_t pk[KM];  // index pairs (inputs below 65536), clamped into the tile
   float Wa = 0.0f, Wb = 0.0f;
 #pragma unroll
   for (int k = 0; k < KM; ++k) {
-    pk[k] = (uint32_t)P.ia[k] | ((uint32_t)P.ib[k] << 16);
+    pk[k] = min((uint32_t)P.ia[k], lim) | (min((uint32_t)P.ib[k], lim) << 16);
     Wa += P.fa[k];
     Wb += P.fb[k];
   }
@@ -188,11 +189,11 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
   }
 }
 
-// Workspace (in 4-byte words): records | partials | operand gradients | input-gradient part.
+// Workspace (in 4-byte words): partials | operand gradients | input-gradient part.
 struct Bwd8Plan {
   int threads, n_orange, NR, tiles_per_range;
-  int64_t rec, part, gbr, in_ws;
-  int64_t total() const { return rec + part + gbr + in_ws; }
+  int64_t part, gbr, in_ws;
+  int64_t total() const { return part + gbr + in_ws; }
 };
 
 static int64_t bwd8_lds_cap() { return std::min<int64_t>(device_lds_bytes(), 160 * 1024); }
@@ -214,7 +215,6 @@ static Bwd8Plan bwd8_plan(int64_t B, int64_t IN, int64_t OUT, int K) {
   p.tiles_per_range = (int)cdiv(n_tiles, p.NR);
   p.NR = (int)cdiv(n_tiles, p.tiles_per_range);
   auto round4 = [](int64_t n) { return (n + 3) & ~int64_t(3); };
-  p.rec = fc_bwd_record_words(OUT, K);
   p.part = round4((int64_t)p.NR * (2 * K + 4) * OUT);
   p.gbr = round4(2 * OUT * n_tiles * kRows8Tile);  // the last tile's rows whole
   p.in_ws = fc_input_grad_floats(B, IN, OUT, 2, K);
@@ -226,7 +226,8 @@ struct Bwd8Args {
   const float* rows;
   int64_t B, IN, OUT;
   int K;
-  const float* rec;
+  const int* cand;
+  const float *w, *np;
   float inv_tau;
   const float* gy;
   float *part, *gbr;
@@ -244,8 +245,9 @@ static int launch_bwd8(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
                                              (int)lds);
     SLG_REQUIRE(e == hipSuccess, (int)e, "fc_soft_bwd8: LDS %zu: %s", lds, hipGetErrorString(e));
   }
-  ParamView pv{};
-  pv.rec = a.rec;
+  // a thread reads its output's parameters once, from where they are: records
+  // (as the fp32 kernels take) would be a launch and 5 us to save less
+  const ParamView pv{a.cand, a.cand + a.K, a.w, a.w + a.K, a.np, 2 * a.K, 2 * a.K, 4, nullptr};
   hipLaunchKernelGGL(kern, dim3((unsigned)(cdiv((int64_t)p.n_orange * p.NR, 8) * 8)), dim3(bwd8_threads<KC>()),
                      lds, st, a.codes, a.rows, (int)a.B, (int)a.IN, (int)ld, (int)a.OUT, a.K, pv,
                      a.inv_tau, a.gy, p.n_orange, p.NR, p.tiles_per_range, a.part, a.gbr);
@@ -255,7 +257,7 @@ static int launch_bwd8(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
 
 template <int NODE>
 static int launch_bwd8_k(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
-  if (a.K == 8) return launch_bwd8<NODE, 8>(a, p, st);
+  if (a.K == 8) return launch_bwd8<NODE, 8>(a, p, st);  // 16-byte loads: alignment checked
   if (a.K == 4) return launch_bwd8<NODE, 4>(a, p, st);
   return launch_bwd8<NODE, 0>(a, p, st);
 }
@@ -281,21 +283,20 @@ int slg_fc_soft_bwd8(const uint8_t* codes, const float* rows, int64_t B, int64_t
               SLG_E_ARG, "fc_soft_bwd8: node_kind %d", node_kind);
   SLG_REQUIRE(bwd8_takes(B, IN, OUT, K), SLG_E_SHAPE, "fc_soft_bwd8: B %lld, IN %lld, OUT %lld, K %d",
               (long long)B, (long long)IN, (long long)OUT, K);
-  SLG_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)workspace % 16 == 0, SLG_E_ARG,
-              "fc_soft_bwd8: codes or workspace not at a multiple of 16 bytes");
+  SLG_REQUIRE((((uintptr_t)codes | (uintptr_t)cand | (uintptr_t)w | (uintptr_t)node_param |
+                (uintptr_t)workspace) & 15) == 0,
+              SLG_E_ARG, "fc_soft_bwd8: codes, cand, w, node_param or workspace not at a multiple of 16 bytes");
   const Bwd8Plan p = bwd8_plan(B, IN, OUT, K);
   SLG_REQUIRE(workspace_floats >= p.total(), SLG_E_ARG, "fc_soft_bwd8: workspace of %lld floats, %lld needed",
               (long long)workspace_floats, (long long)p.total());
   hipStream_t st = as_stream(stream);
-  float* part = workspace + p.rec;
+  float* part = workspace;
   float* gbr = part + p.part;
   float* in_ws = gbr + p.gbr;
   const bool want_w = gw || gnp, want_x = gx != nullptr && B > 0;
   if (B > 0 && (want_w || want_x)) {
-    fc_bwd_pack_records(cand, w, node_param, OUT, K, IN, reinterpret_cast<uint32_t*>(workspace), st);
-    SLG_LAUNCH_CHECK("fc_soft_bwd8 records");
-    const Bwd8Args a{reinterpret_cast<const uint32_t*>(codes), rows, B, IN, OUT, K, workspace, inv_tau, gy,
-                     want_w ? part : nullptr, want_x ? gbr : nullptr};
+    const Bwd8Args a{reinterpret_cast<const uint32_t*>(codes), rows, B, IN, OUT, K, cand, w, node_param, inv_tau,
+                     gy, want_w ? part : nullptr, want_x ? gbr : nullptr};
     const int rc = node_kind == SLG_NODE_GATE16  ? launch_bwd8_k<SLG_NODE_GATE16>(a, p, st)
                    : node_kind == SLG_NODE_WALSH ? launch_bwd8_k<SLG_NODE_WALSH>(a, p, st)
                                                  : launch_bwd8_k<SLG_NODE_MULTILINEAR2>(a, p, st);

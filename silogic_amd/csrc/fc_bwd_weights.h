@@ -34,14 +34,6 @@ __device__ inline void node_grad(float a, float b, float g, const float4& p, flo
   }
 }
 
-// Records of a layer from its separate arrays (fc_soft_pack_records_kernel),
-// rec: fc_bwd_record_words(OUT, K) words.
-void fc_bwd_pack_records(const int* cand, const float* w, const float* np, int64_t OUT, int K, int64_t IN,
-                         uint32_t* rec, hipStream_t st);
-inline int64_t fc_bwd_record_words(int64_t OUT, int K) {
-  return cdiv(OUT, 64) * 64 * (int64_t)rec_quads(K) * 4;
-}
-
 // gw [OUT,2,K], gnp [OUT,4] (either may be null) from the partials
 // part [NR][2K+4][OUT] of the sample ranges (NR = 0: zeros).
 void fc_bwd_reduce(const float* part, int NR, int64_t OUT, int K, float* gw, float* gnp, hipStream_t st);

@@ -304,12 +304,6 @@ fc_soft_bwd_reduce_kernel(const float* __restrict__ part, int NR, int OUT, int K
 // ---------------------------------------------------------------------------
 // launch helpers
 // ---------------------------------------------------------------------------
-void fc_bwd_pack_records(const int* cand, const float* w, const float* np, int64_t OUT, int K, int64_t IN,
-                         uint32_t* rec, hipStream_t st) {
-  hipLaunchKernelGGL(fc_soft_pack_records_kernel, dim3((unsigned)cdiv(fc_bwd_record_words(OUT, K), 256)),
-                     dim3(256), 0, st, cand, w, np, (int)OUT, K, (int)IN, rec);
-}
-
 void fc_bwd_reduce(const float* part, int NR, int64_t OUT, int K, float* gw, float* gnp, hipStream_t st) {
   hipLaunchKernelGGL(fc_soft_bwd_reduce_kernel, dim3((unsigned)cdiv((2 * K + 4) * OUT, kSumCols)),
                      dim3(kSumThreads), 0, st, part, NR, (int)OUT, K, gw, gnp);
@@ -353,7 +347,7 @@ static BwdPlan bwd_plan(int64_t B, int64_t IN, int64_t OUT, int K) {
   p.NR = (int)std::max<int64_t>(1, std::min<int64_t>(n_tiles, slots / p.n_orange));
   p.tiles_per_range = (int)cdiv(n_tiles, p.NR);
   p.NR = (int)cdiv(n_tiles, p.tiles_per_range);
-  p.rec_floats = p.SL ? 0 : fc_bwd_record_words(OUT, K);
+  p.rec_floats = p.SL ? 0 : cdiv(OUT, 64) * 64 * (int64_t)rec_quads(K) * 4;
   p.part_floats = round4((int64_t)p.NR * (2 * K + 4) * OUT);
   p.gbr_floats = round4(2 * OUT * n_tiles * p.Sw);  // the last tile's rows whole
   p.in_floats = fc_input_grad_floats(B, IN, OUT, 2, K);
@@ -450,7 +444,9 @@ int slg_fc_soft_bwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t 
   float* gbr = part + p.part_floats;
   float* in_ws = gbr + p.gbr_floats;
   if (!p.SL) {
-    fc_bwd_pack_records(cand, w, node_param, OUT, K, IN, reinterpret_cast<uint32_t*>(rec), st);
+    hipLaunchKernelGGL(fc_soft_pack_records_kernel, dim3((unsigned)cdiv(p.rec_floats, 256)),
+                       dim3(256), 0, st, cand, w, node_param, (int)OUT, K, (int)IN,
+                       reinterpret_cast<uint32_t*>(rec));
     SLG_LAUNCH_CHECK("fc_soft_pack_records");
   }
   const bool want_w = gw || gnp;

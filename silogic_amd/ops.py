@@ -120,7 +120,7 @@ def fc_soft_bwd8(codes, rows, in_dim, cand, w, npar, node_kind, inv_tau, gy, nee
     wide for the kernel on codes are unpacked for the one on fp32."""
     require_gpu(codes, rows, cand, w, npar, gy)
     same_device("fc_soft_bwd8", codes, rows, cand, w, npar, gy)
-    cand, w, npar = _c(cand, torch.int32), _c(w, torch.float32), _c(npar, torch.float32)
+    cand, w, npar = (_quads(_c(t, d)) for t, d in ((cand, torch.int32), (w, torch.float32), (npar, torch.float32)))
     gy = _c(gy, torch.float32)
     B, (OUT, _, K) = rows.shape[0], cand.shape
     if gy.shape != (B, OUT):
@@ -358,7 +358,7 @@ def _layer8_args(x, cand, conn, raw, node_kind):
     same_device("fc_layer8", x, cand, conn, raw)
     check_layer8(x, cand, conn=(conn, cand.shape),
                  raw=(raw, (cand.shape[0], 16 if node_kind == GATE16 else 4)))
-    return (_as_f32(x), _c(cand, torch.int32), _c(conn, torch.float32), _quads(_c(raw, torch.float32)),
+    return (_as_f32(x), _quads(_c(cand, torch.int32)), _c(conn, torch.float32), _quads(_c(raw, torch.float32)),
             (*x.shape, cand.shape[0], cand.shape[2]))
 
 
