@@ -24,6 +24,7 @@ namespace slg {
 
 constexpr int kRadixThreads = 512, kRadixWaves = kRadixThreads / 64;
 constexpr int kRadixBits = 10, kRadixSmallBits = 9;  // of a digit, at most (the small sort's LDS holds entries too)
+constexpr int kRadixScanBlocks = 4096;               // workgroups at most
 constexpr int kRadixSmall = 8 * kRadixThreads;       // entries of the one-launch sort, at most
 
 // A range of 4-byte words that the first launch clears beside its own work,
@@ -38,9 +39,10 @@ struct RadixPlan {
   int64_t N;
   int64_t tile;  // entries a workgroup, whole rounds of kRadixThreads * items
   int blocks, nbp, items, passes, bits;
-  // Workspace in 4-byte words: two entry arrays and the counts.
+  bool scan;  // many workgroups: their first places by a launch of its own
+  // Workspace in 4-byte words: two entry arrays, the counts, the digits' sums.
   int64_t ent, hist;
-  int64_t words() const { return 2 * ent + hist; }
+  int64_t words() const { return 2 * ent + hist + (1 << kRadixBits); }
   // Which of the two entry arrays holds the result.
   int result() const { return (passes - 1) & 1; }
 };
@@ -54,11 +56,15 @@ inline RadixPlan radix_plan(int64_t N, int64_t nkeys) {
   const int most = N <= kRadixSmall ? kRadixSmallBits : kRadixBits;
   p.passes = (key + most - 1) / most;
   p.bits = (key + p.passes - 1) / p.passes;
-  // short rounds spread few entries over more CUs; past 256 workgroups longer
-  // ones keep the counts that every workgroup reads few
-  p.items = N <= 256 * 4 * kRadixThreads ? 4 : 8;
+  // short rounds spread few entries over more CUs. Past 256 workgroups each
+  // would read too many counts: a launch scans them first, and several
+  // workgroups a CU take a round each (a pass over 4.2 M entries by 9 bits: 55
+  // us, in 256 workgroups of four rounds 79; at 524288 entries the launch is
+  // the dearer, 25 to 21)
+  p.scan = N > 256 * 4 * kRadixThreads;
+  p.items = p.scan ? 8 : 4;
   const int64_t round = (int64_t)p.items * kRadixThreads;
-  p.tile = std::max<int64_t>(1, cdiv(N, 256 * round)) * round;
+  p.tile = std::max<int64_t>(1, cdiv(N, kRadixScanBlocks * round)) * round;
   p.blocks = (int)std::max<int64_t>(1, cdiv(N, p.tile));
   p.nbp = (p.blocks + 3) & ~3;
   p.ent = (2 * N + 3) & ~int64_t(3);
@@ -219,15 +225,37 @@ radix_count_kernel(Src src, const int2* __restrict__ in, RadixPlan p, int shift,
       for (int b = p.blocks; b < p.nbp; ++b) hist[(int64_t)d * p.nbp + b] = 0;
 }
 
+// Counts [digit][nbp] to first places within the digit, a workgroup a digit;
+// tot: the digit's entries.
+static __global__ void __launch_bounds__(kRadixThreads)
+radix_scan_kernel(int nbp, int* __restrict__ hist, int* __restrict__ tot) {
+  __shared__ int part[2][kRadixWaves];
+  int* h = hist + (int64_t)blockIdx.x * nbp;
+  int run = 0;
+  for (int b0 = 0, k = 0; b0 < nbp; b0 += kRadixThreads, k ^= 1) {
+    const int b = b0 + threadIdx.x, c = b < nbp ? h[b] : 0;
+    const int x = radix_scan(c, part[k]);
+    if (b < nbp) h[b] = run + x - c;
+#pragma unroll
+    for (int w = 0; w < kRadixWaves; ++w) run += part[k][w];
+  }
+  if (threadIdx.x == 0) tot[blockIdx.x] = run;
+}
+
 template <typename Src, int I>
 __global__ void __launch_bounds__(kRadixThreads)
 radix_scatter_kernel(Src src, const int2* __restrict__ in, RadixPlan p, int shift,
-                     const int* __restrict__ hist, int2* __restrict__ out) {
+                     const int* __restrict__ hist, const int* __restrict__ sums, int2* __restrict__ out) {
   __shared__ int cnt[kRadixWaves << kRadixBits];
   __shared__ int tot[1 << kRadixBits], base[1 << kRadixBits], part[kRadixWaves];
   const int R = 1 << p.bits, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int mine = blockIdx.x;
-  {  // P neighbouring threads to a digit
+  if (p.scan) {
+    for (int d = tid; d < R; d += kRadixThreads) {
+      tot[d] = sums[d];
+      base[d] = hist[(int64_t)d * p.nbp + mine];
+    }
+  } else {  // P neighbouring threads to a digit
     const int P = max(1, min(kRadixThreads >> p.bits, 64)), q = tid % P, nq = p.nbp >> 2;
     for (int d0 = 0; d0 < R; d0 += kRadixThreads / P) {  // every lane takes part in the sums
       const int d = d0 + tid / P;
@@ -313,7 +341,7 @@ template <typename Src>
 inline const int2* radix_sort(const Src& src, const RadixPlan& p, int* ws, const RadixClear& clear,
                               hipStream_t st) {
   int2* ent[2] = {reinterpret_cast<int2*>(ws), reinterpret_cast<int2*>(ws + p.ent)};
-  int* hist = ws + 2 * p.ent;
+  int *hist = ws + 2 * p.ent, *sums = hist + p.hist;
   const int extra = (int)std::min<int64_t>(cdiv(clear.bytes, 16 * kRadixThreads), 2048);
   if (p.N <= kRadixSmall) {
     hipLaunchKernelGGL((radix_small_kernel<Src>), dim3(1 + extra), dim3(kRadixThreads), 0, st, src, (int)p.N,
@@ -325,12 +353,14 @@ inline const int2* radix_sort(const Src& src, const RadixPlan& p, int* ws, const
     const RadixClear c = k == 0 ? clear : RadixClear{};
     hipLaunchKernelGGL((radix_count_kernel<Src>), dim3(p.blocks + (k == 0 ? std::max(extra, clear.word ? 1 : 0) : 0)),
                        dim3(kRadixThreads), 0, st, src, in, p, shift, hist, c);
+    if (p.scan)
+      hipLaunchKernelGGL(radix_scan_kernel, dim3(1 << p.bits), dim3(kRadixThreads), 0, st, p.nbp, hist, sums);
     if (p.items == 4)
       hipLaunchKernelGGL((radix_scatter_kernel<Src, 4>), dim3(p.blocks), dim3(kRadixThreads), 0, st, src, in, p,
-                         shift, hist, ent[k & 1]);
+                         shift, hist, sums, ent[k & 1]);
     else
       hipLaunchKernelGGL((radix_scatter_kernel<Src, 8>), dim3(p.blocks), dim3(kRadixThreads), 0, st, src, in, p,
-                         shift, hist, ent[k & 1]);
+                         shift, hist, sums, ent[k & 1]);
     in = ent[k & 1];
   }
   return in;

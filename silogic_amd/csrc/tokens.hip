@@ -66,57 +66,68 @@ __device__ inline float tok_slope(float e, float scale) {
   return scale * (t * r) * r;
 }
 
-// VU values of a table's row, or of a gradient's.
-template <int DT, int VU>
+// VU neighbouring values of a table's row or of a gradient's. Rows of whole
+// groups of VU are aligned as such; RAG: rows that start at any element, whose
+// last group is moved back to end with the row (the columns that two lanes then
+// hold come out the same from both).
+template <int DT, int VU, bool RAG>
+struct RowVec {
+  using T = typename TabType<DT>::t;
+  typedef T t __attribute__((ext_vector_type(VU), aligned(sizeof(T) * (RAG ? 1 : VU))));
+};
+template <int DT, int VU, bool RAG = false>
 __device__ inline void tab_load(const typename TabType<DT>::t* __restrict__ p, float (&v)[VU]) {
   using T = typename TabType<DT>::t;
-  typedef T Vt __attribute__((ext_vector_type(VU)));
-  const Vt r = *reinterpret_cast<const Vt*>(p);
+  const typename RowVec<DT, VU, RAG>::t r = *reinterpret_cast<const typename RowVec<DT, VU, RAG>::t*>(p);
 #pragma unroll
   for (int j = 0; j < VU; ++j) v[j] = tab_get<DT>(VU == 1 ? ((const T*)&r)[0] : r[j]);
 }
-template <int DT, int VU, bool NT = false>
+template <int DT, int VU, bool RAG = false, bool NT = false>
 __device__ inline void tab_store(typename TabType<DT>::t* __restrict__ p, const float (&v)[VU]) {
-  using T = typename TabType<DT>::t;
-  typedef T Vt __attribute__((ext_vector_type(VU)));
+  using Vt = typename RowVec<DT, VU, RAG>::t;
   Vt r;
 #pragma unroll
   for (int j = 0; j < VU; ++j) r[j] = tab_put<DT>(v[j]);
   if constexpr (NT) __builtin_nontemporal_store(r, reinterpret_cast<Vt*>(p));
   else *reinterpret_cast<Vt*>(p) = r;
 }
+// The first column of group c.
+template <int VU, bool RAG>
+__device__ inline int group_col(int c, int D) {
+  return RAG ? min(c * VU, D - VU) : c * VU;
+}
 
-// A thread takes kEncUnits units of VU values of one token (D a multiple of
-// VU), a workgroup's units next to each other. The values stream past the
-// caches, which are left to the table's rows (524288 tokens of 128 values, 25.6
-// MB of table: 55 against 68 us). upr: units per row. Idx: the
-// type that counts units.
+// A thread takes kEncUnits units of VU values of one token, a workgroup's units
+// next to each other (upr units a row). The values stream past the caches,
+// which are left to the table's rows (524288 tokens of 128 values, 25.6 MB of
+// table: 55 against 68 us). Idx: the type that counts units.
 constexpr int kEncUnits = 4;
-template <int DT, typename IdT, int VU, typename Idx>
+template <int DT, typename IdT, int VU, bool RAG, typename Idx>
 __global__ void __launch_bounds__(256)
-tok_encode_kernel(const IdT* __restrict__ ids, Idx units, Idx upr, int V, int64_t pad,
+tok_encode_kernel(const IdT* __restrict__ ids, Idx units, Idx upr, int D, int V, int64_t pad,
                   const typename TabType<DT>::t* __restrict__ tab, float nlog2, int ste, float* __restrict__ y) {
   for (Idx u0 = (Idx)blockIdx.x * (256 * kEncUnits) + threadIdx.x; u0 < units;
        u0 += (Idx)gridDim.x * (256 * kEncUnits)) {
-    int r[kEncUnits];
-    Idx c[kEncUnits];
+    int r[kEncUnits], col[kEncUnits];
+    int64_t at[kEncUnits];
     float e[kEncUnits][VU];
 #pragma unroll
     for (int k = 0; k < kEncUnits; ++k) {
       const Idx u = min(u0 + k * 256, units - 1), n = u / upr;
-      c[k] = u - n * upr;
+      col[k] = group_col<VU, RAG>((int)(u - n * upr), D);
+      at[k] = (int64_t)n * D + col[k];
       r[k] = tok_row(ids, (int64_t)n, V, pad);
     }
 #pragma unroll
     for (int k = 0; k < kEncUnits; ++k)  // an absent token reads row 0
-      tab_load<DT, VU>(tab + ((int64_t)(r[k] < V ? r[k] : 0) * upr + c[k]) * VU, e[k]);
+      tab_load<DT, VU, RAG>(tab + (int64_t)(r[k] < V ? r[k] : 0) * D + col[k], e[k]);
 #pragma unroll
     for (int k = 0; k < kEncUnits; ++k) {
       if (u0 + k * 256 < units) {
         float v[VU];
 #pragma unroll
         for (int j = 0; j < VU; ++j) v[j] = r[k] < V ? tok_value(e[k][j], nlog2, ste != 0) : 0.0f;
-        tab_store<kTabF32, VU, true>(y + (int64_t)(u0 + k * 256) * VU, v);
+        tab_store<kTabF32, VU, RAG, true>(y + at[k], v);
       }
     }
   }
@@ -140,13 +151,13 @@ struct SegArgs {
   float scale;
 };
 
-template <int DT, int VU>
+template <int DT, int VU, bool RAG>
 __device__ inline void seg_write(const SegArgs& a, int v, int d, const float (&sum)[VU], const float (&e)[VU],
                                  typename TabType<DT>::t* __restrict__ gtab) {
   float g[VU];
 #pragma unroll
   for (int j = 0; j < VU; ++j) g[j] = sum[j] * tok_slope(e[j], a.scale);
-  tab_store<DT, VU>(gtab + (int64_t)v * a.D + d, g);
+  tab_store<DT, VU, RAG>(gtab + (int64_t)v * a.D + d, g);
 }
 
 // G lanes sum a chunk of C entries, VU columns each, kSegAhead rows of the
@@ -158,7 +169,7 @@ __device__ inline void seg_write(const SegArgs& a, int v, int d, const float (&s
 // adds its runs at once (one atomic a run on one address took most of the
 // kernel: 17 us at 65536 tokens of 64 values).
 constexpr int kSegAhead = 4;
-template <int DT, int VU>
+template <int DT, int VU, bool RAG>
 __global__ void __launch_bounds__(256)
 tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict__ gy,
                    const typename TabType<DT>::t* __restrict__ tab,
@@ -174,7 +185,8 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
   const bool begun = i0 > 0 && ent[i0 - 1].x == first;
   const int after = i1 < a.N ? ent[i1].x : -1;
   // absent tokens from the chunk's start to the end: nothing
-  for (int d = c < a.chunks && first < a.V ? l * VU : a.D; d < a.D; d += a.G * VU) {
+  for (int q = c < a.chunks && first < a.V ? l : a.D; q * VU < a.D; q += a.G) {
+    const int d = group_col<VU, RAG>(q, a.D);
     bool from_before = begun;
     float sum[VU];
 #pragma unroll
@@ -189,7 +201,7 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
 #pragma unroll
       for (int u = 0; u < kSegAhead; ++u) {
         e[u] = next[u];
-        tab_load<kTabF32, VU>(gy + (int64_t)(uint32_t)e[u].y * a.D + d, g[u]);
+        tab_load<kTabF32, VU, RAG>(gy + (int64_t)(uint32_t)e[u].y * a.D + d, g[u]);
       }
 #pragma unroll
       for (int u = 0; u < kSegAhead; ++u) next[u] = ent[min(i + kSegAhead + u, i1 - 1)];
@@ -198,7 +210,7 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
         const int64_t at = i + u + 1;
         const int then = at < i1 ? (u + 1 < kSegAhead ? e[(u + 1) % kSegAhead].x : next[0].x) : after;
         ends[u] = i + u < i1 && e[u].x < a.V && e[u].x != then;
-        if (ends[u]) tab_load<DT, VU>(tab + (int64_t)e[u].x * a.D + d, t[u]);
+        if (ends[u]) tab_load<DT, VU, RAG>(tab + (int64_t)e[u].x * a.D + d, t[u]);
       }
 #pragma unroll
       for (int u = 0; u < kSegAhead; ++u) {
@@ -206,8 +218,8 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
 #pragma unroll
         for (int j = 0; j < VU; ++j) sum[j] += g[u][j];
         if (ends[u]) {
-          if (from_before) tab_store<kTabF32, VU>(edge + c * a.D + d, sum);
-          else seg_write<DT, VU>(a, e[u].x, d, sum, t[u], gtab);
+          if (from_before) tab_store<kTabF32, VU, RAG>(edge + c * a.D + d, sum);
+          else seg_write<DT, VU, RAG>(a, e[u].x, d, sum, t[u], gtab);
           from_before = false;
 #pragma unroll
           for (int j = 0; j < VU; ++j) sum[j] = 0.0f;
@@ -218,10 +230,10 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
     const int row = ent[i1 - 1].x;
     if (row < a.V && after == row) {  // the last run goes on
       if (from_before) {
-        tab_store<kTabF32, VU>(edge + c * a.D + d, sum);
+        tab_store<kTabF32, VU, RAG>(edge + c * a.D + d, sum);
       } else {
-        tab_store<kTabF32, VU>(edge + (a.chunks + c) * a.D + d, sum);
-        if (d == 0) runs[atomicAdd(&n_runs, 1)] = (int)c;
+        tab_store<kTabF32, VU, RAG>(edge + (a.chunks + c) * a.D + d, sum);
+        if (q == 0) runs[atomicAdd(&n_runs, 1)] = (int)c;
       }
     }
   }
@@ -231,74 +243,111 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
   for (int k = threadIdx.x; k < n_runs; k += 256) list[at_list + k] = runs[k];
 }
 
-// The runs that cross chunks, a workgroup each: G lanes a row, the chunks'
-// parts dealt to kJoinThreads / G groups (each in ascending order), whose sums
-// are added in order.
-constexpr int kJoinThreads = 256;
-template <int DT, int VU>
-__global__ void __launch_bounds__(kJoinThreads)
+// The runs that cross chunks. A group of G lanes takes a run of up to kJoinNear
+// chunks past the one where it begins; the workgroup then takes its groups'
+// longer runs one by one, their chunks' parts dealt to the groups (each in
+// ascending order), whose sums are added in order. T = 1024 for few long runs
+// (tok_join_threads).
+constexpr int kJoinNear = 8;
+template <int DT, int VU, bool RAG, int T>
+__global__ void __launch_bounds__(T)
 tok_join_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict__ edge,
                 const typename TabType<DT>::t* __restrict__ tab,
                 typename TabType<DT>::t* __restrict__ gtab, const int* __restrict__ list,
                 const int* __restrict__ listed) {
-  __shared__ float red[kJoinThreads * VU];
-  __shared__ int end[kJoinThreads / 64];
+  constexpr int W = T / 64;
+  __shared__ float red[T * VU];
+  __shared__ int end[W], far[T], n_far;
   const int tid = threadIdx.x, wave = tid >> 6;
-  const int P = kJoinThreads / a.G, part = tid / a.G, l = tid % a.G;
+  const int P = T / a.G, part = tid / a.G, l = tid % a.G;
   const int n = *listed;
-  for (int k = blockIdx.x; k < n; k += gridDim.x) {
-    const int64_t c = list[k];
-    const int row = ent[min(a.N, (c + 1) * a.C) - 1].x;
-    // chunks past c that begin with the row: the first that does not ends it
-    int64_t last = c;
-    for (;;) {
-      const int64_t q = last + 1 + tid;
-      const uint64_t off = __ballot(!(q < a.chunks && ent[q * a.C].x == row));
-      if ((tid & 63) == 0) end[wave] = off ? __ffsll((unsigned long long)off) - 1 : 64;
-      __syncthreads();
-      int m = 0;
-      bool more = true;
+  // runs dealt to the workgroups one by one, so that long ones meet in few
+  for (int64_t k0 = blockIdx.x; k0 < n; k0 += (int64_t)gridDim.x * P) {
+    if (tid == 0) n_far = 0;
+    __syncthreads();
+    const int64_t k = k0 + (int64_t)part * gridDim.x;
+    if (k < n) {
+      const int64_t c = list[k];
+      int x[kJoinNear];
 #pragma unroll
-      for (int w = 0; w < kJoinThreads / 64; ++w) {
-        m += more ? end[w] : 0;
-        more &= end[w] == 64;
-      }
-      __syncthreads();
-      last += m;
-      if (!more) break;
-    }
-    for (int d0 = 0; d0 < a.D; d0 += a.G * VU) {
-      const int d = d0 + l * VU;
-      float sum[VU];
+      for (int u = 0; u < kJoinNear; ++u) x[u] = ent[min(c + 1 + u, a.chunks - 1) * a.C].x;
+      const int row = ent[(c + 1) * a.C - 1].x;
+      int m = 0;  // chunks past c that begin with the row
 #pragma unroll
-      for (int j = 0; j < VU; ++j) sum[j] = 0.0f;
-      if (d < a.D) {
-        constexpr int U = 8;
-        for (int64_t q = c + 1 + part; q <= last; q += (int64_t)U * P) {
-          float g[U][VU];
+      for (int u = 0; u < kJoinNear; ++u) m += m == u && c + 1 + u < a.chunks && x[u] == row;
+      if (m == kJoinNear) {
+        if (l == 0) far[atomicAdd(&n_far, 1)] = (int)c;
+      } else {
+        for (int q = l; q * VU < a.D; q += a.G) {
+          const int d = group_col<VU, RAG>(q, a.D);
+          float s[VU], e[VU], g[kJoinNear - 1][VU];
+          tab_load<kTabF32, VU, RAG>(edge + (a.chunks + c) * a.D + d, s);
+          tab_load<DT, VU, RAG>(tab + (int64_t)row * a.D + d, e);
 #pragma unroll
-          for (int u = 0; u < U; ++u)
-            tab_load<kTabF32, VU>(edge + min(q + (int64_t)u * P, last) * a.D + d, g[u]);
+          for (int u = 0; u < kJoinNear - 1; ++u)
+            tab_load<kTabF32, VU, RAG>(edge + (c + 1 + min(u, m - 1)) * a.D + d, g[u]);
 #pragma unroll
-          for (int u = 0; u < U; ++u)
+          for (int u = 0; u < kJoinNear - 1; ++u)
 #pragma unroll
-            for (int j = 0; j < VU; ++j) sum[j] += q + (int64_t)u * P <= last ? g[u][j] : 0.0f;
+            for (int j = 0; j < VU; ++j) s[j] += u < m ? g[u][j] : 0.0f;
+          seg_write<DT, VU, RAG>(a, row, d, s, e, gtab);
         }
       }
-#pragma unroll
-      for (int j = 0; j < VU; ++j) red[(part * a.G + l) * VU + j] = sum[j];
-      __syncthreads();
-      if (part == 0 && d < a.D) {
-        float s[VU], e[VU];
-        tab_load<kTabF32, VU>(edge + (a.chunks + c) * a.D + d, s);
-        tab_load<DT, VU>(tab + (int64_t)row * a.D + d, e);
-        for (int p = 0; p < P; ++p)
-#pragma unroll
-          for (int j = 0; j < VU; ++j) s[j] += red[(p * a.G + l) * VU + j];
-        seg_write<DT, VU>(a, row, d, s, e, gtab);
-      }
-      __syncthreads();
     }
+    __syncthreads();
+    for (int f = 0; f < n_far; ++f) {
+      const int64_t c = far[f];
+      const int row = ent[(c + 1) * a.C - 1].x;
+      int64_t last = c + kJoinNear;
+      for (bool more = true; more;) {
+        const int64_t q = last + 1 + tid;
+        const uint64_t off = __ballot(q >= a.chunks || ent[min(q, a.chunks - 1) * a.C].x != row);
+        if ((tid & 63) == 0) end[wave] = off ? __ffsll((unsigned long long)off) - 1 : 64;
+        __syncthreads();
+        int m = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          m += more ? end[w] : 0;
+          more &= end[w] == 64;
+        }
+        __syncthreads();
+        last += m;
+      }
+      for (int q0 = 0; q0 * VU < a.D; q0 += a.G) {
+        const bool on = (q0 + l) * VU < a.D;
+        const int d = on ? group_col<VU, RAG>(q0 + l, a.D) : 0;
+        float sum[VU];
+#pragma unroll
+        for (int j = 0; j < VU; ++j) sum[j] = 0.0f;
+        if (on) {
+          constexpr int U = 8;
+          for (int64_t q = c + 1 + part; q <= last; q += (int64_t)U * P) {
+            float g[U][VU];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+              tab_load<kTabF32, VU, RAG>(edge + min(q + (int64_t)u * P, last) * a.D + d, g[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+              for (int j = 0; j < VU; ++j) sum[j] += q + (int64_t)u * P <= last ? g[u][j] : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < VU; ++j) red[(part * a.G + l) * VU + j] = sum[j];
+        __syncthreads();
+        if (part == 0 && on) {
+          float s[VU], e[VU];
+          tab_load<kTabF32, VU, RAG>(edge + (a.chunks + c) * a.D + d, s);
+          tab_load<DT, VU, RAG>(tab + (int64_t)row * a.D + d, e);
+          for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int j = 0; j < VU; ++j) s[j] += red[(p * a.G + l) * VU + j];
+          seg_write<DT, VU, RAG>(a, row, d, s, e, gtab);
+        }
+        __syncthreads();
+      }
+    }
+    __syncthreads();  // n_far is cleared
   }
 }
 
@@ -366,7 +415,7 @@ __device__ inline uint64_t wave_transpose(uint64_t m) {
 // j then holds feature j's word. Word-major rows of features are written as
 // they are; for the rows [F][nw] a workgroup's waves take TW neighbouring
 // words, which leave through LDS in runs of TW.
-constexpr int kPackTokens = 4;
+constexpr int kPackTokens = 4, kPackFew = 8;
 template <typename IdT, bool WM, int TW>
 __global__ void __launch_bounds__(64 * TW)
 tok_packed_kernel(const IdT* __restrict__ ids, int64_t B, int64_t L, int V, int64_t pad, int D, int DW,
@@ -374,7 +423,8 @@ tok_packed_kernel(const IdT* __restrict__ ids, int64_t B, int64_t L, int V, int6
   __shared__ uint64_t tile[WM ? 1 : kPackTokens][WM ? 1 : 64][WM ? 1 : TW + 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t F = L * D, wt = (nw + TW - 1) / TW, lt = (L + kPackTokens - 1) / kPackTokens, jobs = wt * lt * DW;
-  for (int64_t k = blockIdx.x; k < jobs; k += gridDim.x) {
+  // the jobs that share ids' lines on one XCD, whose L2 then reads them once
+  for (int64_t k = xcd_logical_id(blockIdx.x, gridDim.x); k < jobs; k += gridDim.x) {
     const int64_t t = k / (lt * DW), r = k - t * (lt * DW), l0 = r / DW * kPackTokens;
     const int dw = (int)(r % DW);
     const int64_t w = t * TW + wave, b = w * 64 + lane;
@@ -388,7 +438,16 @@ tok_packed_kernel(const IdT* __restrict__ ids, int64_t B, int64_t L, int V, int6
     const int d = dw * 64 + lane;
 #pragma unroll
     for (int u = 0; u < kPackTokens; ++u) {
-      const uint64_t v = wave_transpose(m[u]);
+      uint64_t v = 0;
+      if (D <= kPackFew) {  // a ballot a bit
+#pragma unroll
+        for (int j = 0; j < kPackFew; ++j) {
+          const uint64_t all = __ballot((m[u] >> j) & 1);
+          v = lane == j ? all : v;
+        }
+      } else {
+        v = wave_transpose(m[u]);
+      }
       if constexpr (WM) {
         if (w < nw && d < D && l0 + u < L) out[w * F + (l0 + u) * D + d] = v;
       } else {
@@ -426,12 +485,23 @@ static void tok_dispatch(int dtype, int id_bytes, F&& f) {
   else ids(std::integral_constant<int, kTabF16>{});
 }
 
-// f(values a lane takes) by the width and the alignment of every row.
+// f(values a lane takes, whether rows are ragged) by the width and the
+// alignment of every row.
 template <typename F>
 static void tok_vector(int64_t D, bool aligned, F&& f) {
-  if (D % 4 == 0 && aligned) f(std::integral_constant<int, 4>{});
-  else f(std::integral_constant<int, 1>{});
+  using Yes = std::true_type;
+  using No = std::false_type;
+  if (D % 4 == 0 && aligned) f(std::integral_constant<int, 4>{}, No{});
+  else if (D >= 4) f(std::integral_constant<int, 4>{}, Yes{});
+  else f(std::integral_constant<int, 1>{}, No{});
 }
+
+// Threads of a join's workgroup: 256, or 1024 where a few rows have all tokens,
+// whose runs a workgroup each then reads (131072 tokens of 512 values over 2
+// rows: 243 us in all with 256, 185 with 1024; 65536 x 64 over 32000 rows: the
+// join 7 and 17 us; 4.1 M tokens of one value over 1000 rows: 271 and 332 in
+// all).
+static int tok_join_threads(int64_t chunks, int64_t V) { return V <= 256 && chunks >= 32 * V ? 1024 : 256; }
 
 struct TokBwdPlan {
   RadixPlan sort;
@@ -440,16 +510,17 @@ struct TokBwdPlan {
   int64_t total() const { return sort.words() + edge + list; }
 };
 
-// Lanes a row: a power of two up to the wave. Chunks: 64 entries, fewer where
-// that leaves less than about 8 waves a CU.
+// Lanes a row: a power of two up to the wave. Chunks: 256 entries, fewer where
+// that leaves less than 16 waves a CU (524288 x 128 tokens: 64; 65536 x 64: 8,
+// of which 16 and 32 took 1 and 7 us longer with their joins).
 static TokBwdPlan tok_bwd_plan(int64_t N, int64_t V, int64_t D) {
   TokBwdPlan p{};
   p.sort = radix_plan(N, V + 1);
-  p.VU = D % 4 == 0 ? 4 : 1;
+  p.VU = D >= 4 ? 4 : 1;
   p.G = 1;
   while (p.G < 64 && p.G * p.VU < D) p.G *= 2;
-  p.C = 64;
-  while (p.C > 8 && cdiv(N, p.C) * p.G < 131072) p.C /= 2;
+  p.C = 256;
+  while (p.C > 8 && cdiv(N, p.C) * p.G < 262144) p.C /= 2;
   p.chunks = cdiv(N, p.C);
   p.edge = (2 * p.chunks * D + 3) & ~int64_t(3);
   p.list = p.chunks + 1;
@@ -480,18 +551,19 @@ int slg_token_encode(const void* ids, int32_t id_bytes, int64_t N, int64_t V, in
     constexpr int DT = decltype(dt)::value;
     using Id = decltype(it);
     using T = typename TabType<DT>::t;
-    tok_vector(D, (uintptr_t)table % (4 * sizeof(T)) == 0 && (uintptr_t)y % 16 == 0, [&](auto vu) {
+    tok_vector(D, (uintptr_t)table % (4 * sizeof(T)) == 0 && (uintptr_t)y % 16 == 0, [&](auto vu, auto rag) {
       constexpr int VU = decltype(vu)::value;
-      const int64_t units = N * D / VU;
+      constexpr bool RAG = decltype(rag)::value;
+      const int64_t upr = cdiv(D, VU), units = N * upr;
       auto go = [&](auto kern, auto idx) {
         using Idx = decltype(idx);
         hipLaunchKernelGGL(kern, dim3(grid_of(cdiv(units, 256 * kEncUnits))), dim3(256), 0, st,
-                           static_cast<const Id*>(ids), (Idx)units, (Idx)(D / VU), (int)V, pad,
+                           static_cast<const Id*>(ids), (Idx)units, (Idx)upr, (int)D, (int)V, pad,
                            static_cast<const T*>(table), nlog2, ste, y);
       };
       // a round of the grid past the last unit still counts within 32 bits
-      if (units < (1LL << 31)) go(tok_encode_kernel<DT, Id, VU, uint32_t>, uint32_t(0));
-      else go(tok_encode_kernel<DT, Id, VU, int64_t>, int64_t(0));
+      if (units < (1LL << 31)) go(tok_encode_kernel<DT, Id, VU, RAG, uint32_t>, uint32_t(0));
+      else go(tok_encode_kernel<DT, Id, VU, RAG, int64_t>, int64_t(0));
     });
   });
   SLG_LAUNCH_CHECK("token_encode");
@@ -528,15 +600,17 @@ int slg_token_encode_bwd(const void* ids, int32_t id_bytes, int64_t N, int64_t V
     }
     const int2* ent = radix_sort(TokenKeys<Id>{static_cast<const Id*>(ids), (int)V, pad}, p.sort, workspace, clear, st);
     const bool aligned = (uintptr_t)table % (4 * sizeof(T)) == 0 && (uintptr_t)gy % 16 == 0;
-    tok_vector(D, aligned, [&](auto vu) {
+    tok_vector(D, aligned, [&](auto vu, auto rag) {
       constexpr int VU = decltype(vu)::value;
+      constexpr bool RAG = decltype(rag)::value;
       const SegArgs s{N, p.chunks, (int)V, (int)D, p.C, p.G, scale};
-      hipLaunchKernelGGL((tok_segment_kernel<DT, VU>), dim3((unsigned)cdiv(p.chunks, 256 / p.G)), dim3(256), 0, st,
+      hipLaunchKernelGGL((tok_segment_kernel<DT, VU, RAG>), dim3((unsigned)cdiv(p.chunks, 256 / p.G)), dim3(256), 0, st,
                          s, ent, gy, static_cast<const T*>(table), static_cast<T*>(gtable), edge, listed + 1,
                          listed);
-      hipLaunchKernelGGL((tok_join_kernel<DT, VU>), dim3((unsigned)std::min<int64_t>(p.chunks, 2048)),
-                         dim3(kJoinThreads), 0, st, s, ent, edge, static_cast<const T*>(table),
-                         static_cast<T*>(gtable), listed + 1, listed);
+      const int T2 = tok_join_threads(p.chunks, V);
+      hipLaunchKernelGGL((T2 == 1024 ? tok_join_kernel<DT, VU, RAG, 1024> : tok_join_kernel<DT, VU, RAG, 256>),
+                         dim3((unsigned)std::min<int64_t>(p.chunks, 512 * 1024 / T2)), dim3(T2), 0, st, s, ent, edge,
+                         static_cast<const T*>(table), static_cast<T*>(gtable), listed + 1, listed);
     });
   });
   SLG_LAUNCH_CHECK("token_encode_bwd");
@@ -573,15 +647,16 @@ int slg_token_encode_hard(const void* ids, int32_t id_bytes, int64_t B, int64_t 
     using Id = decltype(it);
     const Id* id = static_cast<const Id*>(ids);
     if (layout == 2) {
-      tok_vector(D, (uintptr_t)out % 4 == 0, [&](auto vu) {
-        constexpr int VU = decltype(vu)::value;
-        hipLaunchKernelGGL((tok_bytes_kernel<Id, VU>), dim3(grid_of(cdiv(N * D / VU, 256))), dim3(256), 0, st, id,
-                           N * D / VU, (int)(D / VU), (int)V, pad, (int)DW, bits, static_cast<uint8_t*>(out));
-      });
+      auto go = [&](auto kern, int64_t vu) {
+        hipLaunchKernelGGL(kern, dim3(grid_of(cdiv(N * D / vu, 256))), dim3(256), 0, st, id, N * D / vu,
+                           (int)(D / vu), (int)V, pad, (int)DW, bits, static_cast<uint8_t*>(out));
+      };
+      if (D % 4 == 0 && (uintptr_t)out % 4 == 0) go(tok_bytes_kernel<Id, 4>, 4);
+      else go(tok_bytes_kernel<Id, 1>, 1);
       return;
     }
     auto go = [&](auto kern, int tw) {
-      hipLaunchKernelGGL(kern, dim3(grid_of(cdiv(nw, tw) * cdiv(L, kPackTokens) * DW)), dim3(64 * tw), 0, st, id, B, L, (int)V, pad,
+      hipLaunchKernelGGL(kern, dim3(grid_of(cdiv(cdiv(nw, tw) * cdiv(L, kPackTokens) * DW, 8) * 8)), dim3(64 * tw), 0, st, id, B, L, (int)V, pad,
                          (int)D, (int)DW, nw, bits, static_cast<uint64_t*>(out));
     };
     if (layout == 1) go(tok_packed_kernel<Id, true, 4>, 4);

@@ -77,7 +77,8 @@ def _check(B, L, V, D, how="zipf", dtype=torch.float32, ste=False, pad=None, sca
 @pytest.mark.parametrize("B,L,V,D", [(1, 1, 1, 1), (1, 1, 2, 16), (1, 3, 5, 7), (2, 1, 300, 64), (63, 2, 17, 3),
                                      (64, 5, 100, 65), (65, 4, 1000, 32), (130, 33, 70, 10), (257, 16, 511, 24),
                                      (100, 50, 512, 4), (33, 200, 513, 130), (7, 1, 70000, 8), (5, 3, 9, 600),
-                                     (300, 40, 3, 12), (513, 64, 4001, 5)])
+                                     (300, 40, 3, 12), (513, 64, 4001, 5), (41, 7, 60, 27), (3, 3, 40, 301), (70, 3, 90, 8),
+                                     (66, 9, 30, 9)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_sizes(B, L, V, D, dtype):
     _check(B, L, V, D, dtype=dtype, pad=0 if V > 1 else None)
@@ -97,6 +98,13 @@ def test_sorts_of_several_workgroups(how):
     _check(700, 30, 40, 8, how=how)
     _check(500, 41, 30000, 8, how=how, pad=5)
     _check(301, 30, 300000, 4, how=how)
+
+
+@pytest.mark.parametrize("how", ["one", "zipf"])
+def test_sorts_whose_counts_are_scanned_first(how):
+    """More than 524288 tokens; runs over thousands of chunks."""
+    _check(2100, 260, 1000, 1, how=how, int32=True)
+    _check(1100, 500, 70000, 6, how=how)
 
 
 def test_large_values_and_scales():
