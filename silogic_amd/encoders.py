@@ -152,28 +152,28 @@ class TokenEncoder(nn.Module):
     def _bit_table(self, weight):
         """Bit words of the weight, made once per version of it (its storage and
         version counter, as ``derived`` keys tables; ``derived.clear`` drops
-        them). Another stream than the one that made them waits for them; a
-        captured call that finds none of its own stream makes them inside the
-        graph, so that a replay reads the weight afresh."""
-        here = ops._stream(weight).value
-        slot = self.__dict__.get("_derived_bits")
-        if slot is not None and slot[0] == (weight.data_ptr(), weight._version):
-            if slot[1] == here:
-                return slot[2]
-        else:
-            slot = None
-        w = weight.detach()
+        them). Another stream than the one that made them waits for them. A
+        captured call makes its own inside the graph, which then keeps them
+        and reads the weight afresh on every replay."""
         if torch.cuda.is_current_stream_capturing():
-            return ops.token_bits(ops._c(w))
-        stream = torch.cuda.current_stream(w.device)
-        if slot is None:
+            return ops.token_bits(ops._c(weight.detach()))
+        here = ops._stream(weight).value
+        key = (weight.data_ptr(), weight._version)
+        slot = self.__dict__.get("_derived_bits")
+        if slot is None or slot[0] != key:
+            w = weight.detach()   # kept: its address stays taken while the key holds it
             bits = ops.token_bits(ops._c(w))
-            # w itself: its address stays taken while the key holds it
-            self._derived_bits = ((w.data_ptr(), w._version), here, bits, stream.record_event(), w)
+            done = torch.cuda.current_stream(w.device).record_event()
+            self._derived_bits = (key, here, bits, done, w)
             return bits
-        stream.wait_event(slot[3])
-        slot[2].record_stream(stream)
+        if slot[1] != here:
+            stream = torch.cuda.current_stream(weight.device)
+            stream.wait_event(slot[3])
+            slot[2].record_stream(stream)
         return slot[2]
+
+    def __getstate__(self):   # copies and pickles make their own bit table
+        return {k: v for k, v in self.__dict__.items() if k != "_derived_bits"}
 
     def _hard(self, ids, layout):
         w = self.weight

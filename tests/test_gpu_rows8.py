@@ -371,3 +371,37 @@ def test_custom_ops_check():
     torch.library.opcheck(torch.ops.silogic_hip.fc_layer8, (args[0], cand.to(DEV), args[1], args[2], orc.GATE16, 1.0))
     w, p = torch.softmax(conn, -1).to(DEV).requires_grad_(), torch.rand(8, 4, device=DEV, requires_grad=True)
     torch.library.opcheck(torch.ops.silogic_hip.fc_soft8, (args[0], cand.to(DEV), w, p, orc.WALSH, 0.5))
+
+
+def test_under_autocast():
+    layer = sl.LogicLayer(30, 40, k=4, seed=1).to(DEV)
+    sl.save_activations(layer)
+    x = torch.rand(10, 30, device=DEV)
+    y = layer(x)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert torch.equal(layer(x), y)
+
+
+def test_no_second_derivative():
+    x, cand, conn, raw, _ = _problem(orc.GATE16, 6, 9, 8, 3)
+    x = x.to(DEV).requires_grad_()
+    (g,) = torch.autograd.grad(ops.fc_layer8(x, cand.to(DEV), conn.to(DEV), raw.to(DEV), orc.GATE16).sum(), [x],
+                               create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), [x])
+
+
+def test_sizes_past_32_bit_offsets():
+    """2.2e9 values packed, and a layer over 2.2e9 inputs: the last samples as in a call of their own."""
+    B, D = 270001, 8190
+    x = torch.rand(B, D, device=DEV)
+    codes, rows = sl.pack_rows8(x)
+    part = slice(B - B % 4 - 8, B)
+    c, r = sl.pack_rows8(x[part])
+    assert torch.equal(codes[-c.shape[0]:], c) and torch.equal(rows[part], r)
+    assert torch.equal(sl.unpack_rows8(codes, rows)[part], sl.unpack_rows8(c, r))
+    _, cand, conn, raw, gy = _problem(orc.GATE16, B, D, 40, 2, x=torch.zeros(1))
+    y, gx, _, _ = _grads(x, cand, conn, raw, gy, orc.GATE16, 1.0)
+    ys, gs, _, _ = _grads(x[part], cand, conn, raw, gy[part], orc.GATE16, 1.0)
+    assert torch.equal(y[part], ys)
+    assert (gx[part] - gs).abs().max() <= 64 * orc.EPS * gs.abs().max()   # one order or another of an input's sum

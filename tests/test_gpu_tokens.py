@@ -275,20 +275,97 @@ def test_compiled_and_checked():
     torch.library.opcheck(torch.ops.silogic_hip.token_encode, (ids, w, 1.5, False, 2))
 
 
+def test_copies_and_pickles():
+    import copy
+    import io
+    enc = sl.TokenEncoder(9, 70, padding_idx=1).to(DEV)
+    ids = torch.arange(9, device=DEV)
+    want = enc.forward_packed(ids)   # the bit table is there
+    other = copy.deepcopy(enc)
+    with torch.no_grad():
+        other.weight.neg_()
+    assert torch.equal(enc.forward_packed(ids), want)
+    assert torch.equal(other.forward_hard(ids)[0].bool(), other.weight[0] > 0)
+    f = io.BytesIO()
+    torch.save(enc, f)
+    f.seek(0)
+    back = torch.load(f, weights_only=False)   # the file is this test's own
+    assert torch.equal(back.forward_packed(ids), want) and back.padding_idx == 1
+
+
+def test_no_second_derivative():
+    enc = sl.TokenEncoder(9, 7).to(DEV)
+    (g,) = torch.autograd.grad(enc(torch.arange(9, device=DEV)).sum(), [enc.weight], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), [enc.weight])
+
+
+def test_ids_far_outside_the_table():
+    enc = sl.TokenEncoder(9, 7).to(DEV)
+    ids = torch.tensor([3, 2 ** 40 + 3, -2 ** 62, 2 ** 63 - 1, -1, 9], device=DEV)
+    y = enc(ids)
+    assert y[0].all() and not y[1:].any() and not enc.forward_hard(ids)[1:].any()
+    (g,) = torch.autograd.grad(y.sum(), [enc.weight])
+    assert g[3].all() and not g[:3].any() and not g[4:].any()
+
+
+def test_under_autocast():
+    enc = sl.TokenEncoder(9, 7).to(DEV)
+    ids = torch.arange(9, device=DEV)
+    y = enc(ids)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert torch.equal(enc(ids), y)
+
+
+def test_values_past_32_bit_offsets():
+    """2.2e9 values: the last tokens' values, and counts exact in fp32 as every row's sum."""
+    V, D, N = 1000, 130, 2 ** 24 + 5
+    enc = sl.TokenEncoder(V, D, scale=0.5).to(DEV)
+    ids = (torch.arange(N, device=DEV) * 7919) % V
+    y = enc(ids)
+    for part in (slice(0, 64), slice(N // 2, N // 2 + 64), slice(N - 64, N)):
+        assert torch.equal(y[part], enc(ids[part]))
+    (g,) = torch.autograd.grad(y, [enc.weight], torch.ones_like(y))
+    count = torch.bincount(ids, minlength=V)
+    (one,) = torch.autograd.grad(enc(torch.arange(V, device=DEV)).sum(), [enc.weight])
+    # the sums are whole numbers below 2^24; a product's rounding each way
+    orc.close(g, one.cpu().to(F64) * count.cpu().to(F64)[:, None], 2 * orc.EPS * (one.cpu().to(F64) * count.cpu()[:, None]))
+
+
 def test_feeds_a_network():
-    """Tokens through the encoder and gate layers that keep bytes: a training step's gradients against the
-    64-bit gradient of the same function, and the circuit against the hard layers' own path."""
+    """Tokens through the encoder, gate layers that keep bytes and the head: a training step's gradients against
+    the 64-bit ones at the values that each layer kept, and the circuit against the hard layers' own path."""
     torch.manual_seed(0)
     enc = sl.TokenEncoder(40, 8, padding_idx=0).to(DEV)
     net = sl.LogicNet(6 * 8, 60, 2, num_classes=10, k=4, tau=3.0, seed=0).to(DEV)
     assert sl.save_activations(net) == 2
     net.train()
     ids = torch.randint(0, 40, (100, 6), device=DEV)
-    logits = net(enc(ids))
-    loss = torch.nn.functional.cross_entropy(logits, torch.randint(0, 10, (100,), device=DEV))
-    loss.backward()
-    grads = {n: p.grad for m in (enc, net) for n, p in m.named_parameters()}
-    assert all(g is not None and torch.isfinite(g).all() for g in grads.values())
+    label = torch.randint(0, 10, (100,), device=DEV)
+    torch.nn.functional.cross_entropy(net(enc(ids)), label).backward()
+    # the same step layer by layer, for what each kept and the gradient at the head's input
+    x = [enc(ids).detach()]
+    for layer in net.layers:
+        x.append(layer(x[-1]).detach())
+    top = x[-1].clone().requires_grad_()
+    (g,) = torch.autograd.grad(torch.nn.functional.cross_entropy(net.head(top), label), [top])
+    g = g.cpu().to(F64)
+    mag, n = g.abs(), 0
+    for layer, kept in zip(reversed(list(net.layers)), (x[1], x[0])):
+        cand, conn, raw = layer._conn.cand_i32, layer._conn.conn.detach().cpu(), layer.node.raw().detach().cpu()
+        w = torch.softmax(conn.to(F64), -1)
+        p, pmag, back, back_mag = orc.poly(orc.GATE16, raw)
+        v = orc.values_of(kept)
+        (_, gx, gw, gp), _ = orc.layer(v, cand, w, p, orc.GATE16, 1.0, g, pmag)
+        # errors of the gradient from above go on with its mag in the place of its size
+        _, (_, gxm, gwm, gpm) = orc.layer(v, cand, w, p, orc.GATE16, 1.0, mag, pmag)
+        n += 4 * 4 + 80 + 100 + 2 * 4 * 60   # as in the layers' own tests, references at most all
+        orc.close(layer._conn.conn.grad, orc.softmax_back(w, gw), n * orc.EPS * orc.softmax_back_mag(w, gwm), "conn")
+        orc.close(layer.node.raw().grad, back(gp), n * orc.EPS * back_mag(gpm), "node")
+        g, mag = gx, gxm
+    _, _, want, _, _ = _oracle(ids, enc.weight, 1.0, False, 0, g)
+    _, _, _, _, size = _oracle(ids, enc.weight, 1.0, False, 0, mag)
+    orc.close(enc.weight.grad, want, (n + 600 + 30) * orc.EPS * size, "table")
     assert not enc.weight.grad[0].any() and enc.weight.grad[1:].any()
     net.eval()
     hard = net.forward_hard(enc.forward_hard(ids).float())
