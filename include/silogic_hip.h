@@ -328,9 +328,9 @@ int slg_fc_soft_bwd8(const uint8_t* codes, const float* rows, int64_t B, int64_t
 /* A gate layer's training step from its own parameters, its input kept in 8
  * bits: slg_layer_params and slg_fc_soft_fwd8 one way (w [OUT,2,K] and kept as
  * the former gives them: kept [OUT,4], gate16: followed by its probabilities
- * [OUT,16]), slg_fc_soft_bwd8 and slg_layer_params_bwd the other (any of gx,
- * gconn, graw may be NULL). conn NULL: fixed wiring. raw and kept at multiples
- * of 16 bytes. */
+ * [OUT,16]); the other way the gradients of slg_fc_soft_bwd8 down to conn and
+ * raw (any of gx, gconn, graw may be NULL). conn NULL: fixed wiring. raw, w and
+ * kept at multiples of 16 bytes. */
 int slg_fc_layer8_fwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t K,
                       const int32_t* cand, const float* conn, const float* raw, int32_t node_kind,
                       float inv_tau, float* y, uint8_t* codes, float* rows, float* w, float* kept,

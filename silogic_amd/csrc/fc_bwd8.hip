@@ -189,6 +189,79 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
   }
 }
 
+// From the sample ranges' partials to the gradients of a layer's own
+// parameters in one launch: the sums over ranges, the connection softmax's
+// chain rule and the node's. A workgroup takes 16 outputs; a wave a component
+// at a time, its lanes 16 outputs by 4 parts of the ranges (each part
+// ascending, the parts added in order of a butterfly), so that a narrow layer
+// with many ranges is not walked by one lane. 9.6 us at 16000 outputs with 8
+// candidates; as two launches through memory (the sums, then
+// slg_layer_params_bwd) 14 us.
+constexpr int kPbThreads = 1024, kPbOut = 16;
+template <int NODE>
+__global__ void __launch_bounds__(kPbThreads)
+fc_bwd8_params_kernel(const float* __restrict__ part, int NR, int OUT, int K, const float* __restrict__ w,
+                      const float* __restrict__ kept, float* __restrict__ gconn, float* __restrict__ graw) {
+  __shared__ float g[36][kPbOut + 1];  // 2 K + 4 components
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int o0 = blockIdx.x * kPbOut, n = 2 * K + 4;
+  const int o = min(o0 + (lane & 15), OUT - 1);
+  for (int c = wave; c < n; c += kPbThreads / 64) {
+    float sum = 0.0f;
+    for (int r0 = lane >> 4; r0 < NR; r0 += 32) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = part[((int64_t)min(r0 + 4 * u, NR - 1) * n + c) * OUT + o];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sum += r0 + 4 * u < NR ? v[u] : 0.0f;
+    }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (lane < kPbOut) g[c][lane] = sum;
+  }
+  __syncthreads();
+  if (tid < 2 * kPbOut) {  // a softmax row: an output's operand
+    const int side = tid / kPbOut, l = tid % kPbOut;
+    if (gconn && o0 + l < OUT) {
+      const int64_t at = ((int64_t)(o0 + l) * 2 + side) * K;
+      float dot = 0.0f;
+      for (int k = 0; k < K; ++k) dot = fmaf(w[at + k], g[side * K + k][l], dot);
+      for (int k = 0; k < K; ++k) gconn[at + k] = w[at + k] * (g[side * K + k][l] - dot);
+    }
+  } else if (tid >= 64 && tid < 64 + kPbOut) {
+    const int l = tid - 64;
+    if (graw && o0 + l < OUT) {
+      const int64_t out = o0 + l;
+      const float q0 = g[2 * K][l], q1 = g[2 * K + 1][l], q2 = g[2 * K + 2][l], q3 = g[2 * K + 3][l];
+      if constexpr (NODE == SLG_NODE_GATE16) {
+        // gate i's values by the bits of i: f(a, b) = bit 3 - (2 a + b), in {1, a, b, ab}
+        const float* p = kept + 4 * (int64_t)OUT + 16 * out;
+        float d[16], dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int f0 = (i >> 3) & 1, f1 = (i >> 2) & 1, f2 = (i >> 1) & 1, f3 = i & 1;
+          d[i] = f0 * q0 + (f2 - f0) * q1 + (f1 - f0) * q2 + (f3 - f2 - f1 + f0) * q3;
+          dot = fmaf(p[i], d[i], dot);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) graw[16 * out + i] = p[i] * (d[i] - dot);
+      } else if constexpr (NODE == SLG_NODE_WALSH) {
+        graw[4 * out] = q0;
+        graw[4 * out + 1] = 2.0f * q1 - q0;
+        graw[4 * out + 2] = 2.0f * q2 - q0;
+        graw[4 * out + 3] = q0 + 4.0f * q3 - 2.0f * (q1 + q2);
+      } else {
+        const float q[4] = {q0, q1, q2, q3};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = kept[4 * out + i];
+          graw[4 * out + i] = q[i] * (v * (1.0f - v));
+        }
+      }
+    }
+  }
+}
+
 // Workspace (in 4-byte words): partials | operand gradients | input-gradient part.
 struct Bwd8Plan {
   int threads, n_orange, NR, tiles_per_range;
@@ -262,6 +335,38 @@ static int launch_bwd8_k(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
   return launch_bwd8<NODE, 0>(a, p, st);
 }
 
+// Checks, the weight kernel and the input gradient: partials of the weights'
+// and node parameters' gradients (want_w) at the workspace's start, p.NR of
+// them (none for an empty batch).
+static int bwd8_run(Bwd8Args a, int node_kind, bool want_w, float* gx, float* workspace, int64_t workspace_floats,
+                    hipStream_t st, Bwd8Plan& p) {
+  SLG_REQUIRE(a.cand && a.w && a.np && workspace && ((a.codes && a.rows && a.gy) || a.B == 0), SLG_E_ARG,
+              "fc_soft_bwd8: null pointer");
+  SLG_REQUIRE(node_kind == SLG_NODE_GATE16 || node_kind == SLG_NODE_WALSH ||
+                  node_kind == SLG_NODE_MULTILINEAR2,
+              SLG_E_ARG, "fc_soft_bwd8: node_kind %d", node_kind);
+  SLG_REQUIRE(bwd8_takes(a.B, a.IN, a.OUT, a.K), SLG_E_SHAPE, "fc_soft_bwd8: B %lld, IN %lld, OUT %lld, K %d",
+              (long long)a.B, (long long)a.IN, (long long)a.OUT, a.K);
+  SLG_REQUIRE((((uintptr_t)a.codes | (uintptr_t)a.cand | (uintptr_t)a.w | (uintptr_t)a.np |
+                (uintptr_t)workspace) & 15) == 0,
+              SLG_E_ARG, "fc_soft_bwd8: codes, cand, w, node_param or workspace not at a multiple of 16 bytes");
+  p = bwd8_plan(a.B, a.IN, a.OUT, a.K);
+  SLG_REQUIRE(workspace_floats >= p.total(), SLG_E_ARG, "fc_soft_bwd8: workspace of %lld floats, %lld needed",
+              (long long)workspace_floats, (long long)p.total());
+  if (a.B == 0) {  // no samples: zero gradients
+    p.NR = 0;
+    return 0;
+  }
+  if (!want_w && !gx) return 0;
+  float* gbr = workspace + p.part;
+  a.part = want_w ? workspace : nullptr;
+  a.gbr = gx ? gbr : nullptr;
+  const int rc = node_kind == SLG_NODE_GATE16  ? launch_bwd8_k<SLG_NODE_GATE16>(a, p, st)
+                 : node_kind == SLG_NODE_WALSH ? launch_bwd8_k<SLG_NODE_WALSH>(a, p, st)
+                                               : launch_bwd8_k<SLG_NODE_MULTILINEAR2>(a, p, st);
+  return rc || !gx ? rc : fc_input_grad(gbr, a.B, a.IN, a.OUT, 2, a.K, a.cand, a.w, gbr + p.gbr, gx, st);
+}
+
 }  // namespace slg
 
 using namespace slg;
@@ -276,40 +381,13 @@ int slg_fc_soft_bwd8(const uint8_t* codes, const float* rows, int64_t B, int64_t
                      const int32_t* cand, const float* w, int32_t node_kind, const float* node_param,
                      float inv_tau, const float* gy, float* gx, float* gw, float* gnp, float* workspace,
                      int64_t workspace_floats, slg_stream_t stream) {
-  SLG_REQUIRE(cand && w && node_param && workspace && ((codes && rows && gy) || B == 0), SLG_E_ARG,
-              "fc_soft_bwd8: null pointer");
-  SLG_REQUIRE(node_kind == SLG_NODE_GATE16 || node_kind == SLG_NODE_WALSH ||
-                  node_kind == SLG_NODE_MULTILINEAR2,
-              SLG_E_ARG, "fc_soft_bwd8: node_kind %d", node_kind);
-  SLG_REQUIRE(bwd8_takes(B, IN, OUT, K), SLG_E_SHAPE, "fc_soft_bwd8: B %lld, IN %lld, OUT %lld, K %d",
-              (long long)B, (long long)IN, (long long)OUT, K);
-  SLG_REQUIRE((((uintptr_t)codes | (uintptr_t)cand | (uintptr_t)w | (uintptr_t)node_param |
-                (uintptr_t)workspace) & 15) == 0,
-              SLG_E_ARG, "fc_soft_bwd8: codes, cand, w, node_param or workspace not at a multiple of 16 bytes");
-  const Bwd8Plan p = bwd8_plan(B, IN, OUT, K);
-  SLG_REQUIRE(workspace_floats >= p.total(), SLG_E_ARG, "fc_soft_bwd8: workspace of %lld floats, %lld needed",
-              (long long)workspace_floats, (long long)p.total());
-  hipStream_t st = as_stream(stream);
-  float* part = workspace;
-  float* gbr = part + p.part;
-  float* in_ws = gbr + p.gbr;
-  const bool want_w = gw || gnp, want_x = gx != nullptr && B > 0;
-  if (B > 0 && (want_w || want_x)) {
-    const Bwd8Args a{reinterpret_cast<const uint32_t*>(codes), rows, B, IN, OUT, K, cand, w, node_param, inv_tau,
-                     gy, want_w ? part : nullptr, want_x ? gbr : nullptr};
-    const int rc = node_kind == SLG_NODE_GATE16  ? launch_bwd8_k<SLG_NODE_GATE16>(a, p, st)
-                   : node_kind == SLG_NODE_WALSH ? launch_bwd8_k<SLG_NODE_WALSH>(a, p, st)
-                                                 : launch_bwd8_k<SLG_NODE_MULTILINEAR2>(a, p, st);
-    if (rc) return rc;
-  }
-  if (want_x) {
-    const int rc = fc_input_grad(gbr, B, IN, OUT, 2, K, cand, w, in_ws, gx, st);
-    if (rc) return rc;
-  }
-  if (want_w) {
-    fc_bwd_reduce(part, B > 0 ? p.NR : 0, OUT, K, gw, gnp, st);  // no samples: zero gradients
-    SLG_LAUNCH_CHECK("fc_soft_bwd8 sums");
-  }
+  const Bwd8Args a{reinterpret_cast<const uint32_t*>(codes), rows, B, IN, OUT, K, cand, w, node_param, inv_tau,
+                   gy, nullptr, nullptr};
+  Bwd8Plan p{};
+  const int rc = bwd8_run(a, node_kind, gw || gnp, gx, workspace, workspace_floats, as_stream(stream), p);
+  if (rc || !(gw || gnp)) return rc;
+  fc_bwd_reduce(workspace, p.NR, OUT, K, gw, gnp, as_stream(stream));
+  SLG_LAUNCH_CHECK("fc_soft_bwd8 sums");
   return 0;
 }
 
@@ -329,29 +407,26 @@ int slg_fc_layer8_fwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_
 }
 
 int64_t slg_fc_layer8_bwd_workspace(int64_t B, int64_t IN, int64_t OUT, int32_t K) {
-  const int64_t n = slg_fc_soft_bwd8_workspace(B, IN, OUT, K);
-  return n < 0 ? n : n + ((2 * OUT * K + 3) & ~int64_t(3)) + 4 * OUT;
+  return slg_fc_soft_bwd8_workspace(B, IN, OUT, K);
 }
 
 int slg_fc_layer8_bwd(const uint8_t* codes, const float* rows, int64_t B, int64_t IN, int64_t OUT, int32_t K,
                       const int32_t* cand, const float* w, const float* kept, int32_t node_kind, float inv_tau,
                       const float* gy, float* gx, float* gconn, float* graw, float* workspace,
                       int64_t workspace_floats, slg_stream_t stream) {
-  SLG_REQUIRE(kept && workspace, SLG_E_ARG, "fc_layer8_bwd: null pointer");
-  SLG_REQUIRE(bwd8_takes(B, IN, OUT, K), SLG_E_SHAPE, "fc_layer8_bwd: B %lld, IN %lld, OUT %lld, K %d",
-              (long long)B, (long long)IN, (long long)OUT, K);
-  const int64_t own = ((2 * OUT * K + 3) & ~int64_t(3)) + 4 * OUT;  // the weights' and node parameters' gradients
-  float* gn = workspace;
-  float* gw = gn + 4 * OUT;
-  int rc = slg_fc_soft_bwd8(codes, rows, B, IN, OUT, K, cand, w, node_kind, kept, inv_tau, gy, gx,
-                            gconn ? gw : nullptr, graw ? gn : nullptr, workspace + own, workspace_floats - own,
-                            stream);
-  if (rc || (!gconn && !graw)) return rc;
-  const int32_t one = 1;
-  // gate16 kept its probabilities behind the coefficients; walsh needs neither
-  const float* from = node_kind == SLG_NODE_GATE16 ? kept + 4 * OUT : node_kind == SLG_NODE_WALSH ? nullptr : kept;
-  return slg_layer_params_bwd(w, gconn ? gw : nullptr, 2 * OUT, K, 1, &one, OUT, node_kind, 2, 1.0f, from,
-                              graw ? gn : nullptr, gconn, &graw, stream);
+  const Bwd8Args a{reinterpret_cast<const uint32_t*>(codes), rows, B, IN, OUT, K, cand, w, kept, inv_tau, gy,
+                   nullptr, nullptr};
+  Bwd8Plan p{};
+  hipStream_t st = as_stream(stream);
+  const int rc = bwd8_run(a, node_kind, gconn || graw, gx, workspace, workspace_floats, st, p);
+  if (rc || !(gconn || graw)) return rc;
+  auto kern = node_kind == SLG_NODE_GATE16  ? fc_bwd8_params_kernel<SLG_NODE_GATE16>
+              : node_kind == SLG_NODE_WALSH ? fc_bwd8_params_kernel<SLG_NODE_WALSH>
+                                            : fc_bwd8_params_kernel<SLG_NODE_MULTILINEAR2>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)cdiv(OUT, kPbOut)), dim3(kPbThreads), 0, st, workspace, p.NR, (int)OUT,
+                     K, w, kept, gconn, graw);
+  SLG_LAUNCH_CHECK("fc_layer8_bwd parameters");
+  return 0;
 }
 
 }  // extern "C"

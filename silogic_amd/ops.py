@@ -354,12 +354,18 @@ def fc_soft8_fwd(x, cand, w, npar, node_kind, inv_tau):
 
 def _layer8_args(x, cand, conn, raw, node_kind):
     """The arguments as the kernels read them, and ``(B, IN, OUT, K)``."""
-    require_gpu(x, cand, conn, raw)
-    same_device("fc_layer8", x, cand, conn, raw)
-    check_layer8(x, cand, conn=(conn, cand.shape),
-                 raw=(raw, (cand.shape[0], 16 if node_kind == GATE16 else 4)))
-    return (_as_f32(x), _quads(_c(cand, torch.int32)), _c(conn, torch.float32), _quads(_c(raw, torch.float32)),
-            (*x.shape, cand.shape[0], cand.shape[2]))
+    d, (OUT, two, K) = x.get_device(), cand.shape if cand.dim() == 3 else (0, 0, 0)
+    # all in order (the usual call), or the check that says what is not
+    if not (d >= 0 and cand.get_device() == d and raw.get_device() == d and x.dim() == 2 and two == 2 and
+            0 < K <= 16 and OUT > 0 and x.shape[1] > 0 and
+            raw.shape == (OUT, 16 if node_kind == GATE16 else 4) and
+            (conn is None or (conn.get_device() == d and conn.shape == cand.shape))):
+        require_gpu(x, cand, conn, raw)
+        same_device("fc_layer8", x, cand, conn, raw)
+        check_layer8(x, cand, conn=(conn, cand.shape),
+                     raw=(raw, (cand.shape[0], 16 if node_kind == GATE16 else 4)))
+    return (_as_f32(x), _quads(_c(cand, torch.int32)), _c(conn, torch.float32),
+            _quads(_c(raw, torch.float32)), (*x.shape, OUT, K))
 
 
 def fc_layer8_fwd(x, cand, conn, raw, node_kind, inv_tau):
