@@ -20,6 +20,7 @@
 
 namespace slg {
 
+constexpr bool bwd8_compiled(int K) { return K == 1 || K == 2 || K == 4 || K == 8; }
 template <int KC>
 constexpr int bwd8_threads() { return KC > 0 ? 1024 : 512; }
 
@@ -278,7 +279,7 @@ static bool bwd8_takes(int64_t B, int64_t IN, int64_t OUT, int K) {
 
 static Bwd8Plan bwd8_plan(int64_t B, int64_t IN, int64_t OUT, int K) {
   Bwd8Plan p{};
-  p.threads = K == 8 || K == 4 ? 1024 : 512;
+  p.threads = bwd8_compiled(K) ? 1024 : 512;
   p.n_orange = (int)cdiv(OUT, p.threads);
   const int64_t n_tiles = cdiv(std::max<int64_t>(B, 1), kRows8Tile);
   // one round of workgroups: as many sample ranges as resident slots allow
@@ -332,6 +333,8 @@ template <int NODE>
 static int launch_bwd8_k(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
   if (a.K == 8) return launch_bwd8<NODE, 8>(a, p, st);  // 16-byte loads: alignment checked
   if (a.K == 4) return launch_bwd8<NODE, 4>(a, p, st);
+  if (a.K == 2) return launch_bwd8<NODE, 2>(a, p, st);
+  if (a.K == 1) return launch_bwd8<NODE, 1>(a, p, st);  // fixed wiring
   return launch_bwd8<NODE, 0>(a, p, st);
 }
 

@@ -9,6 +9,9 @@
 // at most half a step: (max - min) / 510. A row that holds an infinity or a
 // NaN, or whose span overflows, has lo = NaN: it comes back as NaN everywhere
 // rather than as finite values that were not there.
+//
+// Both ways are bound by memory: 5 bytes a value. 4096 x 16380 (335 MB): packed
+// in 69 us (4.9 TB/s; a copy of as much takes 71), unpacked in 54 (6.2 TB/s).
 #include <algorithm>
 
 #include "rows8.h"
@@ -17,21 +20,33 @@ namespace slg {
 
 constexpr int64_t kRows8Grid = 1 << 20;  // workgroups at most; the rest in turn
 
-// VU neighbouring values or words as one access.
+// VU neighbouring values or words as one access, from any multiple of 4 bytes
+// (aligned ones are as fast), so that odd widths take 16 bytes too: a row's
+// last run is moved back to end with the row, the values that two threads then
+// hold come out the same from both.
+template <typename E, int VU>
+struct Rows8Run {
+  typedef E t __attribute__((ext_vector_type(VU), aligned(4)));
+};
 template <int VU>
 __device__ inline void rows8_load(const float* __restrict__ p, float (&v)[VU]) {
-  if constexpr (VU == 4) {
-    const float4 r = *reinterpret_cast<const float4*>(p);
-    v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
-  } else {
-    v[0] = *p;
-  }
+  using R = typename Rows8Run<float, VU>::t;
+  const R r = *reinterpret_cast<const R*>(p);
+#pragma unroll
+  for (int j = 0; j < VU; ++j) v[j] = VU == 1 ? ((const float*)&r)[0] : r[j];
+}
+template <typename E, int VU>
+__device__ inline void rows8_store(E* __restrict__ p, const E (&v)[VU]) {
+  using R = typename Rows8Run<E, VU>::t;
+  R r;
+#pragma unroll
+  for (int j = 0; j < VU; ++j) r[j] = v[j];
+  *reinterpret_cast<R*>(p) = r;
 }
 
 // One workgroup per tile of 4 samples. NU > 0: the tile's values stay in
 // registers between the range and the codes (NU runs of VU inputs of each row
-// a thread, D <= NU * VU * T); NU = 0: they are read again. VU = 4: D a
-// multiple of 4 and x at one of 16 bytes.
+// a thread, D <= NU * VU * T); NU = 0: they are read again. D >= VU.
 template <int NU, int VU, int T>
 __global__ void __launch_bounds__(T)
 rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_t* __restrict__ codes,
@@ -44,7 +59,7 @@ rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_
     const int nb = (int)min((int64_t)kRows8Tile, B - b0);
     const float* p[kRows8Tile];
 #pragma unroll
-    for (int v = 0; v < kRows8Tile; ++v) p[v] = x + (b0 + min(v, nb - 1)) * D;  // past the batch: its last row
+    for (int v = 0; v < kRows8Tile; ++v) p[v] = x + min(b0 + v, B - 1) * D;  // past the batch: its last row
     Rows8Range r[kRows8Tile];
     float keep[NU > 0 ? NU : 1][kRows8Tile][VU];
     if constexpr (NU > 0) {
@@ -64,7 +79,7 @@ rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_
       for (int i = tid * VU; i < D; i += T * VU)
 #pragma unroll
         for (int v = 0; v < kRows8Tile; ++v) {
-          rows8_load<VU>(p[v] + i, keep[0][v]);
+          rows8_load<VU>(p[v] + min(i, D - VU), keep[0][v]);
 #pragma unroll
           for (int j = 0; j < VU; ++j) r[v].take(keep[0][v][j]);
         }
@@ -101,17 +116,17 @@ rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_
 #pragma unroll
         for (int v = 0; v < kRows8Tile; ++v) w[j] = rows8_code(w[j], v, e[v][j], lo[v], inv[v]);
       }
-      if constexpr (VU == 4) *reinterpret_cast<uint4*>(c + i) = make_uint4(w[0], w[1], w[2], w[3]);
-      else c[i] = w[0];
+      rows8_store<uint32_t, VU>(c + i, w);
     };
     if constexpr (NU > 0) {
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         const int i = (tid + u * T) * VU;
-        if (i < D) put(i, keep[u]);
+        if (i < D) put(min(i, D - VU), keep[u]);
       }
     } else {
-      for (int i = tid * VU; i < D; i += T * VU) {
+      for (int k = tid * VU; k < D; k += T * VU) {
+        const int i = min(k, D - VU);
 #pragma unroll
         for (int v = 0; v < kRows8Tile; ++v) rows8_load<VU>(p[v] + i, keep[0][v]);
         put(i, keep[0]);
@@ -123,22 +138,20 @@ rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_
 }
 
 // Values that the codes stand for: a thread takes VU neighbouring words and
-// writes four rows of them (VU = 4: as above).
+// writes four rows of them.
 template <int VU>
 __global__ void __launch_bounds__(256)
 rows8_unpack_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ rows, int64_t B, int D,
                     int ld, int per_tile, int64_t blocks, float* __restrict__ x) {
+  using W = typename Rows8Run<uint32_t, VU>::t;
   for (int64_t k = blockIdx.x; k < blocks; k += gridDim.x) {
     const int64_t t = k / per_tile;
-    const int i = ((int)(k - t * per_tile) * 256 + threadIdx.x) * VU;
-    if (i >= D) continue;
+    const int i0 = ((int)(k - t * per_tile) * 256 + threadIdx.x) * VU, i = min(i0, D - VU);
+    if (i0 >= D) continue;
+    const W r = *reinterpret_cast<const W*>(codes + t * ld + i);
     uint32_t w[VU];
-    if constexpr (VU == 4) {
-      const uint4 r = *reinterpret_cast<const uint4*>(codes + t * ld + i);
-      w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
-    } else {
-      w[0] = codes[t * ld + i];
-    }
+#pragma unroll
+    for (int j = 0; j < VU; ++j) w[j] = VU == 1 ? ((const uint32_t*)&r)[0] : r[j];
 #pragma unroll
     for (int v = 0; v < kRows8Tile; ++v) {
       const int64_t b = t * kRows8Tile + v;
@@ -147,8 +160,7 @@ rows8_unpack_kernel(const uint32_t* __restrict__ codes, const float* __restrict_
       float e[VU];
 #pragma unroll
       for (int j = 0; j < VU; ++j) e[j] = fmaf((float)((w[j] >> (8 * v)) & 255u), step, lo);
-      if constexpr (VU == 4) *reinterpret_cast<float4*>(x + b * D + i) = make_float4(e[0], e[1], e[2], e[3]);
-      else x[b * D + i] = e[0];
+      rows8_store<float, VU>(x + b * D + i, e);
     }
   }
 }
@@ -160,24 +172,26 @@ static void launch_pack(const float* x, int64_t B, int64_t D, uint32_t* codes, f
                      (int)D, (int)rows8_ld(D), codes, rows);
 }
 
-// Workgroups that hold a tile in registers: 16 values of each row a thread at
-// most.
-template <int VU>
-static void launch_pack_v(const float* x, int64_t B, int64_t D, uint32_t* codes, float* rows, hipStream_t st) {
-  constexpr int Q = 4 / VU;  // runs that make 4 values
-  if (D <= 256 * VU) launch_pack<1, VU, 256>(x, B, D, codes, rows, st);
-  else if (D <= 4096 && Q * VU * 256 >= D) launch_pack<Q, VU, 256>(x, B, D, codes, rows, st);
-  else if (D <= 4096) launch_pack<Q, VU, 1024>(x, B, D, codes, rows, st);
-  else if (D <= 8192) launch_pack<2 * Q, VU, 1024>(x, B, D, codes, rows, st);
-  else if (D <= 16384) launch_pack<4 * Q, VU, 1024>(x, B, D, codes, rows, st);
-  else launch_pack<0, VU, 1024>(x, B, D, codes, rows, st);
-}
-
-static bool rows8_vector(const float* x, int64_t D) { return D % 4 == 0 && (uintptr_t)x % 16 == 0; }
-
+// The fewest threads that hold a tile in 16 values of each row a thread (32
+// for the widest): fewer, longer threads have less of the range's sums over
+// lanes and waves to do. Measured (us; threads x values a thread):
+//   65536 x 256     64 x 4   15.7   256 x 4    44    read again by 64    21
+//   32768 x 1000    64 x 16  26.2   256 x 4    27.5  read again by 256   38
+//   16384 x 2000   256 x 8   26.3  1024 x 4    67    read again by 256   42
+//   8192 x 4001    256 x 16  26.1  1024 x 4    39    read again by 256   43
+//   4096 x 8001    512 x 16  26.6  1024 x 8    29    read again by 512   43
+//   4096 x 16380   512 x 32  68.7  1024 x 16   72    read again by 1024  85
+// Wider rows are read again, from the caches (2048 x 32000: 84).
 void rows8_pack(const float* x, int64_t B, int64_t D, uint32_t* codes, float* rows, hipStream_t st) {
-  if (rows8_vector(x, D)) launch_pack_v<4>(x, B, D, codes, rows, st);
-  else launch_pack_v<1>(x, B, D, codes, rows, st);
+  if (D < 4) launch_pack<1, 1, 64>(x, B, D, codes, rows, st);
+  else if (D <= 256) launch_pack<1, 4, 64>(x, B, D, codes, rows, st);
+  else if (D <= 512) launch_pack<2, 4, 64>(x, B, D, codes, rows, st);
+  else if (D <= 1024) launch_pack<4, 4, 64>(x, B, D, codes, rows, st);
+  else if (D <= 2048) launch_pack<2, 4, 256>(x, B, D, codes, rows, st);
+  else if (D <= 4096) launch_pack<4, 4, 256>(x, B, D, codes, rows, st);
+  else if (D <= 8192) launch_pack<4, 4, 512>(x, B, D, codes, rows, st);
+  else if (D <= 16384) launch_pack<8, 4, 512>(x, B, D, codes, rows, st);
+  else launch_pack<0, 4, 512>(x, B, D, codes, rows, st);
 }
 
 }  // namespace slg
@@ -206,7 +220,7 @@ int slg_rows8_unpack(const uint8_t* codes, const float* rows, int64_t B, int64_t
               "rows8_unpack: B %lld, D %lld", (long long)B, (long long)D);
   SLG_REQUIRE((uintptr_t)codes % 16 == 0, SLG_E_ARG, "rows8_unpack: codes not at a multiple of 16 bytes");
   if (B == 0) return 0;
-  const bool vec = rows8_vector(x, D);
+  const bool vec = D >= 4;
   const int64_t per = cdiv(D, vec ? 1024 : 256), blocks = cdiv(B, kRows8Tile) * per;
   hipLaunchKernelGGL(vec ? rows8_unpack_kernel<4> : rows8_unpack_kernel<1>,
                      dim3((unsigned)std::min(blocks, kRows8Grid)), dim3(256), 0, as_stream(stream),
