@@ -12,6 +12,16 @@
 // LDS and a copy of a row of the codes (no transpose), and the 2K gathered
 // words stay in registers from the operands to the weight gradients, where
 // the fp32 kernel gathers twice.
+//
+// Bound by the vector units: each (sample, output) takes 2K conversions and
+// 2K products twice, and the node's derivatives. 10000 -> 10000, K = 8, B =
+// 4096: 113 us for the weights (1.3 G fused products: 23 TFLOP/s of the 79
+// without packed instructions, and as many conversions), 147 with the operand
+// gradients' 328 MB written too, where the fp32 kernel's weights' part takes
+// 318. Halves multiplied straight from
+// registers (fp16 of the codes by a byte permutation, mixed-precision products)
+// took the same time with fewer instructions; kept from the operands to the
+// weights they spilled (482 us).
 #include <algorithm>
 
 #include "fc_bwd_input.h"
@@ -20,6 +30,12 @@
 
 namespace slg {
 
+// Candidates known to the compiler, 1024 threads: they take half of the time
+// that the loop for any K does, whose 16 slots need 512 threads of twice the
+// registers (weights' part, us: 10000 -> 10000, K = 8, B = 4096 113 for 218;
+// 16380 -> 16380, K = 4, B = 1024 45 for 91; 8000 -> 8000, B = 1024 K = 2 25 for
+// 43, K = 1 22 for 39; with 512 threads 145 and 71 for K = 8 and 4, the loop
+// with 1024 118 for 52 at K = 5).
 constexpr bool bwd8_compiled(int K) { return K == 1 || K == 2 || K == 4 || K == 8; }
 template <int KC>
 constexpr int bwd8_threads() { return KC > 0 ? 1024 : 512; }

@@ -11,7 +11,7 @@
 // rather than as finite values that were not there.
 //
 // Both ways are bound by memory: 5 bytes a value. 4096 x 16380 (335 MB): packed
-// in 69 us (4.9 TB/s; a copy of as much takes 71), unpacked in 54 (6.2 TB/s).
+// in 74 us (4.6 TB/s; a copy of as much takes 71), unpacked in 54 (6.2 TB/s).
 #include <algorithm>
 
 #include "rows8.h"

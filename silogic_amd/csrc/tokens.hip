@@ -66,23 +66,23 @@ __device__ inline float tok_slope(float e, float scale) {
   return scale * (t * r) * r;
 }
 
-// VU neighbouring values of a table's row or of a gradient's. Rows of whole
-// groups of VU are aligned as such; RAG: rows that start at any element, whose
-// last group is moved back to end with the row (the columns that two lanes then
-// hold come out the same from both).
-template <int DT, int VU, bool RAG>
+// VU neighbouring values of a table's row or of a gradient's, from any element
+// on: a row's last group is moved back to end with the row (the columns that
+// two lanes then hold come out the same from both). RAG = false: rows of whole
+// groups, aligned as such.
+template <int DT, int VU, bool RAG = true>
 struct RowVec {
   using T = typename TabType<DT>::t;
   typedef T t __attribute__((ext_vector_type(VU), aligned(sizeof(T) * (RAG ? 1 : VU))));
 };
-template <int DT, int VU, bool RAG = false>
+template <int DT, int VU, bool RAG = true>
 __device__ inline void tab_load(const typename TabType<DT>::t* __restrict__ p, float (&v)[VU]) {
   using T = typename TabType<DT>::t;
   const typename RowVec<DT, VU, RAG>::t r = *reinterpret_cast<const typename RowVec<DT, VU, RAG>::t*>(p);
 #pragma unroll
   for (int j = 0; j < VU; ++j) v[j] = tab_get<DT>(VU == 1 ? ((const T*)&r)[0] : r[j]);
 }
-template <int DT, int VU, bool RAG = false, bool NT = false>
+template <int DT, int VU, bool RAG = true, bool NT = false>
 __device__ inline void tab_store(typename TabType<DT>::t* __restrict__ p, const float (&v)[VU]) {
   using Vt = typename RowVec<DT, VU, RAG>::t;
   Vt r;
@@ -92,7 +92,7 @@ __device__ inline void tab_store(typename TabType<DT>::t* __restrict__ p, const 
   else *reinterpret_cast<Vt*>(p) = r;
 }
 // The first column of group c.
-template <int VU, bool RAG>
+template <int VU, bool RAG = true>
 __device__ inline int group_col(int c, int D) {
   return RAG ? min(c * VU, D - VU) : c * VU;
 }
@@ -102,21 +102,21 @@ __device__ inline int group_col(int c, int D) {
 // which are left to the table's rows (524288 tokens of 128 values, 25.6 MB of
 // table: 55 against 68 us). Idx: the type that counts units.
 constexpr int kEncUnits = 4;
-template <int DT, typename IdT, int VU, bool RAG, typename Idx>
+template <int DT, typename IdT, int VU, bool RAG>
 __global__ void __launch_bounds__(256)
-tok_encode_kernel(const IdT* __restrict__ ids, Idx units, Idx upr, int D, int V, int64_t pad,
+tok_encode_kernel(const IdT* __restrict__ ids, int64_t units, int64_t upr, int D, int V, int64_t pad,
                   const typename TabType<DT>::t* __restrict__ tab, float nlog2, int ste, float* __restrict__ y) {
-  for (Idx u0 = (Idx)blockIdx.x * (256 * kEncUnits) + threadIdx.x; u0 < units;
-       u0 += (Idx)gridDim.x * (256 * kEncUnits)) {
+  for (int64_t u0 = (int64_t)blockIdx.x * (256 * kEncUnits) + threadIdx.x; u0 < units;
+       u0 += (int64_t)gridDim.x * (256 * kEncUnits)) {
     int r[kEncUnits], col[kEncUnits];
     int64_t at[kEncUnits];
     float e[kEncUnits][VU];
 #pragma unroll
     for (int k = 0; k < kEncUnits; ++k) {
-      const Idx u = min(u0 + k * 256, units - 1), n = u / upr;
+      const int64_t u = min(u0 + k * 256, units - 1), n = u / upr;
       col[k] = group_col<VU, RAG>((int)(u - n * upr), D);
-      at[k] = (int64_t)n * D + col[k];
-      r[k] = tok_row(ids, (int64_t)n, V, pad);
+      at[k] = n * D + col[k];
+      r[k] = tok_row(ids, n, V, pad);
     }
 #pragma unroll
     for (int k = 0; k < kEncUnits; ++k)  // an absent token reads row 0
@@ -151,13 +151,13 @@ struct SegArgs {
   float scale;
 };
 
-template <int DT, int VU, bool RAG>
+template <int DT, int VU>
 __device__ inline void seg_write(const SegArgs& a, int v, int d, const float (&sum)[VU], const float (&e)[VU],
                                  typename TabType<DT>::t* __restrict__ gtab) {
   float g[VU];
 #pragma unroll
   for (int j = 0; j < VU; ++j) g[j] = sum[j] * tok_slope(e[j], a.scale);
-  tab_store<DT, VU, RAG>(gtab + (int64_t)v * a.D + d, g);
+  tab_store<DT, VU>(gtab + (int64_t)v * a.D + d, g);
 }
 
 // G lanes sum a chunk of C entries, VU columns each, kSegAhead rows of the
@@ -169,7 +169,7 @@ __device__ inline void seg_write(const SegArgs& a, int v, int d, const float (&s
 // adds its runs at once (one atomic a run on one address took most of the
 // kernel: 17 us at 65536 tokens of 64 values).
 constexpr int kSegAhead = 4;
-template <int DT, int VU, bool RAG>
+template <int DT, int VU>
 __global__ void __launch_bounds__(256)
 tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict__ gy,
                    const typename TabType<DT>::t* __restrict__ tab,
@@ -186,7 +186,7 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
   const int after = i1 < a.N ? ent[i1].x : -1;
   // absent tokens from the chunk's start to the end: nothing
   for (int q = c < a.chunks && first < a.V ? l : a.D; q * VU < a.D; q += a.G) {
-    const int d = group_col<VU, RAG>(q, a.D);
+    const int d = group_col<VU>(q, a.D);
     bool from_before = begun;
     float sum[VU];
 #pragma unroll
@@ -201,7 +201,7 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
 #pragma unroll
       for (int u = 0; u < kSegAhead; ++u) {
         e[u] = next[u];
-        tab_load<kTabF32, VU, RAG>(gy + (int64_t)(uint32_t)e[u].y * a.D + d, g[u]);
+        tab_load<kTabF32, VU>(gy + (int64_t)(uint32_t)e[u].y * a.D + d, g[u]);
       }
 #pragma unroll
       for (int u = 0; u < kSegAhead; ++u) next[u] = ent[min(i + kSegAhead + u, i1 - 1)];
@@ -210,7 +210,7 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
         const int64_t at = i + u + 1;
         const int then = at < i1 ? (u + 1 < kSegAhead ? e[(u + 1) % kSegAhead].x : next[0].x) : after;
         ends[u] = i + u < i1 && e[u].x < a.V && e[u].x != then;
-        if (ends[u]) tab_load<DT, VU, RAG>(tab + (int64_t)e[u].x * a.D + d, t[u]);
+        if (ends[u]) tab_load<DT, VU>(tab + (int64_t)e[u].x * a.D + d, t[u]);
       }
 #pragma unroll
       for (int u = 0; u < kSegAhead; ++u) {
@@ -218,8 +218,8 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
 #pragma unroll
         for (int j = 0; j < VU; ++j) sum[j] += g[u][j];
         if (ends[u]) {
-          if (from_before) tab_store<kTabF32, VU, RAG>(edge + c * a.D + d, sum);
-          else seg_write<DT, VU, RAG>(a, e[u].x, d, sum, t[u], gtab);
+          if (from_before) tab_store<kTabF32, VU>(edge + c * a.D + d, sum);
+          else seg_write<DT, VU>(a, e[u].x, d, sum, t[u], gtab);
           from_before = false;
 #pragma unroll
           for (int j = 0; j < VU; ++j) sum[j] = 0.0f;
@@ -230,9 +230,9 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
     const int row = ent[i1 - 1].x;
     if (row < a.V && after == row) {  // the last run goes on
       if (from_before) {
-        tab_store<kTabF32, VU, RAG>(edge + c * a.D + d, sum);
+        tab_store<kTabF32, VU>(edge + c * a.D + d, sum);
       } else {
-        tab_store<kTabF32, VU, RAG>(edge + (a.chunks + c) * a.D + d, sum);
+        tab_store<kTabF32, VU>(edge + (a.chunks + c) * a.D + d, sum);
         if (q == 0) runs[atomicAdd(&n_runs, 1)] = (int)c;
       }
     }
@@ -249,7 +249,7 @@ tok_segment_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restr
 // ascending order), whose sums are added in order. T = 1024 for few long runs
 // (tok_join_threads).
 constexpr int kJoinNear = 8;
-template <int DT, int VU, bool RAG, int T>
+template <int DT, int VU, int T>
 __global__ void __launch_bounds__(T)
 tok_join_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict__ edge,
                 const typename TabType<DT>::t* __restrict__ tab,
@@ -279,18 +279,18 @@ tok_join_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict
         if (l == 0) far[atomicAdd(&n_far, 1)] = (int)c;
       } else {
         for (int q = l; q * VU < a.D; q += a.G) {
-          const int d = group_col<VU, RAG>(q, a.D);
+          const int d = group_col<VU>(q, a.D);
           float s[VU], e[VU], g[kJoinNear - 1][VU];
-          tab_load<kTabF32, VU, RAG>(edge + (a.chunks + c) * a.D + d, s);
-          tab_load<DT, VU, RAG>(tab + (int64_t)row * a.D + d, e);
+          tab_load<kTabF32, VU>(edge + (a.chunks + c) * a.D + d, s);
+          tab_load<DT, VU>(tab + (int64_t)row * a.D + d, e);
 #pragma unroll
           for (int u = 0; u < kJoinNear - 1; ++u)
-            tab_load<kTabF32, VU, RAG>(edge + (c + 1 + min(u, m - 1)) * a.D + d, g[u]);
+            tab_load<kTabF32, VU>(edge + (c + 1 + min(u, m - 1)) * a.D + d, g[u]);
 #pragma unroll
           for (int u = 0; u < kJoinNear - 1; ++u)
 #pragma unroll
             for (int j = 0; j < VU; ++j) s[j] += u < m ? g[u][j] : 0.0f;
-          seg_write<DT, VU, RAG>(a, row, d, s, e, gtab);
+          seg_write<DT, VU>(a, row, d, s, e, gtab);
         }
       }
     }
@@ -315,7 +315,7 @@ tok_join_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict
       }
       for (int q0 = 0; q0 * VU < a.D; q0 += a.G) {
         const bool on = (q0 + l) * VU < a.D;
-        const int d = on ? group_col<VU, RAG>(q0 + l, a.D) : 0;
+        const int d = on ? group_col<VU>(q0 + l, a.D) : 0;
         float sum[VU];
 #pragma unroll
         for (int j = 0; j < VU; ++j) sum[j] = 0.0f;
@@ -325,7 +325,7 @@ tok_join_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict
             float g[U][VU];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-              tab_load<kTabF32, VU, RAG>(edge + min(q + (int64_t)u * P, last) * a.D + d, g[u]);
+              tab_load<kTabF32, VU>(edge + min(q + (int64_t)u * P, last) * a.D + d, g[u]);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -337,12 +337,12 @@ tok_join_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict
         __syncthreads();
         if (part == 0 && on) {
           float s[VU], e[VU];
-          tab_load<kTabF32, VU, RAG>(edge + (a.chunks + c) * a.D + d, s);
-          tab_load<DT, VU, RAG>(tab + (int64_t)row * a.D + d, e);
+          tab_load<kTabF32, VU>(edge + (a.chunks + c) * a.D + d, s);
+          tab_load<DT, VU>(tab + (int64_t)row * a.D + d, e);
           for (int p = 0; p < P; ++p)
 #pragma unroll
             for (int j = 0; j < VU; ++j) s[j] += red[(p * a.G + l) * VU + j];
-          seg_write<DT, VU, RAG>(a, row, d, s, e, gtab);
+          seg_write<DT, VU>(a, row, d, s, e, gtab);
         }
         __syncthreads();
       }
@@ -368,19 +368,33 @@ tok_bits_kernel(const typename TabType<DT>::t* __restrict__ tab, int64_t words, 
   }
 }
 
-// Bits as uint8 [N, D], VU of a token a thread (D a multiple of VU).
+// Bits as uint8 [N, D], VU of a token a thread (D >= VU), written at any byte;
+// a token's last run is moved back to end with it. 4.2 M tokens of 100 bits:
+// 132 us with 16 bits a thread, 250 with 4 (and 8.4 M of 6: 82 us a bit a
+// thread, 48 with 4).
 template <typename IdT, int VU>
 __global__ void __launch_bounds__(256)
-tok_bytes_kernel(const IdT* __restrict__ ids, int64_t units, int upr, int V, int64_t pad, int DW,
+tok_bytes_kernel(const IdT* __restrict__ ids, int64_t units, int upr, int D, int V, int64_t pad, int DW,
                  const uint64_t* __restrict__ bits, uint8_t* __restrict__ out) {
+  constexpr int VW = VU < 4 ? 1 : VU / 4;
+  typedef uint32_t run __attribute__((ext_vector_type(VW), aligned(1)));
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < units; i += (int64_t)gridDim.x * 256) {
     const int64_t n = i / upr;
-    const int d = (int)(i - n * upr) * VU, r = tok_row(ids, n, V, pad);
-    const uint32_t b = r < V ? (uint32_t)(bits[(int64_t)r * DW + (d >> 6)] >> (d & 63)) : 0u;
-    if constexpr (VU == 4)
-      reinterpret_cast<uint32_t*>(out)[i] = ((b & 15u) * 0x00204081u) & 0x01010101u;  // bit j to byte j
-    else
+    const int d = group_col<VU>((int)(i - n * upr), D), r = tok_row(ids, n, V, pad), s = d & 63;
+    uint32_t b = 0;
+    if (r < V) {
+      const uint64_t* w = bits + (int64_t)r * DW + (d >> 6);
+      b = (uint32_t)(w[0] >> s);
+      if (s + VU > 64) b |= (uint32_t)(w[1] << (64 - s));
+    }
+    if constexpr (VU >= 4) {
+      run v;
+#pragma unroll
+      for (int j = 0; j < VW; ++j) v[j] = (((b >> (4 * j)) & 15u) * 0x00204081u) & 0x01010101u;  // bit j to byte j
+      *reinterpret_cast<run*>(out + n * D + d) = v;
+    } else {
       out[i] = (uint8_t)(b & 1u);
+    }
   }
 }
 
@@ -410,12 +424,31 @@ __device__ inline uint64_t wave_transpose(uint64_t m) {
   return (uint64_t)hi << 32 | lo;
 }
 
+constexpr int kPackTokens = 4;
+// The rows of kPackTokens neighbouring tokens of which n are there (the rest:
+// absent), as 16-byte loads where all are.
+template <typename IdT>
+__device__ inline void tok_rows(const IdT* __restrict__ p, int64_t n, int V, int64_t pad, int (&row)[kPackTokens]) {
+  IdT t[kPackTokens];
+  if (n >= kPackTokens) {
+    typedef IdT t4 __attribute__((ext_vector_type(kPackTokens), aligned(sizeof(IdT))));
+    const t4 r = *reinterpret_cast<const t4*>(p);
+#pragma unroll
+    for (int u = 0; u < kPackTokens; ++u) t[u] = r[u];
+  } else {
+#pragma unroll
+    for (int u = 0; u < kPackTokens; ++u) t[u] = u < n ? p[u] : (IdT)-1;
+  }
+#pragma unroll
+  for (int u = 0; u < kPackTokens; ++u) row[u] = tok_row(t, u, V, pad);
+}
 // Bits packed 64 samples a word. A wave takes 64 samples' word dw of kPackTokens
 // neighbouring tokens (whose ids share memory lines) and transposes each: lane
 // j then holds feature j's word. Word-major rows of features are written as
 // they are; for the rows [F][nw] a workgroup's waves take TW neighbouring
-// words, which leave through LDS in runs of TW.
-constexpr int kPackTokens = 4, kPackFew = 8;
+// words, which leave through LDS in runs of TW. Bound by the loads of
+// single rows of bits, a line each: 65536 x 16 tokens of 64 bits 9.7 us (25 MB,
+// 2.6 TB/s; with the ids loaded one by one 13.4), 65536 x 128 of 2 bits 43.
 template <typename IdT, bool WM, int TW>
 __global__ void __launch_bounds__(64 * TW)
 tok_packed_kernel(const IdT* __restrict__ ids, int64_t B, int64_t L, int V, int64_t pad, int D, int DW,
@@ -430,24 +463,16 @@ tok_packed_kernel(const IdT* __restrict__ ids, int64_t B, int64_t L, int V, int6
     const int64_t w = t * TW + wave, b = w * 64 + lane;
     int row[kPackTokens];
     uint64_t m[kPackTokens];
+    tok_rows(ids + min(b, B - 1) * L + l0, L - l0, V, pad, row);
+    if (b >= B)
 #pragma unroll
-    for (int u = 0; u < kPackTokens; ++u)
-      row[u] = b < B && l0 + u < L ? tok_row(ids, b * L + l0 + u, V, pad) : V;
+      for (int u = 0; u < kPackTokens; ++u) row[u] = V;
 #pragma unroll
     for (int u = 0; u < kPackTokens; ++u) m[u] = row[u] < V ? bits[(int64_t)row[u] * DW + dw] : 0ull;
     const int d = dw * 64 + lane;
 #pragma unroll
     for (int u = 0; u < kPackTokens; ++u) {
-      uint64_t v = 0;
-      if (D <= kPackFew) {  // a ballot a bit
-#pragma unroll
-        for (int j = 0; j < kPackFew; ++j) {
-          const uint64_t all = __ballot((m[u] >> j) & 1);
-          v = lane == j ? all : v;
-        }
-      } else {
-        v = wave_transpose(m[u]);
-      }
+      const uint64_t v = wave_transpose(m[u]);
       if constexpr (WM) {
         if (w < nw && d < D && l0 + u < L) out[w * F + (l0 + u) * D + d] = v;
       } else {
@@ -485,16 +510,6 @@ static void tok_dispatch(int dtype, int id_bytes, F&& f) {
   else ids(std::integral_constant<int, kTabF16>{});
 }
 
-// f(values a lane takes, whether rows are ragged) by the width and the
-// alignment of every row.
-template <typename F>
-static void tok_vector(int64_t D, bool aligned, F&& f) {
-  using Yes = std::true_type;
-  using No = std::false_type;
-  if (D % 4 == 0 && aligned) f(std::integral_constant<int, 4>{}, No{});
-  else if (D >= 4) f(std::integral_constant<int, 4>{}, Yes{});
-  else f(std::integral_constant<int, 1>{}, No{});
-}
 
 // Threads of a join's workgroup: 256, or 1024 where a few rows have all tokens,
 // whose runs a workgroup each then reads (131072 tokens of 512 values over 2
@@ -551,20 +566,18 @@ int slg_token_encode(const void* ids, int32_t id_bytes, int64_t N, int64_t V, in
     constexpr int DT = decltype(dt)::value;
     using Id = decltype(it);
     using T = typename TabType<DT>::t;
-    tok_vector(D, (uintptr_t)table % (4 * sizeof(T)) == 0 && (uintptr_t)y % 16 == 0, [&](auto vu, auto rag) {
-      constexpr int VU = decltype(vu)::value;
-      constexpr bool RAG = decltype(rag)::value;
-      const int64_t upr = cdiv(D, VU), units = N * upr;
-      auto go = [&](auto kern, auto idx) {
-        using Idx = decltype(idx);
-        hipLaunchKernelGGL(kern, dim3(grid_of(cdiv(units, 256 * kEncUnits))), dim3(256), 0, st,
-                           static_cast<const Id*>(ids), (Idx)units, (Idx)upr, (int)D, (int)V, pad,
-                           static_cast<const T*>(table), nlog2, ste, y);
-      };
-      // a round of the grid past the last unit still counts within 32 bits
-      if (units < (1LL << 31)) go(tok_encode_kernel<DT, Id, VU, RAG, uint32_t>, uint32_t(0));
-      else go(tok_encode_kernel<DT, Id, VU, RAG, int64_t>, int64_t(0));
-    });
+    auto go = [&](auto kern, int vu) {
+      const int64_t upr = cdiv(D, vu), units = N * upr;
+      hipLaunchKernelGGL(kern, dim3(grid_of(cdiv(units, 256 * kEncUnits))), dim3(256), 0, st,
+                         static_cast<const Id*>(ids), units, upr, (int)D, (int)V, pad,
+                         static_cast<const T*>(table), nlog2, ste, y);
+    };
+    // whole aligned groups (524288 x 256: 84 us, taken as ragged ones 92), any
+    // rows of 4 values (2.4 M x 27: 62 us, a value a thread 102), narrower ones
+    const bool whole = D % 4 == 0 && (uintptr_t)table % (4 * sizeof(T)) == 0 && (uintptr_t)y % 16 == 0;
+    if (whole) go(tok_encode_kernel<DT, Id, 4, false>, 4);
+    else if (D >= 4) go(tok_encode_kernel<DT, Id, 4, true>, 4);
+    else go(tok_encode_kernel<DT, Id, 1, true>, 1);
   });
   SLG_LAUNCH_CHECK("token_encode");
   return 0;
@@ -599,19 +612,18 @@ int slg_token_encode_bwd(const void* ids, int32_t id_bytes, int64_t N, int64_t V
       return;
     }
     const int2* ent = radix_sort(TokenKeys<Id>{static_cast<const Id*>(ids), (int)V, pad}, p.sort, workspace, clear, st);
-    const bool aligned = (uintptr_t)table % (4 * sizeof(T)) == 0 && (uintptr_t)gy % 16 == 0;
-    tok_vector(D, aligned, [&](auto vu, auto rag) {
+    auto go = [&](auto vu) {
       constexpr int VU = decltype(vu)::value;
-      constexpr bool RAG = decltype(rag)::value;
       const SegArgs s{N, p.chunks, (int)V, (int)D, p.C, p.G, scale};
-      hipLaunchKernelGGL((tok_segment_kernel<DT, VU, RAG>), dim3((unsigned)cdiv(p.chunks, 256 / p.G)), dim3(256), 0, st,
-                         s, ent, gy, static_cast<const T*>(table), static_cast<T*>(gtable), edge, listed + 1,
-                         listed);
+      hipLaunchKernelGGL((tok_segment_kernel<DT, VU>), dim3((unsigned)cdiv(p.chunks, 256 / p.G)), dim3(256), 0, st, s,
+                         ent, gy, static_cast<const T*>(table), static_cast<T*>(gtable), edge, listed + 1, listed);
       const int T2 = tok_join_threads(p.chunks, V);
-      hipLaunchKernelGGL((T2 == 1024 ? tok_join_kernel<DT, VU, RAG, 1024> : tok_join_kernel<DT, VU, RAG, 256>),
+      hipLaunchKernelGGL((T2 == 1024 ? tok_join_kernel<DT, VU, 1024> : tok_join_kernel<DT, VU, 256>),
                          dim3((unsigned)std::min<int64_t>(p.chunks, 512 * 1024 / T2)), dim3(T2), 0, st, s, ent, edge,
                          static_cast<const T*>(table), static_cast<T*>(gtable), listed + 1, listed);
-    });
+    };
+    if (p.VU == 4) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 1>{});
   });
   SLG_LAUNCH_CHECK("token_encode_bwd");
   return 0;
@@ -648,10 +660,12 @@ int slg_token_encode_hard(const void* ids, int32_t id_bytes, int64_t B, int64_t 
     const Id* id = static_cast<const Id*>(ids);
     if (layout == 2) {
       auto go = [&](auto kern, int64_t vu) {
-        hipLaunchKernelGGL(kern, dim3(grid_of(cdiv(N * D / vu, 256))), dim3(256), 0, st, id, N * D / vu,
-                           (int)(D / vu), (int)V, pad, (int)DW, bits, static_cast<uint8_t*>(out));
+        const int64_t upr = cdiv(D, vu), units = N * upr;
+        hipLaunchKernelGGL(kern, dim3(grid_of(cdiv(units, 256))), dim3(256), 0, st, id, units, (int)upr, (int)D,
+                           (int)V, pad, (int)DW, bits, static_cast<uint8_t*>(out));
       };
-      if (D % 4 == 0 && (uintptr_t)out % 4 == 0) go(tok_bytes_kernel<Id, 4>, 4);
+      if (D >= 16) go(tok_bytes_kernel<Id, 16>, 16);
+      else if (D >= 4) go(tok_bytes_kernel<Id, 4>, 4);
       else go(tok_bytes_kernel<Id, 1>, 1);
       return;
     }
@@ -659,8 +673,13 @@ int slg_token_encode_hard(const void* ids, int32_t id_bytes, int64_t B, int64_t 
       hipLaunchKernelGGL(kern, dim3(grid_of(cdiv(cdiv(nw, tw) * cdiv(L, kPackTokens) * DW, 8) * 8)), dim3(64 * tw), 0, st, id, B, L, (int)V, pad,
                          (int)D, (int)DW, nw, bits, static_cast<uint64_t*>(out));
     };
-    if (layout == 1) go(tok_packed_kernel<Id, true, 4>, 4);
-    else if (nw == 1) go(tok_packed_kernel<Id, false, 1>, 1);
+    // as many neighbouring words a workgroup as there are, so that no wave
+    // idles (one word's tokens, 64 x 20000 x 64 bits: 11 us; with 4 and 8
+    // words a workgroup 15 and 27), up to 8, whose rows leave in runs of 64
+    // bytes (65536 x 64 x 100 bits: 32 us; with 4 the same, with 1 52). One
+    // word a feature lies the same in both layouts.
+    if (nw == 1) go(tok_packed_kernel<Id, false, 1>, 1);
+    else if (layout == 1) go(tok_packed_kernel<Id, true, 4>, 4);
     else if (nw <= 4) go(tok_packed_kernel<Id, false, 4>, 4);
     else go(tok_packed_kernel<Id, false, 8>, 8);
   });
