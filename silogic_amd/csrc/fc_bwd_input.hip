@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(256) ig_entries_kernel(IgArgs a, const int2* _
 
 // The whole table in one launch, a workgroup per input block, for one pass
 // (ig_small): the references that fall in the block are counted, placed and
-// ranked in LDS, where the eight launches of the general way pass everything
+// ranked in LDS, where the launches of the general way (the sort's, three more) pass everything
 // through memory. Each workgroup reads all candidates, twice.
 __global__ void __launch_bounds__(1024)
 ig_table_kernel(IgArgs a, const int* __restrict__ cand, const float* __restrict__ w,
@@ -649,7 +649,11 @@ static IwPlan iw_plan(int64_t B, int64_t IN, int64_t OUT, int nsides, int K) {
 // row and the block's references. Wide: the transpose and the gather over 256
 // samples at a time, and the list of one input, which is walked alone. FC
 // backward from LDS / wide, K = 8: 10000 -> 10000, B = 1024: 186 / 273 us; 60000
-// -> 60000, B = 124: 1332 / 1175; 172000 -> 172000, B = 3: 3046 / 1207.
+// -> 60000, B = 124: 1332 / 1175; 172000 -> 172000, B = 3: 3046 / 1207. The fit is
+// that of a slower reference table; it stays, so that layers keep their sums'
+// order. With the sort (8-bit backward, us from LDS / wide): K = 8 10000 ->
+// 10000, B = 1024 143 / 196, B = 256 99 / 87; 40000 -> 40000, B = 124 336 / 217;
+// K = 4 12000 -> 12000, B = 300 134 / 92; 16380 -> 16380, B = 1024 222 / 248.
 static bool ig_small(const IgArgs& a);
 static bool ig_fits(const IgPlan& p) {
   return p.a.R + p.groups * ig_slack(p.a.IB) < (1LL << 31) && p.nkeys < (1LL << 31) &&
@@ -700,11 +704,11 @@ static int fc_input_grad_wide(const float* gbr, int64_t B, int64_t IN, int64_t O
 // One launch for the whole table: one pass, lists of 32 references on average
 // at most (an element's rank reads its list) and at most 4096 references a
 // block, 48K in all: a workgroup's scattered loads and stores bound it, so it
-// follows the references of a block, and every block reads all of them. FC
-// backward, K = 8, this against the general way, captured: 250 -> 250, B = 64:
-// 40 / 46 us; 1000, B = 256 (4000 a block): 57 / 63; 3000, B = 64 (4000 a
-// block, 48000 in all): 67 / 68; past the rule 4000, B = 64: 77 / 75; 2000,
-// B = 256 (8000 a block): 81 / 73; 1000, B = 1024 (16000): 98 / 76.
+// follows the references of a block, and every block reads all of them. 8-bit
+// backward, K = 8, this against the general way, captured, us: 250 -> 250, B =
+// 64: 35 / 38; 1000, B = 256 (4000 a block): 41 / 48; 3000, B = 64 (4000 a
+// block, 48000 in all): 51 / 58; past the rule 4000, B = 64: 57 / 61; 2000,
+// B = 256 (8000 a block): 58 / 58; 1000, B = 1024 (16000): 73 / 51.
 static size_t ig_small_lds(const IgArgs& a) {
   return (size_t)(a.IB + 1) * 4 + (size_t)a.R * 2;
 }
