@@ -154,8 +154,9 @@ class TokenEncoder(nn.Module):
         version counter, as ``derived`` keys tables; ``derived.clear`` drops
         them). Another stream than the one that made them waits for them. A
         captured call makes its own inside the graph, which then keeps them
-        and reads the weight afresh on every replay."""
-        if torch.cuda.is_current_stream_capturing():
+        and reads the weight afresh on every replay; so does a call on a weight
+        without a version (made in inference mode)."""
+        if torch.cuda.is_current_stream_capturing() or weight.is_inference():
             return ops.token_bits(ops._c(weight.detach()))
         here = ops._stream(weight).value
         key = (weight.data_ptr(), weight._version)

@@ -371,3 +371,16 @@ def test_feeds_a_network():
     hard = net.forward_hard(enc.forward_hard(ids).float())
     for wm in (False, True):
         assert torch.equal(net.forward_hard_packed(enc.forward_packed(ids, word_major=wm), 100, wm), hard)
+
+
+def test_a_weight_made_in_inference_mode():
+    """It has no version counter: every call reads it afresh."""
+    ids = torch.arange(40, device=DEV).view(8, 5) % 9
+    with torch.inference_mode():
+        enc = sl.TokenEncoder(9, 12).to(DEV)
+        for _ in range(2):
+            assert torch.equal(enc.forward_hard(ids).view(40, 12).bool(), enc.weight[ids.view(-1)] > 0)
+            enc.weight.neg_()
+        e = enc.weight[ids.view(-1)].double()
+        want = torch.sigmoid(e)
+        orc.close(enc(ids).view(40, 12), want, (2 * e.abs().max() + 8) * orc.EPS * want, "values")   # as _check
