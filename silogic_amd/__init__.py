@@ -17,7 +17,9 @@ Compute is GPU-only; CPU tensors raise. Covered: nodes ``gate16``,
 ``walsh`` (any arity), ``multilinear`` and ``hybrid`` (arity 2-6) in FC
 layers and conv trees (binary trees of depth 1-5, LUT trees of at most 36
 leaves); wiring ``topk``, ``blocktopk``, ``fixed``; ``GroupSum`` heads;
-``ConvLogicTree`` + ``OrPool``; the layer and network presets.
+``ConvLogicTree`` + ``OrPool``; the layer and network presets; learned bits of
+token ids (``TokenEncoder``) and training activations kept in 8 bits
+(``save_activations``), which the reference has not.
 """
 
 __version__ = "0.1.0"
