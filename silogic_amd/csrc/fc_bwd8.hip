@@ -15,13 +15,14 @@
 //
 // Bound by the vector units: each (sample, output) takes 2K conversions and
 // 2K products twice, and the node's derivatives. 10000 -> 10000, K = 8, B =
-// 4096: 113 us for the weights (1.3 G fused products: 23 TFLOP/s of the 79
-// without packed instructions, and as many conversions), 147 with the operand
-// gradients' 328 MB written too, where the fp32 kernel's weights' part takes
-// 318. Halves multiplied straight from
-// registers (fp16 of the codes by a byte permutation, mixed-precision products)
-// took the same time with fewer instructions; kept from the operands to the
-// weights they spilled (482 us).
+// 4096: 113 us for the weights' part alone (1.3 G fused products and as many
+// conversions), 146 with the operand gradients written too (348 MB of 575 in
+// all, 3.9 TB/s, and 64% of the vector issue), where the fp32 kernel's weights'
+// part takes 318. Halves multiplied straight from registers (fp16 of the codes
+// by a byte permutation, mixed-precision products) took the same time with
+// fewer instructions; kept from the operands to the weights they spilled (482
+// us). The next tile's gy and rows loaded before this one's stores, so that no
+// load waits for a store, took 131 us and 169.
 #include <algorithm>
 
 #include "fc_bwd_input.h"
