@@ -431,20 +431,24 @@ struct IwKeys {
   __device__ int key(int64_t r) const { return min(max(cand[r], 0), IN - 1); }
 };
 
-__global__ void __launch_bounds__(256) iw_entries_kernel(const int2* __restrict__ sorted,
-                                                                  int R, int OUT, int NS, int K,
-                                                                  const float* __restrict__ w,
-                                                                  int2* __restrict__ ent) {
-  const int j = blockIdx.x * blockDim.x + threadIdx.x;
+// Where each input's entries start (the first workgroups), and the entries (the
+// others).
+__global__ void __launch_bounds__(256) iw_entries_kernel(const int2* __restrict__ sorted, int R, int IN,
+                                                         int start_blocks, int OUT, int NS, int K,
+                                                         const float* __restrict__ w, int* __restrict__ start,
+                                                         int2* __restrict__ ent) {
+  if ((int)blockIdx.x < start_blocks) {
+    const int k = blockIdx.x * 256 + threadIdx.x;
+    if (k <= IN) start[k] = ref_start(sorted, R, k);
+    return;
+  }
+  const int j = (blockIdx.x - start_blocks) * 256 + threadIdx.x;
   if (j >= R) return;
   const int r = sorted[j].y, SK = NS * K;  // r = (o * NS + side) * K + k
   const int o = r / SK, side = (r - o * SK) / K;
   ent[j] = make_int2(side * OUT + o, __float_as_int(w[r]));
 }
 
-// gab [R2][LB] = transpose of gbr [B][R2] (rows b >= B of gab's columns are
-// zero), through a 64 x 64 LDS tile; float4 loads along gbr rows when R2 is
-// a multiple of 4, float4 stores along gab rows (LB is a multiple of 64).
 __global__ void __launch_bounds__(256) iw_transpose_kernel(const float* __restrict__ gbr,
                                                                     int B, int R2, int64_t LB,
                                                                     int n_rtiles,
@@ -689,9 +693,9 @@ static int fc_input_grad_wide(const float* gbr, int64_t B, int64_t IN, int64_t O
   int2* ent = reinterpret_cast<int2*>(sort + q.sort);  // offsets are multiples of 4
   const int R = (int)q.R, R2 = (int)q.R2;
   const int2* sorted = radix_sort(IwKeys{cand, (int)IN}, radix_plan(R, IN), sort, RadixClear{}, st);
-  ref_starts(sorted, R, IN, start, nullptr, st);
-  hipLaunchKernelGGL(iw_entries_kernel, dim3((unsigned)cdiv(R, 256)), dim3(256), 0, st, sorted, R,
-                     (int)OUT, nsides, K, w, ent);
+  const int start_blocks = (int)cdiv(IN + 1, 256);
+  hipLaunchKernelGGL(iw_entries_kernel, dim3((unsigned)(start_blocks + cdiv(R, 256))), dim3(256), 0, st, sorted, R,
+                     (int)IN, start_blocks, (int)OUT, nsides, K, w, start, ent);
   hipLaunchKernelGGL(iw_transpose_kernel, dim3((unsigned)n_tr), dim3(256), 0, st, gbr, (int)B, R2, q.LB,
                      (int)n_rtiles, gab);
   // a multiple of 8 workgroups for the XCD order

@@ -21,8 +21,19 @@ int64_t ref_table_ints(int64_t R, int64_t nkeys);
 int build_ref_table(const int* keys, int64_t R, int64_t nkeys, int* ws, hipStream_t st,
                     RefTable* out);
 
-// start[k] = how many of R entries sorted by key (x) lie below key k, k in
-// [0, nkeys]; with sorted, also their references (y) alone.
+// How many of R entries sorted by key (x) lie below key k.
+__device__ inline int ref_start(const int2* __restrict__ ent, int R, int64_t k) {
+  int lo = 0, hi = R;
+  while (lo < hi) {
+    const int mid = lo + ((hi - lo) >> 1);
+    if (ent[mid].x < k) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// start[k] = ref_start of every key k in [0, nkeys]; with sorted, also the
+// entries' references (y) alone.
 void ref_starts(const int2* ent, int64_t R, int64_t nkeys, int* start, int* sorted, hipStream_t st);
 
 }  // namespace slg

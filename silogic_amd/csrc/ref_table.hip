@@ -28,13 +28,7 @@ __global__ void __launch_bounds__(256) ref_start_kernel(const int2* __restrict__
   }
   const int64_t k = b * 256 + threadIdx.x;
   if (k > nkeys) return;
-  int lo = 0, hi = R;
-  while (lo < hi) {
-    const int mid = lo + ((hi - lo) >> 1);
-    if (ent[mid].x < k) lo = mid + 1;
-    else hi = mid;
-  }
-  start[k] = lo;
+  start[k] = ref_start(ent, R, k);
 }
 
 static inline int64_t round4i(int64_t n) { return (n + 3) & ~int64_t(3); }
