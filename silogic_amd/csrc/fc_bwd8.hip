@@ -31,15 +31,15 @@
 
 namespace slg {
 
-// Candidates known to the compiler, 1024 threads: they take half of the time
-// that the loop for any K does, whose 16 slots need 512 threads of twice the
-// registers (weights' part, us: 10000 -> 10000, K = 8, B = 4096 113 for 218;
-// 16380 -> 16380, K = 4, B = 1024 45 for 91; 8000 -> 8000, B = 1024 K = 2 25 for
-// 43, K = 1 22 for 39; with 512 threads 145 and 71 for K = 8 and 4, the loop
-// with 1024 118 for 52 at K = 5).
-constexpr bool bwd8_compiled(int K) { return K == 1 || K == 2 || K == 4 || K == 8; }
-template <int KC>
-constexpr int bwd8_threads() { return KC > 0 ? 1024 : 512; }
+// Candidate slots of a thread: those past K have input 0 and weight 0, which the
+// codes, always finite, leave without a trace; a loop that skips them (16
+// slots, 512 threads of twice the registers) only past 8. Weights' part, us,
+// against that loop for any K: 10000 -> 10000, B = 4096, K = 8 110 for 218; 16380
+// -> 16380, B = 1024, K = 4 45 for 91; 8000 -> 8000, B = 1024, K = 1 22 for 39, 2 25
+// for 44, 3 24 for 43, 5 36 for 52, 7 37 for 56. With 512 threads K = 8 and 4 took
+// 145 and 71, the loop with 1024 118 for 52 at K = 5.
+constexpr int bwd8_slots(int K) { return K <= 1 ? 1 : K <= 2 ? 2 : K <= 4 ? 4 : K <= 8 ? 8 : 16; }
+constexpr int bwd8_threads(int KM) { return KM <= 8 ? 1024 : 512; }
 
 // The four codes of a word as floats (v_cvt_f32_ubyte0..3).
 __device__ inline float code_of(uint32_t w, int v) { return (float)((w >> (8 * v)) & 255u); }
@@ -48,16 +48,15 @@ __device__ inline float code_of(uint32_t w, int v) { return (float)((w >> (8 * v
 // fc_soft_bwd_w_kernel writes them. AHEAD: two tiles in LDS, the next one's
 // codes on their way in registers (up to bwd8_quads quads a thread) while this
 // one computes, one barrier a tile; else one tile and two barriers.
-template <int KC>
-constexpr int bwd8_quads() { return KC == 8 ? 3 : KC == 4 ? 5 : 8; }
-template <int NODE, int KC, bool AHEAD>
-__global__ void __launch_bounds__((bwd8_threads<KC>()))
+constexpr int bwd8_quads(int KM) { return KM == 8 ? 3 : KM == 4 ? 5 : 8; }
+template <int NODE, int KM, bool AHEAD>
+__global__ void __launch_bounds__(bwd8_threads(KM))
 fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ rows, int B, int IN, int ld,
-                 int OUT, int Kr, ParamView pv, float inv_tau, const float* __restrict__ gy, int n_orange,
+                 int OUT, int K, ParamView pv, float inv_tau, const float* __restrict__ gy, int n_orange,
                  int n_range, int tiles_per_range, float* __restrict__ part, float* __restrict__ gbr) {
-  constexpr int S = kRows8Tile, KM = KC > 0 ? KC : 16, NQ = bwd8_quads<KC>();
+  constexpr int S = kRows8Tile, NQ = bwd8_quads(KM);
+  constexpr bool SKIP = KM > 8;  // more slots to skip than the branches cost
   extern __shared__ __align__(16) unsigned char smem[];
-  const int K = KC > 0 ? KC : Kr;
   // the output ranges of one sample range on one XCD: they stage the same codes
   const uint32_t lid = xcd_logical_id(blockIdx.x, gridDim.x);
   const int r_o = (int)(lid % (uint32_t)n_orange);
@@ -66,7 +65,8 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
   const int o = r_o * blockDim.x + threadIdx.x;
   const bool valid = o < OUT;
   FcParams<KM> P;
-  load_params<KC, KM, false>(P, min(o, OUT - 1), K, pv);
+  if (K == KM) load_params<KM, KM, false>(P, min(o, OUT - 1), K, pv);
+  else load_params<0, KM, false>(P, min(o, OUT - 1), K, pv);  // free slots: input 0, weight 0
   const uint32_t lim = (uint32_t)IN - 1u;
   uint32_t pk[KM];  // index pairs (inputs below 65536), clamped into the tile
   float Wa = 0.0f, Wb = 0.0f;
@@ -135,7 +135,7 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
     uint32_t qa[KM], qb[KM];
 #pragma unroll
     for (int k = 0; k < KM; ++k) {
-      if (KC > 0 || k < K) {
+      if (!SKIP || k < K) {
         qa[k] = xs[pk[k] & 0xffffu];
         qb[k] = xs[pk[k] >> 16];
       }
@@ -143,7 +143,7 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
     float A[S] = {0.f, 0.f, 0.f, 0.f}, Bv[S] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < KM; ++k) {
-      if (KC > 0 || k < K) {
+      if (!SKIP || k < K) {
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           A[s] = fmaf(P.fa[k], code_of(qa[k], s), A[s]);
@@ -180,7 +180,7 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
     }
 #pragma unroll
     for (int k = 0; k < KM; ++k) {
-      if (KC > 0 || k < K) {
+      if (!SKIP || k < K) {
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           swa[k] = fmaf(ga[s], code_of(qa[k], s), swa[k]);
@@ -197,7 +197,7 @@ fc_bwd8_w_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ r
     float* base = part + (int64_t)r_b * (2 * K + 4) * OUT + o;
 #pragma unroll
     for (int k = 0; k < KM; ++k) {
-      if (KC > 0 || k < K) {
+      if (k < K) {
         base[(int64_t)k * OUT] = swa[k] + sla;
         base[(int64_t)(K + k) * OUT] = swb[k] + slb;
       }
@@ -296,7 +296,7 @@ static bool bwd8_takes(int64_t B, int64_t IN, int64_t OUT, int K) {
 
 static Bwd8Plan bwd8_plan(int64_t B, int64_t IN, int64_t OUT, int K) {
   Bwd8Plan p{};
-  p.threads = bwd8_compiled(K) ? 1024 : 512;
+  p.threads = bwd8_threads(bwd8_slots(K));
   p.n_orange = (int)cdiv(OUT, p.threads);
   const int64_t n_tiles = cdiv(std::max<int64_t>(B, 1), kRows8Tile);
   // one round of workgroups: as many sample ranges as resident slots allow
@@ -324,12 +324,12 @@ struct Bwd8Args {
   float *part, *gbr;
 };
 
-template <int NODE, int KC>
+template <int NODE, int KM>
 static int launch_bwd8(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
   const int64_t ld = rows8_ld(a.IN);
-  const bool ahead = p.tiles_per_range > 1 && ld <= bwd8_quads<KC>() * 4 * bwd8_threads<KC>() &&
+  const bool ahead = p.tiles_per_range > 1 && ld <= bwd8_quads(KM) * 4 * bwd8_threads(KM) &&
                      ld * 8 <= bwd8_lds_cap();
-  auto kern = ahead ? fc_bwd8_w_kernel<NODE, KC, true> : fc_bwd8_w_kernel<NODE, KC, false>;
+  auto kern = ahead ? fc_bwd8_w_kernel<NODE, KM, true> : fc_bwd8_w_kernel<NODE, KM, false>;
   const size_t lds = (size_t)ld * 4 * (ahead ? 2 : 1);
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -339,7 +339,7 @@ static int launch_bwd8(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
   // a thread reads its output's parameters once, from where they are: records
   // (as the fp32 kernels take) would be a launch and 5 us to save less
   const ParamView pv{a.cand, a.cand + a.K, a.w, a.w + a.K, a.np, 2 * a.K, 2 * a.K, 4, nullptr};
-  hipLaunchKernelGGL(kern, dim3((unsigned)(cdiv((int64_t)p.n_orange * p.NR, 8) * 8)), dim3(bwd8_threads<KC>()),
+  hipLaunchKernelGGL(kern, dim3((unsigned)(cdiv((int64_t)p.n_orange * p.NR, 8) * 8)), dim3(bwd8_threads(KM)),
                      lds, st, a.codes, a.rows, (int)a.B, (int)a.IN, (int)ld, (int)a.OUT, a.K, pv,
                      a.inv_tau, a.gy, p.n_orange, p.NR, p.tiles_per_range, a.part, a.gbr);
   SLG_LAUNCH_CHECK("fc_soft_bwd8");
@@ -348,11 +348,13 @@ static int launch_bwd8(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
 
 template <int NODE>
 static int launch_bwd8_k(const Bwd8Args& a, const Bwd8Plan& p, hipStream_t st) {
-  if (a.K == 8) return launch_bwd8<NODE, 8>(a, p, st);  // 16-byte loads: alignment checked
-  if (a.K == 4) return launch_bwd8<NODE, 4>(a, p, st);
-  if (a.K == 2) return launch_bwd8<NODE, 2>(a, p, st);
-  if (a.K == 1) return launch_bwd8<NODE, 1>(a, p, st);  // fixed wiring
-  return launch_bwd8<NODE, 0>(a, p, st);
+  switch (bwd8_slots(a.K)) {
+    case 1: return launch_bwd8<NODE, 1>(a, p, st);  // fixed wiring
+    case 2: return launch_bwd8<NODE, 2>(a, p, st);
+    case 4: return launch_bwd8<NODE, 4>(a, p, st);
+    case 8: return launch_bwd8<NODE, 8>(a, p, st);
+    default: return launch_bwd8<NODE, 16>(a, p, st);
+  }
 }
 
 // Checks, the weight kernel and the input gradient: partials of the weights'
