@@ -35,8 +35,36 @@ struct HeadArgs {
 
 // Widest workgroup per variant: 1024 threads keeps <= 128 VGPRs per lane,
 // which fits the lean variants; the others get 512 threads and more registers.
+// Slots of a thread for a candidate count known when compiled (KC > 0), of at
+// most -KC (KC < 0) or of at most 16.
+template <int KC>
+constexpr int soft_slots() { return KC > 0 ? KC : KC < 0 ? -KC : 16; }
 template <int KC, int S>
 constexpr int soft_max_threads() { return (KC == 0 || S >= 8) ? 512 : 1024; }
+
+// acc += sum over k < K of w[k] src[idx[k]], k ascending. With K known only at
+// run time, quads of gathers are issued together (a slot past K gathers input 0
+// and is not added: 0 times an infinity is none).
+template <int KC, int KM, typename vt>
+__device__ inline void slot_sum(vt& acc, const float (&w)[KM], const vt* src, const uint32_t (&idx)[KM], int K) {
+  if constexpr (KC > 0) {
+#pragma unroll
+    for (int k = 0; k < KM; ++k) fma_acc(acc, w[k], src[idx[k]]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < KM; q += 4) {
+      if (q < K) {
+        vt v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = src[idx[q + e]];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (q + e < K) fma_acc(acc, w[q + e], v[e]);
+      }
+    }
+  }
+}
 
 // PACK: the input also in 8 bits (rows8.h), from the staged tile: what a
 // training layer keeps of it, without reading it again (10000 -> 10000, K = 8,
@@ -48,7 +76,7 @@ fc_soft_kernel(const float* __restrict__ x, int B, int IN, int OUT, int Kr, Para
                Rows8Out po) {
   constexpr int V = S >= 4 ? 4 : S;
   constexpr int G = S / V;
-  constexpr int KM = KC > 0 ? KC : 16;
+  constexpr int KM = soft_slots<KC>();
   using vt = typename vecf<V>::t;
   extern __shared__ __align__(16) unsigned char smem[];
   vt* lds = reinterpret_cast<vt*>(smem);
@@ -127,13 +155,9 @@ fc_soft_kernel(const float* __restrict__ x, int B, int IN, int OUT, int Kr, Para
       // slot a, then slot b: at most K gathers in flight per wave keeps the
       // two parameter sets and the gathered vectors within 128 VGPRs
       vt A = zero_vec<vt>(), Bv = zero_vec<vt>();
-#pragma unroll
-      for (int k = 0; k < KM; ++k)
-        if (KC > 0 || k < K) fma_acc(A, P.fa[k], src[ia[k]]);
+      slot_sum<KC>(A, P.fa, src, ia, K);
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int k = 0; k < KM; ++k)
-        if (KC > 0 || k < K) fma_acc(Bv, P.fb[k], src[ib[k]]);
+      slot_sum<KC>(Bv, P.fb, src, ib, K);
 #pragma unroll
       for (int v = 0; v < V; ++v)
         yv[g * V + v] = node_eval<NODE>(lanev(A, v), lanev(Bv, v), P.p, inv_tau);
@@ -985,6 +1009,12 @@ static int launch_soft_node(const SoftArgs& a, hipStream_t st) {
                      v.cstride % 4 == 0 && v.wstride % 4 == 0;
     if (a.K == 8 && vec) return launch_soft_k<NODE, 8, false, false>(a, st);
     if (a.K == 4 && vec) return launch_soft_k<NODE, 4, false, false>(a, st);
+    // other counts, us, as compiled / as at most 8 / as at most 16 (8000 -> 8000, B =
+    // 1024): K = 1 24 / 33 / 35, K = 2 24 / 35 / 37, K = 3 - / 35 / 36, K = 5 - / 44 /
+    // 48 (2000 -> 2000, B = 4096: 33 / 47), K = 16 - / - / 85
+    if (a.K == 1) return launch_soft_k<NODE, 1, false, false>(a, st);
+    if (a.K == 2) return launch_soft_k<NODE, 2, false, false>(a, st);
+    if (a.K <= 8) return launch_soft_k<NODE, -8, false, false>(a, st);
     return launch_soft_k<NODE, 0, false, false>(a, st);
   }
   set_error("fc_soft: the fused GroupSum takes records");
