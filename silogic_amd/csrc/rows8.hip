@@ -137,6 +137,70 @@ rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_
   }
 }
 
+// Rows too wide for that: the tile's four rows one after the other, NU runs of
+// 4 of one row a thread, while their codes gather in as many words (D <= 4096 *
+// NU; 1024 threads). The next row's values are on their way as soon as the last
+// one's are coded. 2048 x 32000: 73 us, with every value read twice 104 (1500 x
+// 40960: 72 and 99; 64 x 20000: 10.1 and 9.5).
+template <int NU>
+__global__ void __launch_bounds__(1024)
+rows8_pack_wide_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_t* __restrict__ codes,
+                       float* __restrict__ rows) {
+  constexpr int T = 1024, VU = 4, W = T / 64;
+  struct Ends { float lo, hi; };
+  __shared__ Ends part[2][W];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  float e[NU][VU];
+  auto load = [&](const float* p, int u) { rows8_load<VU>(p + min((tid + u * T) * VU, D - VU), e[u]); };
+  for (int64_t t = blockIdx.x; t * kRows8Tile < B; t += gridDim.x) {
+    const int64_t b0 = t * kRows8Tile;
+    const int nb = (int)min((int64_t)kRows8Tile, B - b0);
+    uint32_t w[NU][VU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      load(x + b0 * D, u);
+#pragma unroll
+      for (int j = 0; j < VU; ++j) w[u][j] = 0;
+    }
+    for (int v = 0; v < nb; ++v) {
+      Rows8Range r;
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int j = 0; j < VU; ++j) r.take(e[u][j]);
+      r.wave();
+      if (lane == 0) part[v & 1][wave] = {r.lo, r.hi};
+      __syncthreads();  // part[v & 1] is written again two rows on, past the next one's
+      Ends a = part[v & 1][0];
+#pragma unroll
+      for (int k = 1; k < W; ++k) {
+        a.lo = fminf(a.lo, part[v & 1][k].lo);
+        a.hi = fmaxf(a.hi, part[v & 1][k].hi);
+      }
+      float lo, step, inv;
+      rows8_scale(a.lo, a.hi, lo, step, inv);
+      if (tid == 0) {
+        rows[2 * (b0 + v)] = lo;
+        rows[2 * (b0 + v) + 1] = step;
+      }
+      const float* next = x + (b0 + min(v + 1, nb - 1)) * D;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+#pragma unroll
+        for (int j = 0; j < VU; ++j) w[u][j] |= rows8_code(0, 0, e[u][j], lo, inv) << (8 * v);
+        load(next, u);
+      }
+    }
+    uint32_t* c = codes + t * ld;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int i = (tid + u * T) * VU;
+      if (i < D) rows8_store<uint32_t, VU>(c + min(i, D - VU), w[u]);
+    }
+    if (tid < ld - D) c[D + tid] = 0u;
+  }
+}
+
 // Values that the codes stand for: a thread takes VU neighbouring words and
 // writes four rows of them.
 template <int VU>
@@ -172,6 +236,12 @@ static void launch_pack(const float* x, int64_t B, int64_t D, uint32_t* codes, f
                      (int)D, (int)rows8_ld(D), codes, rows);
 }
 
+template <int NU>
+static void launch_pack_wide(const float* x, int64_t B, int64_t D, uint32_t* codes, float* rows, hipStream_t st) {
+  hipLaunchKernelGGL((rows8_pack_wide_kernel<NU>), dim3((unsigned)std::min<int64_t>(cdiv(B, kRows8Tile), kRows8Grid)),
+                     dim3(1024), 0, st, x, B, (int)D, (int)rows8_ld(D), codes, rows);
+}
+
 // The fewest threads that hold a tile in 16 values of each row a thread (32
 // for the widest): fewer, longer threads have less of the range's sums over
 // lanes and waves to do. Measured (us; threads x values a thread):
@@ -181,7 +251,8 @@ static void launch_pack(const float* x, int64_t B, int64_t D, uint32_t* codes, f
 //   8192 x 4001    256 x 16  26.1  1024 x 4    39    read again by 256   43
 //   4096 x 8001    512 x 16  26.6  1024 x 8    29    read again by 512   43
 //   4096 x 16380   512 x 32  68.7  1024 x 16   72    read again by 1024  85
-// Wider rows are read again, from the caches (2048 x 32000: 84).
+// Wider rows go row by row, and those past 40960 (what a workgroup's registers
+// hold) are read again.
 void rows8_pack(const float* x, int64_t B, int64_t D, uint32_t* codes, float* rows, hipStream_t st) {
   if (D < 4) launch_pack<1, 1, 64>(x, B, D, codes, rows, st);
   else if (D <= 256) launch_pack<1, 4, 64>(x, B, D, codes, rows, st);
@@ -191,6 +262,9 @@ void rows8_pack(const float* x, int64_t B, int64_t D, uint32_t* codes, float* ro
   else if (D <= 4096) launch_pack<4, 4, 256>(x, B, D, codes, rows, st);
   else if (D <= 8192) launch_pack<4, 4, 512>(x, B, D, codes, rows, st);
   else if (D <= 16384) launch_pack<8, 4, 512>(x, B, D, codes, rows, st);
+  else if (D <= 24576) launch_pack_wide<6>(x, B, D, codes, rows, st);
+  else if (D <= 32768) launch_pack_wide<8>(x, B, D, codes, rows, st);
+  else if (D <= 40960) launch_pack_wide<10>(x, B, D, codes, rows, st);
   else launch_pack<0, 4, 512>(x, B, D, codes, rows, st);
 }
 

@@ -30,7 +30,8 @@ def _rows(B, D):
 @pytest.mark.parametrize("B,D", [(1, 1), (1, 2), (3, 5), (4, 64), (5, 255), (7, 257), (6, 1000), (9, 1025),
                                  (3, 4097), (2, 8193), (5, 16384), (3, 16387), (2, 70001), (70, 33),
                                  (5, 3), (9, 4), (6, 256), (3, 512), (4, 513), (6, 1024), (3, 2048), (5, 2049), (2, 4096),
-                                 (3, 8192), (2, 16381), (1, 16383)])
+                                 (3, 8192), (2, 16381), (1, 16383), (5, 16385), (3, 24576), (6, 24577), (9, 32771), (4, 40959),
+                                 (7, 40961)])
 def test_pack_and_unpack(B, D):
     x = _rows(B, D)
     codes, rows = sl.pack_rows8(x.to(DEV))
