@@ -330,11 +330,13 @@ int slg_fc_soft_bwd8(const uint8_t* codes, const float* rows, int64_t B, int64_t
  * the former gives them: kept [OUT,4], gate16: followed by its probabilities
  * [OUT,16]); the other way the gradients of slg_fc_soft_bwd8 down to conn and
  * raw (any of gx, gconn, graw may be NULL). conn NULL: fixed wiring. raw, w and
- * kept at multiples of 16 bytes. */
+ * kept at multiples of 16 bytes. Workspaces in floats; the forward's may be
+ * NULL where it takes none. */
+int64_t slg_fc_layer8_fwd_workspace(int64_t B, int64_t IN, int64_t OUT, int32_t K);
 int slg_fc_layer8_fwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t K,
                       const int32_t* cand, const float* conn, const float* raw, int32_t node_kind,
                       float inv_tau, float* y, uint8_t* codes, float* rows, float* w, float* kept,
-                      slg_stream_t stream);
+                      float* workspace, int64_t workspace_floats, slg_stream_t stream);
 int64_t slg_fc_layer8_bwd_workspace(int64_t B, int64_t IN, int64_t OUT, int32_t K);
 int slg_fc_layer8_bwd(const uint8_t* codes, const float* rows, int64_t B, int64_t IN, int64_t OUT,
                       int32_t K, const int32_t* cand, const float* w, const float* kept,

@@ -59,8 +59,9 @@ SIGNATURES = {
     "slg_fc_soft_bwd8_workspace": (_I64, [_I64, _I64, _I64, _I32]),
     "slg_fc_soft_bwd8": (C.c_int, [_P, _P, _I64, _I64, _I64, _I32, _P, _P, _I32, _P, _F32, _P, _P, _P,
                                    _P, _P, _I64, _P]),
+    "slg_fc_layer8_fwd_workspace": (_I64, [_I64, _I64, _I64, _I32]),
     "slg_fc_layer8_fwd": (C.c_int, [_P, _I64, _I64, _I64, _I32, _P, _P, _P, _I32, _F32, _P, _P, _P, _P,
-                                    _P, _P]),
+                                    _P, _P, _I64, _P]),
     "slg_fc_layer8_bwd_workspace": (_I64, [_I64, _I64, _I64, _I32]),
     "slg_fc_layer8_bwd": (C.c_int, [_P, _P, _I64, _I64, _I64, _I32, _P, _P, _P, _I32, _F32, _P, _P, _P,
                                     _P, _P, _I64, _P]),

@@ -27,6 +27,7 @@
 
 #include "fc_bwd_input.h"
 #include "fc_bwd_weights.h"
+#include "fc_soft_common.h"
 #include "rows8.h"
 
 namespace slg {
@@ -413,9 +414,14 @@ int slg_fc_soft_bwd8(const uint8_t* codes, const float* rows, int64_t B, int64_t
   return 0;
 }
 
+int64_t slg_fc_layer8_fwd_workspace(int64_t B, int64_t IN, int64_t OUT, int32_t K) {
+  return fc_soft8_rec_floats(B, IN, OUT, K);
+}
+
 int slg_fc_layer8_fwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t K, const int32_t* cand,
                       const float* conn, const float* raw, int32_t node_kind, float inv_tau, float* y,
-                      uint8_t* codes, float* rows, float* w, float* kept, slg_stream_t stream) {
+                      uint8_t* codes, float* rows, float* w, float* kept, float* workspace, int64_t workspace_floats,
+                      slg_stream_t stream) {
   SLG_REQUIRE(cand && raw && w && kept, SLG_E_ARG, "fc_layer8_fwd: null pointer");
   SLG_REQUIRE(node_kind == SLG_NODE_GATE16 || node_kind == SLG_NODE_WALSH ||
                   node_kind == SLG_NODE_MULTILINEAR2,
@@ -425,7 +431,13 @@ int slg_fc_layer8_fwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_
   const int32_t one = 1;
   const int rc = slg_layer_params(conn, 2 * OUT, K, 1, &raw, &one, OUT, node_kind, 2, 1.0f, w, kept,
                                   node_kind == SLG_NODE_GATE16 ? kept + 4 * OUT : nullptr, stream);
-  return rc ? rc : slg_fc_soft_fwd8(x, B, IN, OUT, K, cand, w, node_kind, kept, inv_tau, y, codes, rows, stream);
+  if (rc) return rc;
+  const int64_t rec = fc_soft8_rec_floats(B, IN, OUT, K);
+  SLG_REQUIRE(workspace_floats >= rec && (rec == 0 || (workspace && (uintptr_t)workspace % 16 == 0)), SLG_E_ARG,
+              "fc_layer8_fwd: workspace of %lld floats, %lld at a multiple of 16 bytes needed",
+              (long long)workspace_floats, (long long)rec);
+  return fc_soft_fwd8(x, B, IN, OUT, K, cand, w, node_kind, kept, inv_tau, y, codes, rows, rec ? workspace : nullptr,
+                      as_stream(stream));
 }
 
 int64_t slg_fc_layer8_bwd_workspace(int64_t B, int64_t IN, int64_t OUT, int32_t K) {

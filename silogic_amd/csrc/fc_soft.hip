@@ -265,11 +265,11 @@ __device__ inline T lds_at(uint32_t off) {
 //  * index halves become LDS byte offsets with one SDWA shift each;
 //  * a slot's KC gathers are issued together before they are accumulated;
 //  * stores take the sample row as a scalar offset.
-template <int NODE, int KC, int S, bool HEAD>
+template <int NODE, int KC, int S, bool HEAD, bool PACK = false>
 __global__ void __launch_bounds__((soft_max_threads<KC, S>()))
 fc_soft_rec_kernel(const float* __restrict__ x, int B, int IN, int OUT,
                    const uint32_t* __restrict__ rec, float inv_tau, float* __restrict__ y,
-                   int n_chunks, int chunk, HeadArgs hd) {
+                   int n_chunks, int chunk, HeadArgs hd, Rows8Out po) {
   static_assert(KC == 4 || KC == 8, "records kernel takes 4 or 8 candidates");
   constexpr int V = S >= 4 ? 4 : S;
   constexpr int G = S / V;
@@ -316,6 +316,10 @@ fc_soft_rec_kernel(const float* __restrict__ x, int B, int IN, int OUT,
   constexpr int NB = V == 4 ? 3 : (V == 2 ? 5 : 10);
   for (int g = 0; g < G; ++g) stage_rows<V, true, NB>(lds + g * IN, x, B, IN, b0 + g * V);
   __syncthreads();
+
+  if constexpr (PACK) {  // as fc_soft_kernel's
+    if (ch == 0) rows8_pack_tile<S>(lds, IN, b0, B, reinterpret_cast<float*>(lds + G * IN), po);
+  }
 
   __amdgpu_buffer_rsrc_t yrows;
   if constexpr (!HEAD) yrows = uniform_rsrc(y + (int64_t)b0 * OUT, rows * OUT * 4);
@@ -935,14 +939,17 @@ static int launch_soft_s(const SoftArgs& a, hipStream_t st) {
   auto kern = fc_soft_kernel<NODE, KC, S, HEAD, REC>;
   const int threads = std::min(a.threads, soft_max_threads<KC, S>());
   size_t lds = (size_t)a.IN * S * sizeof(float) + (HEAD ? (size_t)S * a.hd.C * 4 : 0);
-  if constexpr (!HEAD && !REC && S >= 4) {
+  if constexpr (!HEAD && S >= 4) {
     if (a.po.codes) {
-      kern = fc_soft_kernel<NODE, KC, S, HEAD, REC, true>;
       lds += sizeof(float) * rows8_scratch(S, threads / 64);
+      if constexpr (!REC) kern = fc_soft_kernel<NODE, KC, S, HEAD, REC, true>;
     }
   }
   if constexpr (REC && (KC == 4 || KC == 8)) {
     auto rk = fc_soft_rec_kernel<NODE, KC, S, HEAD>;
+    if constexpr (!HEAD && S >= 4) {
+      if (a.po.codes) rk = fc_soft_rec_kernel<NODE, KC, S, HEAD, true>;
+    }
     SLG_REQUIRE(lds <= (size_t)device_lds_bytes(), SLG_E_SHAPE, "fc_soft: %zu B LDS needed", lds);
     static const size_t static_lds = [&] {
       hipFuncAttributes fa{};
@@ -961,7 +968,7 @@ static int launch_soft_s(const SoftArgs& a, hipStream_t st) {
     }
     hipLaunchKernelGGL(rk, dim3((unsigned)grid), dim3(threads), lds, st, a.x, (int)a.B,
                        (int)a.IN, (int)a.OUT, reinterpret_cast<const uint32_t*>(a.pv.rec),
-                       a.inv_tau, a.y, (int)n_chunks, (int)chunk, a.hd);
+                       a.inv_tau, a.y, (int)n_chunks, (int)chunk, a.hd, a.po);
     SLG_LAUNCH_CHECK("fc_soft");
     return 0;
   }
@@ -1413,6 +1420,36 @@ static ParamView records_view(const float* rec) {
   return ParamView{nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0, 0, rec};
 }
 
+// A tile reads every output's parameters, from the arrays in 16-byte loads that
+// touch a line a lane; records are read as whole lines and cost a launch. They
+// win where many tiles read many outputs (K = 8, tiles of 4 samples or less;
+// with the pack of the input, us, records / arrays): 10000 -> 10000, B = 4096 139 /
+// 165; 16000 -> 16000, B = 512 48 / 59; 100 -> 20000, B = 1024 52 / 62; 8000 -> 8000,
+// B = 2048 63 / 68, B = 1024 37 / 39, B = 512 40 / 40; 2000 -> 2000, B = 1024 27 / 26;
+// tiles of 8 samples, 2000 -> 2000, B = 4096 47 / 36. Four candidates gain nothing
+// (16380 -> 16380, B = 1024 64 / 66; 8000 -> 8000 31 / 29).
+int64_t fc_soft8_rec_floats(int64_t B, int64_t IN, int64_t OUT, int K) {
+  if (B < 1 || IN < 1 || OUT < 1 || K != 8 || IN > 65536 || rec_floats(OUT, K) >= (1LL << 29)) return 0;
+  const int S = pick_tile(IN, 0, B);
+  return S > 0 && S <= 4 && cdiv(B, S) * OUT > (1LL << 21) ? rec_floats(OUT, K) : 0;
+}
+
+int fc_soft_fwd8(const float* x, int64_t B, int64_t IN, int64_t OUT, int K, const int32_t* cand, const float* w,
+                 int node_kind, const float* np, float inv_tau, float* out, uint8_t* codes, float* rows, float* rec,
+                 hipStream_t st) {
+  SLG_REQUIRE(cand && w && np && ((codes && rows) || B == 0), SLG_E_ARG, "fc_soft_fwd8: null pointer");
+  SLG_REQUIRE((uintptr_t)codes % 16 == 0, SLG_E_ARG, "fc_soft_fwd8: codes not at a multiple of 16 bytes");
+  SoftArgs a{x, B, IN, OUT, K, arrays_view(cand, cand + K, 2 * K, w, w + K, 2 * K, np), inv_tau, out, 0, 0,
+             HeadArgs{nullptr, 0, 0, 1.0f},
+             Rows8Out{reinterpret_cast<uint32_t*>(codes), rows, (int)rows8_ld(IN)}};
+  if (rec && B > 0) {
+    fc_soft_pack_records(cand, w, np, OUT, K, IN, rec, st);
+    SLG_LAUNCH_CHECK("fc_soft_fwd8 records");
+    a.pv.rec = rec;
+  }
+  return fc_soft_dispatch8(a, node_kind, st);
+}
+
 }  // namespace slg
 
 using namespace slg;
@@ -1433,12 +1470,8 @@ int slg_fc_soft_fwd8(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t
                      const int32_t* cand, const float* w, int32_t node_kind,
                      const float* node_param, float inv_tau, float* out, uint8_t* codes, float* rows,
                      slg_stream_t stream) {
-  SLG_REQUIRE(cand && w && ((codes && rows) || B == 0), SLG_E_ARG, "fc_soft_fwd8: null pointer");
-  SLG_REQUIRE((uintptr_t)codes % 16 == 0, SLG_E_ARG, "fc_soft_fwd8: codes not at a multiple of 16 bytes");
-  SoftArgs a{x, B, IN, OUT, K, arrays_view(cand, cand + K, 2 * K, w, w + K, 2 * K, node_param),
-             inv_tau, out, 0, 0, HeadArgs{nullptr, 0, 0, 1.0f},
-             Rows8Out{reinterpret_cast<uint32_t*>(codes), rows, (int)rows8_ld(IN)}};
-  return fc_soft_dispatch8(a, node_kind, as_stream(stream));
+  return fc_soft_fwd8(x, B, IN, OUT, K, cand, w, node_kind, node_param, inv_tau, out, codes, rows, nullptr,
+                      as_stream(stream));
 }
 
 int slg_dense_logic_fwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t K,

@@ -61,6 +61,12 @@ __global__ void __launch_bounds__(256) fc_soft_pack_records_kernel(const int* __
   rec[t] = v;
 }
 
+void fc_soft_pack_records(const int* cand, const float* w, const float* np, int64_t OUT, int K, int64_t IN,
+                          float* rec, hipStream_t st) {
+  hipLaunchKernelGGL(fc_soft_pack_records_kernel, dim3((unsigned)cdiv(rec_floats(OUT, K), 256)), dim3(256), 0, st,
+                     cand, w, np, (int)OUT, K, (int)IN, reinterpret_cast<uint32_t*>(rec));
+}
+
 constexpr int kBwdAheadQuads = 3;
 template <int KC>
 constexpr int bwd_threads() { return KC > 0 && KC <= 8 ? 1024 : 512; }
@@ -444,9 +450,7 @@ int slg_fc_soft_bwd(const float* x, int64_t B, int64_t IN, int64_t OUT, int32_t 
   float* gbr = part + p.part_floats;
   float* in_ws = gbr + p.gbr_floats;
   if (!p.SL) {
-    hipLaunchKernelGGL(fc_soft_pack_records_kernel, dim3((unsigned)cdiv(p.rec_floats, 256)),
-                       dim3(256), 0, st, cand, w, node_param, (int)OUT, K, (int)IN,
-                       reinterpret_cast<uint32_t*>(rec));
+    fc_soft_pack_records(cand, w, node_param, OUT, K, IN, rec, st);
     SLG_LAUNCH_CHECK("fc_soft_pack_records");
   }
   const bool want_w = gw || gnp;

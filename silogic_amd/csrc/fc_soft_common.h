@@ -144,6 +144,18 @@ struct ParamView {
 // 65536), K words w_a, K words w_b, zero padding to a whole quad, then one
 // quad of node parameters.
 __host__ __device__ constexpr int rec_quads(int K) { return (3 * K + 3) / 4 + 1; }
+// Floats of a layer's records.
+inline int64_t rec_floats(int64_t OUT, int K) { return (OUT + 63) / 64 * 64 * rec_quads(K) * 4; }
+// Records from separate arrays (candidates in their order).
+void fc_soft_pack_records(const int* cand, const float* w, const float* np, int64_t OUT, int K, int64_t IN,
+                          float* rec, hipStream_t st);
+
+// slg_fc_soft_fwd8; with rec (fc_soft8_rec_floats of them, none: 0) on records
+// packed there first.
+int64_t fc_soft8_rec_floats(int64_t B, int64_t IN, int64_t OUT, int K);
+int fc_soft_fwd8(const float* x, int64_t B, int64_t IN, int64_t OUT, int K, const int32_t* cand, const float* w,
+                 int node_kind, const float* np, float inv_tau, float* out, uint8_t* codes, float* rows, float* rec,
+                 hipStream_t st);
 
 // Per-output parameters held in registers: 2K candidate indices, 2K weights,
 // 4 node coefficients.

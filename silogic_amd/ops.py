@@ -375,8 +375,10 @@ def fc_layer8_fwd(x, cand, conn, raw, node_kind, inv_tau):
     codes, rows = _rows8_empty(x)
     y, w = x.new_empty((B, OUT)), x.new_empty(cand.shape)
     kept = x.new_empty((OUT * (5 if node_kind == GATE16 else 1), 4))
+    ws = _lib.lib().slg_fc_layer8_fwd_workspace(B, IN, OUT, K)
+    work = x.new_empty(ws) if ws else None
     call_on(x, "slg_fc_layer8_fwd", _p(x), B, IN, OUT, K, _p(cand), _p(conn), _p(raw), node_kind,
-            float(inv_tau), _p(y), _p(codes), _p(rows), _p(w), _p(kept))
+            float(inv_tau), _p(y), _p(codes), _p(rows), _p(w), _p(kept), _p(work), ws)
     return y, codes, rows, w, kept
 
 
@@ -405,8 +407,10 @@ class _FcLayer8(torch.autograd.Function):
         y = x.new_empty((B, OUT))
         saved = x.new_empty(at[2] + 16 * OUT * (5 if node_kind == GATE16 else 1), dtype=torch.uint8)
         p = saved.data_ptr()
+        ws = _lib.lib().slg_fc_layer8_fwd_workspace(B, IN, OUT, K)
+        work = x.new_empty(ws) if ws else None
         call_on(x, "slg_fc_layer8_fwd", x.data_ptr(), B, IN, OUT, K, cand.data_ptr(), _p(conn),
-                raw.data_ptr(), node_kind, inv_tau, y.data_ptr(), p, p + at[0], p + at[1], p + at[2])
+                raw.data_ptr(), node_kind, inv_tau, y.data_ptr(), p, p + at[0], p + at[1], p + at[2], _p(work), ws)
         ctx.save_for_backward(cand, saved)
         ctx.meta = (B, IN, OUT, K, node_kind, inv_tau, at)
         return y

@@ -139,10 +139,13 @@ def test_wide_rows(IN):
 
 @pytest.mark.parametrize("B,IN,OUT,K", [(1, 1, 1, 1), (5, 64, 70, 8), (9, 1280, 700, 4), (130, 1281, 40, 8),
                                         (4100, 1300, 64, 4), (4099, 4099, 65, 3), (33, 10000, 129, 8),
-                                        (7, 10177, 30, 8), (6, 16380, 200, 4), (5, 30001, 40, 2), (3, 41000, 50, 8)])
+                                        (7, 10177, 30, 8), (6, 16380, 200, 4), (5, 30001, 40, 2), (3, 41000, 50, 8),
+                                        (130, 40, 70001, 8), (70, 16400, 60007, 8), (41, 30001, 60001, 8)])
 def test_forward_writes_what_pack_writes(B, IN, OUT, K):
     """The codes that a layer's forward makes from its staged tiles (4 and 8 samples, several output chunks a
-    tile) or beside them (narrower tiles), and its output, are those of the separate calls."""
+    tile) or beside them (narrower tiles), and its output, are those of the separate calls; also where the
+    layer reads its parameters from records."""
+    assert (ops._lib.lib().slg_fc_layer8_fwd_workspace(B, IN, OUT, K) > 0) == (OUT > 60000)
     x, cand, conn, raw, _ = _problem(orc.GATE16, B, IN, OUT, K, x=_rows(B, IN))
     if B > 2:
         x[2, IN // 2] = float("nan")
