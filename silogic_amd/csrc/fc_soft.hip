@@ -68,7 +68,8 @@ __device__ inline void slot_sum(vt& acc, const float (&w)[KM], const vt* src, co
 
 // PACK: the input also in 8 bits (rows8.h), from the staged tile: what a
 // training layer keeps of it, without reading it again (10000 -> 10000, K = 8,
-// B = 4096: 165 us, against 144 + 71 for the layer and slg_rows8_pack).
+// B = 4096: 165 us, against 144 + 71 for the layer and slg_rows8_pack; on
+// records 133).
 template <int NODE, int KC, int S, bool HEAD, bool REC, bool PACK = false>
 __global__ void __launch_bounds__((soft_max_threads<KC, S>()))
 fc_soft_kernel(const float* __restrict__ x, int B, int IN, int OUT, int Kr, ParamView pv,
