@@ -107,17 +107,30 @@ class TokenEncoder(nn.Module):
         return enc
 
     def _settle(self, weight, scale, ste, padding_idx):
+        self._check_weight(weight)
+        V = weight.shape[0]
+        if padding_idx is not None:
+            if not -V <= padding_idx < V:
+                raise ValueError(f"TokenEncoder: padding_idx {padding_idx} for {V} tokens")
+            padding_idx %= V
+        self.scale, self.ste, self.padding_idx = float(scale), bool(ste), padding_idx
+        self.weight = weight if isinstance(weight, nn.Parameter) else nn.Parameter(weight)
+
+    @staticmethod
+    def _check_weight(weight):
         if weight.dim() != 2 or 0 in weight.shape:
             raise ValueError(f"TokenEncoder: weight {tuple(weight.shape)}, [num_tokens, bits] expected")
         if weight.dtype not in ops.TABLE_DTYPES:
             raise TypeError(f"TokenEncoder: weight of {weight.dtype} (fp32, bf16 or fp16)")
-        self.num_tokens, self.bits = weight.shape
-        if padding_idx is not None:
-            if not -self.num_tokens <= padding_idx < self.num_tokens:
-                raise ValueError(f"TokenEncoder: padding_idx {padding_idx} for {self.num_tokens} tokens")
-            padding_idx %= self.num_tokens
-        self.scale, self.ste, self.padding_idx = float(scale), bool(ste), padding_idx
-        self.weight = weight if isinstance(weight, nn.Parameter) else nn.Parameter(weight)
+
+    # the present weight's sizes: a weight may be replaced by one of others
+    @property
+    def num_tokens(self):
+        return self.weight.shape[0]
+
+    @property
+    def bits(self):
+        return self.weight.shape[1]
 
     def extra_repr(self):
         return (f"{self.num_tokens}, {self.bits}, scale={self.scale}, ste={self.ste}, "
@@ -133,8 +146,7 @@ class TokenEncoder(nn.Module):
             raise TypeError(f"TokenEncoder: ids of {ids.dtype} (int32 or int64)")
         if ids.dim() not in (1, 2):
             raise ValueError(f"TokenEncoder: ids {tuple(ids.shape)}, [B] or [B, L] expected")
-        if weight.dtype not in ops.TABLE_DTYPES:
-            raise TypeError(f"TokenEncoder: weight of {weight.dtype} (fp32, bf16 or fp16)")
+        self._check_weight(weight)
         ops.require_gpu(ids, weight)
         ops.same_device("TokenEncoder", ids, weight)
         return ops._c(ids if ids.dim() == 2 else ids.unsqueeze(1))
@@ -179,7 +191,7 @@ class TokenEncoder(nn.Module):
     def _hard(self, ids, layout):
         w = self.weight
         ids = self._ids(ids, w)
-        return ops.token_encode_hard(ids, self._bit_table(w), self.bits, self._pad, layout)
+        return ops.token_encode_hard(ids, self._bit_table(w), w.shape[1], self._pad, layout)
 
     def forward_hard(self, ids):
         """uint8 bits ``[B, L*bits]``."""

@@ -532,6 +532,8 @@ def token_encode_hard(ids, bits, D, pad, layout):
     """Bits of ``ids [B, L]``'s tokens: layout 0 ``[L*D, nw]``, 1 ``[nw, L*D]``,
     2 uint8 ``[B, L*D]``."""
     B, L = ids.shape
+    if D < 1 or bits.dim() != 2 or bits.shape[1] != -(-D // 64):
+        raise ValueError(f"token_encode_hard: words {tuple(bits.shape)} for rows of {D} bits")
     nw = n_words(B)
     if layout == 2:
         out = bits.new_empty((B, L * D), dtype=torch.uint8)

@@ -1,0 +1,51 @@
+"""The token encoder's hard bits after its weight was replaced, without a GPU: entry points are recorded, not
+launched."""
+import pytest
+import torch
+
+import silogic_amd as sl
+from silogic_amd import ops
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """Names and arguments of the entry points that a call would launch."""
+    made = []
+    monkeypatch.setattr(ops, "require_gpu", lambda *ts: None)
+    monkeypatch.setattr(ops, "call_on", lambda t, name, *args: made.append((name, args)))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)   # bits of every call's own
+    return made
+
+
+def test_words_of_another_width_are_refused(calls):
+    ids = torch.zeros((2, 3), dtype=torch.int64)
+    for D, words in ((65, 1), (128, 1), (64, 2), (1, 0)):
+        with pytest.raises(ValueError, match="words"):
+            ops.token_encode_hard(ids, torch.zeros((5, words), dtype=torch.int64), D, -1, 2)
+    assert not calls
+    assert ops.token_encode_hard(ids, torch.zeros((5, 2), dtype=torch.int64), 65, -1, 2).shape == (2, 195)
+
+
+@pytest.mark.parametrize("before,after", [(128, 64), (64, 65), (200, 3)])
+def test_a_weight_of_another_width(calls, before, after):
+    """The bits' width is the present weight's in every form, not the first one's."""
+    enc = sl.TokenEncoder(4, before)
+    enc.weight = torch.nn.Parameter(torch.randn(7, after))
+    assert (enc.num_tokens, enc.bits) == (7, after)
+    ids = torch.zeros((2, 3), dtype=torch.int64)
+    assert enc.forward_hard(ids).shape == (2, 3 * after)
+    assert enc.forward_packed(ids).shape == (3 * after, 1)
+    for name, args in calls:
+        if name == "slg_token_encode_hard":
+            assert args[4:6] == (7, after)   # V, D
+    assert len(calls) == 4
+
+
+def test_a_weight_that_is_no_table(calls):
+    enc = sl.TokenEncoder(4, 5)
+    for w in (torch.randn(20), torch.randn(2, 2, 5), torch.randn(0, 5), torch.randn(5, 0)):
+        enc.weight = torch.nn.Parameter(w)
+        for form in (enc, enc.forward_hard, enc.forward_packed):
+            with pytest.raises(ValueError, match="weight"):
+                form(torch.zeros(3, dtype=torch.int64))
+    assert not calls
