@@ -9,8 +9,9 @@ come from changes. The key of a table is the storage address and version
 counter of every parameter and buffer of the modules it reads: in-place
 updates (optimizer steps, ``copy_``, ``load_state_dict``) bump the version,
 and moving or replacing a tensor changes its storage. Writes through
-``tensor.data`` bypass the version counter; call :func:`clear` on a model
-after such writes. Tracing under ``torch.compile`` builds the tables afresh.
+``tensor.data`` bypass the version counter, and so does a replayed graph that
+updates a parameter; call :func:`clear` on a model after such writes. Tracing
+under ``torch.compile`` builds the tables afresh.
 """
 import torch
 

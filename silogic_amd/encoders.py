@@ -162,28 +162,31 @@ class TokenEncoder(nn.Module):
         return _TokenFn.apply(ids, w, self.scale, self.ste, self._pad)
 
     def _bit_table(self, weight):
-        """Bit words of the weight, made once per version of it (its storage and
-        version counter, as ``derived`` keys tables; ``derived.clear`` drops
-        them). Another stream than the one that made them waits for them. A
-        captured call makes its own inside the graph, which then keeps them
-        and reads the weight afresh on every replay; so does a call on a weight
-        without a version (made in inference mode)."""
+        """Bit words of the weight, made once per version of it: the parameter
+        itself, its storage, version counter and layout (writes through
+        ``.data`` and replays of a graph that updates the weight count no
+        version: ``derived.clear`` drops the words). Another stream than the
+        one that made them waits for them. A captured call makes its own inside
+        the graph, which then keeps them and reads the weight afresh on every
+        replay; so does a call on a weight without a version (made in inference
+        mode)."""
         if torch.cuda.is_current_stream_capturing() or weight.is_inference():
             return ops.token_bits(ops._c(weight.detach()))
         here = ops._stream(weight).value
-        key = (weight.data_ptr(), weight._version)
+        key = (weight.data_ptr(), weight._version, weight.shape, weight.stride(), weight.dtype)
         slot = self.__dict__.get("_derived_bits")
-        if slot is None or slot[0] != key:
+        if slot is None or slot[0] is not weight or slot[1] != key:
             w = weight.detach()   # kept: its address stays taken while the key holds it
             bits = ops.token_bits(ops._c(w))
             done = torch.cuda.current_stream(w.device).record_event()
-            self._derived_bits = (key, here, bits, done, w)
+            self._derived_bits = (weight, key, here, bits, done, w)
             return bits
-        if slot[1] != here:
+        _, _, made_on, bits, done, _ = slot
+        if made_on != here:
             stream = torch.cuda.current_stream(weight.device)
-            stream.wait_event(slot[3])
-            slot[2].record_stream(stream)
-        return slot[2]
+            stream.wait_event(done)
+            bits.record_stream(stream)
+        return bits
 
     def __getstate__(self):   # copies and pickles make their own bit table
         return {k: v for k, v in self.__dict__.items() if k != "_derived_bits"}

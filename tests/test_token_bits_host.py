@@ -49,3 +49,63 @@ def test_a_weight_that_is_no_table(calls):
             with pytest.raises(ValueError, match="weight"):
                 form(torch.zeros(3, dtype=torch.int64))
     assert not calls
+
+
+class _Stream:
+    cuda_stream = 0
+
+    def record_event(self):
+        return object()
+
+
+@pytest.fixture
+def made(calls, monkeypatch):
+    """The weights that bit tables were made of, outside a capture."""
+    tables = []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: _Stream())
+    monkeypatch.setattr(ops, "_stream", lambda t: type("", (), {"value": 0}))
+    real = ops.token_bits
+    monkeypatch.setattr(ops, "token_bits", lambda t: (tables.append(t), real(t))[1])
+    return tables
+
+
+# replacements that start at the old weight's address
+VIEWS = {
+    "prefix": lambda w: torch.nn.Parameter(w.detach()[:2]),
+    "columns": lambda w: torch.nn.Parameter(w.detach()[:, :2]),
+    "transposed": lambda w: torch.nn.Parameter(w.detach().t()),
+    "type": lambda w: torch.nn.Parameter(w.detach().view(torch.float16)[:, :4]),
+    "counter of its own": lambda w: torch.nn.Parameter(w.data),
+}
+
+
+@pytest.mark.parametrize("how", list(VIEWS))
+def test_a_weight_replaced_by_a_view_of_it(made, how):
+    enc = sl.TokenEncoder(4, 4)
+    ids = torch.zeros(3, dtype=torch.int64)
+    enc.forward_hard(ids)
+    enc.forward_packed(ids)
+    assert len(made) == 1   # one table for both
+    old = enc.weight
+    enc.weight = VIEWS[how](old)
+    assert enc.weight.data_ptr() == old.data_ptr() and enc.weight._version == old._version
+    enc.forward_hard(ids)
+    enc.forward_packed(ids)
+    assert len(made) == 2 and torch.equal(made[1], enc.weight)
+
+
+def test_a_new_weight_of_the_same_version(made):
+    """Another parameter on the same memory counts its changes by itself."""
+    enc = sl.TokenEncoder(4, 4)
+    ids = torch.zeros(3, dtype=torch.int64)
+    with torch.no_grad():
+        enc.weight.neg_()
+    enc.forward_hard(ids)
+    old = enc.weight
+    enc.weight = torch.nn.Parameter(old.data)
+    with torch.no_grad():
+        enc.weight.neg_()
+    assert enc.weight.data_ptr() == old.data_ptr() and enc.weight._version == old._version
+    enc.forward_hard(ids)
+    assert len(made) == 2
