@@ -360,10 +360,10 @@ def _layer8_args(x, cand, conn, raw, node_kind):
             0 < K <= 16 and OUT > 0 and x.shape[1] > 0 and
             raw.shape == (OUT, 16 if node_kind == GATE16 else 4) and
             (conn is None or (conn.get_device() == d and conn.shape == cand.shape))):
-        require_gpu(x, cand, conn, raw)
-        same_device("fc_layer8", x, cand, conn, raw)
         check_layer8(x, cand, conn=(conn, cand.shape),
                      raw=(raw, (cand.shape[0], 16 if node_kind == GATE16 else 4)))
+        require_gpu(x, cand, conn, raw)
+        same_device("fc_layer8", x, cand, conn, raw)
     return (_as_f32(x), _quads(_c(cand, torch.int32)), _c(conn, torch.float32),
             _quads(_c(raw, torch.float32)), (*x.shape, OUT, K))
 
@@ -476,7 +476,8 @@ def fc_layer8(x, cand, conn, raw, node_kind, inv_tau=1.0):
     if torch.compiler.is_compiling():
         return torch.ops.silogic_hip.fc_layer8(x, cand, conn, raw, node_kind, float(inv_tau))[0]
     if not _grad_path(x, conn, raw):   # nothing to keep
-        w, npar = fc_soft_prep(conn, raw, node_kind, *cand.shape[::2])
+        x, cand, conn, raw, (_, _, OUT, K) = _layer8_args(x, cand, conn, raw, node_kind)
+        w, npar = fc_soft_prep(conn, raw, node_kind, OUT, K)
         return fc_soft(x, cand, w, npar, node_kind, inv_tau)
     return _FcLayer8.apply(x, cand, conn, raw, node_kind, float(inv_tau))
 
