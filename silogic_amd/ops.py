@@ -106,6 +106,16 @@ def rows8_pack(x):
     return codes, rows
 
 
+def check_rows8(codes, rows, D):
+    """Raise unless ``codes`` and ``rows`` are :func:`rows8_pack`'s of rows of
+    ``D`` values."""
+    if rows.dtype != torch.float32 or rows.dim() != 2 or rows.shape[1] != 2:
+        raise ValueError(f"8-bit activations: rows {rows.dtype} {tuple(rows.shape)}, fp32 [B, 2] expected")
+    shape = ((rows.shape[0] + 3) // 4, (D + 3) // 4 * 4, 4)
+    if D < 1 or codes.dtype != torch.uint8 or tuple(codes.shape) != shape:
+        raise ValueError(f"8-bit activations: codes {codes.dtype} {tuple(codes.shape)}, uint8 {shape} expected")
+
+
 def rows8_unpack(codes, rows, D):
     """The values that the codes stand for, ``[B, D]`` fp32."""
     B = rows.shape[0]
@@ -118,10 +128,12 @@ def fc_soft_bwd8(codes, rows, in_dim, cand, w, npar, node_kind, inv_tau, gy, nee
                  need_w=True, need_np=True):
     """:func:`fc_soft_bwd` of an input kept as ``codes`` and ``rows``. Rows too
     wide for the kernel on codes are unpacked for the one on fp32."""
+    check_rows8(codes, rows, in_dim)
+    check_layer8(rows, cand, w=(w, cand.shape), npar=(npar, (*cand.shape[:1], 4)))
     require_gpu(codes, rows, cand, w, npar, gy)
     same_device("fc_soft_bwd8", codes, rows, cand, w, npar, gy)
     cand, w, npar = (_quads(_c(t, d)) for t, d in ((cand, torch.int32), (w, torch.float32), (npar, torch.float32)))
-    gy = _c(gy, torch.float32)
+    codes, rows, gy = _quads(_c(codes)), _c(rows), _c(gy, torch.float32)
     B, (OUT, _, K) = rows.shape[0], cand.shape
     if gy.shape != (B, OUT):
         raise ValueError(f"fc_soft_bwd8: gradient {tuple(gy.shape)} for {(B, OUT)}")

@@ -38,3 +38,28 @@ def test_on_the_cpu(grad):
     args["x"].requires_grad_(grad)
     with pytest.raises(RuntimeError, match="GPU"):
         ops.fc_layer8(**args)
+
+
+def _back(B=6, IN=9, OUT=5, K=3):
+    return dict(codes=torch.zeros(((B + 3) // 4, (IN + 3) // 4 * 4, 4), dtype=torch.uint8), rows=torch.zeros(B, 2),
+                in_dim=IN, cand=torch.zeros((OUT, 2, K), dtype=torch.int32), w=torch.rand(OUT, 2, K),
+                npar=torch.rand(OUT, 4), node_kind=ops.GATE16, inv_tau=1.0, gy=torch.rand(B, OUT))
+
+
+@pytest.mark.parametrize("bad", [dict(in_dim=13), dict(in_dim=8), dict(in_dim=0), dict(rows=torch.zeros(9, 2)),
+                                 dict(rows=torch.zeros(6, 1)), dict(rows=torch.zeros(6, 2).double()),
+                                 dict(codes=torch.zeros(2, 12, 4)), dict(codes=torch.zeros(2, 9, 4, dtype=torch.uint8)),
+                                 dict(codes=torch.zeros(1, 12, 4, dtype=torch.uint8)),
+                                 dict(codes=torch.zeros(96, dtype=torch.uint8)), dict(w=torch.rand(4, 2, 3)),
+                                 dict(w=torch.rand(5, 2, 2)), dict(npar=torch.rand(4, 4)), dict(npar=torch.rand(5, 3))])
+def test_backward_on_codes(bad):
+    """Sizes that the kernel would read past: of the codes, of their rows and of the parameters."""
+    with pytest.raises(ValueError, match="8-bit activations"):
+        ops.fc_soft_bwd8(**{**_back(), **bad})
+
+
+def test_backward_on_codes_on_the_cpu():
+    with pytest.raises(RuntimeError, match="GPU"):
+        ops.fc_soft_bwd8(**_back())
+    with pytest.raises(NotImplementedError):
+        ops.fc_soft_bwd8(**{**_back(), "cand": torch.zeros(5, 2, 17)})
