@@ -460,7 +460,7 @@ fc_soft8.register_autograd(_fc_soft8_backward, setup_context=_fc_soft8_setup)
 @torch.library.custom_op(f"{_NS}::token_encode", mutates_args=())
 def token_encode(ids: Tensor, table: Tensor, scale: float, ste: bool, pad: int) -> Tensor:
     """``ids [B,L]``, ``table [V,D]`` -> ``[B, L*D]`` fp32."""
-    ops.require_gpu(ids, table)
+    ops.check_tokens(ids, table)
     return ops.token_encode(ops._c(ids), ops._c(table), scale, ste, pad)
 
 
@@ -471,6 +471,7 @@ def _(ids, table, scale, ste, pad):
 
 @torch.library.custom_op(f"{_NS}::token_encode_bwd", mutates_args=())
 def token_encode_bwd(ids: Tensor, table: Tensor, scale: float, pad: int, gy: Tensor) -> Tensor:
+    ops.check_tokens(ids, table, gy)
     return ops.token_encode_bwd(ops._c(ids), ops._c(table), scale, pad, gy)
 
 

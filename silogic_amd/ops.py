@@ -509,6 +509,17 @@ def fc_soft8(x, cand, w, npar, node_kind, inv_tau=1.0):
 TABLE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
+def check_tokens(ids, table, *others):
+    """Raise unless ``ids [B, L]`` and ``table [V, D]`` are what the encoder's
+    kernels take, on one device with ``others``."""
+    if ids.dtype not in (torch.int32, torch.int64) or ids.dim() != 2:
+        raise ValueError(f"token encoder: ids {ids.dtype} {tuple(ids.shape)}, int32 or int64 [B, L] expected")
+    if table.dtype not in TABLE_DTYPES or table.dim() != 2 or 0 in table.shape:
+        raise ValueError(f"token encoder: table {table.dtype} {tuple(table.shape)}, fp32, bf16 or fp16 [V, D] expected")
+    require_gpu(ids, table, *others)
+    same_device("token encoder", ids, table, *others)
+
+
 def token_encode(ids, table, scale, ste, pad):
     """``ids [B, L]`` int32 / int64, ``table [V, D]`` -> ``[B, L * D]`` fp32
     (``slg_token_encode``)."""

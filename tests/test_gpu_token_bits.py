@@ -63,3 +63,14 @@ def test_a_graph_that_updates_the_weight():
         derived.clear(enc)
         _check(enc)
         torch.cuda.synchronize()
+
+
+def test_operators_want_their_tensors_on_the_gpu():
+    op = torch.ops.silogic_hip
+    ids, table, gy = torch.zeros((2, 3), dtype=torch.int64), torch.rand(4, 5), torch.rand(2, 15)
+    on = [t.to(DEV) for t in (ids, table, gy)]
+    assert op.token_encode_bwd(on[0], on[1], 1.0, -1, on[2]).shape == (4, 5)
+    for i, t in enumerate((ids, table, gy)):
+        args = on[:i] + [t] + on[i + 1:]
+        with pytest.raises(RuntimeError, match="GPU"):
+            op.token_encode_bwd(args[0], args[1], 1.0, -1, args[2])

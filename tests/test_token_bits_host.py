@@ -109,3 +109,23 @@ def test_a_new_weight_of_the_same_version(made):
     assert enc.weight.data_ptr() == old.data_ptr() and enc.weight._version == old._version
     enc.forward_hard(ids)
     assert len(made) == 2
+
+
+@pytest.mark.parametrize("ids,table", [(torch.zeros(2, 3), torch.rand(4, 5)), (torch.zeros(2, 3, dtype=torch.int16), torch.rand(4, 5)),
+                                       (torch.zeros(3, dtype=torch.int64), torch.rand(4, 5)),
+                                       (torch.zeros((2, 3), dtype=torch.int64), torch.rand(4, 5).double()),
+                                       (torch.zeros((2, 3), dtype=torch.int64), torch.rand(0, 5)),
+                                       (torch.zeros((2, 3), dtype=torch.int64), torch.rand(4))])
+def test_operators_refuse_what_the_kernels_do_not_take(ids, table):
+    with pytest.raises(ValueError, match="token encoder"):
+        torch.ops.silogic_hip.token_encode(ids, table, 1.0, False, -1)
+    with pytest.raises(ValueError, match="token encoder"):
+        torch.ops.silogic_hip.token_encode_bwd(ids, table, 1.0, -1, torch.rand(2, 15))
+
+
+def test_operators_on_the_cpu():
+    ids, table = torch.zeros((2, 3), dtype=torch.int64), torch.rand(4, 5)
+    with pytest.raises(RuntimeError, match="GPU"):
+        torch.ops.silogic_hip.token_encode(ids, table, 1.0, False, -1)
+    with pytest.raises(RuntimeError, match="GPU"):
+        torch.ops.silogic_hip.token_encode_bwd(ids, table, 1.0, -1, torch.rand(2, 15))
