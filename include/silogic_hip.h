@@ -267,9 +267,9 @@ int slg_learned_thermo_bwd(const float* x, int64_t B, int64_t F, int32_t T, cons
 
 /* Token encoder (no counterpart in the reference, whose encoders take numbers):
  * a learned row of D soft bits per token id. table [V,D] (dtype 0: fp32, 1:
- * bf16, 2: fp16), ids [N] of id_bytes 4 or 8 (signed). A token with id pad, or
- * outside 0..V-1, is absent: values and bits 0, no gradient (pad < 0: every id
- * of the table counts).
+ * bf16, 2: fp16), ids [N] of id_bytes 4 or 8 (signed), 0 < scale <= 2e38. A
+ * token with id pad, or outside 0..V-1, is absent: values and bits 0, no
+ * gradient (pad < 0: every id of the table counts).
  *   slg_token_encode       y [N,D] fp32 = sigmoid(scale * table[id]); ste: 1
  *                          where table[id] > 0, else 0
  *   slg_token_encode_bwd   gtable [V,D] (the table's type, all of it written) =

@@ -1,6 +1,7 @@
 // Token encoder for gfx950: a learned row of D soft bits per token id.
 //   soft   y[n, d] = sigmoid(scale * E[t_n, d]) (ste: 1 where E > 0, else 0)
-//   hard   bit (n, d) = E[t_n, d] > 0, the soft form past 1/2
+//   hard   bit (n, d) = E[t_n, d] > 0, the soft form past 1/2 (scale > 0: a
+//          negative one would put the soft form and the bits at odds)
 //   back   gE[v, d] = scale * sigmoid'(scale * E[v, d]) * sum over n with t_n = v of gy[n, d]
 // A token that is the padding id, or that no row of the table has (negative,
 // or V and above), is absent: its values and bits are 0 and it adds to no
@@ -552,6 +553,10 @@ using namespace slg;
   SLG_REQUIRE(tok_sizes(N, V, D), SLG_E_SHAPE, name ": N %lld, V %lld, D %lld", (long long)N,        \
               (long long)V, (long long)D)
 
+// scale log2 e has to be finite too: 0 times an infinity has no value.
+#define TOK_CHECK_SCALE(name) \
+  SLG_REQUIRE(scale > 0.0f && scale <= 2e38f, SLG_E_ARG, name ": scale %g outside (0, 2e38]", (double)scale)
+
 extern "C" {
 
 int slg_token_encode(const void* ids, int32_t id_bytes, int64_t N, int64_t V, int64_t D, int64_t pad,
@@ -559,6 +564,7 @@ int slg_token_encode(const void* ids, int32_t id_bytes, int64_t N, int64_t V, in
                      slg_stream_t stream) {
   SLG_REQUIRE(table && ((ids && y) || N == 0), SLG_E_ARG, "token_encode: null pointer");
   TOK_CHECK("token_encode");
+  TOK_CHECK_SCALE("token_encode");
   if (N == 0) return 0;
   hipStream_t st = as_stream(stream);
   const float nlog2 = (float)(-1.4426950408889634 * (double)scale);
@@ -593,6 +599,7 @@ int slg_token_encode_bwd(const void* ids, int32_t id_bytes, int64_t N, int64_t V
   SLG_REQUIRE(table && gtable && ((ids && gy && workspace) || N == 0), SLG_E_ARG,
               "token_encode_bwd: null pointer");
   TOK_CHECK("token_encode_bwd");
+  TOK_CHECK_SCALE("token_encode_bwd");
   const TokBwdPlan p = tok_bwd_plan(N, V, D);
   SLG_REQUIRE(workspace_words >= p.total() && (uintptr_t)workspace % 16 == 0, SLG_E_ARG,
               "token_encode_bwd: workspace of %lld words, %lld at a multiple of 16 bytes needed",

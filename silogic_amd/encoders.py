@@ -86,7 +86,7 @@ class TokenEncoder(nn.Module):
     encoders take numbers): ids ``[B]`` or ``[B, L]`` (int32 or int64) ->
     ``[B, L*bits]``, feature ``l*bits + d`` of token ``l``.
 
-    The soft forward is ``sigmoid(scale * weight[id])`` in fp32, with ``ste``
+    The soft forward is ``sigmoid(scale * weight[id])`` (``scale > 0``) in fp32, with ``ste``
     the hard bits ``weight[id] > 0`` under the same gradient (straight
     through); :meth:`forward_hard` and :meth:`forward_packed` are the hard
     bits. A token with id ``padding_idx``, or outside the table, is absent: its
@@ -113,6 +113,8 @@ class TokenEncoder(nn.Module):
             if not -V <= padding_idx < V:
                 raise ValueError(f"TokenEncoder: padding_idx {padding_idx} for {V} tokens")
             padding_idx %= V
+        if not 0 < scale <= 2e38:   # the soft form falls where the bits rise; scale log2 e overflows
+            raise ValueError(f"TokenEncoder: scale {scale} outside (0, 2e38]")
         self.scale, self.ste, self.padding_idx = float(scale), bool(ste), padding_idx
         self.weight = weight if isinstance(weight, nn.Parameter) else nn.Parameter(weight)
 

@@ -1,10 +1,12 @@
 """The token encoder's hard bits after its weight was replaced, without a GPU: entry points are recorded, not
 launched."""
+import ctypes
+
 import pytest
 import torch
 
 import silogic_amd as sl
-from silogic_amd import ops
+from silogic_amd import _lib, ops
 
 
 @pytest.fixture
@@ -129,3 +131,16 @@ def test_operators_on_the_cpu():
         torch.ops.silogic_hip.token_encode(ids, table, 1.0, False, -1)
     with pytest.raises(RuntimeError, match="GPU"):
         torch.ops.silogic_hip.token_encode_bwd(ids, table, 1.0, -1, torch.rand(2, 15))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, -1.0, float("nan"), float("inf"), -float("inf"), 3e38])
+def test_scales_that_part_the_soft_form_from_the_bits(scale):
+    with pytest.raises(ValueError, match="scale"):
+        sl.TokenEncoder(4, 5, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        sl.TokenEncoder.from_weight(torch.randn(4, 5), scale=scale)
+    at = ctypes.c_void_p(16)   # an address that is only looked at
+    lib = _lib.lib()
+    assert lib.slg_token_encode(at, 8, 4, 5, 6, -1, at, 0, scale, 0, at, None) == -1
+    n = lib.slg_token_encode_bwd_workspace(4, 5, 6)
+    assert lib.slg_token_encode_bwd(at, 8, 4, 5, 6, -1, at, 0, scale, at, at, at, n, None) == -1
