@@ -33,12 +33,12 @@ struct HeadArgs {
   float tau;
 };
 
-// Widest workgroup per variant: 1024 threads keeps <= 128 VGPRs per lane,
-// which fits the lean variants; the others get 512 threads and more registers.
 // Slots of a thread for a candidate count known when compiled (KC > 0), of at
 // most -KC (KC < 0) or of at most 16.
 template <int KC>
 constexpr int soft_slots() { return KC > 0 ? KC : KC < 0 ? -KC : 16; }
+// Widest workgroup per variant: 1024 threads keeps <= 128 VGPRs per lane,
+// which fits the lean variants; the others get 512 threads and more registers.
 template <int KC, int S>
 constexpr int soft_max_threads() { return (KC == 0 || S >= 8) ? 512 : 1024; }
 
@@ -904,7 +904,7 @@ struct SoftArgs {
   float inv_tau; float* y;
   int S, threads;
   HeadArgs hd;  // hd.logits != nullptr: fused GroupSum, y unused
-  Rows8Out po{};  // po.codes != nullptr: the input in 8 bits too (no head, no records)
+  Rows8Out po{};  // po.codes != nullptr: the input in 8 bits too (launch_soft_s says where)
 };
 
 // Output chunks per sample tile: enough workgroups to fill the chip twice
@@ -927,8 +927,8 @@ static void soft_grid(const SoftArgs& a, int64_t* n_chunks_out, int64_t* chunk_o
   *chunk_out = chunk;
 }
 
-template <int NODE, int KC, int S, bool HEAD, bool REC>
-static int launch_soft_s(const SoftArgs& a, hipStream_t st) {
+template <int NODE, int KC, int S, bool HEAD, bool REC, bool PACK>
+static int launch_soft_pack(const SoftArgs& a, hipStream_t st) {
   int64_t n_chunks, chunk;
   soft_grid(a, &n_chunks, &chunk);
   SLG_REQUIRE(!HEAD || n_chunks == 1, SLG_E_UNSUPPORTED,
@@ -937,20 +937,11 @@ static int launch_soft_s(const SoftArgs& a, hipStream_t st) {
   SLG_REQUIRE(grid < (1LL << 31), SLG_E_SHAPE, "fc_soft: grid too large");
   SLG_REQUIRE(a.OUT * S * 4 < (1LL << 31), SLG_E_SHAPE, "fc_soft: OUT %lld too large",
               (long long)a.OUT);
-  auto kern = fc_soft_kernel<NODE, KC, S, HEAD, REC>;
   const int threads = std::min(a.threads, soft_max_threads<KC, S>());
-  size_t lds = (size_t)a.IN * S * sizeof(float) + (HEAD ? (size_t)S * a.hd.C * 4 : 0);
-  if constexpr (!HEAD && S >= 4) {
-    if (a.po.codes) {
-      lds += sizeof(float) * rows8_scratch(S, threads / 64);
-      if constexpr (!REC) kern = fc_soft_kernel<NODE, KC, S, HEAD, REC, true>;
-    }
-  }
+  const size_t lds = (size_t)a.IN * S * sizeof(float) + (HEAD ? (size_t)S * a.hd.C * 4 : 0) +
+                     (PACK ? sizeof(float) * rows8_scratch(S, threads / 64) : 0);
   if constexpr (REC && (KC == 4 || KC == 8)) {
-    auto rk = fc_soft_rec_kernel<NODE, KC, S, HEAD>;
-    if constexpr (!HEAD && S >= 4) {
-      if (a.po.codes) rk = fc_soft_rec_kernel<NODE, KC, S, HEAD, true>;
-    }
+    auto rk = fc_soft_rec_kernel<NODE, KC, S, HEAD, PACK>;
     SLG_REQUIRE(lds <= (size_t)device_lds_bytes(), SLG_E_SHAPE, "fc_soft: %zu B LDS needed", lds);
     static const size_t static_lds = [&] {
       hipFuncAttributes fa{};
@@ -972,21 +963,35 @@ static int launch_soft_s(const SoftArgs& a, hipStream_t st) {
                        a.inv_tau, a.y, (int)n_chunks, (int)chunk, a.hd, a.po);
     SLG_LAUNCH_CHECK("fc_soft");
     return 0;
-  }
-  SLG_REQUIRE(lds <= (size_t)device_lds_bytes(), SLG_E_SHAPE, "fc_soft: %zu B LDS needed", lds);
-  if (lds > 65536) {
-    hipError_t e = hipFuncSetAttribute((const void*)kern,
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) {
-      set_error("fc_soft: cannot reserve %zu B LDS: %s", lds, hipGetErrorString(e));
-      return (int)e;
+  } else {
+    auto kern = fc_soft_kernel<NODE, KC, S, HEAD, REC, PACK>;
+    SLG_REQUIRE(lds <= (size_t)device_lds_bytes(), SLG_E_SHAPE, "fc_soft: %zu B LDS needed", lds);
+    if (lds > 65536) {
+      hipError_t e = hipFuncSetAttribute((const void*)kern,
+                                         hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      if (e != hipSuccess) {
+        set_error("fc_soft: cannot reserve %zu B LDS: %s", lds, hipGetErrorString(e));
+        return (int)e;
+      }
     }
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(threads), lds, st, a.x, (int)a.B,
+                       (int)a.IN, (int)a.OUT, a.K, a.pv, a.inv_tau, a.y, (int)n_chunks, (int)chunk,
+                       a.hd, a.po);
+    SLG_LAUNCH_CHECK("fc_soft");
+    return 0;
   }
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(threads), lds, st, a.x, (int)a.B,
-                     (int)a.IN, (int)a.OUT, a.K, a.pv, a.inv_tau, a.y, (int)n_chunks, (int)chunk,
-                     a.hd, a.po);
-  SLG_LAUNCH_CHECK("fc_soft");
-  return 0;
+}
+
+// The input's codes come from tiles of 4 samples or more, from records where
+// fc_soft8_rec_floats takes them (8 candidates, tiles of 4).
+template <int NODE, int KC, int S, bool HEAD, bool REC>
+static int launch_soft_s(const SoftArgs& a, hipStream_t st) {
+  constexpr bool packs = !HEAD && (REC ? KC == 8 && S == 4 : S >= 4);
+  SLG_REQUIRE(packs || !a.po.codes, SLG_E_UNSUPPORTED, "fc_soft: no codes from tiles of %d, %d candidates", S, a.K);
+  if constexpr (packs) {
+    if (a.po.codes) return launch_soft_pack<NODE, KC, S, HEAD, REC, true>(a, st);
+  }
+  return launch_soft_pack<NODE, KC, S, HEAD, REC, false>(a, st);
 }
 
 template <int NODE, int KC, bool HEAD, bool REC>
