@@ -74,3 +74,26 @@ def test_operators_want_their_tensors_on_the_gpu():
         args = on[:i] + [t] + on[i + 1:]
         with pytest.raises(RuntimeError, match="GPU"):
             op.token_encode_bwd(args[0], args[1], 1.0, -1, args[2])
+
+
+def test_a_stream_waits_for_the_words_of_another():
+    """The words are made on the main stream behind work of some milliseconds; the side stream is idle and has
+    waited for nothing since."""
+    enc = sl.TokenEncoder(3000, 200).to(DEV)
+    ids = torch.randint(0, 3000, (500, 4), device=DEV)
+    a, b = torch.rand(2, 1 << 28, device=DEV)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        enc.forward_packed(ids)   # memory of the side stream's own
+    for k in range(3):
+        torch.cuda.synchronize()
+        for _ in range(20):
+            b.copy_(a)
+        with torch.no_grad():
+            enc.weight.neg_()
+        mine = enc.forward_packed(ids)
+        with torch.cuda.stream(side):
+            other = enc.forward_packed(ids)
+        torch.cuda.synchronize()
+        want = _packed((enc.weight > 0)[ids].reshape(500, -1))
+        assert torch.equal(mine, want) and torch.equal(other, want), f"call {k}"

@@ -144,3 +144,34 @@ def test_scales_that_part_the_soft_form_from_the_bits(scale):
     assert lib.slg_token_encode(at, 8, 4, 5, 6, -1, at, 0, scale, 0, at, None) == -1
     n = lib.slg_token_encode_bwd_workspace(4, 5, 6)
     assert lib.slg_token_encode_bwd(at, 8, 4, 5, 6, -1, at, 0, scale, at, at, at, n, None) == -1
+
+
+def test_another_stream_waits_for_the_words(made, monkeypatch):
+    """The event of the stream that made them, before their first use on another."""
+    did, now = [], ["main"]
+
+    class Stream:
+        def record_event(self):
+            return ("made on", now[0])
+
+        def wait_event(self, event):
+            did.append((now[0], event))
+
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream())
+    monkeypatch.setattr(ops, "_stream", lambda t: type("", (), {"value": now[0]}))
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, stream: did.append((now[0], "kept")))
+    enc = sl.TokenEncoder(4, 5)
+    ids = torch.zeros(3, dtype=torch.int64)
+    enc.forward_hard(ids)
+    enc.forward_hard(ids)
+    assert not did
+    now[0] = "side"
+    enc.forward_hard(ids)
+    assert did == [("side", ("made on", "main")), ("side", "kept")] and len(made) == 1
+    with torch.no_grad():
+        enc.weight.neg_()
+    enc.forward_hard(ids)   # made anew, here
+    assert len(did) == 2 and len(made) == 2
+    now[0] = "main"
+    enc.forward_hard(ids)
+    assert did[2:] == [("main", ("made on", "side")), ("main", "kept")]
