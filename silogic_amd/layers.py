@@ -148,7 +148,8 @@ class LogicLayer(nn.Module):
 
     def takes_rows8(self):
         """Whether the layer can keep its input in 8 bits for the backward."""
-        return self.arity == 2 and not self.is_lut and self._conn.k <= 16
+        return (self.arity == 2 and not self.is_lut and self._conn.k <= 16
+                and 2 * self.out_dim * self._conn.k < 1 << 31)
 
     def records_ok(self):
         """Whether the forward without gradients runs on per-output records:

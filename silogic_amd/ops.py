@@ -344,9 +344,10 @@ def layer_params_bwd(w, gw, kept, nodes, kind, arity, scale, gnp, need_conn, nee
 # ---------------------------------------------------------------------------
 def check_layer8(x, cand, **shapes):
     """Raise for sizes that the 8-bit backward does not take."""
-    if cand.dim() != 3 or cand.shape[1] != 2 or not 1 <= cand.shape[2] <= 16 or cand.shape[0] < 1:
+    if cand.dim() != 3 or cand.shape[1] != 2 or not 1 <= cand.shape[2] <= 16 or cand.shape[0] < 1 or \
+            cand.numel() >= 1 << 31:
         raise NotImplementedError(f"8-bit activations: candidates {tuple(cand.shape)} "
-                                  "(gate layers [OUT, 2, K] of 1 to 16 candidates)")
+                                  "(gate layers [OUT, 2, K] of 1 to 16 candidates, fewer than 2^31 in all)")
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"8-bit activations: input {tuple(x.shape)}, [B, IN] expected")
     for name, (t, shape) in shapes.items():

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import silogic_amd as sl
 from silogic_amd import ops
 
 
@@ -63,3 +64,18 @@ def test_backward_on_codes_on_the_cpu():
         ops.fc_soft_bwd8(**_back())
     with pytest.raises(NotImplementedError):
         ops.fc_soft_bwd8(**{**_back(), "cand": torch.zeros(5, 2, 17)})
+
+
+def test_more_candidates_than_the_backwards_take():
+    """2^31 of them: the forward says so, not the backward."""
+    few = torch.zeros(1, 1, 1, dtype=torch.int32)
+    x = torch.rand(2, 9)
+    with pytest.raises(NotImplementedError, match="candidates"):
+        ops.check_layer8(x, few.expand(1 << 26, 2, 16))
+    ops.check_layer8(x, few.expand((1 << 26) - 1, 2, 16))
+    layer = sl.LogicLayer(16, 20, k=16)
+    assert layer.takes_rows8()
+    layer.out_dim = 1 << 26
+    assert not layer.takes_rows8()
+    with pytest.raises(ValueError):
+        sl.save_activations(layer)
