@@ -410,6 +410,7 @@ def fc_soft8(x: Tensor, cand: Tensor, w: Tensor, npar: Tensor, node_kind: int,
              inv_tau: float) -> Tuple[Tensor, Tensor, Tensor]:
     """``(y, codes, rows)`` of :func:`ops.fc_soft8`."""
     ops.require_gpu(x, cand, w, npar)
+    ops.same_device("fc_soft8", x, cand, w, npar)
     ops.check_layer8(x, cand, w=(w, cand.shape), npar=(npar, (cand.shape[0], 4)))
     return ops.fc_soft8_fwd(ops._as_f32(x), ops._c(cand, torch.int32), ops._c(w, torch.float32),
                             ops._c(npar, torch.float32), node_kind, inv_tau)

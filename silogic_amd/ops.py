@@ -12,6 +12,7 @@ the autograd backward differentiates the op's torch expression
 (``fc_soft_torch``, ``conv_soft_torch``). Without gradients the wrappers
 launch the kernels directly.
 """
+import contextlib
 import ctypes
 
 import torch
@@ -68,6 +69,11 @@ def _as_f32(x):
     if x.dtype != torch.float32:
         x = x.float()
     return x.contiguous()
+
+
+def on_device(t):
+    """A context in which ``t``'s device is the current one."""
+    return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def call_on(t, name, *args):
@@ -140,7 +146,8 @@ def fc_soft_bwd8(codes, rows, in_dim, cand, w, npar, node_kind, inv_tau, gy, nee
     ws = _lib.lib().slg_fc_soft_bwd8_workspace(B, in_dim, OUT, K)
     if ws < 0:
         x = rows8_unpack(codes, rows, in_dim)
-        return fc_soft_bwd(x, cand, w, npar, node_kind, inv_tau, gy, need_x, need_w, need_np)
+        with on_device(x):
+            return fc_soft_bwd(x, cand, w, npar, node_kind, inv_tau, gy, need_x, need_w, need_np)
     dev, f32 = codes.device, torch.float32
     gx = torch.empty((B, in_dim), device=dev, dtype=f32) if need_x else None
     gw = torch.empty((OUT, 2, K), device=dev, dtype=f32) if need_w else None
@@ -400,8 +407,9 @@ def fc_layer8_bwd(codes, rows, cand, w, kept, in_dim, node_kind, inv_tau, gy, ne
     """``(gx, gconn, graw)`` of :func:`fc_layer8`; None where not needed."""
     gx, gw, gn = fc_soft_bwd8(codes, rows, in_dim, cand, w, kept[:cand.shape[0]], node_kind, inv_tau,
                               gy, need_x, need_conn, need_raw)
-    gconn, (graw,) = layer_params_bwd(w, gw, kept, [1], node_kind, 2, 1.0, gn, need_conn, [need_raw],
-                                      4 * w.shape[0] if node_kind == GATE16 else 0)
+    with on_device(w):
+        gconn, (graw,) = layer_params_bwd(w, gw, kept, [1], node_kind, 2, 1.0, gn, need_conn, [need_raw],
+                                          4 * w.shape[0] if node_kind == GATE16 else 0)
     return gx, gconn, None if graw is None else graw.squeeze(1)
 
 
@@ -490,8 +498,9 @@ def fc_layer8(x, cand, conn, raw, node_kind, inv_tau=1.0):
         return torch.ops.silogic_hip.fc_layer8(x, cand, conn, raw, node_kind, float(inv_tau))[0]
     if not _grad_path(x, conn, raw):   # nothing to keep
         x, cand, conn, raw, (_, _, OUT, K) = _layer8_args(x, cand, conn, raw, node_kind)
-        w, npar = fc_soft_prep(conn, raw, node_kind, OUT, K)
-        return fc_soft(x, cand, w, npar, node_kind, inv_tau)
+        with on_device(x):
+            w, npar = fc_soft_prep(conn, raw, node_kind, OUT, K)
+            return fc_soft(x, cand, w, npar, node_kind, inv_tau)
     return _FcLayer8.apply(x, cand, conn, raw, node_kind, float(inv_tau))
 
 
@@ -500,7 +509,10 @@ def fc_soft8(x, cand, w, npar, node_kind, inv_tau=1.0):
     if torch.compiler.is_compiling():
         return torch.ops.silogic_hip.fc_soft8(x, cand, w, npar, node_kind, float(inv_tau))[0]
     if not _grad_path(x, w, npar):
-        return fc_soft(x, cand, w, npar, node_kind, inv_tau)
+        require_gpu(x, cand, w, npar)
+        same_device("fc_soft8", x, cand, w, npar)
+        with on_device(x):
+            return fc_soft(x, cand, w, npar, node_kind, inv_tau)
     return _FcSoft8.apply(x, cand, w, npar, node_kind, float(inv_tau))
 
 

@@ -79,3 +79,42 @@ def test_more_candidates_than_the_backwards_take():
     assert not layer.takes_rows8()
     with pytest.raises(ValueError):
         sl.save_activations(layer)
+
+
+@pytest.mark.parametrize("call", ["layer", "soft", "layer backward", "wide backward"])
+def test_launched_from_the_tensors_device(monkeypatch, call):
+    """Every launch of a call is made with its tensors' device current: without gradients, where nothing is kept,
+    and in backwards that unpack wide rows or share the fp32 layers' kernels."""
+    here, launches = [7], []
+
+    class Device:
+        def __init__(self, d):
+            self.d = torch.device(d)
+
+        def __enter__(self):
+            self.old, here[0] = here[0], self.d
+
+        def __exit__(self, *exc):
+            here[0] = self.old
+
+    class Lib:
+        slg_fc_soft_bwd8_workspace = staticmethod(lambda B, IN, OUT, K: -1 if call == "wide backward" else 16)
+        slg_fc_soft_bwd_workspace = staticmethod(lambda B, IN, OUT, K: 16)
+
+    monkeypatch.setattr(ops, "require_gpu", lambda *ts: None)
+    monkeypatch.setattr(ops, "_stream", lambda t: None)
+    monkeypatch.setattr(ops._lib, "lib", lambda: Lib)
+    monkeypatch.setattr(ops._lib, "call", lambda name, *args: launches.append((name, here[0])))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 7)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    a, b = _args(), _back()
+    kept = torch.rand(25, 4)
+    if call == "layer":
+        ops.fc_layer8(**a)
+    elif call == "soft":
+        ops.fc_soft8(a["x"], a["cand"], b["w"], b["npar"], ops.GATE16)
+    elif call == "layer backward":
+        ops.fc_layer8_bwd(b["codes"], b["rows"], b["cand"], b["w"], kept, 9, ops.GATE16, 1.0, b["gy"], True, True, True)
+    else:
+        ops.fc_soft_bwd8(**b)
+    assert launches and all(at == torch.device("cpu") for _, at in launches), launches
