@@ -120,7 +120,7 @@ class TokenEncoder(nn.Module):
 
     @staticmethod
     def _check_weight(weight):
-        if weight.dim() != 2 or 0 in weight.shape:
+        if weight.dim() != 2 or weight.numel() == 0:
             raise ValueError(f"TokenEncoder: weight {tuple(weight.shape)}, [num_tokens, bits] expected")
         if weight.dtype not in ops.TABLE_DTYPES:
             raise TypeError(f"TokenEncoder: weight of {weight.dtype} (fp32, bf16 or fp16)")
@@ -143,18 +143,18 @@ class TokenEncoder(nn.Module):
         return -1 if self.padding_idx is None else self.padding_idx
 
     def _ids(self, ids, weight):
-        """``ids`` as ``[B, L]``, checked against ``weight``."""
+        """``ids`` as ``[B, L]``, on ``weight``'s device."""
         if ids.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"TokenEncoder: ids of {ids.dtype} (int32 or int64)")
         if ids.dim() not in (1, 2):
             raise ValueError(f"TokenEncoder: ids {tuple(ids.shape)}, [B] or [B, L] expected")
-        self._check_weight(weight)
         ops.require_gpu(ids, weight)
         ops.same_device("TokenEncoder", ids, weight)
         return ops._c(ids if ids.dim() == 2 else ids.unsqueeze(1))
 
     def forward(self, ids):
         w = self.weight
+        self._check_weight(w)
         ids = self._ids(ids, w)
         if torch.compiler.is_compiling():
             return torch.ops.silogic_hip.token_encode(ids, w, self.scale, self.ste, self._pad)
@@ -173,21 +173,24 @@ class TokenEncoder(nn.Module):
         replay; so does a call on a weight without a version (made in inference
         mode)."""
         if torch.cuda.is_current_stream_capturing() or weight.is_inference():
+            self._check_weight(weight)
             return ops.token_bits(ops._c(weight.detach()))
         here = ops._stream(weight).value
-        key = (weight.data_ptr(), weight._version, weight.shape, weight.stride(), weight.dtype)
         slot = self.__dict__.get("_derived_bits")
-        if slot is None or slot[0] is not weight or slot[1] != key:
-            w = weight.detach()   # kept: its address stays taken while the key holds it
-            bits = ops.token_bits(ops._c(w))
-            done = torch.cuda.current_stream(w.device).record_event()
-            self._derived_bits = (weight, key, here, bits, done, w)
-            return bits
-        _, _, made_on, bits, done, _ = slot
-        if made_on != here:
-            stream = torch.cuda.current_stream(weight.device)
-            stream.wait_event(done)
-            bits.record_stream(stream)
+        # w: the weight as it was, whose memory stays taken by it
+        if slot is not None:
+            of, version, w, made_on, bits, done = slot
+            if of is weight and version == weight._version and w.dtype == weight.dtype and w.is_set_to(weight):
+                if made_on != here:
+                    stream = torch.cuda.current_stream(weight.device)
+                    stream.wait_event(done)
+                    bits.record_stream(stream)
+                return bits
+        self._check_weight(weight)
+        w = weight.detach()
+        bits = ops.token_bits(ops._c(w))
+        done = torch.cuda.current_stream(w.device).record_event()
+        self._derived_bits = (weight, weight._version, w, here, bits, done)
         return bits
 
     def __getstate__(self):   # copies and pickles make their own bit table

@@ -568,15 +568,15 @@ def token_bits(table):
 def token_encode_hard(ids, bits, D, pad, layout):
     """Bits of ``ids [B, L]``'s tokens: layout 0 ``[L*D, nw]``, 1 ``[nw, L*D]``,
     2 uint8 ``[B, L*D]``."""
-    B, L = ids.shape
-    if D < 1 or bits.dim() != 2 or bits.shape[1] != -(-D // 64):
+    (B, L), (V, words) = ids.shape, bits.shape
+    if D < 1 or words != (D + 63) >> 6:
         raise ValueError(f"token_encode_hard: words {tuple(bits.shape)} for rows of {D} bits")
     nw = n_words(B)
     if layout == 2:
         out = bits.new_empty((B, L * D), dtype=torch.uint8)
     else:
         out = bits.new_empty((nw, L * D) if layout else (L * D, nw))
-    call_on(bits, "slg_token_encode_hard", ids.data_ptr(), ids.element_size(), B, L, bits.shape[0], D,
+    call_on(bits, "slg_token_encode_hard", ids.data_ptr(), ids.element_size(), B, L, V, D,
             pad, bits.data_ptr(), layout, out.data_ptr())
     return out
 
