@@ -63,6 +63,7 @@ struct IgKeys {
   const int* cand;
   __device__ int key(int64_t r) const {
     const int i = min(max(cand[r], 0), a.IN - 1);
+    if (a.NP == 1) return i;  // the groups' inputs follow each other: no divisions (1.5 us of a launch)
     const int SK = a.NS * a.K, o = (int)r / SK, side = ((int)r - o * SK) / a.K;
     const int q = i / a.IB;
     return ((side * a.OUT + o) / a.RB * a.NB + q) * a.IB + (i - q * a.IB);
@@ -170,8 +171,8 @@ __global__ void __launch_bounds__(256) ig_entries_kernel(IgArgs a, const int2* _
 
 // The whole table in one launch, a workgroup per input block, for one pass
 // (ig_small): the references that fall in the block are counted, placed and
-// ranked in LDS, where the launches of the general way (the sort's, three more) pass everything
-// through memory. Each workgroup reads all candidates, twice.
+// ranked in LDS, where the launches of the general way (the sort's, three more)
+// pass everything through memory. Each workgroup reads all candidates, twice.
 __global__ void __launch_bounds__(1024)
 ig_table_kernel(IgArgs a, const int* __restrict__ cand, const float* __restrict__ w,
                 int* __restrict__ start, int* __restrict__ perm, int* __restrict__ slot,
@@ -449,6 +450,9 @@ __global__ void __launch_bounds__(256) iw_entries_kernel(const int2* __restrict_
   ent[j] = make_int2(side * OUT + o, __float_as_int(w[r]));
 }
 
+// gab [R2][LB] = transpose of gbr [B][R2] (rows b >= B of gab's columns are
+// zero), through a 64 x 64 LDS tile; float4 loads along gbr rows when R2 is
+// a multiple of 4, float4 stores along gab rows (LB is a multiple of 64).
 __global__ void __launch_bounds__(256) iw_transpose_kernel(const float* __restrict__ gbr,
                                                                     int B, int R2, int64_t LB,
                                                                     int n_rtiles,
@@ -645,19 +649,20 @@ static IwPlan iw_plan(int64_t B, int64_t IN, int64_t OUT, int nsides, int K) {
   return q;
 }
 
-// Whether the wide way is the shorter, by the nanoseconds that the two differ in
-// (fitted to 700 random layers of 100-400000 inputs and outputs, 1-4096 samples,
-// K 1-16; the choice is within 3% of the better way for nineteen in twenty and 1%
-// slower than it on average). From LDS: the key scan, keys per
-// (pass, input), then per round of workgroups the passes, the staging of every
-// row and the block's references. Wide: the transpose and the gather over 256
-// samples at a time, and the list of one input, which is walked alone. FC
-// backward from LDS / wide, K = 8: 10000 -> 10000, B = 1024: 186 / 273 us; 60000
-// -> 60000, B = 124: 1332 / 1175; 172000 -> 172000, B = 3: 3046 / 1207. The fit is
-// that of a slower reference table; it stays, so that layers keep their sums'
-// order. With the sort (8-bit backward, us from LDS / wide): K = 8 10000 ->
-// 10000, B = 1024 143 / 196, B = 256 99 / 87; 40000 -> 40000, B = 124 336 / 217;
-// K = 4 12000 -> 12000, B = 300 134 / 92; 16380 -> 16380, B = 1024 222 / 248.
+// Whether the wide way is taken, by the nanoseconds that the two differ in. From
+// LDS: the key scan, keys per (pass, input), then per round of workgroups the
+// passes, the staging of every row and the block's references. Wide: the
+// transpose and the gather over 256 samples at a time, and the list of one
+// input, which is walked alone. The constants were fitted to 700 random layers
+// (100-400000 inputs and outputs, 1-4096 samples, K 1-16) with a reference table
+// that took 10 us and 0.3 ns a key more than the sort does; they stay, so that
+// fp32 layers keep their sums' order, and no longer take the shorter way
+// everywhere. As it is, captured, us from LDS / wide (* taken): fp32 backward, K =
+// 8: 10000 -> 10000, B = 1024 190* / 249; 60000 -> 60000, B = 124 1014 / 1067*;
+// 172000 -> 172000, B = 3 838 / 853*; 100000 -> 100000, B = 1 359 / 419*. 8-bit
+// backward: K = 8 10000 -> 10000, B = 1024 151* / 201, B = 256 109* / 94; 40000 ->
+// 40000, B = 124 355 / 227*; K = 4 12000 -> 12000, B = 300 143 / 99*; 16380 ->
+// 16380, B = 1024 242 / 257*.
 static bool ig_small(const IgArgs& a);
 static bool ig_fits(const IgPlan& p) {
   return p.a.R + p.groups * ig_slack(p.a.IB) < (1LL << 31) && p.nkeys < (1LL << 31) &&
@@ -709,10 +714,10 @@ static int fc_input_grad_wide(const float* gbr, int64_t B, int64_t IN, int64_t O
 // at most (an element's rank reads its list) and at most 4096 references a
 // block, 48K in all: a workgroup's scattered loads and stores bound it, so it
 // follows the references of a block, and every block reads all of them. 8-bit
-// backward, K = 8, this against the general way, captured, us: 250 -> 250, B =
-// 64: 35 / 38; 1000, B = 256 (4000 a block): 41 / 48; 3000, B = 64 (4000 a
-// block, 48000 in all): 51 / 58; past the rule 4000, B = 64: 57 / 61; 2000,
-// B = 256 (8000 a block): 58 / 58; 1000, B = 1024 (16000): 73 / 51.
+// backward to the parameters, K = 8, this against the general way, captured, us:
+// 250 -> 250, B = 64: 38 / 41; 1000, B = 256 (4000 a block): 50 / 56; 3000, B = 64
+// (4000 a block, 48000 in all): 58 / 60; past the rule 4000, B = 64: 67 / 65; 2000,
+// B = 256 (8000 a block): 71 / 65; 1000, B = 1024 (16000): 94 / 69.
 static size_t ig_small_lds(const IgArgs& a) {
   return (size_t)(a.IB + 1) * 4 + (size_t)a.R * 2;
 }

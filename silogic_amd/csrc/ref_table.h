@@ -21,13 +21,16 @@ int64_t ref_table_ints(int64_t R, int64_t nkeys);
 int build_ref_table(const int* keys, int64_t R, int64_t nkeys, int* ws, hipStream_t st,
                     RefTable* out);
 
-// How many of R entries sorted by key (x) lie below key k.
+// How many of R entries sorted by key (x) lie below key k: three reads a step
+// leave a quarter of the range (by halves, twice as many reads one after the
+// other).
 __device__ inline int ref_start(const int2* __restrict__ ent, int R, int64_t k) {
-  int lo = 0, hi = R;
-  while (lo < hi) {
-    const int mid = lo + ((hi - lo) >> 1);
-    if (ent[mid].x < k) lo = mid + 1;
-    else hi = mid;
+  int lo = 0, n = R;  // between lo and lo + n
+  while (n > 0) {
+    const int a = lo + (n >> 2), b = lo + (n >> 1), c = b + (n >> 2), end = lo + n;
+    const bool pa = ent[a].x < k, pb = ent[b].x < k, pc = ent[c].x < k;
+    lo = pc ? c + 1 : pb ? b + 1 : pa ? a + 1 : lo;
+    n = (pc ? end : pb ? c : pa ? b : a) - lo;
   }
   return lo;
 }
