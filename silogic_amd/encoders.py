@@ -148,8 +148,10 @@ class TokenEncoder(nn.Module):
             raise TypeError(f"TokenEncoder: ids of {ids.dtype} (int32 or int64)")
         if ids.dim() not in (1, 2):
             raise ValueError(f"TokenEncoder: ids {tuple(ids.shape)}, [B] or [B, L] expected")
-        ops.require_gpu(ids, weight)
-        ops.same_device("TokenEncoder", ids, weight)
+        d = ids.get_device()
+        if d < 0 or d != weight.get_device():   # the check that says what is wrong
+            ops.require_gpu(ids, weight)
+            ops.same_device("TokenEncoder", ids, weight)
         return ops._c(ids if ids.dim() == 2 else ids.unsqueeze(1))
 
     def forward(self, ids):
