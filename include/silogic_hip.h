@@ -274,8 +274,9 @@ int slg_learned_thermo_bwd(const float* x, int64_t B, int64_t F, int32_t T, cons
  *                          where table[id] > 0, else 0
  *   slg_token_encode_bwd   gtable [V,D] (the table's type, all of it written) =
  *                          scale * sigmoid'(scale * table) * (gy [N,D] summed
- *                          over each id's tokens, in ascending order of n: the
- *                          same bits on every call). workspace: that many
+ *                          over each id's tokens, in an order that follows from
+ *                          the ids alone: the same bits on every call).
+ *                          workspace: that many
  *                          4-byte words, at a multiple of 16 bytes
  *   slg_token_bits         bits [V, ceil(D/64)] = table > 0, bit d % 64 of word
  *                          d / 64: the table of slg_token_encode_hard, made

@@ -47,9 +47,9 @@ def save_activations(model, bits=8):
     input in ``bits`` bits for the backward: 8, or 32 to go back. Outputs do
     not change; gradients are taken at the 8-bit values. Returns how many
     layers were set; a model without one raises. LUT layers and conv blocks
-    keep fp32: a conv block's backward routes each pooled gradient by
-    comparing the forward's exact values, which 8 bits would move at
-    near-ties."""
+    keep fp32: the LUT layers' backward has no form on codes, and a conv
+    block's routes each pooled gradient by comparing the forward's exact
+    values, which 8 bits would move at near-ties."""
     from .layers import LogicLayer
     if bits not in (8, 32):
         raise ValueError(f"save_activations: {bits} bits (8 or 32)")

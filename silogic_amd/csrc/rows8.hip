@@ -140,7 +140,8 @@ rows8_pack_kernel(const float* __restrict__ x, int64_t B, int D, int ld, uint32_
 // Rows too wide for that: the tile's four rows one after the other, NU runs of
 // 4 of one row a thread, while their codes gather in as many words (D <= 4096 *
 // NU; 1024 threads). The next row's values are on their way as soon as the last
-// one's are coded. 2048 x 32000: 73 us, with every value read twice 104 (1500 x
+// one's are coded (behind the tile's last row that row again, from the caches,
+// unused). 2048 x 32000: 73 us, with every value read twice 104 (1500 x
 // 40960: 72 and 99; 64 x 20000: 10.1 and 9.5).
 template <int NU>
 __global__ void __launch_bounds__(1024)

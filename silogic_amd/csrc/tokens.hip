@@ -355,7 +355,9 @@ tok_join_kernel(SegArgs a, const int2* __restrict__ ent, const float* __restrict
 // ---------------------------------------------------------------------------
 // Hard bits
 // ---------------------------------------------------------------------------
-// bits [V][DW] words: bit d % 64 of word d / 64 of a row = E > 0. A wave per word.
+// bits [V][DW] words: bit d % 64 of word d / 64 of a row = E > 0. A wave per word,
+// with one load of 64 values in flight: 32000 x 64 in fp32 7 us (8.4 MB, 1.2
+// TB/s), once a version of the weight.
 template <int DT>
 __global__ void __launch_bounds__(256)
 tok_bits_kernel(const typename TabType<DT>::t* __restrict__ tab, int64_t words, int D, int DW,
@@ -448,8 +450,10 @@ __device__ inline void tok_rows(const IdT* __restrict__ p, int64_t n, int V, int
 // j then holds feature j's word. Word-major rows of features are written as
 // they are; for the rows [F][nw] a workgroup's waves take TW neighbouring
 // words, which leave through LDS in runs of TW. Bound by the loads of
-// single rows of bits, a line each: 65536 x 16 tokens of 64 bits 9.7 us (25 MB,
-// 2.6 TB/s; with the ids loaded one by one 13.4), 65536 x 128 of 2 bits 43.
+// single rows of bits, a line each: 65536 x 16 tokens of 64 bits 9.7 us (17 MB
+// of ids and words, 1.8 TB/s; with the ids loaded one by one 13.4), 65536 x 128
+// of 2 bits 43. Word-major the same to 5% (calls of 65536 x 64 x 100 bits: 42.5
+// us, word-major 39.9).
 template <typename IdT, bool WM, int TW>
 __global__ void __launch_bounds__(64 * TW)
 tok_packed_kernel(const IdT* __restrict__ ids, int64_t B, int64_t L, int V, int64_t pad, int D, int DW,
