@@ -298,6 +298,62 @@ int slg_token_encode_hard(const void* ids, int32_t id_bytes, int64_t B, int64_t 
                           int64_t D, int64_t pad, const uint64_t* bits, int32_t layout, void* out,
                           slg_stream_t stream);
 
+/* On a network's logits [N,V] (no counterpart in the reference): dtype 0 fp32, 1
+ * bf16, 2 fp16, rows `ld` values apart (0: one row for all). A NaN or -inf is
+ * absent in the first two of
+ *   slg_top_logits         the K largest of each row (K <= V, at most 1024; V at
+ *                          most 2^24): values [N,K] in the logits' type, ids
+ *                          [N,K], by value, equal values by the lower id; -inf
+ *                          and -1 past the tokens that are there
+ *   slg_sample_logits      one token of each row from u [N] in [0,1): by masses
+ *                          exp((s - max) / temperature) in the order above, kept
+ *                          are the first top_k (0: all), of these those before
+ *                          which lies less than top_p of their mass, of these
+ *                          those with at least min_p of the largest mass; drawn
+ *                          is the first whose running sum passes u times theirs.
+ *                          A temperature that is not over 0 takes the first. -1
+ *                          where no token is there. allowed: NULL, or bytes
+ *                          [N,V], rows allowed_ld apart, 0 for a token that is
+ *                          not. Limits of each row instead of the numbers where
+ *                          the pointer is not NULL ([N]; those out of their
+ *                          range act as their nearest bound)
+ *   slg_distill_fwd        loss of the logits against a teacher's entries, values
+ *                          [N,K] (vtype as dtype; K <= 1024) at ids [N,K] of
+ *                          id_bytes 4 or 8 (absent: outside 0..V-1, or a value of
+ *                          -inf), and labels [N] (NULL: none; absent: outside
+ *                          0..V-1): (1 - alpha) T^2 KL(softmax(values / T) ||
+ *                          softmax(logits / T)) + alpha * cross entropy, the KL
+ *                          alone without labels. A term without entries or label
+ *                          counts 0. reduction 0: loss [N], 1: their sum, 2: the
+ *                          mean over rows with an entry or a label. 1e-4 <= T <=
+ *                          1e4. kept: slg_distill_kept(N) floats for
+ *   slg_distill_bwd        grad [N,V] (the logits' type) = scale * upstream (NULL:
+ *                          1; [N], or [1] with a reduction) * d loss / d logits;
+ *                          0 in rows whose upstream is 0 or that have no term
+ *   slg_distill_loss_grad  both with an upstream of `scale` */
+int slg_top_logits(const void* logits, int32_t dtype, int64_t N, int64_t V, int64_t ld, int64_t K,
+                   void* values, int64_t* ids, slg_stream_t stream);
+int slg_sample_logits(const void* logits, int32_t dtype, int64_t N, int64_t V, int64_t ld,
+                      const uint8_t* allowed, int64_t allowed_ld, const float* u, double temperature,
+                      int64_t top_k, double top_p, double min_p, const float* temperatures,
+                      const int64_t* top_ks, const float* top_ps, const float* min_ps, int64_t* ids,
+                      slg_stream_t stream);
+int64_t slg_distill_kept(int64_t N);
+int slg_distill_fwd(const void* logits, int32_t dtype, int64_t N, int64_t V, int64_t ld,
+                    const void* values, int32_t vtype, const void* ids, int32_t id_bytes, int32_t K,
+                    const void* labels, int32_t label_bytes, float T, float alpha, int32_t reduction,
+                    float* loss, float* kept, slg_stream_t stream);
+int slg_distill_bwd(const void* logits, int32_t dtype, int64_t N, int64_t V, int64_t ld,
+                    const void* values, int32_t vtype, const void* ids, int32_t id_bytes, int32_t K,
+                    const void* labels, int32_t label_bytes, float T, float alpha, int32_t reduction,
+                    const float* kept, const float* upstream, float scale, void* grad,
+                    slg_stream_t stream);
+int slg_distill_loss_grad(const void* logits, int32_t dtype, int64_t N, int64_t V, int64_t ld,
+                          const void* values, int32_t vtype, const void* ids, int32_t id_bytes,
+                          int32_t K, const void* labels, int32_t label_bytes, float T, float alpha,
+                          int32_t reduction, float scale, float* loss, void* grad, float* kept,
+                          slg_stream_t stream);
+
 /* Activations kept in 8 bits between a layer's forward and its backward (no
  * counterpart in the reference). x [B,D] fp32 -> codes [ceil(B/4)][ld][4] uint8
  * (at a multiple of 16 bytes), ld = slg_rows8_ld(D), byte v of (t, i) the code

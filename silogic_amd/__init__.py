@@ -18,8 +18,10 @@ Compute is GPU-only; CPU tensors raise. Covered: nodes ``gate16``,
 layers and conv trees (binary trees of depth 1-5, LUT trees of at most 36
 leaves); wiring ``topk``, ``blocktopk``, ``fixed``; ``GroupSum`` heads;
 ``ConvLogicTree`` + ``OrPool``; the layer and network presets; learned bits of
-token ids (``TokenEncoder``) and training activations kept in 8 bits
-(``save_activations``), which the reference has not.
+token ids (``TokenEncoder``), training activations kept in 8 bits
+(``save_activations``), a loss against a teacher's largest logits
+(``top_logits``, ``distill_loss``) and tokens drawn from logits
+(``sample_logits``), which the reference has not.
 """
 
 __version__ = "0.1.0"
@@ -35,6 +37,7 @@ from .layers import (LogicLayer, WARPLayer, WARPLayerN, LUTkLayer, LUTNodeLayer,
 from .models import LogicNet, WARPNet, WARPNetN, LUTkNet, LUTNodeNet, LogicConvNet, LogicTreeNet
 from .encoders import LearnedThermometerEncoder, TokenEncoder
 from .activations import pack_rows8, unpack_rows8, save_activations
+from .logits import top_logits, sample_logits, distill_loss, distill_loss_and_grad
 from .data import (binarize, binarize_spatial, binarize_packed, edge_bits, MNIST_THRESH,
                    SEVEN_THRESH, FOUR_THRESH, FIVE_THRESH, CIFAR3_THRESH, EDGE_THRESH)
 from . import derived, kernels, library, ops
@@ -47,6 +50,7 @@ __all__ = [
     "ConvLogicLayer", "OrPool", "LogicNet", "WARPNet", "WARPNetN", "LUTkNet", "LUTNodeNet",
     "LogicConvNet", "LogicTreeNet", "kernels", "ops",
     "LearnedThermometerEncoder", "TokenEncoder", "pack_rows8", "unpack_rows8", "save_activations",
+    "top_logits", "sample_logits", "distill_loss", "distill_loss_and_grad",
     "binarize", "binarize_spatial", "binarize_packed", "edge_bits",
     "MNIST_THRESH", "SEVEN_THRESH", "FOUR_THRESH", "FIVE_THRESH", "CIFAR3_THRESH", "EDGE_THRESH",
 ]

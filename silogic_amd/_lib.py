@@ -11,7 +11,7 @@ import threading
 
 from . import _build
 
-_P, _I32, _I64, _F32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float
+_P, _I32, _I64, _F32, _F64 = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_double
 
 # name -> (restype, argtypes); mirrors include/silogic_hip.h one to one
 SIGNATURES = {
@@ -71,6 +71,16 @@ SIGNATURES = {
                                        _I64, _P]),
     "slg_token_bits": (C.c_int, [_P, _I32, _I64, _I64, _P, _P]),
     "slg_token_encode_hard": (C.c_int, [_P, _I32, _I64, _I64, _I64, _I64, _I64, _P, _I32, _P, _P]),
+    "slg_top_logits": (C.c_int, [_P, _I32, _I64, _I64, _I64, _I64, _P, _P, _P]),
+    "slg_sample_logits": (C.c_int, [_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _F64, _I64, _F64, _F64, _P, _P,
+                                    _P, _P, _P, _P]),
+    "slg_distill_kept": (_I64, [_I64]),
+    "slg_distill_fwd": (C.c_int, [_P, _I32, _I64, _I64, _I64, _P, _I32, _P, _I32, _I32, _P, _I32, _F32, _F32,
+                                  _I32, _P, _P, _P]),
+    "slg_distill_bwd": (C.c_int, [_P, _I32, _I64, _I64, _I64, _P, _I32, _P, _I32, _I32, _P, _I32, _F32, _F32,
+                                  _I32, _P, _P, _F32, _P, _P]),
+    "slg_distill_loss_grad": (C.c_int, [_P, _I32, _I64, _I64, _I64, _P, _I32, _P, _I32, _I32, _P, _I32, _F32,
+                                        _F32, _I32, _F32, _P, _P, _P, _P]),
     "slg_conv_soft_bwd_workspace": (C.c_int64, [_I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32,
                                                 _I32, _I32, _I32]),
     "slg_conv_soft_bwd": (C.c_int, [_P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _P,

@@ -496,6 +496,101 @@ token_encode.register_autograd(_token_backward, setup_context=_token_setup)
 
 
 # ---------------------------------------------------------------------------
+# A network's logits: what torch.compile traces (rows [N, V] as ops takes them)
+# ---------------------------------------------------------------------------
+@torch.library.custom_op(f"{_NS}::top_logits", mutates_args=())
+def top_logits(logits: Tensor, k: int) -> Tuple[Tensor, Tensor]:
+    ops.require_gpu(logits)
+    return ops.top_logits(ops.check_logits("top_logits", logits), k)
+
+
+@top_logits.register_fake
+def _(logits, k):
+    return logits.new_empty((logits.shape[0], k)), logits.new_empty((logits.shape[0], k), dtype=torch.int64)
+
+
+@torch.library.custom_op(f"{_NS}::sample_logits", mutates_args=())
+def sample_logits(logits: Tensor, u: Tensor, temperature: float, top_k: int, top_p: float, min_p: float,
+                  temperatures: Optional[Tensor], top_ks: Optional[Tensor], top_ps: Optional[Tensor],
+                  min_ps: Optional[Tensor], mask: Optional[Tensor]) -> Tensor:
+    from . import logits as lg
+    limits = [v if each is None else each for v, each in
+              ((temperature, temperatures), (top_k, top_ks), (top_p, top_ps), (min_p, min_ps))]
+    return lg.sample_logits(logits, u, *limits, mask)
+
+
+@sample_logits.register_fake
+def _(logits, u, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps, mask):
+    return logits.new_empty((logits.shape[0],), dtype=torch.int64)
+
+
+def _distill_checked(logits, values, ids, labels, temperature, alpha, reduction):
+    from . import logits as lg
+    names = {v: k for k, v in ops.REDUCTIONS.items()}
+    return lg._distill("distill_loss", logits, values, ids, labels, temperature, alpha, names.get(reduction))
+
+
+def _distill_shapes(logits, reduction):
+    f32 = torch.float32
+    return (logits.new_empty((logits.shape[0],) if reduction == 0 else (), dtype=f32),
+            logits.new_empty((9 * logits.shape[0] + 1,), dtype=f32))
+
+
+@torch.library.custom_op(f"{_NS}::distill_loss", mutates_args=())
+def distill_loss(logits: Tensor, values: Tensor, ids: Tensor, labels: Optional[Tensor], temperature: float,
+                 alpha: float, reduction: int) -> Tuple[Tensor, Tensor]:
+    return ops.distill_fwd(*_distill_checked(logits, values, ids, labels, temperature, alpha, reduction))
+
+
+@distill_loss.register_fake
+def _(logits, values, ids, labels, temperature, alpha, reduction):
+    return _distill_shapes(logits, reduction)
+
+
+@torch.library.custom_op(f"{_NS}::distill_loss_bwd", mutates_args=())
+def distill_loss_bwd(logits: Tensor, values: Tensor, ids: Tensor, labels: Optional[Tensor], temperature: float,
+                     alpha: float, reduction: int, kept: Tensor, upstream: Tensor) -> Tensor:
+    args = _distill_checked(logits, values, ids, labels, temperature, alpha, reduction)
+    if kept.dtype != torch.float32 or kept.shape != (9 * logits.shape[0] + 1,) or not kept.is_contiguous() or \
+            upstream.shape != (logits.shape[:1] if reduction == 0 else ()):
+        raise ValueError(f"distill_loss_bwd: kept {kept.dtype} {tuple(kept.shape)}, upstream {tuple(upstream.shape)}")
+    ops.require_gpu(kept, upstream)
+    ops.same_device("distill_loss_bwd", logits, kept, upstream)
+    return ops.distill_bwd(*args, kept, upstream)
+
+
+@distill_loss_bwd.register_fake
+def _(logits, values, ids, labels, temperature, alpha, reduction, kept, upstream):
+    return logits.new_empty(logits.shape)
+
+
+def _distill_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:4], output[1])
+    ctx.how = inputs[4:]
+    ctx.mark_non_differentiable(output[1])
+
+
+def _distill_backward(ctx, g, _):
+    *given, kept = ctx.saved_tensors
+    gx = distill_loss_bwd(*given, *ctx.how, kept, g) if ctx.needs_input_grad[0] else None
+    return gx, None, None, None, None, None, None
+
+
+distill_loss.register_autograd(_distill_backward, setup_context=_distill_setup)
+
+
+@torch.library.custom_op(f"{_NS}::distill_loss_grad", mutates_args=())
+def distill_loss_grad(logits: Tensor, values: Tensor, ids: Tensor, labels: Optional[Tensor], temperature: float,
+                      alpha: float, reduction: int, scale: float) -> Tuple[Tensor, Tensor]:
+    return ops.distill_loss_grad(*_distill_checked(logits, values, ids, labels, temperature, alpha, reduction), scale)
+
+
+@distill_loss_grad.register_fake
+def _(logits, values, ids, labels, temperature, alpha, reduction, scale):
+    return _distill_shapes(logits, reduction)[0], logits.new_empty(logits.shape)
+
+
+# ---------------------------------------------------------------------------
 # LUT FC layer (multilinear_logic)
 # ---------------------------------------------------------------------------
 @torch.library.custom_op(f"{_NS}::fc_lut_soft", mutates_args=())

@@ -25,6 +25,7 @@ import torch.nn as nn
 from . import derived, ops
 from .heads import GroupSum, build_decoder
 from .layers import LogicLayer, ConvLogicTree, OrPool, _needs_grad
+from .logits import sample_logits
 
 
 def _per_layer(v, i):
@@ -138,7 +139,21 @@ def _hard_fc_stack(layers, x, in_kind, B, in_dim, C, wire_r):
     return ops.groupsum_packed(xp, B, C)
 
 
-class LogicNet(nn.Module):
+class _Samples:
+    @torch.no_grad()
+    def sample(self, x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None, hard=False):
+        """A class (or token) of each sample of ``x``, drawn from the network's
+        logits with the random numbers ``u [B]`` (:func:`sample_logits`):
+        the soft ones, or with ``hard`` the bit-packed circuit's counts over
+        the head's ``tau``."""
+        if hard:
+            logits, temperature = self.forward_hard(x), temperature * self.head.tau
+        else:
+            logits = self(x)
+        return sample_logits(logits, u, temperature, top_k, top_p, min_p, mask)
+
+
+class LogicNet(_Samples, nn.Module):
     """Stack of logic layers followed by a GroupSum head (arguments as
     silogic.models.LogicNet)."""
 
@@ -272,7 +287,7 @@ class LUTNodeNet(LogicNet):
                          arity=arity, k=k, tau=tau, residual_p=residual_p, seed=seed)
 
 
-class LogicConvNet(nn.Module):
+class LogicConvNet(_Samples, nn.Module):
     """Convolutional logic-gate-tree network with a logic head (arguments as
     silogic.models.LogicConvNet)."""
 

@@ -582,6 +582,88 @@ def token_encode_hard(ids, bits, D, pad, layout):
 
 
 # ---------------------------------------------------------------------------
+# a network's logits: largest ones, draws, a teacher's loss
+# ---------------------------------------------------------------------------
+def check_logits(what, logits):
+    """``logits`` as rows ``[N, V]`` of neighbouring values."""
+    if logits.dtype not in TABLE_DTYPES:
+        raise TypeError(f"{what}: logits of {logits.dtype} (fp32, bf16 or fp16)")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{what}: logits {tuple(logits.shape)}, [..., V] expected")
+    if logits.dim() != 2:
+        logits = logits.reshape(-1, logits.shape[-1])
+    return logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
+
+
+def top_logits(logits, k):
+    """``(values, ids)`` ``[N, k]`` of rows ``logits [N, V]`` (``slg_top_logits``)."""
+    N, V = logits.shape
+    if not 1 <= k <= min(V, 1024):
+        raise ValueError(f"top_logits: {k} of {V} logits (1 to 1024, and no more than there are)")
+    values, ids = logits.new_empty((N, k)), logits.new_empty((N, k), dtype=torch.int64)
+    call_on(logits, "slg_top_logits", logits.data_ptr(), TABLE_DTYPES[logits.dtype], N, V, logits.stride(0), k,
+            values.data_ptr(), ids.data_ptr())
+    return values, ids
+
+
+def sample_logits(logits, u, t, k, p, m, mask):
+    """Tokens ``[N]`` of rows ``logits [N, V]``; ``u [N]`` fp32, ``t``, ``k``,
+    ``p``, ``m`` numbers or ``[N]`` (``k`` int64, the others fp32), ``mask``
+    None or bool ``[N, V]`` (``slg_sample_logits``)."""
+    N, V = logits.shape
+    ids = logits.new_empty((N,), dtype=torch.int64)
+    number = [0 if isinstance(v, torch.Tensor) else v for v in (t, k, p, m)]
+    each = [v.data_ptr() if isinstance(v, torch.Tensor) else None for v in (t, k, p, m)]
+    call_on(logits, "slg_sample_logits", logits.data_ptr(), TABLE_DTYPES[logits.dtype], N, V, logits.stride(0),
+            None if mask is None else mask.data_ptr(), 0 if mask is None else mask.stride(0), u.data_ptr(),
+            *number, *each, ids.data_ptr())
+    return ids
+
+
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+def _distill_args(logits, values, ids, labels, t, alpha, reduction):
+    N, V = logits.shape
+    return (logits.data_ptr(), TABLE_DTYPES[logits.dtype], N, V, logits.stride(0), values.data_ptr(),
+            TABLE_DTYPES[values.dtype], ids.data_ptr(), ids.element_size(), values.shape[1],
+            None if labels is None else labels.data_ptr(), 0 if labels is None else labels.element_size(),
+            t, alpha, reduction)
+
+
+def _distill_out(logits, reduction):
+    N = logits.shape[0]
+    loss = logits.new_empty((N,) if reduction == 0 else (), dtype=torch.float32)
+    return loss, logits.new_empty(_lib.lib().slg_distill_kept(N), dtype=torch.float32)
+
+
+def distill_fwd(logits, values, ids, labels, t, alpha, reduction):
+    """``(loss, kept)`` of rows ``logits [N, V]``, contiguous ``values``, ``ids``
+    ``[N, K]`` and ``labels [N]`` or None (``slg_distill_fwd``)."""
+    loss, kept = _distill_out(logits, reduction)
+    call_on(logits, "slg_distill_fwd", *_distill_args(logits, values, ids, labels, t, alpha, reduction),
+            loss.data_ptr(), kept.data_ptr())
+    return loss, kept
+
+
+def distill_bwd(logits, values, ids, labels, t, alpha, reduction, kept, upstream):
+    """The logits' gradient ``[N, V]`` in their type."""
+    grad, upstream = logits.new_empty(logits.shape), _c(upstream, torch.float32)
+    call_on(logits, "slg_distill_bwd", *_distill_args(logits, values, ids, labels, t, alpha, reduction),
+            kept.data_ptr(), upstream.data_ptr(), 1.0, grad.data_ptr())
+    return grad
+
+
+def distill_loss_grad(logits, values, ids, labels, t, alpha, reduction, scale):
+    """``(loss, grad)`` with an upstream gradient of ``scale``."""
+    loss, kept = _distill_out(logits, reduction)
+    grad = logits.new_empty(logits.shape)
+    call_on(logits, "slg_distill_loss_grad", *_distill_args(logits, values, ids, labels, t, alpha, reduction),
+            scale, loss.data_ptr(), grad.data_ptr(), kept.data_ptr())
+    return loss, grad
+
+
+# ---------------------------------------------------------------------------
 # FC layers of n-input LUT nodes (multilinear of any arity, hybrid)
 # ---------------------------------------------------------------------------
 def _fc_lut_launch(x, cand, w, s, hybrid):
