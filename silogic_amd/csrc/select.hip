@@ -6,14 +6,18 @@
 // Drawing (temperature T, limits k, p and m, a random number u in [0, 1)): masses w = exp((s - max) / T), of which
 // the first k tokens stay, of these those before which lies less than p of their mass, of these those with w >= m;
 // drawn is the first whose running sum passes u times theirs. Masses are held as whole numbers of 2^-F, F = 62 -
-// log2 V and at most 52 (45 bits at 131072 tokens, where exp in 64 bits is off by 2^-52): their sums are exact, the
+// log2 V and at most 50 (47 bits at 32000 tokens, where exp in 64 bits is off by 2^-51): their sums are exact, the
 // same in any order, so LDS atomics may make them, and a border between two tokens is where 64-bit sums have it up
 // to about V 2^-F.
 //
-// Finding a place in the order by its running count or mass goes by histogram: 2048 bins of equal width over the
-// values (where a logit's mass goes by e^value, bins of equal keys would put most of a row into few bins), a scan,
-// then the bin's own tokens, sorted if a thread can hold each, else by bins of their place numbers again until they
-// are few.
+// A workgroup takes a row, in registers where it fits (the only read of it). What the limits keep is found by value
+// first: k tokens are at least as large as a threshold that k lanes' own maxima reach, min_p is a threshold by
+// itself. If a thread can hold each of the tokens past it, they are sorted and summed in order. Else places in the
+// order are found by histogram: bins of equal width over the values (where a logit's mass goes by e^value, bins of
+// equal keys would put most of a row into few bins), a scan, then the bin's own tokens, sorted if a thread can hold
+// each, else by bins of their place numbers until they are few.
+#include <float.h>
+
 #include <algorithm>
 
 #include "block_ops.h"
@@ -21,10 +25,9 @@
 
 namespace slg {
 
-constexpr int kBins = 2048;
 constexpr int kMaxTop = 1024;
 
-// Rising with x, 0 for absent.
+// Rising with x.
 __device__ inline uint32_t key_of(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);   // -0 and 0 are equal
   return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
@@ -33,77 +36,195 @@ __device__ inline float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
+// Bins of a histogram: enough that a long row's fullest bin seldom holds more tokens than threads, few enough to
+// clear and scan.
+template <int TH>
+constexpr int kBins = TH == 64 ? 256 : TH == 256 ? 1024 : 2048;
+
 template <int TH>
 struct SelectLds {
-  uint64_t hist[kBins];
+  uint64_t hist[kBins<TH>];
   uint64_t list[TH];
   uint64_t part[TH / 64];
   uint64_t at, base;
   int n;
 };
 
-// A row of logits, its order, and the masses of its tokens.
-template <int DT, int TH>
+// 2^f on [-1/2, 1/2] by the polynomial of degree 10 with value 1 at 0 and the least largest relative error, 3e-16
+// (fitted by exchange of its extremes). In memory, so that they come to scalar registers: a literal of 64 bits would
+// be moved to vector ones before each product.
+__constant__ double kExp2[10] = {0x1.62e42fefa3a28p-1,  0x1.ebfbdff82c61fp-3,  0x1.c6b08d7039559p-5,  0x1.3b2ab6fb8208ep-7,
+                                 0x1.5d87fea4a755ap-10, 0x1.43091387c719ep-13, 0x1.ffcb3f1b1dfa2p-17, 0x1.62be68640a005p-20,
+                                 0x1.b689b4ad4f65fp-24, 0x1.e8b761c675c38p-28};
+__device__ __forceinline__ double exp2_small(double f) {
+  double p = kExp2[9];
+#pragma unroll
+  for (int i = 8; i >= 0; --i) p = fma(p, f, kExp2[i]);
+  return fma(p, f, 1.0);
+}
+
+// A row of logits over the threads of a workgroup, group j of thread t the row's (j TH + t)th of 16 bytes: the first NV
+// in registers, others read again by each pass (NV = 0: rows shorter than a group too).
+template <int DT, int TH, int NV>
 struct Row {
   using T = typename TabType<DT>::t;
+  static constexpr int VU = 16 / (int)sizeof(T);
+  static constexpr int BINS = kBins<TH>;
+  static constexpr bool MORE = NV == 0 || NV == 8;   // rows may be longer than the registers hold
+  typedef T Vec __attribute__((ext_vector_type(VU), aligned(sizeof(T))));
+  typedef uint8_t Bytes __attribute__((ext_vector_type(VU), aligned(1)));
   const T* logits;
   const uint8_t* allowed;   // null: all
   int V, bits;
   uint64_t id_mask;
   SelectLds<TH>* lds;
-  // set by masses()
-  float top, scale_bins;
-  double inv_t, one;
-  double least;   // masses under it count nothing
-  uint64_t from;  // tokens before it in the numbers count nothing
+  Vec r[NV ? NV : 1];
+  bool infinite;
+  float top, bin_scale;
+  double top64, slope, shifter, least;   // slope: log2 e / T; masses under `least` (in units of 2^-F) count nothing
+  int F;
+  uint64_t from;   // tokens whose place number is under it count nothing
 
-  __device__ Row(const T* l, const uint8_t* m, int v, SelectLds<TH>* s) : logits(l), allowed(m), V(v), lds(s) {
+  __device__ __forceinline__ Row(const T* l, const uint8_t* m, int v, SelectLds<TH>* s) : logits(l), allowed(m), V(v), lds(s) {
     bits = 32 - __clz(v);
     id_mask = (1ull << bits) - 1;
-    from = 1;
+    infinite = false;
+    from = 0;
     least = 0.0;
-  }
-  __device__ uint64_t comp(float x, int i) const { return ((uint64_t)key_of(x) << bits) | (id_mask - (uint64_t)i); }
-  __device__ int id_of(uint64_t c) const { return (int)(id_mask - (c & id_mask)); }
-  __device__ float of(uint64_t c) const { return value_of((uint32_t)(c >> bits)); }
-
-  // f(comp, x) of the tokens that are there.
-  template <class F>
-  __device__ void each(F f) const {
-    for (int i = threadIdx.x; i < V; i += TH) {
-      const float x = tab_get<DT>(logits[i]);
-      if (x > -INFINITY && (!allowed || allowed[i])) f(comp(x, i), x);
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) r[j] = read((j * TH + (int)threadIdx.x) * VU);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (allowed || (j + 1) * TH * VU > V) strike(r[j], (j * TH + (int)threadIdx.x) * VU);
     }
   }
 
-  __device__ void masses(float max, float min, double t) {
-    top = max;
-    inv_t = 1.0 / t;
-    const int f = min_(52, 62 - bits);
-    one = (double)(1ull << f);
-    // masses end where they fall under 2^-(F+1), values where the row does
-    const float range = fmaxf(fminf((float)((f + 2) * 0.6931472 * t), max - min), 1e-30f);
-    scale_bins = (float)kBins / range;
+  static __device__ T absent() {
+    if constexpr (DT == kTabBf16) return (T)0x7fc0;
+    else return (T)NAN;
   }
-  static __device__ int min_(int a, int b) { return a < b ? a : b; }
-  __device__ uint64_t mass(float x) const {
-    const double e = exp((x == top ? 0.0 : (double)x - (double)top) * inv_t);
-    return e >= least ? (uint64_t)rint(e * one) : 0;   // a NaN (0 times an infinity) is none
+  // The first token of the group that begins at token i: a row's last group is moved back to end with the row, and
+  // those past it come to lie there too. Tokens before i in it are another group's.
+  __device__ __forceinline__ int base(int i) const { return NV == 0 && V < VU ? i : min(i, V - VU); }
+  __device__ __forceinline__ Vec read(int i) const {
+    if (NV > 0 || V >= VU) return *reinterpret_cast<const Vec*>(reinterpret_cast<const char*>(logits) + (uint32_t)base(i) * (uint32_t)sizeof(T));
+    Vec x;
+#pragma unroll
+    for (int u = 0; u < VU; ++u) x[u] = logits[min(i + u, V - 1)];
+    return x;
   }
-  __device__ int bin(float x) const { return (int)fminf((top - x) * scale_bins, (float)(kBins - 1)); }
+  // NaN for tokens that are another group's, past the row or not allowed.
+  __device__ __forceinline__ void strike(Vec& x, int i) const {
+    const int b = base(i);
+#pragma unroll
+    for (int u = 0; u < VU; ++u) x[u] = b + u >= i && b + u < V ? x[u] : absent();
+    if (allowed) {
+      if (NV > 0 || V >= VU) {
+        const Bytes m = *reinterpret_cast<const Bytes*>(allowed + b);
+#pragma unroll
+        for (int u = 0; u < VU; ++u) x[u] = m[u] ? x[u] : absent();
+      } else {
+#pragma unroll
+        for (int u = 0; u < VU; ++u) x[u] = allowed[min(b + u, V - 1)] ? x[u] : absent();
+      }
+    }
+  }
+  // f(x, token) of all tokens, absent ones (-inf, NaN) among them, and NaN past the row.
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      // a group at a time, and nothing of it kept from an earlier pass: what is computed of all values at once, or
+      // kept, does not fit the registers beside them
+      Vec x = r[j];
+      int t = threadIdx.x;
+      asm volatile("" : "+v"(x), "+v"(t));
+      const int i = base((j * TH + t) * VU);
+#pragma unroll
+      for (int u = 0; u < VU; ++u) {
+        f(tab_get<DT>(x[u]), i + u);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (MORE) each_again<NV>(f);
+  }
+  // The same from memory, from group FIRST TH on: for what the registers do not hold, and passes that few rows need.
+  template <int FIRST, class F>
+  __device__ __forceinline__ void each_again(F f) const {
+#pragma unroll 1
+    for (int i = (FIRST * TH + (int)threadIdx.x) * VU; i < V; i += TH * VU) {
+      Vec x = read(i);
+      const int b = base(i);
+      if (allowed || i + VU > V) strike(x, i);
+#pragma unroll
+      for (int u = 0; u < VU; ++u) {
+        f(value(x[u]), b + u);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  __device__ __forceinline__ float value(T v) const {
+    const float x = tab_get<DT>(v);
+    return infinite ? (x == INFINITY ? 0.0f : -INFINITY) : x;
+  }
+  // The largest is +inf: those that are count as 0, the others are absent.
+  __device__ __forceinline__ void set_infinite() {
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int u = 0; u < VU; ++u) r[j][u] = tab_get<DT>(r[j][u]) == INFINITY ? (T)0 : absent();
+    }
+    infinite = true;
+  }
+  __device__ __forceinline__ uint64_t comp(float x, int i) const { return ((uint64_t)key_of(x) << bits) | (id_mask - (uint64_t)i); }
+  __device__ __forceinline__ int id_of(uint64_t c) const { return (int)(id_mask - (c & id_mask)); }
+  __device__ __forceinline__ float of(uint64_t c) const { return value_of((uint32_t)(c >> bits)); }
 
-  __device__ void clear() const {
-    for (int i = threadIdx.x; i < kBins; i += TH) lds->hist[i] = 0;
-    __syncthreads();
+  __device__ __forceinline__ void masses(float max, float min, double t) {
+    top = max;
+    top64 = uniform((double)max);
+    slope = uniform(fmin(1.4426950408889634 / t, 1e300));
+    F = bits > 12 ? 62 - bits : 50;
+    shifter = uniform(0x1.8p52 + (double)F);
+    // bins end where masses fall under 2^-(F+1), or where the row does
+    const float range = fmaxf(fminf((float)((F + 2) * 0.6931472 * t), max - min), 1e-30f);
+    bin_scale = uniform((float)BINS / range);
   }
-  // The bin in which the running sum passes `target`, and the sum before it; the sum of all bins. None passes: -1.
-  __device__ int find(uint64_t target, uint64_t& before, uint64_t& total) const {
-    constexpr int B = kBins / TH;
-    uint64_t sum = 0;
-    for (int b = 0; b < B; ++b) sum += lds->hist[threadIdx.x * B + b];
-    uint64_t run = block_scan<TH>(sum, lds->part, total);
-    if (target >= total) return -1;
-    if (target >= run && target - run < sum) {
+  __device__ __forceinline__ uint64_t mass(float x) const {
+    // the bound takes in -inf and NaN
+    const double y = fmax(((double)x - top64) * slope, -100.0);
+    // where 1.5 2^52 is added the sum's low bits are the nearest whole number, here n + F
+    const double z = y + shifter, n = z - shifter;
+    const long long p = __double_as_longlong(exp2_small(y - n));
+    const double e = __longlong_as_double(p + ((long long)(int)__double_as_longlong(z) << 52));
+    if (!(e >= least)) return 0;
+    // at most 2^50: rounded to a whole number where 2^52 is added, whose bits it then leaves
+    return (uint64_t)__double_as_longlong(e + 0x1p52) & ((1ull << 52) - 1);
+  }
+  // Falling with x; infinite for -inf.
+  __device__ __forceinline__ float bin_at(float x) const { return (top - x) * bin_scale; }
+  __device__ __forceinline__ uint32_t bin(float x) const { return (uint32_t)fminf(bin_at(x), (float)(BINS - 1)); }
+
+  // What the threads know of a histogram: the sum before a thread's own bins, of its own, of all.
+  struct Prefix {
+    uint64_t run, sum, total;
+  };
+  __device__ __forceinline__ Prefix prefix() const {
+    constexpr int B = BINS / TH;
+    Prefix p;
+    p.sum = 0;
+#pragma unroll
+    for (int b = 0; b < B; ++b) p.sum += lds->hist[threadIdx.x * B + b];
+    p.run = block_scan<TH>(p.sum, lds->part, p.total);
+    return p;
+  }
+  // The bin in which the running sum passes `target` (less than the total), and the sum before it.
+  __device__ __forceinline__ int find(const Prefix& p, uint64_t target, uint64_t& before) const {
+    constexpr int B = BINS / TH;
+    if (target >= p.run && target - p.run < p.sum) {
+      uint64_t run = p.run;
       int b = 0;
       for (; b < B - 1; ++b) {
         const uint64_t h = lds->hist[threadIdx.x * B + b];
@@ -114,38 +235,45 @@ struct Row {
       lds->base = run;
     }
     __syncthreads();
-    const int got = (int)lds->at;
-    before = lds->base;
+    const int got = (int)uniform(lds->at);
+    before = uniform(lds->base);
     __syncthreads();
     return got;
   }
-
-  // Sums of weight(x) over the bins of the tokens' values.
-  template <class W>
-  __device__ void histogram(W weight) const {
-    clear();
-    each([&](uint64_t c, float x) {
-      if (c < from) return;
-      const uint64_t w = weight(x);
-      if (w) atomicAdd((unsigned long long*)&lds->hist[bin(x)], (unsigned long long)w);
-    });
+  __device__ __forceinline__ void clear() const {
+    for (int i = threadIdx.x; i < BINS; i += TH) lds->hist[i] = 0;
     __syncthreads();
   }
+  // Masses over the bins of the tokens' values; AGAIN: from memory, of the tokens from `from` on.
+  template <bool AGAIN>
+  __device__ __forceinline__ Prefix histogram() const {
+    clear();
+    const auto add = [&](float x, int i) {
+      const uint64_t w = mass(x);
+      if (w && (!AGAIN || comp(x, i) >= from)) atomicAdd((unsigned long long*)&lds->hist[bin(x)], (unsigned long long)w);
+    };
+    if constexpr (AGAIN) each_again<0>(add);
+    else each(add);
+    __syncthreads();
+    return prefix();
+  }
 
-  // The tokens for which in(c, x) holds, in falling order, one a thread (0: none), if there are at most TH; how many.
-  template <class P>
-  __device__ int collect(P in, uint64_t& mine) const {
+  // The tokens for which in(x, i) holds, in falling order, one a thread (0: none), if there are at most TH; how many.
+  template <bool AGAIN, class P>
+  __device__ __forceinline__ int collect(P in, uint64_t& mine) const {
     if (threadIdx.x == 0) lds->n = 0;
     lds->list[threadIdx.x] = 0;
     __syncthreads();
-    each([&](uint64_t c, float x) {
-      if (c >= from && in(c, x)) {
+    const auto take = [&](float x, int i) {
+      if (in(x, i)) {
         const int at = atomicAdd(&lds->n, 1);
-        if (at < TH) lds->list[at] = c;
+        if (at < TH) lds->list[at] = comp(x, i);
       }
-    });
+    };
+    if constexpr (AGAIN) each_again<0>(take);
+    else each(take);
     __syncthreads();
-    const int n = lds->n;
+    const int n = uniform(lds->n);
     mine = lds->list[threadIdx.x];
     __syncthreads();
     if (n <= TH) {
@@ -156,85 +284,134 @@ struct Row {
     return n;
   }
 
-  // The place of the token whose running weight, on from `before` at the first token of bin b, passes `target`.
-  // before: the sum before that token.
+  // Of the tokens with place numbers in [lo, hi], the one whose running weight, on from `before` at the first of them,
+  // passes `target`, and the sum before it. By bins of the place numbers until a thread can hold each token of one.
   template <class W>
-  __device__ uint64_t within(int b, uint64_t target, uint64_t& before, W weight) const {
-    uint64_t mine, total;
-    int n = collect([&](uint64_t, float x) { return bin(x) == b; }, mine);
-    if (n > TH) {
-      uint64_t lo = ~0ull, hi = 0;
-      each([&](uint64_t c, float x) {
-        if (c >= from && bin(x) == b) {
-          lo = c < lo ? c : lo;
-          hi = c > hi ? c : hi;
-        }
+  __device__ __forceinline__ uint64_t descend(uint64_t lo, uint64_t hi, uint64_t target, uint64_t& before, W weight) const {
+    uint64_t mine;
+    int n = TH + 1;
+    for (int round = 0; round < 16 && n > TH; ++round) {   // each cuts the numbers' range to a 128th at most, or to one number
+      int shift = 0;
+      while (((hi - lo) >> shift) >= (uint64_t)BINS) ++shift;
+      clear();
+      each_again<0>([&](float x, int i) {
+        const uint64_t c = comp(x, i);
+        if (!(x > -INFINITY) || c < lo || c > hi) return;
+        const uint64_t w = weight(x);
+        if (w) atomicAdd((unsigned long long*)&lds->hist[(hi - c) >> shift], (unsigned long long)w);
       });
-      lo = block_reduce<TH>(lo, lds->part, [](uint64_t p, uint64_t q) { return p < q ? p : q; });
-      hi = block_reduce<TH>(hi, lds->part, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
-      while (n > TH) {   // each round at least halves the numbers' range
-        int shift = 0;
-        while (((hi - lo) >> shift) >= (uint64_t)kBins) ++shift;
-        clear();
-        each([&](uint64_t c, float x) {
-          if (c < lo || c > hi) return;
-          const uint64_t w = weight(x);
-          if (w) atomicAdd((unsigned long long*)&lds->hist[(hi - c) >> shift], (unsigned long long)w);
-        });
-        __syncthreads();
-        uint64_t run;
-        const uint64_t d = (uint64_t)find(target - before, run, total);
-        before += run;
-        hi -= d << shift;
-        const uint64_t width = (1ull << shift) - 1;
-        if (hi - lo > width) lo = hi - width;
-        n = collect([&](uint64_t c, float) { return c >= lo && c <= hi; }, mine);
-      }
+      __syncthreads();
+      uint64_t run;
+      const uint64_t d = (uint64_t)find(prefix(), target - before, run);
+      before += run;
+      hi -= d << shift;
+      const uint64_t width = (1ull << shift) - 1;
+      if (hi - lo > width) lo = hi - width;
+      n = collect<true>([&](float x, int i) { return x > -INFINITY && comp(x, i) >= lo && comp(x, i) <= hi; }, mine);
     }
+    return among(mine, target, before, weight);
+  }
+  // The same of tokens in order, one a thread.
+  template <class W>
+  __device__ __forceinline__ uint64_t among(uint64_t mine, uint64_t target, uint64_t& before, W weight) const {
     const uint64_t w = mine ? weight(of(mine)) : 0;
+    uint64_t total;
     const uint64_t run = before + block_scan<TH>(w, lds->part, total);
     if (w && target >= run && target - run < w) {
       lds->at = mine;
       lds->base = run;
     }
     __syncthreads();
-    const uint64_t c = lds->at;
-    before = lds->base;
+    const uint64_t c = uniform(lds->at);
+    before = uniform(lds->base);
     __syncthreads();
     return c;
   }
+  // c: the token of bin b at which the running mass, on from `before` at the bin's first, passes `target`. False if
+  // the bin holds more tokens than there are threads: then nothing is found, or with AGAIN it is, and the bins of the
+  // values are overwritten.
+  template <bool AGAIN>
+  __device__ __forceinline__ bool within(int b, uint64_t target, uint64_t& before, uint64_t& c) const {
+    const float lo = b ? (float)b : -INFINITY, hi = b < BINS - 1 ? (float)(b + 1) : INFINITY;
+    const auto in = [&](float x, int i) {
+      const float at = bin_at(x);
+      return at >= lo && at < hi && (!AGAIN || comp(x, i) >= from);
+    };
+    const auto weight = [&](float x) { return mass(x); };
+    uint64_t mine;
+    if (collect<AGAIN>(in, mine) <= TH) {
+      c = among(mine, target, before, weight);
+      return true;
+    }
+    if constexpr (AGAIN) {
+      uint64_t first = ~0ull, last = 0;
+      each_again<0>([&](float x, int i) {
+        if (in(x, i)) {
+          const uint64_t at = comp(x, i);
+          first = at < first ? at : first;
+          last = at > last ? at : last;
+        }
+      });
+      first = block_reduce<TH>(first, lds->part, [](uint64_t p, uint64_t q) { return p < q ? p : q; });
+      last = block_reduce<TH>(last, lds->part, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
+      c = descend(first, last, target, before, weight);
+    }
+    return false;
+  }
+  // The kth token in order, one at least as large as `least_value`; there are more than k such.
+  __device__ __forceinline__ uint64_t kth(int64_t k, float least_value) const {
+    uint64_t before = 0;
+    return descend((uint64_t)key_of(least_value) << bits, ~0ull >> (32 - bits), (uint64_t)(k - 1), before,
+                   [](float) { return (uint64_t)1; });
+  }
+  // A value that at least k tokens (at most TH) reach, if there are as many: in each wave as many lanes as make k of
+  // all waves have a token of that size, own: each lane's largest.
+  __device__ __forceinline__ float reached(float own, int k) const {
+    const int t = threadIdx.x & 63;
+    for (int s = 2; s <= 64; s <<= 1)
+      for (int d = s >> 1; d; d >>= 1) {
+        const float o = __shfl_xor(own, d);
+        own = ((t & s) == 0) == ((t & d) == 0) ? fmaxf(own, o) : fminf(own, o);
+      }
+    constexpr int W = TH / 64;
+    own = __shfl(own, (k + W - 1) / W - 1);
+    return block_reduce<TH>(own, reinterpret_cast<float*>(lds->part), [](float p, float q) { return fminf(p, q); });
+  }
+  // Largest and smallest of the tokens that are there, and a thread's own largest.
+  __device__ __forceinline__ void extremes(float& max, float& min, float& own) const {
+    own = -INFINITY;
+    min = INFINITY;
+    each([&](float x, int) {   // both pass over a NaN
+      own = fmaxf(own, x);
+      min = fminf(min, x);
+    });
+    const auto smaller = [](float p, float q) { return fminf(p, q); };
+    max = block_reduce<TH>(own, reinterpret_cast<float*>(lds->part), [](float p, float q) { return fmaxf(p, q); });
+    min = block_reduce<TH>(min, reinterpret_cast<float*>(lds->part), smaller);
+    if (min == -INFINITY) {
+      min = INFINITY;
+      each_again<0>([&](float x, int) { min = x > -INFINITY ? fminf(min, x) : min; });
+      min = block_reduce<TH>(min, reinterpret_cast<float*>(lds->part), smaller);
+    }
+  }
 };
 
-// Largest and smallest place of the row's tokens; 0 where there is none.
-template <int DT, int TH>
-__device__ inline void extremes(const Row<DT, TH>& r, uint64_t& first, uint64_t& last) {
-  uint64_t hi = 0, lo = ~0ull;
-  r.each([&](uint64_t c, float) {
-    hi = c > hi ? c : hi;
-    lo = c < lo ? c : lo;
-  });
-  first = block_reduce<TH>(hi, r.lds->part, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
-  last = block_reduce<TH>(lo, r.lds->part, [](uint64_t p, uint64_t q) { return p < q ? p : q; });
-}
-
-template <int DT, int TH>
+template <int DT, int TH, int NV>
 __global__ void __launch_bounds__(TH)
 top_logits_kernel(const typename TabType<DT>::t* logits, int64_t ld, int V, int K, typename TabType<DT>::t* values, int64_t* ids) {
   __shared__ SelectLds<TH> lds;
   const int64_t n = blockIdx.x;
-  Row<DT, TH> r(logits + n * ld, nullptr, V, &lds);
-  uint64_t first, last, mine = 0;
-  extremes(r, first, last);
-  if (first) {
-    const auto one = [](float) { return (uint64_t)1; };
-    if (V > TH) {
-      r.masses(r.of(first), r.of(last), INFINITY);
-      r.histogram(one);
-      uint64_t before, total;
-      const int b = r.find(K - 1, before, total);
-      if (b >= 0) r.from = r.within(b, K - 1, before, one);
-    }
-    r.collect([](uint64_t, float) { return true; }, mine);
+  Row<DT, TH, NV> r(logits + n * ld, nullptr, V, &lds);
+  float least = -FLT_MAX;
+  if (V > TH) {
+    float own = -FLT_MAX;
+    r.each([&](float x, int) { own = fmaxf(own, x); });
+    least = r.reached(own, K);
+  }
+  uint64_t mine;
+  if (r.template collect<false>([&](float x, int) { return x >= least; }, mine) > TH) {
+    const uint64_t c = r.kth(K, least);
+    r.template collect<true>([&](float x, int i) { return x >= least && r.comp(x, i) >= c; }, mine);
   }
   if (threadIdx.x < K) {
     values[n * K + threadIdx.x] = tab_put<DT>(mine ? r.of(mine) : -INFINITY);
@@ -249,53 +426,113 @@ struct Limits {   // of all rows, or with a pointer of each; 64 bits, in which 0
   const int64_t* ks;
 };
 
-template <int DT, int TH>
-__global__ void __launch_bounds__(TH)
-sample_kernel(const typename TabType<DT>::t* logits, int64_t ld, int V, const uint8_t* allowed, int64_t allowed_ld, const float* u,
+// The running sum that is passed by the last token before which lies less than p of `total`.
+__device__ inline uint64_t reach_of(double p, uint64_t total) {
+  const double mass = p * (double)total;
+  const uint64_t reach = mass > 0.0 ? (uint64_t)ceil(mass) - 1 : 0;
+  return reach < total ? reach : total - 1;
+}
+__device__ inline uint64_t target_of(float u, uint64_t total) {
+  const uint64_t t = u > 0.0f ? (uint64_t)(fmin((double)u, 1.0) * (double)total) : 0;
+  return t < total ? t : total - 1;
+}
+
+template <int DT, int TH, int NV>
+__global__ void __launch_bounds__(TH, 4)
+sample_kernel(const typename TabType<DT>::t* logits, int64_t ld, int V, const uint8_t* allowed, int64_t allowed_ld, const float* us,
               Limits lim, int64_t* ids) {
   __shared__ SelectLds<TH> lds;
   const int64_t n = blockIdx.x;
-  Row<DT, TH> r(logits + n * ld, allowed ? allowed + n * allowed_ld : nullptr, V, &lds);
-  uint64_t first, last;
-  extremes(r, first, last);
+  Row<DT, TH, NV> r(logits + n * ld, allowed ? allowed + n * allowed_ld : nullptr, V, &lds);
   const double t = lim.ts ? lim.ts[n] : lim.t, p = lim.ps ? lim.ps[n] : lim.p, m = lim.ms ? lim.ms[n] : lim.m;
   const int64_t k = lim.ks ? lim.ks[n] : lim.k;
-  if (!first || !(t > 0.0)) {
-    if (threadIdx.x == 0) ids[n] = first ? r.id_of(first) : -1;
+  const float u = us[n];
+  float max, min, own;
+  r.extremes(max, min, own);
+  if (max == -INFINITY || !(t > 0.0)) {
+    int first = V;
+    r.template each_again<0>([&](float x, int i) { first = x == max && max > -INFINITY && i < first ? i : first; });
+    first = block_reduce<TH>(first, reinterpret_cast<int*>(lds.part), [](int a, int b) { return a < b ? a : b; });
+    if (threadIdx.x == 0) ids[n] = first < V ? first : -1;
     return;
   }
-  const bool by_p = p < 1.0;
-  r.masses(r.of(first), r.of(last), t);
-  const double least = m > 0.0 ? fmin(m, 1.0) : 0.0;
-  const auto weight = [&](float x) { return r.mass(x); };
-  const auto one = [](float) { return (uint64_t)1; };
-  uint64_t before, total;
-  uint64_t got = first;
-  if (k > 0 && k < V) {
-    r.histogram(one);
-    const int b = r.find(k - 1, before, total);
-    if (b >= 0) r.from = r.within(b, k - 1, before, one);
+  if (max == INFINITY) {
+    r.set_infinite();
+    max = min = 0.0f;
+    own = own == INFINITY ? 0.0f : -INFINITY;
   }
-  if (!by_p) r.least = least;
-  r.histogram(weight);
-  r.find(~0ull, before, total);
-  if (by_p) {
-    // the last token before which lies less than p of the mass: the one at which the running sum reaches it
-    const double mass = p * (double)total;
-    const uint64_t reach = mass > 0.0 ? (uint64_t)ceil(mass) - 1 : 0;   // the running sum passes this
-    const int b = r.find(min(reach, total - 1), before, total);
-    const uint64_t c = r.within(b, min(reach, total - 1), before, weight);
-    total = before + r.mass(r.of(c));
-    r.from = c;
-    r.least = least;
-    r.histogram(weight);
-    r.find(~0ull, before, total);
+  r.masses(max, min, t);
+  const bool by_p = p < 1.0, by_m = m > 0.0, by_k = k > 0 && k < V;
+  const double least = by_m ? fmin(m, 1.0) : 0.0;
+  float lower = -FLT_MAX;
+  if (by_k && k <= TH && V > TH) lower = fmaxf(lower, r.reached(own, (int)k));
+  if (by_m && !by_p) {
+    // under the border by more than its rounding and the bound's own
+    const double b = (double)max + t * log(least);
+    lower = fmaxf(lower, (float)(b - 1e-6 * (fabs(b) + t) - 1e-37));
   }
-  const float v = u[n];
-  const uint64_t target = min((uint64_t)(v > 0.0f ? fmin((double)v, 1.0) * (double)total : 0.0), total - 1);
-  const int b = r.find(target, before, total);
-  got = r.within(b, target, before, weight);
-  if (threadIdx.x == 0) ids[n] = r.id_of(got);
+  uint64_t mine = 0, total;
+  int many = TH + 1;
+  if (V <= TH || (by_k && k <= TH) || (by_m && !by_p))
+    many = r.template collect<false>([&](float x, int) { return x >= lower; }, mine);
+  if (many <= TH) {   // a token a thread, in order
+    if (by_k && threadIdx.x >= k) mine = 0;
+    uint64_t w = mine ? r.mass(r.of(mine)) : 0;
+    const uint64_t run = block_scan<TH>(w, lds.part, total);
+    if (by_p || by_m) {
+      if (by_p && run > reach_of(p, total)) w = 0;
+      r.least = ldexp(least, r.F);
+      if (by_m && mine && w) w = r.mass(r.of(mine));
+      total = block_reduce<TH>(w ? run + w : 0, lds.part, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+    }
+    const uint64_t target = target_of(u, total);
+    if (w && target >= run && target - run < w) ids[n] = r.id_of(mine);
+    return;
+  }
+  if (by_k && many > TH) {
+    // without a threshold the kth may not be there
+    int there = 0;
+    r.template each_again<0>([&](float x, int) { there += x > -INFINITY; });
+    there = block_reduce<TH>(there, reinterpret_cast<int*>(lds.part), [](int a, int b) { return a + b; });
+    if (there > k) r.from = r.kth(k, k <= TH && V > TH ? lower : min);
+  }
+  uint64_t before = 0, c = 0;
+  if (!by_p) r.least = uniform(ldexp(least, r.F));
+  if (!r.from) {
+    const auto hist = r.template histogram<false>();
+    total = hist.total;
+    bool found = true;
+#pragma unroll 1
+    for (int step = by_p ? 0 : 1; step < 2 && found; ++step) {   // the last token that top_p keeps, the token drawn
+      const uint64_t target = step ? target_of(u, total) : reach_of(p, total);
+      const int b = r.find(hist, target, before);
+      found = r.template within<false>(b, target, before, c);
+      if (step == 0 && found) {
+        const uint64_t w = r.mass(r.of(c));
+        total = before + w;
+        found = !by_m || (double)w >= ldexp(least, r.F) + 1.0;   // min_p keeps them all
+      }
+    }
+    if (found) {
+      if (threadIdx.x == 0) ids[n] = r.id_of(c);
+      return;
+    }
+  }
+  auto hist = r.template histogram<true>();
+  total = hist.total;
+#pragma unroll 1
+  for (int step = by_p ? 0 : 1; step < 2; ++step) {
+    const uint64_t target = step ? target_of(u, total) : reach_of(p, total);
+    const int b = r.find(hist, target, before);
+    r.template within<true>(b, target, before, c);
+    if (step == 0) {
+      r.from = c;
+      r.least = ldexp(least, r.F);
+      hist = r.template histogram<true>();
+      total = hist.total;
+    }
+  }
+  if (threadIdx.x == 0) ids[n] = r.id_of(c);
 }
 
 }  // namespace slg
@@ -304,17 +541,30 @@ using namespace slg;
 
 namespace {
 
-// f with the type and the threads of a row: a token a thread where that can be, at most 1024
-template <class F>
+// f with the type, the threads and the groups of 16 bytes a thread of a row of V logits. Listing up to k tokens takes
+// as many threads.
+template <bool LIST, class F>
 void dispatch(int dtype, int64_t V, int64_t k, F f) {
-  const auto by_threads = [&](auto dt) {
-    if (V <= 64) f(dt, std::integral_constant<int, 64>{});
-    else if (V <= 4096 && k <= 256) f(dt, std::integral_constant<int, 256>{});
-    else f(dt, std::integral_constant<int, 1024>{});
+  using std::integral_constant;
+  const auto by_size = [&](auto dt) {
+    constexpr int VU = 16 / (int)sizeof(typename TabType<decltype(dt)::value>::t);
+    const auto go = [&](auto th, auto nv) { f(dt, th, nv); };
+    const int64_t groups = cdiv(V, VU);
+    // a row that fills no group is read token by token
+    if (V < VU) return go(integral_constant<int, 64>{}, integral_constant<int, 0>{});
+    if (groups <= 128 && k <= 24) return go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    if (groups <= 1024 && k <= 96) return go(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    if constexpr (LIST) {
+      if (groups <= 2048) go(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+      else go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
+    } else {
+      if (groups <= 2048) go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
+      else go(integral_constant<int, 512>{}, integral_constant<int, 8>{});
+    }
   };
-  if (dtype == kTabF32) by_threads(std::integral_constant<int, kTabF32>{});
-  else if (dtype == kTabBf16) by_threads(std::integral_constant<int, kTabBf16>{});
-  else by_threads(std::integral_constant<int, kTabF16>{});
+  if (dtype == kTabF32) by_size(integral_constant<int, kTabF32>{});
+  else if (dtype == kTabBf16) by_size(integral_constant<int, kTabBf16>{});
+  else by_size(integral_constant<int, kTabF16>{});
 }
 
 bool sizes(int64_t N, int64_t V, int64_t ld) { return N >= 0 && N < (1LL << 31) && V >= 1 && V <= (1LL << 24) && ld >= 0; }
@@ -330,9 +580,9 @@ int slg_top_logits(const void* logits, int32_t dtype, int64_t N, int64_t V, int6
   SLG_REQUIRE(sizes(N, V, ld) && K >= 1 && K <= V && K <= kMaxTop, SLG_E_SHAPE, "top_logits: N %lld, V %lld, K %lld", (long long)N,
               (long long)V, (long long)K);
   if (N == 0) return 0;
-  dispatch(dtype, V, K, [&](auto dt, auto th) {
+  dispatch<true>(dtype, V, K, [&](auto dt, auto th, auto nv) {
     using T = typename TabType<decltype(dt)::value>::t;
-    hipLaunchKernelGGL((top_logits_kernel<decltype(dt)::value, decltype(th)::value>), dim3((unsigned)N), dim3(decltype(th)::value), 0,
+    hipLaunchKernelGGL((top_logits_kernel<decltype(dt)::value, decltype(th)::value, decltype(nv)::value>), dim3((unsigned)N), dim3(decltype(th)::value), 0,
                        as_stream(stream), static_cast<const T*>(logits), ld, (int)V, (int)K, static_cast<T*>(values), ids);
   });
   SLG_LAUNCH_CHECK("top_logits");
@@ -351,9 +601,9 @@ int slg_sample_logits(const void* logits, int32_t dtype, int64_t N, int64_t V, i
   SLG_REQUIRE(min_ps || (min_p >= 0.0 && min_p <= 1.0), SLG_E_ARG, "sample_logits: min_p %g outside [0, 1]", min_p);
   if (N == 0) return 0;
   const Limits lim{temperature, top_p, min_p, top_k, temperatures, top_ps, min_ps, top_ks};
-  dispatch(dtype, V, 1, [&](auto dt, auto th) {
+  dispatch<false>(dtype, V, 1, [&](auto dt, auto th, auto nv) {
     using T = typename TabType<decltype(dt)::value>::t;
-    hipLaunchKernelGGL((sample_kernel<decltype(dt)::value, decltype(th)::value>), dim3((unsigned)N), dim3(decltype(th)::value), 0,
+    hipLaunchKernelGGL((sample_kernel<decltype(dt)::value, decltype(th)::value, decltype(nv)::value>), dim3((unsigned)N), dim3(decltype(th)::value), 0,
                        as_stream(stream), static_cast<const T*>(logits), ld, (int)V, allowed, allowed_ld, u, lim, ids);
   });
   SLG_LAUNCH_CHECK("sample_logits");
