@@ -10,8 +10,11 @@
 //
 // Both softmaxes share their maximum m: what is kept of a row is m, 1/Z and 1/Z1 (and the teacher's own), so that a
 // probability is exp((s - m) / T) / Z with the difference exact where it matters. Sums are fp32, those over rows 64
-// bits; the gradient is rounded once.
+// bits; the gradient is rounded once. All kernels are bound by the logits' bytes: one pass for the loss (the running
+// maximum and sums of each thread joined at the end), another with the write for the gradient. Both from one call
+// hold the row in registers between them.
 #include <algorithm>
+#include <type_traits>
 
 #include "block_ops.h"
 #include "float_types.h"
@@ -20,7 +23,9 @@ namespace slg {
 
 constexpr float kLog2e = 1.44269504f;
 constexpr int kMaxEntries = 1024;
-constexpr int kKept = 8;   // floats kept of a row: m, 1/Z, 1/Z1, the teacher's maximum and 1/sum, a_s T, a_h, unused
+constexpr int kKept = 8;      // floats kept of a row: m, 1/Z, 1/Z1, the teacher's maximum and 1/sum, a_s T, a_h, counted
+constexpr int kCounts = 256;  // workgroups that count the rows of a mean
+constexpr int kParts = 1024;  // parts of rows that the loss's first pass is cut into where there are fewer rows
 
 struct Distill {
   const void* logits;
@@ -34,138 +39,252 @@ struct Distill {
   float T, inv_t, alpha;
 };
 
-__device__ inline float load_as(const void* p, int dtype, int64_t i) {
+__device__ __forceinline__ float load_as(const void* p, int dtype, int64_t i) {
   if (dtype == kTabF32) return static_cast<const float*>(p)[i];
   if (dtype == kTabBf16) return tab_get<kTabBf16>(static_cast<const uint16_t*>(p)[i]);
   return (float)static_cast<const _Float16*>(p)[i];
 }
-__device__ inline int64_t load_id(const void* p, int bytes, int64_t i) {
+__device__ __forceinline__ int64_t load_id(const void* p, int bytes, int64_t i) {
   return bytes == 8 ? static_cast<const int64_t*>(p)[i] : (int64_t)static_cast<const int32_t*>(p)[i];
 }
 // Token of the teacher's entry j of row n, or -1, and its value.
-__device__ inline int entry(const Distill& a, int64_t n, int j, float& t) {
+__device__ __forceinline__ int entry(const Distill& a, int64_t n, int j, float& t) {
   const int64_t id = load_id(a.ids, a.id_bytes, n * a.K + j);
   t = load_as(a.values, a.vtype, n * a.K + j);
   return id >= 0 && id < a.V && t != -INFINITY ? (int)id : -1;
 }
-__device__ inline int label_of(const Distill& a, int64_t n) {
+__device__ __forceinline__ int label_of(const Distill& a, int64_t n) {
   if (!a.labels) return -1;
   const int64_t y = load_id(a.labels, a.label_bytes, n);
   return y >= 0 && y < a.V ? (int)y : -1;
 }
 
+// Under 2^-126 it is 0.
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
 struct Sums {   // maximum and sums of exp((s - m) / T), exp(s - m)
   float m, z, z1;
 };
-// exp2((from - to) c) for a change of the maximum; a maximum of -inf has sums of 0.
-__device__ inline Sums join(Sums a, Sums b, float c) {
+// A maximum of -inf has sums of 0; of a NaN they are NaN.
+__device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
   const float m = fmaxf(a.m, b.m), r = m == -INFINITY ? 0.0f : m;
-  const float fa = (a.m - r), fb = (b.m - r);
-  return {m, a.z * exp2f(fa * c) + b.z * exp2f(fb * c), a.z1 * exp2f(fa * kLog2e) + b.z1 * exp2f(fb * kLog2e)};
+  const float fa = a.m - r, fb = b.m - r;
+  return {m, a.z * exp2_fast(fa * c) + b.z * exp2_fast(fb * c), a.z1 * exp2_fast(fa * kLog2e) + b.z1 * exp2_fast(fb * kLog2e)};
 }
 
-template <int DT, class F>
-__device__ inline void each_in(const typename TabType<DT>::t* row, int64_t a, int64_t b, int threads, F f) {
-  for (int64_t i = a + threadIdx.x; i < b; i += threads) f(i, tab_get<DT>(row[i]));
+// Groups of 16 bytes of a row, from any element on.
+template <int DT>
+struct Group {
+  using T = typename TabType<DT>::t;
+  static constexpr int U = 16 / (int)sizeof(T);
+  typedef T Vec __attribute__((ext_vector_type(U), aligned(sizeof(T))));
+  static __device__ __forceinline__ void get(const T* p, float (&v)[U]) {
+    const Vec x = *reinterpret_cast<const Vec*>(p);
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = tab_get<DT>(x[u]);
+  }
+  static __device__ __forceinline__ T round(float v) {
+    if constexpr (DT == kTabBf16) return __builtin_bit_cast(uint16_t, (__bf16)v);
+    else return (T)v;
+  }
+  static __device__ __forceinline__ void put(T* p, const float (&v)[U]) {
+    Vec x;
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = round(v[u]);
+    __builtin_nontemporal_store(x, reinterpret_cast<Vec*>(p));
+  }
+};
+
+// n more values of the running sums. TWO: of both softmaxes, else z1 stays as it is.
+template <bool TWO, int n>
+__device__ __forceinline__ void take(Sums& s, const float (&v)[n], float c) {
+  float m = s.m;
+#pragma unroll
+  for (int u = 0; u < n; ++u) m = fmaxf(m, v[u]);
+  const float r = m == -INFINITY ? 0.0f : m;
+  s.z *= exp2_fast((s.m - r) * c);
+  if (TWO) s.z1 *= exp2_fast((s.m - r) * kLog2e);
+  s.m = m;
+#pragma unroll
+  for (int u = 0; u < n; ++u) {
+    const float d = v[u] - r;
+    s.z += exp2_fast(d * c);
+    if (TWO) s.z1 += exp2_fast(d * kLog2e);
+  }
+}
+
+// Sums of the row's values from `from` to `to` by TH threads, four groups of a thread in flight.
+template <int DT, int TH, bool TWO>
+__device__ __forceinline__ Sums sums_of(const typename TabType<DT>::t* row, int64_t from, int64_t to, float c) {
+  using G = Group<DT>;
+  constexpr int64_t kStep = (int64_t)TH * G::U;
+  Sums s{-INFINITY, 0.0f, 0.0f};
+  int64_t i = from + (int64_t)threadIdx.x * G::U;
+  for (; i + 3 * kStep + G::U <= to; i += 4 * kStep) {
+    float v[4][G::U];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) G::get(row + i + k * kStep, v[k]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) take<TWO>(s, v[k], c);
+  }
+  for (; i + G::U <= to; i += kStep) {
+    float v[G::U];
+    G::get(row + i, v);
+    take<TWO>(s, v, c);
+  }
+  if (i < to) {   // the row's end, in one thread
+    for (int64_t k = i; k < to; ++k) {
+      const float v[1] = {tab_get<DT>(row[k])};
+      take<TWO>(s, v, c);
+    }
+  }
+  return s;
 }
 
 template <int TH>
-__device__ inline Sums block_sums(Sums v, float c, Sums* part) {
+__device__ __forceinline__ Sums block_sums(Sums v, float c, Sums* part) {
+  constexpr int W = TH / 64;
 #pragma unroll
   for (int d = 32; d; d >>= 1) v = join(v, Sums{__shfl_xor(v.m, d), __shfl_xor(v.z, d), __shfl_xor(v.z1, d)}, c);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = part[0];
-  for (int w = 1; w < TH / 64; ++w) v = join(v, part[w], c);
-  __syncthreads();
+  if constexpr (W > 1) {
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = part[threadIdx.x & (W - 1)];
+#pragma unroll
+    for (int d = W / 2; d; d >>= 1) v = join(v, Sums{__shfl_xor(v.m, d), __shfl_xor(v.z, d), __shfl_xor(v.z1, d)}, c);
+  }
   return v;
 }
 
-// The row's loss and what is kept of it, from its sums.
-template <int DT, int TH>
-__device__ inline void finish_row(const Distill& a, int64_t n, Sums s, float* part, float* loss, float* kept, float& a_s,
-                                  float& a_h, float& top, float& rtot) {
-  const auto* row = static_cast<const typename TabType<DT>::t*>(a.logits) + n * a.ld;
-  const auto add = [](float x, float y) { return x + y; };
-  top = -INFINITY;
-  bool any = false, nan = false;
-  for (int j = threadIdx.x; j < a.K; j += TH) {
-    float t;
-    if (entry(a, n, j, t) >= 0) {
-      any = true;
-      nan |= t != t;
-      top = fmaxf(top, t);
-    }
-  }
-  top = block_reduce<TH>(top, part, [](float x, float y) { return fmaxf(x, y); });
-  const float some = block_reduce<TH>(any ? 1.0f : 0.0f, part, add);
-  const float bad = block_reduce<TH>(nan ? 1.0f : 0.0f, part, add);
-  const bool alive = s.z != 0.0f;   // a NaN stays
-  const int y = label_of(a, n);
-  const bool soft = some > 0.0f && alive, hard = y >= 0 && alive;
-  float tot = 0.0f;
-  for (int j = threadIdx.x; j < a.K; j += TH) {
-    float t;
-    if (entry(a, n, j, t) >= 0) tot += expf((t - top) * a.inv_t);
-  }
-  tot = block_reduce<TH>(tot, part, add);
-  rtot = bad > 0.0f ? NAN : 1.0f / tot;
-  const float logs = logf(s.z) - logf(tot);
-  float l = 0.0f;
-  for (int j = threadIdx.x; j < a.K; j += TH) {
+struct Teacher {   // maximum and sum of its entries, and whether there are any
+  float top, total;
+  bool some;
+};
+
+// One wave: the teacher's tokens and probabilities (not yet over `total`) into id[] and q[].
+__device__ __forceinline__ Teacher teacher_of(const Distill& a, int64_t n, int* id, float* q) {
+  const int lane = threadIdx.x & 63;
+  float top = -INFINITY, total = 0.0f;
+  bool any = false;
+  for (int j = lane; j < a.K; j += 64) {
     float t;
     const int i = entry(a, n, j, t);
-    if (i < 0) continue;
-    const float q = expf((t - top) * a.inv_t) * rtot;
-    if (q != 0.0f) l += q * ((t - top) * a.inv_t - (tab_get<DT>(row[i]) - s.m) * a.inv_t + logs);
+    id[j] = i;
+    q[j] = t;
+    any |= i >= 0;
+    if (i >= 0) top = fmaxf(top, t);
   }
-  l = block_reduce<TH>(l, part, add);
+  top = wave_reduce(top, [](float x, float y) { return fmaxf(x, y); });
+  for (int j = lane; j < a.K; j += 64) {
+    const float e = id[j] >= 0 ? expf((q[j] - top) * a.inv_t) : 0.0f;
+    q[j] = e;
+    total += e;
+  }
+  total = wave_reduce(total, [](float x, float y) { return x + y; });
+  return {top, total, __ballot(any) != 0};
+}
+
+// One wave: the row's loss from its sums, and what is kept of it.
+template <int DT>
+__device__ __forceinline__ void finish_row(const Distill& a, int64_t n, const Sums& s, const Teacher& t, const int* id, const float* q,
+                                           float* loss, float* kept, float& a_s, float& a_h) {
+  const auto* row = static_cast<const typename TabType<DT>::t*>(a.logits) + n * a.ld;
+  const int lane = threadIdx.x & 63, y = label_of(a, n);
+  const bool alive = s.z != 0.0f;   // a NaN stays
+  const bool soft = t.some && alive, hard = y >= 0 && alive;
+  const float rtot = 1.0f / t.total, logs = logf(s.z) - logf(t.total);
+  float l = 0.0f;
+  if (soft)
+    for (int j = lane; j < a.K; j += 64) {
+      const float e = q[j];
+      // log q_j from the value itself: the exponential's log would lose what small ones round
+      if (e != 0.0f) {
+        float v;
+        const int i = entry(a, n, j, v);
+        l += e * rtot * ((v - t.top) * a.inv_t - (tab_get<DT>(row[i]) - s.m) * a.inv_t + logs);
+      }
+    }
+  l = wave_reduce(l, [](float x, float y) { return x + y; });
   const float share = a.labels ? 1.0f - a.alpha : 1.0f;
   a_s = soft ? share * a.T : 0.0f;
   a_h = hard ? a.alpha : 0.0f;
-  if (threadIdx.x == 0) {
+  if (lane == 0) {
     float v = soft ? share * a.T * a.T * l : 0.0f;
     if (hard) v += a.alpha * (logf(s.z1) - (tab_get<DT>(row[y]) - s.m));
     loss[n] = v;
     if (kept) {
-      float* k = kept + n * kKept;
-      k[0] = s.m, k[1] = 1.0f / s.z, k[2] = 1.0f / s.z1, k[3] = top, k[4] = rtot, k[5] = a_s, k[6] = a_h;
-      k[7] = some > 0.0f || y >= 0 ? 1.0f : 0.0f;
+      float4* k = reinterpret_cast<float4*>(kept + n * kKept);
+      k[0] = {s.m, 1.0f / s.z, 1.0f / s.z1, t.top};
+      k[1] = {rtot, a_s, a_h, t.some || y >= 0 ? 1.0f : 0.0f};
     }
   }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(256) distill_fwd_kernel(Distill a, float* loss, float* kept) {
-  __shared__ Sums parts[4];
-  __shared__ float part[4];
-  const int64_t n = blockIdx.x;
+// The loss of a row, a workgroup each; with parts > 1 the sums of a part of a row, joined by the next kernel.
+template <int DT, bool TWO>
+__global__ void __launch_bounds__(256) distill_fwd_kernel(Distill a, int parts, int64_t per, Sums* part_sums, float* loss, float* kept) {
+  __shared__ Sums part[4];
+  __shared__ int id[kMaxEntries];
+  __shared__ float q[kMaxEntries];
+  const int64_t n = blockIdx.x / parts, p = blockIdx.x % parts;
   const auto* row = static_cast<const typename TabType<DT>::t*>(a.logits) + n * a.ld;
   const float c = a.inv_t * kLog2e;
+  Sums s = sums_of<DT, 256, TWO>(row, p * per, min(a.V, (p + 1) * per), c);
+  Teacher t{};
+  if (parts == 1 && threadIdx.x < 64) t = teacher_of(a, n, id, q);
+  s = block_sums<256>(s, c, part);
+  if (!TWO) s.z1 = s.z;
+  if (parts > 1) {
+    if (threadIdx.x == 0) part_sums[blockIdx.x] = s;
+  } else if (threadIdx.x < 64) {
+    float a_s, a_h;
+    finish_row<DT>(a, n, s, t, id, q, loss, kept, a_s, a_h);
+  }
+}
+template <int DT>
+__global__ void __launch_bounds__(64) distill_join_kernel(Distill a, int parts, const Sums* part_sums, float* loss, float* kept) {
+  __shared__ int id[kMaxEntries];
+  __shared__ float q[kMaxEntries];
+  const int64_t n = blockIdx.x;
+  const float c = a.inv_t * kLog2e;
   Sums s{-INFINITY, 0.0f, 0.0f};
-  each_in<DT>(row, 0, a.V, 256, [&](int64_t, float x) {
-    const float m = fmaxf(s.m, x), r = m == -INFINITY ? 0.0f : m;
-    s.z = s.z * exp2f((s.m - r) * c) + exp2f((x - r) * c);
-    s.z1 = s.z1 * exp2f((s.m - r) * kLog2e) + exp2f((x - r) * kLog2e);
-    s.m = m;
-  });
-  s = block_sums<256>(s, c, parts);
-  float a_s, a_h, top, rtot;
-  finish_row<DT, 256>(a, n, s, part, loss, kept, a_s, a_h, top, rtot);
+  for (int p = threadIdx.x; p < parts; p += 64) s = join(s, part_sums[n * parts + p], c);
+  const Teacher t = teacher_of(a, n, id, q);
+  s = block_sums<64>(s, c, nullptr);
+  float a_s, a_h;
+  finish_row<DT>(a, n, s, t, id, q, loss, kept, a_s, a_h);
 }
 
-// Sum of the rows' losses, or over the rows that count: out[0]; out[1] is what an upstream gradient is multiplied by.
-__global__ void __launch_bounds__(1024) distill_mean_kernel(const float* loss, const float* kept, int64_t N, int mean, float* out,
-                                                            float* factor) {
+// Rows with an entry or a label, counted by kCounts workgroups of four waves.
+__global__ void __launch_bounds__(256) distill_count_kernel(Distill a, int* counts) {
+  __shared__ int part[4];
+  int c = 0;
+  for (int64_t n = blockIdx.x * 4 + (threadIdx.x >> 6); n < a.N; n += (int64_t)gridDim.x * 4) {
+    bool any = label_of(a, n) >= 0;
+    for (int j = threadIdx.x & 63; !__ballot(any) && j - (int)(threadIdx.x & 63) < a.K; j += 64) {
+      float t;
+      any = j < a.K && entry(a, n, j, t) >= 0;
+    }
+    c += __ballot(any) != 0;
+  }
+  c = block_reduce<256>((threadIdx.x & 63) == 0 ? c : 0, part, [](int x, int y) { return x + y; });
+  if (threadIdx.x == 0) counts[blockIdx.x] = c;
+}
+
+// Sum of the rows' losses, or their mean over the rows that count (by `counted`, or where that is null by what is
+// kept of the rows), and what an upstream gradient is multiplied by.
+__global__ void __launch_bounds__(1024) distill_mean_kernel(const float* loss, const float* kept, const int* counts, int64_t N, int mean,
+                                                            float* out, float* factor) {
   __shared__ double part[16];
   double s = 0.0, c = 0.0;
   for (int64_t n = threadIdx.x; n < N; n += 1024) {
     s += (double)loss[n];
-    c += (double)kept[n * kKept + 7];
+    if (kept) c += (double)kept[n * kKept + 7];
   }
+  if (counts && threadIdx.x < kCounts) c = (double)counts[threadIdx.x];
   const auto add = [](double x, double y) { return x + y; };
   s = block_reduce<1024>(s, part, add);
-  c = block_reduce<1024>(c, part, add);
+  if (mean) c = block_reduce<1024>(c, part, add);
   if (threadIdx.x == 0) {
     const double f = mean ? 1.0 / fmax(c, 1.0) : 1.0;
     out[0] = (float)(s * f);
@@ -173,54 +292,216 @@ __global__ void __launch_bounds__(1024) distill_mean_kernel(const float* loss, c
   }
 }
 
-// grad of `chunk` logits of a row: all of them from their probabilities, then those that the teacher or the label
-// names once more, each by the first entry that names it.
-template <int DT>
-__global__ void __launch_bounds__(256)
-distill_bwd_kernel(Distill a, const float* kept, const float* upstream, int per_row, const float* factor, float scale, int64_t chunk,
-                   int chunks, void* grad) {
-  __shared__ int id[kMaxEntries + 1];
-  __shared__ float share[kMaxEntries + 1];
-  const int64_t n = blockIdx.x / chunks, from = (blockIdx.x % chunks) * chunk, to = min(a.V, from + chunk);
-  const auto* row = static_cast<const typename TabType<DT>::t*>(a.logits) + n * a.ld;
-  auto* out = static_cast<typename TabType<DT>::t*>(grad) + n * a.V;
-  const float* k = kept + n * kKept;
-  float g = scale;
-  if (upstream) g *= upstream[per_row ? n : 0];
-  if (factor) g *= *factor;
-  const float m = k[0], top = k[3], rtot = k[4], c = a.inv_t * kLog2e;
-  const float a_s = k[5], a_h = k[6], w = g * a_s * k[1], w1 = g * a_h * k[2];
-  if (g == 0.0f || (a_s == 0.0f && a_h == 0.0f)) {
-    for (int64_t i = from + threadIdx.x; i < to; i += 256) out[i] = tab_put<DT>(0.0f);
-    return;
+// A logit's gradient but for the entries that name it.
+struct Slope {
+  float m, c, w, w1;
+  bool two;
+  __device__ __forceinline__ float operator()(float x) const {
+    const float d = x - m, v = w * exp2_fast(d * c);
+    return two ? v + w1 * exp2_fast(d * kLog2e) : v;
   }
-  const auto at = [&](float x) {
-    float v = 0.0f;
-    if (a_s != 0.0f) v = w * exp2f((x - m) * c);
-    if (a_h != 0.0f) v += w1 * exp2f((x - m) * kLog2e);
-    return v;
-  };
-  for (int j = threadIdx.x; j < a.K; j += 256) {
-    float t;
-    const int i = a_s != 0.0f ? entry(a, n, j, t) : -1;
-    id[j] = i;
-    share[j] = i < 0 ? 0.0f : g * a_s * expf((t - top) * a.inv_t) * rtot;
-  }
-  if (threadIdx.x == 0) id[a.K] = a_h != 0.0f ? label_of(a, n) : -1, share[a.K] = g * a_h;
-  each_in<DT>(row, from, to, 256, [&](int64_t i, float x) { out[i] = tab_put<DT>(at(x)); });
+};
+// Of a row with shares ws and wh: with one softmax (temperature 1, or one share 0) both are in w.
+__device__ __forceinline__ Slope slope_of(const Distill& a, float m, float rz, float rz1, float ws, float wh) {
+  const float c = a.inv_t * kLog2e;
+  if (wh == 0.0f) return {m, c, ws * rz, 0.0f, false};
+  if (ws == 0.0f) return {m, kLog2e, wh * rz1, 0.0f, false};
+  if (a.T == 1.0f) return {m, kLog2e, (ws + wh) * rz1, 0.0f, false};
+  return {m, c, ws * rz, wh * rz1, true};
+}
+
+// A barrier at which all waves' stores have arrived, before other threads write some of the places again.
+__device__ __forceinline__ void written() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  for (int j = threadIdx.x; j <= a.K; j += 256) {
+}
+
+// The tokens of [from, to) that entries name, written again with their shares taken off, each by the first entry that
+// names it. share[j] of entries 0..K-1 and of the label, the last.
+template <int DT, int TH>
+__device__ __forceinline__ void name_tokens(const typename TabType<DT>::t* row, typename TabType<DT>::t* out, int K, const int* id,
+                                            const float* share, int64_t from, int64_t to, const Slope& slope) {
+  for (int j = threadIdx.x; j <= K; j += TH) {
     const int i = id[j];
     if (i < from || i >= to) continue;
     float q = 0.0f;
     bool first = true;
-    for (int o = 0; o <= a.K; ++o) {
+    for (int o = 0; o <= K; ++o) {
       if (id[o] != i) continue;
       first &= o >= j;
       q += share[o];
     }
-    if (first) out[i] = tab_put<DT>(at(tab_get<DT>(row[i])) - q);
+    if (first) out[i] = Group<DT>::round(slope(tab_get<DT>(row[i])) - q);
   }
+}
+
+// Gradient of `chunk` logits of a row: all of them from their probabilities, then those that are named.
+template <int DT>
+__global__ void __launch_bounds__(256)
+distill_bwd_kernel(Distill a, const float* kept, const float* upstream, int per_row, const float* factor, float scale, int64_t chunk,
+                   int chunks, void* grad) {
+  using G = Group<DT>;
+  using T = typename TabType<DT>::t;
+  __shared__ int id[kMaxEntries + 1];
+  __shared__ float share[kMaxEntries + 1];
+  const int64_t n = blockIdx.x / chunks, from = (blockIdx.x % chunks) * chunk, to = min(a.V, from + chunk);
+  const T* row = static_cast<const T*>(a.logits) + n * a.ld;
+  T* out = static_cast<T*>(grad) + n * a.V;
+  const float4* k = reinterpret_cast<const float4*>(kept + n * kKept);
+  const float4 k0 = k[0], k1 = k[1];
+  float g = scale;
+  if (upstream) g *= upstream[per_row ? n : 0];
+  if (factor) g *= *factor;
+  const float a_s = k1.y, a_h = k1.z;
+  constexpr int64_t kStep = 256 * G::U;
+  int64_t i = from + (int64_t)threadIdx.x * G::U;
+  if (g == 0.0f || (a_s == 0.0f && a_h == 0.0f)) {
+    const float v[G::U] = {};
+    for (; i + G::U <= to; i += kStep) G::put(out + i, v);
+    for (; i < to && i + G::U > to; ++i) out[i] = G::round(0.0f);
+    return;
+  }
+  const Slope slope = slope_of(a, k0.x, k0.y, k0.z, g * a_s, g * a_h);
+  for (int j = threadIdx.x; j < a.K; j += 256) {
+    float t;
+    const int e = a_s != 0.0f ? entry(a, n, j, t) : -1;
+    id[j] = e;
+    share[j] = e < 0 ? 0.0f : g * a_s * expf((t - k0.w) * a.inv_t) * k1.x;
+  }
+  if (threadIdx.x == 0) id[a.K] = a_h != 0.0f ? label_of(a, n) : -1, share[a.K] = g * a_h;
+  for (; i + 3 * kStep + G::U <= to; i += 4 * kStep) {
+    float v[4][G::U];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) G::get(row + i + q * kStep, v[q]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+      for (int u = 0; u < G::U; ++u) v[q][u] = slope(v[q][u]);
+      G::put(out + i + q * kStep, v[q]);
+    }
+  }
+  for (; i + G::U <= to; i += kStep) {
+    float v[G::U];
+    G::get(row + i, v);
+#pragma unroll
+    for (int u = 0; u < G::U; ++u) v[u] = slope(v[u]);
+    G::put(out + i, v);
+  }
+  if (i < to)
+    for (; i < to; ++i) out[i] = G::round(slope(tab_get<DT>(row[i])));
+  written();
+  name_tokens<DT, 256>(row, out, a.K, id, share, from, to, slope);
+}
+
+// Loss and gradient of a row, a workgroup each, the row's first NV groups of each thread in registers between them.
+template <int DT, int TH, int NV, bool TWO>
+__global__ void __launch_bounds__(TH)
+distill_both_kernel(Distill a, const int* counts, float scale, float* loss, void* grad) {
+  using G = Group<DT>;
+  using T = typename TabType<DT>::t;
+  constexpr int U = G::U, kHeld = NV * TH * U;
+  __shared__ int id[kMaxEntries + 1];
+  __shared__ float share[kMaxEntries + 1];
+  __shared__ float part[2][TH / 64];
+  __shared__ int ipart[TH / 64];
+  __shared__ float told[3];
+  const int64_t n = blockIdx.x;
+  const T* row = static_cast<const T*>(a.logits) + n * a.ld;
+  T* out = static_cast<T*>(grad) + n * a.V;
+  const int V = (int)a.V, groups = V / U;   // whole ones; the row's last V % U values are one thread's
+  const int own = V - groups * U ? (int)threadIdx.x : TH;
+  typename G::Vec r[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int at = j * TH + threadIdx.x;
+    if (at < groups) r[j] = *reinterpret_cast<const typename G::Vec*>(row + (int64_t)at * U);
+  }
+  Teacher t{};
+  if (threadIdx.x < 64) t = teacher_of(a, n, id, share);
+  // f(values, first token) of the thread's groups
+  const auto each = [&](auto f) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int at = j * TH + threadIdx.x;
+      if (at < groups) {
+        float v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = tab_get<DT>(r[j][u]);
+        f(v, at * U);
+      }
+    }
+    for (int at = NV * TH + threadIdx.x; at < groups; at += TH) {
+      float v[U];
+      G::get(row + (int64_t)at * U, v);
+      f(v, at * U);
+    }
+  };
+  const auto rest = [&](auto f) {
+    if (own == 0)
+      for (int i = groups * U; i < V; ++i) f(tab_get<DT>(row[i]), i);
+  };
+  float m = -INFINITY;
+  each([&](const float (&v)[U], int) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) m = fmaxf(m, v[u]);
+  });
+  rest([&](float x, int) { m = fmaxf(m, x); });
+  m = block_reduce<TH>(m, part[0], [](float x, float y) { return fmaxf(x, y); });
+  const float c = a.inv_t * kLog2e, from = m == -INFINITY ? 0.0f : m;
+  float z = 0.0f, z1 = 0.0f;
+  const auto add = [&](float x) {
+    const float d = x - from;
+    z += exp2_fast(d * c);
+    if (TWO) z1 += exp2_fast(d * kLog2e);
+  };
+  each([&](const float (&v)[U], int) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) add(v[u]);
+  });
+  rest([&](float x, int) { add(x); });
+  const auto plus = [](float x, float y) { return x + y; };
+  z = block_reduce<TH>(z, part[0], plus);
+  z1 = TWO ? block_reduce<TH>(z1, part[1], plus) : z;
+  if (counts) {
+    int rows = 0;
+    for (int i = threadIdx.x; i < kCounts; i += TH) rows += counts[i];
+    rows = block_reduce<TH>(rows, ipart, [](int x, int y) { return x + y; });
+    scale *= (float)(1.0 / (double)max(rows, 1));
+  }
+  if (threadIdx.x < 64) {
+    float a_s, a_h;
+    finish_row<DT>(a, n, Sums{m, z, z1}, t, id, share, loss, nullptr, a_s, a_h);
+    const float w = scale * a_s / t.total;
+    for (int j = threadIdx.x; j < a.K; j += 64) {
+      share[j] = a_s != 0.0f ? share[j] * w : 0.0f;
+      if (a_s == 0.0f) id[j] = -1;
+    }
+    if (threadIdx.x == 0) {
+      id[a.K] = a_h != 0.0f ? label_of(a, n) : -1;
+      share[a.K] = scale * a_h;
+      told[0] = a_s, told[1] = a_h;
+    }
+  }
+  __syncthreads();
+  const float a_s = told[0], a_h = told[1];
+  if (scale == 0.0f || (a_s == 0.0f && a_h == 0.0f)) {
+    each([&](const float (&)[U], int i) {
+      const float v[U] = {};
+      G::put(out + i, v);
+    });
+    rest([&](float, int i) { out[i] = G::round(0.0f); });
+    return;
+  }
+  const Slope slope = slope_of(a, m, 1.0f / z, 1.0f / z1, scale * a_s, scale * a_h);
+  each([&](const float (&v)[U], int i) {
+    float g[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) g[u] = slope(v[u]);
+    G::put(out + i, g);
+  });
+  rest([&](float x, int i) { out[i] = G::round(slope(x)); });
+  written();
+  name_tokens<DT, TH>(row, out, a.K, id, share, 0, V, slope);
 }
 
 }  // namespace slg
@@ -235,6 +516,14 @@ void by_type(int dtype, F f) {
   else if (dtype == kTabBf16) f(std::integral_constant<int, kTabBf16>{});
   else f(std::integral_constant<int, kTabF16>{});
 }
+// f with the type and whether two softmaxes are summed.
+template <class F>
+void by_form(const Distill& a, int dtype, F f) {
+  by_type(dtype, [&](auto dt) {
+    if (a.labels && a.T != 1.0f) f(dt, std::true_type{});
+    else f(dt, std::false_type{});
+  });
+}
 
 int check(const Distill& a, int dtype, const char* name) {
   SLG_REQUIRE((a.logits && a.values && a.ids) || a.N == 0, SLG_E_ARG, "%s: null pointer", name);
@@ -243,7 +532,7 @@ int check(const Distill& a, int dtype, const char* name) {
               "%s: ids of %d bytes, labels of %d", name, a.id_bytes, a.label_bytes);
   SLG_REQUIRE(a.T >= 1e-4f && a.T <= 1e4f, SLG_E_ARG, "%s: temperature %g outside [1e-4, 1e4]", name, (double)a.T);
   SLG_REQUIRE(a.alpha >= 0.0f && a.alpha <= 1.0f, SLG_E_ARG, "%s: alpha %g outside [0, 1]", name, (double)a.alpha);
-  SLG_REQUIRE(a.N >= 0 && a.N < (1LL << 31) && a.V >= 1 && a.V < (1LL << 31) && a.ld >= 0 && a.K >= 1 && a.K <= kMaxEntries,
+  SLG_REQUIRE(a.N >= 0 && a.N < (1LL << 31) && a.V >= 1 && a.V < (1LL << 31) - 65536 && a.ld >= 0 && a.K >= 1 && a.K <= kMaxEntries,
               SLG_E_SHAPE, "%s: N %lld, V %lld, K %d", name, (long long)a.N, (long long)a.V, a.K);
   return 0;
 }
@@ -253,14 +542,27 @@ Distill args(const void* logits, int64_t N, int64_t V, int64_t ld, const void* v
   return {logits, N, V, ld, values, vtype, ids, id_bytes, K, labels, label_bytes, T, 1.0f / T, alpha};
 }
 
-// grid of the gradient: rows in chunks of 8192 logits
-constexpr int64_t kChunk = 8192;
+// What `kept` holds: the rows' floats and the factor of an upstream gradient, which the gradient reads; behind them
+// the rows' losses, counts and parts' sums.
+struct Kept {
+  float *rows, *loss, *factor;
+  int* counts;
+  Sums* parts;
+};
+Kept layout(float* kept, int64_t N) {
+  float *loss = kept + N * kKept + 4, *counts = loss + N;
+  return {kept, loss, kept + N * kKept, reinterpret_cast<int*>(counts), reinterpret_cast<Sums*>(counts + kCounts)};
+}
+// Parts of a row: one where there are rows for every compute unit, else as many as fill them, of 2048 values at least.
+int64_t parts_of(int64_t N, int64_t V) { return N >= kParts / 2 ? 1 : std::max<int64_t>(1, std::min<int64_t>(kParts / N, V / 2048)); }
 
 }  // namespace
 
 extern "C" {
 
-int64_t slg_distill_kept(int64_t N) { return N < 0 || N >= (1LL << 31) ? -1 : N * (kKept + 1) + 1; }
+int64_t slg_distill_kept(int64_t N) {
+  return N < 0 || N >= (1LL << 31) ? -1 : N * (kKept + 1) + 4 + kCounts + 3 * (N + kParts);
+}
 
 int slg_distill_fwd(const void* logits, int32_t dtype, int64_t N, int64_t V, int64_t ld, const void* values, int32_t vtype,
                     const void* ids, int32_t id_bytes, int32_t K, const void* labels, int32_t label_bytes, float T, float alpha,
@@ -268,16 +570,23 @@ int slg_distill_fwd(const void* logits, int32_t dtype, int64_t N, int64_t V, int
   const Distill a = args(logits, N, V, ld, values, vtype, ids, id_bytes, K, labels, label_bytes, T, alpha);
   if (const int rc = check(a, dtype, "distill_fwd")) return rc;
   SLG_REQUIRE(reduction >= 0 && reduction <= 2, SLG_E_ARG, "distill_fwd: reduction %d", reduction);
-  SLG_REQUIRE(((loss || N == 0) && kept) || (N == 0 && !reduction), SLG_E_ARG, "distill_fwd: null pointer");
+  SLG_REQUIRE((loss && kept) || (N == 0 && !reduction), SLG_E_ARG, "distill_fwd: null pointer");
+  SLG_REQUIRE((uintptr_t)kept % 16 == 0, SLG_E_ARG, "distill_fwd: kept not at a multiple of 16 bytes");
   if (N == 0 && !reduction) return 0;
   hipStream_t st = as_stream(stream);
-  float *rows = reduction ? kept + N * kKept : loss, *factor = kept + N * (kKept + 1);
-  if (N)
-    by_type(dtype, [&](auto dt) {
-      hipLaunchKernelGGL((distill_fwd_kernel<decltype(dt)::value>), dim3((unsigned)N), dim3(256), 0, st, a, rows, kept);
+  const Kept k = layout(kept, N);
+  float* rows = reduction ? k.loss : loss;
+  if (N) {
+    const int64_t parts = parts_of(N, V), per = cdiv(cdiv(V, parts), 8) * 8;
+    by_form(a, dtype, [&](auto dt, auto two) {
+      constexpr int DT = decltype(dt)::value;
+      hipLaunchKernelGGL((distill_fwd_kernel<DT, decltype(two)::value>), dim3((unsigned)(N * parts)), dim3(256), 0, st, a, (int)parts,
+                         per, k.parts, rows, k.rows);
+      if (parts > 1) hipLaunchKernelGGL(distill_join_kernel<DT>, dim3((unsigned)N), dim3(64), 0, st, a, (int)parts, k.parts, rows, k.rows);
     });
+  }
   if (reduction)
-    hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, st, rows, kept, N, reduction == 2, loss, factor);
+    hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, st, rows, k.rows, nullptr, N, reduction == 2, loss, k.factor);
   SLG_LAUNCH_CHECK("distill_fwd");
   return 0;
 }
@@ -289,12 +598,14 @@ int slg_distill_bwd(const void* logits, int32_t dtype, int64_t N, int64_t V, int
   if (const int rc = check(a, dtype, "distill_bwd")) return rc;
   SLG_REQUIRE(reduction >= 0 && reduction <= 2, SLG_E_ARG, "distill_bwd: reduction %d", reduction);
   SLG_REQUIRE((kept && grad) || N == 0, SLG_E_ARG, "distill_bwd: null pointer");
-  const int64_t chunks = cdiv(V, kChunk);
-  SLG_REQUIRE(N * chunks < (1LL << 31), SLG_E_SHAPE, "distill_bwd: N %lld, V %lld", (long long)N, (long long)V);
+  SLG_REQUIRE((uintptr_t)kept % 16 == 0, SLG_E_ARG, "distill_bwd: kept not at a multiple of 16 bytes");
   if (N == 0) return 0;
+  // whole rows where there are enough of them, else chunks that make 2048 workgroups, of 2048 values at least
+  const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>(cdiv(2048, N), V / 2048)), chunk = cdiv(cdiv(V, chunks), 8) * 8;
   by_type(dtype, [&](auto dt) {
     hipLaunchKernelGGL((distill_bwd_kernel<decltype(dt)::value>), dim3((unsigned)(N * chunks)), dim3(256), 0, as_stream(stream), a,
-                       kept, upstream, reduction == 0, reduction ? kept + N * (kKept + 1) : nullptr, scale, kChunk, (int)chunks, grad);
+                       kept, upstream, reduction == 0, reduction ? layout(const_cast<float*>(kept), N).factor : nullptr, scale, chunk,
+                       (int)chunks, grad);
   });
   SLG_LAUNCH_CHECK("distill_bwd");
   return 0;
@@ -305,11 +616,34 @@ int slg_distill_loss_grad(const void* logits, int32_t dtype, int64_t N, int64_t 
                           int32_t reduction, float scale, float* loss, void* grad, float* kept, slg_stream_t stream) {
   SLG_REQUIRE(grad || N == 0, SLG_E_ARG, "distill_loss_grad: null pointer");
   SLG_REQUIRE(isfinite(scale), SLG_E_ARG, "distill_loss_grad: scale %g", (double)scale);
-  if (const int rc = slg_distill_fwd(logits, dtype, N, V, ld, values, vtype, ids, id_bytes, K, labels, label_bytes, T, alpha, reduction,
-                                     loss, kept, stream))
-    return rc;
-  return slg_distill_bwd(logits, dtype, N, V, ld, values, vtype, ids, id_bytes, K, labels, label_bytes, T, alpha, reduction, kept,
-                         nullptr, scale, grad, stream);
+  if (N == 0 || parts_of(N, V) > 1) {   // too few rows for a workgroup each
+    if (const int rc = slg_distill_fwd(logits, dtype, N, V, ld, values, vtype, ids, id_bytes, K, labels, label_bytes, T, alpha, reduction,
+                                       loss, kept, stream))
+      return rc;
+    return slg_distill_bwd(logits, dtype, N, V, ld, values, vtype, ids, id_bytes, K, labels, label_bytes, T, alpha, reduction, kept,
+                           nullptr, scale, grad, stream);
+  }
+  const Distill a = args(logits, N, V, ld, values, vtype, ids, id_bytes, K, labels, label_bytes, T, alpha);
+  if (const int rc = check(a, dtype, "distill_loss_grad")) return rc;
+  SLG_REQUIRE(reduction >= 0 && reduction <= 2, SLG_E_ARG, "distill_loss_grad: reduction %d", reduction);
+  SLG_REQUIRE(loss && kept && (uintptr_t)kept % 16 == 0, SLG_E_ARG, "distill_loss_grad: loss or kept null or unaligned");
+  hipStream_t st = as_stream(stream);
+  const Kept k = layout(kept, N);
+  float* rows = reduction ? k.loss : loss;
+  int* counts = reduction == 2 ? k.counts : nullptr;
+  if (counts) hipLaunchKernelGGL(distill_count_kernel, dim3(kCounts), dim3(256), 0, st, a, counts);
+  by_form(a, dtype, [&](auto dt, auto two) {
+    constexpr int DT = decltype(dt)::value, U = Group<DT>::U;
+    constexpr bool TWO = decltype(two)::value;
+    const auto go = [&](auto kern, int th) { hipLaunchKernelGGL(kern, dim3((unsigned)N), dim3(th), 0, st, a, counts, scale, rows, grad); };
+    if (V <= 64 * 4 * U) go(distill_both_kernel<DT, 64, 4, TWO>, 64);
+    else if (V <= 256 * 4 * U) go(distill_both_kernel<DT, 256, 4, TWO>, 256);
+    else go(distill_both_kernel<DT, 1024, 8, TWO>, 1024);
+  });
+  if (reduction)
+    hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, st, rows, nullptr, counts, N, reduction == 2, loss, k.factor);
+  SLG_LAUNCH_CHECK("distill_loss_grad");
+  return 0;
 }
 
 }  // extern "C"

@@ -533,13 +533,16 @@ def _distill_checked(logits, values, ids, labels, temperature, alpha, reduction)
 def _distill_shapes(logits, reduction):
     f32 = torch.float32
     return (logits.new_empty((logits.shape[0],) if reduction == 0 else (), dtype=f32),
-            logits.new_empty((9 * logits.shape[0] + 1,), dtype=f32))
+            logits.new_empty((8 * logits.shape[0] + 4,), dtype=f32))
 
 
 @torch.library.custom_op(f"{_NS}::distill_loss", mutates_args=())
 def distill_loss(logits: Tensor, values: Tensor, ids: Tensor, labels: Optional[Tensor], temperature: float,
                  alpha: float, reduction: int) -> Tuple[Tensor, Tensor]:
-    return ops.distill_fwd(*_distill_checked(logits, values, ids, labels, temperature, alpha, reduction))
+    loss, kept = ops.distill_fwd(*_distill_checked(logits, values, ids, labels, temperature, alpha, reduction))
+    kept = kept[:8 * logits.shape[0] + 4].clone()   # what the backward reads of it
+    kept[8 * logits.shape[0] + (reduction != 0):] = 1.0
+    return loss, kept
 
 
 @distill_loss.register_fake
@@ -551,7 +554,7 @@ def _(logits, values, ids, labels, temperature, alpha, reduction):
 def distill_loss_bwd(logits: Tensor, values: Tensor, ids: Tensor, labels: Optional[Tensor], temperature: float,
                      alpha: float, reduction: int, kept: Tensor, upstream: Tensor) -> Tensor:
     args = _distill_checked(logits, values, ids, labels, temperature, alpha, reduction)
-    if kept.dtype != torch.float32 or kept.shape != (9 * logits.shape[0] + 1,) or not kept.is_contiguous() or \
+    if kept.dtype != torch.float32 or kept.shape != (8 * logits.shape[0] + 4,) or not kept.is_contiguous() or \
             upstream.shape != (logits.shape[:1] if reduction == 0 else ()):
         raise ValueError(f"distill_loss_bwd: kept {kept.dtype} {tuple(kept.shape)}, upstream {tuple(upstream.shape)}")
     ops.require_gpu(kept, upstream)

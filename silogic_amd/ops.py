@@ -620,6 +620,11 @@ def sample_logits(logits, u, t, k, p, m, mask):
     return ids
 
 
+def distill_kept(N):
+    """``slg_distill_kept``: floats that the loss of ``N`` rows keeps for its gradient, and works in."""
+    return 12 * N + 3332
+
+
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
@@ -634,7 +639,7 @@ def _distill_args(logits, values, ids, labels, t, alpha, reduction):
 def _distill_out(logits, reduction):
     N = logits.shape[0]
     loss = logits.new_empty((N,) if reduction == 0 else (), dtype=torch.float32)
-    return loss, logits.new_empty(_lib.lib().slg_distill_kept(N), dtype=torch.float32)
+    return loss, logits.new_empty(distill_kept(N), dtype=torch.float32)
 
 
 def distill_fwd(logits, values, ids, labels, t, alpha, reduction):

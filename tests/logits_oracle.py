@@ -6,7 +6,8 @@ import torch
 F64 = torch.float64
 EPS = 2.0 ** -24   # unit rounding of fp32
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
-TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
+# exponentials under 2^-126 count 0, times factors of 4 at most; fp16's smallest step
+TINY = {torch.float32: 2.0 ** -124, torch.bfloat16: 2.0 ** -124, torch.float16: 2.0 ** -25}
 
 
 def top(x, k):

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import silogic_amd as sl
-from silogic_amd import _lib
+from silogic_amd import _lib, ops
 
 P = C.c_void_p(16)   # an address that is only looked at
 ARG, SHAPE = -1, -2
@@ -49,11 +49,14 @@ def test_distill_entry_points():
             assert call(**kw) == ARG, kw
         for kw in (dict(N=-1), dict(N=1 << 31), dict(V=0), dict(V=1 << 31), dict(K=0), dict(K=1025), dict(ld=-1)):
             assert call(**kw) == SHAPE, kw
+    assert fwd(kept=C.c_void_p(20)) == ARG and bwd(kept=C.c_void_p(20)) == ARG and both(kept=C.c_void_p(20)) == ARG
     assert fwd(loss=None) == ARG and bwd(grad=None) == ARG and both(loss=None) == ARG
     assert both(grad=None) == ARG and both(scale=math.inf) == ARG
     assert bwd(N=0, x=None, values=None, ids=None, kept=None, grad=None) == 0
     assert fwd(N=0, reduction=0, x=None, values=None, ids=None, kept=None, loss=None) == 0
-    assert [_lib.lib().slg_distill_kept(n) for n in (0, 7, -1, 1 << 31)] == [1, 64, -1, -1]
+    assert [_lib.lib().slg_distill_kept(n) for n in (-1, 1 << 31)] == [-1, -1]
+    for n in (0, 1, 7, 4096, (1 << 31) - 1):
+        assert _lib.lib().slg_distill_kept(n) == ops.distill_kept(n)
 
 
 def test_top_logits_refuses():
