@@ -161,8 +161,8 @@ struct Teacher {   // maximum and sum of its entries, and whether there are any
   bool some;
 };
 
-// One wave: the teacher's tokens and probabilities (not yet over `total`) into id[] and q[].
-__device__ __forceinline__ Teacher teacher_of(const Distill& a, int64_t n, int* id, float* q) {
+// One wave: the teacher's tokens and probabilities (not yet over `total`) into id[] and q[], their logs into lq[].
+__device__ __forceinline__ Teacher teacher_of(const Distill& a, int64_t n, int* id, float* q, float* lq) {
   const int lane = threadIdx.x & 63;
   float top = -INFINITY, total = 0.0f;
   bool any = false;
@@ -176,8 +176,9 @@ __device__ __forceinline__ Teacher teacher_of(const Distill& a, int64_t n, int* 
   }
   top = wave_reduce(top, [](float x, float y) { return fmaxf(x, y); });
   for (int j = lane; j < a.K; j += 64) {
-    const float e = id[j] >= 0 ? expf((q[j] - top) * a.inv_t) : 0.0f;
+    const float l = (q[j] - top) * a.inv_t, e = id[j] >= 0 ? expf(l) : 0.0f;
     q[j] = e;
+    lq[j] = l;
     total += e;
   }
   total = wave_reduce(total, [](float x, float y) { return x + y; });
@@ -187,7 +188,7 @@ __device__ __forceinline__ Teacher teacher_of(const Distill& a, int64_t n, int* 
 // One wave: the row's loss from its sums, and what is kept of it.
 template <int DT>
 __device__ __forceinline__ void finish_row(const Distill& a, int64_t n, const Sums& s, const Teacher& t, const int* id, const float* q,
-                                           float* loss, float* kept, float& a_s, float& a_h) {
+                                           const float* lq, float* loss, float* kept) {
   const auto* row = static_cast<const typename TabType<DT>::t*>(a.logits) + n * a.ld;
   const int lane = threadIdx.x & 63, y = label_of(a, n);
   const bool alive = s.z != 0.0f;   // a NaN stays
@@ -197,17 +198,10 @@ __device__ __forceinline__ void finish_row(const Distill& a, int64_t n, const Su
   if (soft)
     for (int j = lane; j < a.K; j += 64) {
       const float e = q[j];
-      // log q_j from the value itself: the exponential's log would lose what small ones round
-      if (e != 0.0f) {
-        float v;
-        const int i = entry(a, n, j, v);
-        l += e * rtot * ((v - t.top) * a.inv_t - (tab_get<DT>(row[i]) - s.m) * a.inv_t + logs);
-      }
+      if (e != 0.0f) l += e * rtot * (lq[j] - (tab_get<DT>(row[id[j]]) - s.m) * a.inv_t + logs);
     }
   l = wave_reduce(l, [](float x, float y) { return x + y; });
   const float share = a.labels ? 1.0f - a.alpha : 1.0f;
-  a_s = soft ? share * a.T : 0.0f;
-  a_h = hard ? a.alpha : 0.0f;
   if (lane == 0) {
     float v = soft ? share * a.T * a.T * l : 0.0f;
     if (hard) v += a.alpha * (logf(s.z1) - (tab_get<DT>(row[y]) - s.m));
@@ -215,7 +209,7 @@ __device__ __forceinline__ void finish_row(const Distill& a, int64_t n, const Su
     if (kept) {
       float4* k = reinterpret_cast<float4*>(kept + n * kKept);
       k[0] = {s.m, 1.0f / s.z, 1.0f / s.z1, t.top};
-      k[1] = {rtot, a_s, a_h, t.some || y >= 0 ? 1.0f : 0.0f};
+      k[1] = {rtot, soft ? share * a.T : 0.0f, hard ? a.alpha : 0.0f, t.some || y >= 0 ? 1.0f : 0.0f};
     }
   }
 }
@@ -225,34 +219,32 @@ template <int DT, bool TWO>
 __global__ void __launch_bounds__(256) distill_fwd_kernel(Distill a, int parts, int64_t per, Sums* part_sums, float* loss, float* kept) {
   __shared__ Sums part[4];
   __shared__ int id[kMaxEntries];
-  __shared__ float q[kMaxEntries];
+  __shared__ float q[kMaxEntries], lq[kMaxEntries];
   const int64_t n = blockIdx.x / parts, p = blockIdx.x % parts;
   const auto* row = static_cast<const typename TabType<DT>::t*>(a.logits) + n * a.ld;
   const float c = a.inv_t * kLog2e;
   Sums s = sums_of<DT, 256, TWO>(row, p * per, min(a.V, (p + 1) * per), c);
   Teacher t{};
-  if (parts == 1 && threadIdx.x < 64) t = teacher_of(a, n, id, q);
+  if (parts == 1 && threadIdx.x < 64) t = teacher_of(a, n, id, q, lq);
   s = block_sums<256>(s, c, part);
   if (!TWO) s.z1 = s.z;
   if (parts > 1) {
     if (threadIdx.x == 0) part_sums[blockIdx.x] = s;
   } else if (threadIdx.x < 64) {
-    float a_s, a_h;
-    finish_row<DT>(a, n, s, t, id, q, loss, kept, a_s, a_h);
+    finish_row<DT>(a, n, s, t, id, q, lq, loss, kept);
   }
 }
 template <int DT>
 __global__ void __launch_bounds__(64) distill_join_kernel(Distill a, int parts, const Sums* part_sums, float* loss, float* kept) {
   __shared__ int id[kMaxEntries];
-  __shared__ float q[kMaxEntries];
+  __shared__ float q[kMaxEntries], lq[kMaxEntries];
   const int64_t n = blockIdx.x;
   const float c = a.inv_t * kLog2e;
   Sums s{-INFINITY, 0.0f, 0.0f};
   for (int p = threadIdx.x; p < parts; p += 64) s = join(s, part_sums[n * parts + p], c);
-  const Teacher t = teacher_of(a, n, id, q);
+  const Teacher t = teacher_of(a, n, id, q, lq);
   s = block_sums<64>(s, c, nullptr);
-  float a_s, a_h;
-  finish_row<DT>(a, n, s, t, id, q, loss, kept, a_s, a_h);
+  finish_row<DT>(a, n, s, t, id, q, lq, loss, kept);
 }
 
 // Rows with an entry or a label, counted by kCounts workgroups of four waves.
@@ -317,11 +309,13 @@ __device__ __forceinline__ void written() {
 }
 
 // The tokens of [from, to) that entries name, written again with their shares taken off, each by the first entry that
-// names it. share[j] of entries 0..K-1 and of the label, the last.
-template <int DT, int TH>
+// names it; by `threads` threads, of which this is the `own`th. weight * share[j] of entries 0..K-1, share[K] of the
+// label.
+template <int DT>
 __device__ __forceinline__ void name_tokens(const typename TabType<DT>::t* row, typename TabType<DT>::t* out, int K, const int* id,
-                                            const float* share, int64_t from, int64_t to, const Slope& slope) {
-  for (int j = threadIdx.x; j <= K; j += TH) {
+                                            const float* share, float weight, int64_t from, int64_t to, const Slope& slope, int own,
+                                            int threads) {
+  for (int j = own; j <= K; j += threads) {
     const int i = id[j];
     if (i < from || i >= to) continue;
     float q = 0.0f;
@@ -329,7 +323,7 @@ __device__ __forceinline__ void name_tokens(const typename TabType<DT>::t* row, 
     for (int o = 0; o <= K; ++o) {
       if (id[o] != i) continue;
       first &= o >= j;
-      q += share[o];
+      q += o < K ? weight * share[o] : share[o];
     }
     if (first) out[i] = Group<DT>::round(slope(tab_get<DT>(row[i])) - q);
   }
@@ -390,21 +384,21 @@ distill_bwd_kernel(Distill a, const float* kept, const float* upstream, int per_
   if (i < to)
     for (; i < to; ++i) out[i] = G::round(slope(tab_get<DT>(row[i])));
   written();
-  name_tokens<DT, 256>(row, out, a.K, id, share, from, to, slope);
+  name_tokens<DT>(row, out, a.K, id, share, 1.0f, from, to, slope, threadIdx.x, 256);
 }
 
 // Loss and gradient of a row, a workgroup each, the row's first NV groups of each thread in registers between them.
 template <int DT, int TH, int NV, bool TWO>
-__global__ void __launch_bounds__(TH)
+__global__ void __launch_bounds__(TH, TH == 1024 ? 8 : 1)
 distill_both_kernel(Distill a, const int* counts, float scale, float* loss, void* grad) {
   using G = Group<DT>;
   using T = typename TabType<DT>::t;
   constexpr int U = G::U, kHeld = NV * TH * U;
   __shared__ int id[kMaxEntries + 1];
   __shared__ float share[kMaxEntries + 1];
-  __shared__ float part[2][TH / 64];
+  __shared__ float lq[kMaxEntries], part[2][TH / 64];
   __shared__ int ipart[TH / 64];
-  __shared__ float told[3];
+  __shared__ Teacher told;
   const int64_t n = blockIdx.x;
   const T* row = static_cast<const T*>(a.logits) + n * a.ld;
   T* out = static_cast<T*>(grad) + n * a.V;
@@ -416,8 +410,11 @@ distill_both_kernel(Distill a, const int* counts, float scale, float* loss, void
     const int at = j * TH + threadIdx.x;
     if (at < groups) r[j] = *reinterpret_cast<const typename G::Vec*>(row + (int64_t)at * U);
   }
-  Teacher t{};
-  if (threadIdx.x < 64) t = teacher_of(a, n, id, share);
+  const int y = label_of(a, n);
+  if (threadIdx.x < 64) {
+    const Teacher t = teacher_of(a, n, id, share, lq);
+    if (threadIdx.x == 0) told = t;
+  }
   // f(values, first token) of the thread's groups
   const auto each = [&](auto f) {
 #pragma unroll
@@ -468,40 +465,37 @@ distill_both_kernel(Distill a, const int* counts, float scale, float* loss, void
     rows = block_reduce<TH>(rows, ipart, [](int x, int y) { return x + y; });
     scale *= (float)(1.0 / (double)max(rows, 1));
   }
-  if (threadIdx.x < 64) {
-    float a_s, a_h;
-    finish_row<DT>(a, n, Sums{m, z, z1}, t, id, share, loss, nullptr, a_s, a_h);
-    const float w = scale * a_s / t.total;
-    for (int j = threadIdx.x; j < a.K; j += 64) {
-      share[j] = a_s != 0.0f ? share[j] * w : 0.0f;
-      if (a_s == 0.0f) id[j] = -1;
-    }
-    if (threadIdx.x == 0) {
-      id[a.K] = a_h != 0.0f ? label_of(a, n) : -1;
-      share[a.K] = scale * a_h;
-      told[0] = a_s, told[1] = a_h;
-    }
-  }
-  __syncthreads();
-  const float a_s = told[0], a_h = told[1];
-  if (scale == 0.0f || (a_s == 0.0f && a_h == 0.0f)) {
+  if constexpr (TH == 64) __syncthreads();
+  const Teacher t = told;
+  const bool soft = t.some && z != 0.0f, hard = y >= 0 && z != 0.0f;   // as in finish_row
+  const float a_s = soft ? (a.labels ? 1.0f - a.alpha : 1.0f) * a.T : 0.0f, a_h = hard ? a.alpha : 0.0f;
+  const bool dead = scale == 0.0f || (a_s == 0.0f && a_h == 0.0f);
+  const Slope slope = slope_of(a, m, 1.0f / z, 1.0f / z1, scale * a_s, scale * a_h);
+  if (dead) {
     each([&](const float (&)[U], int i) {
       const float v[U] = {};
       G::put(out + i, v);
     });
     rest([&](float, int i) { out[i] = G::round(0.0f); });
-    return;
-  }
-  const Slope slope = slope_of(a, m, 1.0f / z, 1.0f / z1, scale * a_s, scale * a_h);
-  each([&](const float (&v)[U], int i) {
-    float g[U];
+  } else {
+    each([&](const float (&v)[U], int i) {
+      float g[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) g[u] = slope(v[u]);
-    G::put(out + i, g);
-  });
-  rest([&](float x, int i) { out[i] = G::round(slope(x)); });
+      for (int u = 0; u < U; ++u) g[u] = slope(v[u]);
+      G::put(out + i, g);
+    });
+    rest([&](float x, int i) { out[i] = G::round(slope(x)); });
+  }
+  if (threadIdx.x == 0) {
+    id[a.K] = hard ? y : -1;
+    share[a.K] = scale * a_h;
+  }
   written();
-  name_tokens<DT, TH>(row, out, a.K, id, share, 0, V, slope);
+  // the first wave sums the loss while the others write the tokens that are named
+  if (threadIdx.x < 64) finish_row<DT>(a, n, Sums{m, z, z1}, t, id, share, lq, loss, nullptr);
+  if (!dead && (TH == 64 || threadIdx.x >= 64))
+    name_tokens<DT>(row, out, a.K, id, share, scale * a_s / t.total, 0, V, slope, TH == 64 ? threadIdx.x : threadIdx.x - 64,
+                    TH == 64 ? 64 : TH - 64);
 }
 
 }  // namespace slg
@@ -638,7 +632,8 @@ int slg_distill_loss_grad(const void* logits, int32_t dtype, int64_t N, int64_t 
     const auto go = [&](auto kern, int th) { hipLaunchKernelGGL(kern, dim3((unsigned)N), dim3(th), 0, st, a, counts, scale, rows, grad); };
     if (V <= 64 * 4 * U) go(distill_both_kernel<DT, 64, 4, TWO>, 64);
     else if (V <= 256 * 4 * U) go(distill_both_kernel<DT, 256, 4, TWO>, 256);
-    else go(distill_both_kernel<DT, 1024, 8, TWO>, 1024);
+    else if (DT != kTabF32 || V <= 512 * 8 * U) go(distill_both_kernel<DT, 512, 8, TWO>, 512);
+    else if constexpr (DT == kTabF32) go(distill_both_kernel<DT, 1024, 8, TWO>, 1024);
   });
   if (reduction)
     hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, st, rows, nullptr, counts, N, reduction == 2, loss, k.factor);
