@@ -6,9 +6,9 @@
 // Drawing (temperature T, limits k, p and m, a random number u in [0, 1)): masses w = exp((s - max) / T), of which
 // the first k tokens stay, of these those before which lies less than p of their mass, of these those with w >= m;
 // drawn is the first whose running sum passes u times theirs. Masses are held as whole numbers of 2^-F, F = 62 -
-// log2 V and at most 50 (47 bits at 32000 tokens, where exp in 64 bits is off by 2^-51): their sums are exact, the
-// same in any order, so LDS atomics may make them, and a border between two tokens is where 64-bit sums have it up
-// to about V 2^-F.
+// log2 V and at most 50 (47 bits at 32000 tokens), from an exponential that is off by 2^-43 of itself: their sums are
+// exact, the same in any order, so LDS atomics may make them, and a border between two tokens is where 64-bit sums
+// have it up to about 2^-43 of the sum.
 //
 // A workgroup takes a row, in registers where it fits (the only read of it). What the limits keep is found by value
 // first: k tokens are at least as large as a threshold that k lanes' own maxima reach, min_p is a threshold by
@@ -50,16 +50,16 @@ struct SelectLds {
   int n;
 };
 
-// 2^f on [-1/2, 1/2] by the polynomial of degree 10 with value 1 at 0 and the least largest relative error, 3e-16
+// 2^f on [-1/2, 1/2] by the polynomial of degree 9 with value 1 at 0 and the least largest relative error, 2^-43
 // (fitted by exchange of its extremes). In memory, so that they come to scalar registers: a literal of 64 bits would
 // be moved to vector ones before each product.
-__constant__ double kExp2[10] = {0x1.62e42fefa3a28p-1,  0x1.ebfbdff82c61fp-3,  0x1.c6b08d7039559p-5,  0x1.3b2ab6fb8208ep-7,
-                                 0x1.5d87fea4a755ap-10, 0x1.43091387c719ep-13, 0x1.ffcb3f1b1dfa2p-17, 0x1.62be68640a005p-20,
-                                 0x1.b689b4ad4f65fp-24, 0x1.e8b761c675c38p-28};
+__constant__ double kExp2[9] = {0x1.62e42fefa08dcp-1,  0x1.ebfbdff823df0p-3,  0x1.c6b08d7a95072p-5,
+                                0x1.3b2ab717fb0b6p-7,  0x1.5d87ebe42d79dp-10, 0x1.4308acc67a164p-13,
+                                0x1.fffd75179b1a0p-17, 0x1.63d0ec28f10f2p-20, 0x1.89c489e9e3ae4p-24};
 __device__ __forceinline__ double exp2_small(double f) {
-  double p = kExp2[9];
+  double p = kExp2[8];
 #pragma unroll
-  for (int i = 8; i >= 0; --i) p = fma(p, f, kExp2[i]);
+  for (int i = 7; i >= 0; --i) p = fma(p, f, kExp2[i]);
   return fma(p, f, 1.0);
 }
 
@@ -80,8 +80,8 @@ struct Row {
   SelectLds<TH>* lds;
   Vec r[NV ? NV : 1];
   bool infinite;
-  float top, bin_scale;
-  double top64, slope, shifter, least;   // slope: log2 e / T; masses under `least` (in units of 2^-F) count nothing
+  float top, cut, bin_scale, bin_base;   // under `cut` masses are 0
+  double top64, slope, shifter, least;   // slope: log2 e / T; masses under `least` count nothing
   int F;
   uint64_t from;   // tokens whose place number is under it count nothing
 
@@ -114,9 +114,10 @@ struct Row {
     for (int u = 0; u < VU; ++u) x[u] = logits[min(i + u, V - 1)];
     return x;
   }
-  // NaN for tokens that are another group's, past the row or not allowed.
+  // NaN for tokens that are another group's, past the row, not allowed, or under an infinite largest.
   __device__ __forceinline__ void strike(Vec& x, int i) const {
     const int b = base(i);
+    if (infinite) only_infinite(x);
 #pragma unroll
     for (int u = 0; u < VU; ++u) x[u] = b + u >= i && b + u < V ? x[u] : absent();
     if (allowed) {
@@ -156,25 +157,23 @@ struct Row {
     for (int i = (FIRST * TH + (int)threadIdx.x) * VU; i < V; i += TH * VU) {
       Vec x = read(i);
       const int b = base(i);
-      if (allowed || i + VU > V) strike(x, i);
+      if (allowed || infinite || i + VU > V) strike(x, i);
 #pragma unroll
       for (int u = 0; u < VU; ++u) {
-        f(value(x[u]), b + u);
+        f(tab_get<DT>(x[u]), b + u);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
-  __device__ __forceinline__ float value(T v) const {
-    const float x = tab_get<DT>(v);
-    return infinite ? (x == INFINITY ? 0.0f : -INFINITY) : x;
-  }
   // The largest is +inf: those that are count as 0, the others are absent.
+  static __device__ __forceinline__ void only_infinite(Vec& x) {
+#pragma unroll
+    for (int u = 0; u < VU; ++u) x[u] = tab_get<DT>(x[u]) == INFINITY ? (T)0 : absent();
+  }
   __device__ __forceinline__ void set_infinite() {
     if constexpr (NV > 0) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int u = 0; u < VU; ++u) r[j][u] = tab_get<DT>(r[j][u]) == INFINITY ? (T)0 : absent();
+      for (int j = 0; j < NV; ++j) only_infinite(r[j]);
     }
     infinite = true;
   }
@@ -188,24 +187,33 @@ struct Row {
     slope = uniform(fmin(1.4426950408889634 / t, 1e300));
     F = bits > 12 ? 62 - bits : 50;
     shifter = uniform(0x1.8p52 + (double)F);
-    // bins end where masses fall under 2^-(F+1), or where the row does
-    const float range = fmaxf(fminf((float)((F + 2) * 0.6931472 * t), max - min), 1e-30f);
-    bin_scale = uniform((float)BINS / range);
+    // bins end where masses fall under 2^-(F+2), or where the row does
+    const float reach = (float)((F + 2) * 0.6931472 * t), range = fmaxf(fminf(reach, max - min), 1e-30f);
+    cut = uniform(fmaxf(min, max - reach));
+    // where the sums of bin_at round by more than a bin's part (large logits, close together) all is one bin
+    const float scale = ((float)BINS - 1.0f) / range;
+    bin_scale = uniform(fabsf(max) * scale < 4194304.0f ? scale : 0.0f);
+    bin_base = uniform(max * bin_scale);
   }
-  __device__ __forceinline__ uint64_t mass(float x) const {
-    // the bound takes in -inf and NaN
-    const double y = fmax(((double)x - top64) * slope, -100.0);
+  // 2^-F exp((x - top) / T) to a whole number, for finite x from `cut` on.
+  __device__ __forceinline__ uint64_t mass_in(double y) const {
     // where 1.5 2^52 is added the sum's low bits are the nearest whole number, here n + F
     const double z = y + shifter, n = z - shifter;
-    const long long p = __double_as_longlong(exp2_small(y - n));
-    const double e = __longlong_as_double(p + ((long long)(int)__double_as_longlong(z) << 52));
-    if (!(e >= least)) return 0;
+    const uint64_t p = (uint64_t)__double_as_longlong(exp2_small(y - n));
+    const uint32_t hi = (uint32_t)(p >> 32) + ((uint32_t)__double_as_longlong(z) << 20);
+    const double e = __longlong_as_double((long long)(((uint64_t)hi << 32) | (uint32_t)p));
     // at most 2^50: rounded to a whole number where 2^52 is added, whose bits it then leaves
     return (uint64_t)__double_as_longlong(e + 0x1p52) & ((1ull << 52) - 1);
   }
-  // Falling with x; infinite for -inf.
-  __device__ __forceinline__ float bin_at(float x) const { return (top - x) * bin_scale; }
-  __device__ __forceinline__ uint32_t bin(float x) const { return (uint32_t)fminf(bin_at(x), (float)(BINS - 1)); }
+  // The same of any x; 0 under `least`.
+  __device__ __forceinline__ uint64_t mass(float x) const {
+    // the bound takes in -inf and NaN
+    const uint64_t w = mass_in(fmax(((double)x - top64) * slope, -100.0));
+    return (double)w >= least ? w : 0;
+  }
+  // Falling with x.
+  __device__ __forceinline__ float bin_at(float x) const { return fmaf(x, -bin_scale, bin_base); }
+  __device__ __forceinline__ int bin(float x) const { return min((int)bin_at(x), BINS - 1); }
 
   // What the threads know of a histogram: the sum before a thread's own bins, of its own, of all.
   struct Prefix {
@@ -244,13 +252,15 @@ struct Row {
     for (int i = threadIdx.x; i < BINS; i += TH) lds->hist[i] = 0;
     __syncthreads();
   }
-  // Masses over the bins of the tokens' values; AGAIN: from memory, of the tokens from `from` on.
+  // Masses over the bins of the tokens' values; AGAIN: from memory, of the tokens from `from` on, and not under `least`.
   template <bool AGAIN>
   __device__ __forceinline__ Prefix histogram() const {
     clear();
     const auto add = [&](float x, int i) {
-      const uint64_t w = mass(x);
-      if (w && (!AGAIN || comp(x, i) >= from)) atomicAdd((unsigned long long*)&lds->hist[bin(x)], (unsigned long long)w);
+      if (x >= cut && (!AGAIN || comp(x, i) >= from)) {
+        const uint64_t w = AGAIN ? mass(x) : mass_in(((double)x - top64) * slope);
+        atomicAdd((unsigned long long*)&lds->hist[bin(x)], (unsigned long long)w);
+      }
     };
     if constexpr (AGAIN) each_again<0>(add);
     else each(add);
@@ -332,7 +342,7 @@ struct Row {
   // values are overwritten.
   template <bool AGAIN>
   __device__ __forceinline__ bool within(int b, uint64_t target, uint64_t& before, uint64_t& c) const {
-    const float lo = b ? (float)b : -INFINITY, hi = b < BINS - 1 ? (float)(b + 1) : INFINITY;
+    const float lo = b ? (float)b : -INFINITY, hi = b < BINS - 1 ? (float)(b + 1) : bin_at(cut) + 1.0f;
     const auto in = [&](float x, int i) {
       const float at = bin_at(x);
       return at >= lo && at < hi && (!AGAIN || comp(x, i) >= from);
@@ -497,8 +507,7 @@ sample_kernel(const typename TabType<DT>::t* logits, int64_t ld, int V, const ui
     if (there > k) r.from = r.kth(k, k <= TH && V > TH ? lower : min);
   }
   uint64_t before = 0, c = 0;
-  if (!by_p) r.least = uniform(ldexp(least, r.F));
-  if (!r.from) {
+  if (!r.from && (by_p || !by_m)) {
     const auto hist = r.template histogram<false>();
     total = hist.total;
     bool found = true;
@@ -518,6 +527,7 @@ sample_kernel(const typename TabType<DT>::t* logits, int64_t ld, int V, const ui
       return;
     }
   }
+  if (!by_p) r.least = ldexp(least, r.F);
   auto hist = r.template histogram<true>();
   total = hist.total;
 #pragma unroll 1
@@ -555,7 +565,9 @@ void dispatch(int dtype, int64_t V, int64_t k, F f) {
     if (groups <= 128 && k <= 24) return go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
     if (groups <= 1024 && k <= 96) return go(integral_constant<int, 256>{}, integral_constant<int, 4>{});
     if constexpr (LIST) {
-      if (groups <= 2048) go(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+      // about three times k tokens reach the threshold
+      if (groups <= 4096 && k <= 160) go(integral_constant<int, 512>{}, integral_constant<int, 8>{});
+      else if (groups <= 4096) go(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
       else go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
     } else {
       if (groups <= 2048) go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
