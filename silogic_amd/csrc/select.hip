@@ -19,9 +19,12 @@
 #include <float.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "block_ops.h"
 #include "float_types.h"
+
+#pragma clang fp contract(off)
 
 namespace slg {
 
@@ -71,17 +74,18 @@ struct Row {
   static constexpr int VU = 16 / (int)sizeof(T);
   static constexpr int BINS = kBins<TH>;
   static constexpr bool MORE = NV == 0 || NV == 8;   // rows may be longer than the registers hold
-  typedef T Vec __attribute__((ext_vector_type(VU), aligned(sizeof(T))));
+  using E = std::conditional_t<DT == kTabBf16, __bf16, T>;
+  typedef E Vec __attribute__((ext_vector_type(VU), aligned(sizeof(T))));
   typedef uint8_t Bytes __attribute__((ext_vector_type(VU), aligned(1)));
   const T* logits;
   const uint8_t* allowed;   // null: all
   int V, bits;
   uint64_t id_mask;
   SelectLds<TH>* lds;
-  Vec r[NV ? NV : 1];
+  mutable Vec r[NV ? NV : 1];
   bool infinite;
   float top, cut, bin_scale, bin_base;   // under `cut` masses are 0
-  double top64, slope, shifter, least;   // slope: log2 e / T; masses under `least` count nothing
+  double top64, slope, shifter, lowest, least;   // slope: log2 e / T; masses under `least` count nothing
   int F;
   uint64_t from;   // tokens whose place number is under it count nothing
 
@@ -92,18 +96,23 @@ struct Row {
     from = 0;
     least = 0.0;
     if constexpr (NV > 0) {
+      const int own = (int)threadIdx.x * VU;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) r[j] = read((j * TH + (int)threadIdx.x) * VU);
+      for (int j = 0; j < NV; ++j) r[j] = read(j * TH * VU + own);
+      if (allowed) {
+        Bytes b[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) b[j] = bytes(j * TH * VU + own);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) forbid(r[j], b[j]);
+      }
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (allowed || (j + 1) * TH * VU > V) strike(r[j], (j * TH + (int)threadIdx.x) * VU);
+        if ((j + 1) * TH * VU > V) bound(r[j], j * TH * VU + own);
     }
   }
 
-  static __device__ T absent() {
-    if constexpr (DT == kTabBf16) return (T)0x7fc0;
-    else return (T)NAN;
-  }
+  static __device__ __forceinline__ E absent() { return (E)NAN; }
   // The first token of the group that begins at token i: a row's last group is moved back to end with the row, and
   // those past it come to lie there too. Tokens before i in it are another group's.
   __device__ __forceinline__ int base(int i) const { return NV == 0 && V < VU ? i : min(i, V - VU); }
@@ -111,25 +120,25 @@ struct Row {
     if (NV > 0 || V >= VU) return *reinterpret_cast<const Vec*>(reinterpret_cast<const char*>(logits) + (uint32_t)base(i) * (uint32_t)sizeof(T));
     Vec x;
 #pragma unroll
-    for (int u = 0; u < VU; ++u) x[u] = logits[min(i + u, V - 1)];
+    for (int u = 0; u < VU; ++u) x[u] = reinterpret_cast<const E*>(logits)[min(i + u, V - 1)];
     return x;
   }
-  // NaN for tokens that are another group's, past the row, not allowed, or under an infinite largest.
-  __device__ __forceinline__ void strike(Vec& x, int i) const {
+  __device__ __forceinline__ Bytes bytes(int i) const {
+    if (NV > 0 || V >= VU) return *reinterpret_cast<const Bytes*>(allowed + (uint32_t)base(i));
+    Bytes x;
+#pragma unroll
+    for (int u = 0; u < VU; ++u) x[u] = allowed[min(i + u, V - 1)];
+    return x;
+  }
+  // NaN for tokens that are not allowed; that are another group's, or past the row.
+  static __device__ __forceinline__ void forbid(Vec& x, Bytes b) {
+#pragma unroll
+    for (int u = 0; u < VU; ++u) x[u] = b[u] ? x[u] : absent();
+  }
+  __device__ __forceinline__ void bound(Vec& x, int i) const {
     const int b = base(i);
-    if (infinite) only_infinite(x);
 #pragma unroll
     for (int u = 0; u < VU; ++u) x[u] = b + u >= i && b + u < V ? x[u] : absent();
-    if (allowed) {
-      if (NV > 0 || V >= VU) {
-        const Bytes m = *reinterpret_cast<const Bytes*>(allowed + b);
-#pragma unroll
-        for (int u = 0; u < VU; ++u) x[u] = m[u] ? x[u] : absent();
-      } else {
-#pragma unroll
-        for (int u = 0; u < VU; ++u) x[u] = allowed[min(b + u, V - 1)] ? x[u] : absent();
-      }
-    }
   }
   // f(x, token) of all tokens, absent ones (-inf, NaN) among them, and NaN past the row.
   template <class F>
@@ -138,37 +147,45 @@ struct Row {
     for (int j = 0; j < NV; ++j) {
       // a group at a time, and nothing of it kept from an earlier pass: what is computed of all values at once, or
       // kept, does not fit the registers beside them
-      Vec x = r[j];
       int t = threadIdx.x;
-      asm volatile("" : "+v"(x), "+v"(t));
+      asm volatile("" : "+v"(r[j]), "+v"(t));
       const int i = base((j * TH + t) * VU);
 #pragma unroll
       for (int u = 0; u < VU; ++u) {
-        f(tab_get<DT>(x[u]), i + u);
+        f((float)r[j][u], i + u);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if constexpr (MORE) each_again<NV>(f);
+    if constexpr (MORE) each_again<NV, NV == 0 ? 1 : VU == 4 ? 4 : 2>(f);
   }
   // The same from memory, from group FIRST TH on: for what the registers do not hold, and passes that few rows need.
-  template <int FIRST, class F>
+  // AT_ONCE groups of a thread in flight; those past the row are the last one, struck out.
+  template <int FIRST, int AT_ONCE = 1, class F>
   __device__ __forceinline__ void each_again(F f) const {
 #pragma unroll 1
-    for (int i = (FIRST * TH + (int)threadIdx.x) * VU; i < V; i += TH * VU) {
-      Vec x = read(i);
-      const int b = base(i);
-      if (allowed || infinite || i + VU > V) strike(x, i);
+    for (int g = FIRST * TH * VU; g < V; g += AT_ONCE * TH * VU) {
+      int own = g + (int)threadIdx.x * VU;
+      Vec x[AT_ONCE];
 #pragma unroll
-      for (int u = 0; u < VU; ++u) {
-        f(tab_get<DT>(x[u]), b + u);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int k = 0; k < AT_ONCE; ++k) x[k] = read(own + k * TH * VU);
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int i = own + k * TH * VU, b = base(i);
+        if (infinite) only_infinite(x[k]);
+        if (allowed) forbid(x[k], bytes(i));
+        if (g + (k + 1) * TH * VU > V) bound(x[k], i);
+#pragma unroll
+        for (int u = 0; u < VU; ++u) {
+          f((float)x[k][u], b + u);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
   }
   // The largest is +inf: those that are count as 0, the others are absent.
   static __device__ __forceinline__ void only_infinite(Vec& x) {
 #pragma unroll
-    for (int u = 0; u < VU; ++u) x[u] = tab_get<DT>(x[u]) == INFINITY ? (T)0 : absent();
+    for (int u = 0; u < VU; ++u) x[u] = (float)x[u] == INFINITY ? (E)0.0f : absent();
   }
   __device__ __forceinline__ void set_infinite() {
     if constexpr (NV > 0) {
@@ -187,6 +204,7 @@ struct Row {
     slope = uniform(fmin(1.4426950408889634 / t, 1e300));
     F = bits > 12 ? 62 - bits : 50;
     shifter = uniform(0x1.8p52 + (double)F);
+    lowest = fmax(-100.0 / slope, -1e308);   // far enough down for a mass of 0
     // bins end where masses fall under 2^-(F+2), or where the row does
     const float reach = (float)((F + 2) * 0.6931472 * t), range = fmaxf(fminf(reach, max - min), 1e-30f);
     cut = uniform(fmaxf(min, max - reach));
@@ -195,20 +213,19 @@ struct Row {
     bin_scale = uniform(fabsf(max) * scale < 4194304.0f ? scale : 0.0f);
     bin_base = uniform(max * bin_scale);
   }
-  // 2^-F exp((x - top) / T) to a whole number, for finite x from `cut` on.
-  __device__ __forceinline__ uint64_t mass_in(double y) const {
-    // where 1.5 2^52 is added the sum's low bits are the nearest whole number, here n + F
-    const double z = y + shifter, n = z - shifter;
-    const uint64_t p = (uint64_t)__double_as_longlong(exp2_small(y - n));
-    const uint32_t hi = (uint32_t)(p >> 32) + ((uint32_t)__double_as_longlong(z) << 20);
-    const double e = __longlong_as_double((long long)(((uint64_t)hi << 32) | (uint32_t)p));
+  // 2^F exp(d / T) to a whole number. The products are of single roundings in every place that this comes to: sums over
+  // the same tokens have to be the same.
+  __device__ __forceinline__ uint64_t mass_at(double d) const {
+    // where 1.5 2^52 is added the sum's low bits are the nearest whole number, here of log2 plus F
+    const double z = fma(d, slope, shifter), p = exp2_small(fma(d, slope, shifter - z));
+    const double e = __hiloint2double(__double2hiint(p) + (__double2loint(z) << 20), __double2loint(p));
     // at most 2^50: rounded to a whole number where 2^52 is added, whose bits it then leaves
-    return (uint64_t)__double_as_longlong(e + 0x1p52) & ((1ull << 52) - 1);
+    const double w = e + 0x1p52;
+    return ((uint64_t)(__double2hiint(w) & 0xfffff) << 32) | (uint32_t)__double2loint(w);
   }
-  // The same of any x; 0 under `least`.
+  // The mass of a token, 0 if it is under `least`.
   __device__ __forceinline__ uint64_t mass(float x) const {
-    // the bound takes in -inf and NaN
-    const uint64_t w = mass_in(fmax(((double)x - top64) * slope, -100.0));
+    const uint64_t w = mass_at(fmax((double)x - top64, lowest));
     return (double)w >= least ? w : 0;
   }
   // Falling with x.
@@ -258,7 +275,7 @@ struct Row {
     clear();
     const auto add = [&](float x, int i) {
       if (x >= cut && (!AGAIN || comp(x, i) >= from)) {
-        const uint64_t w = AGAIN ? mass(x) : mass_in(((double)x - top64) * slope);
+        const uint64_t w = AGAIN ? mass(x) : mass_at((double)x - top64);
         atomicAdd((unsigned long long*)&lds->hist[bin(x)], (unsigned long long)w);
       }
     };
