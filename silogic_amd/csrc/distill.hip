@@ -144,14 +144,12 @@ __device__ __forceinline__ Sums sums_of(const typename TabType<DT>::t* row, int6
 template <int TH>
 __device__ __forceinline__ Sums block_sums(Sums v, float c, Sums* part) {
   constexpr int W = TH / 64;
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v = join(v, Sums{__shfl_xor(v.m, d), __shfl_xor(v.z, d), __shfl_xor(v.z1, d)}, c);
+  const auto both = [&](Sums x, Sums y) { return join(x, y, c); };
+  v = lanes_reduce(v, both);
   if constexpr (W > 1) {
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = part[threadIdx.x & (W - 1)];
-#pragma unroll
-    for (int d = W / 2; d; d >>= 1) v = join(v, Sums{__shfl_xor(v.m, d), __shfl_xor(v.z, d), __shfl_xor(v.z1, d)}, c);
+    v = lanes_reduce<W>(part[threadIdx.x & (W - 1)], both);
   }
   return v;
 }

@@ -303,11 +303,7 @@ struct Row {
     const int n = uniform(lds->n);
     mine = lds->list[threadIdx.x];
     __syncthreads();
-    if (n <= TH) {
-      int size = 2;
-      while (size < n) size *= 2;
-      mine = block_sort<TH>(mine, size, lds->list);
-    }
+    if (n <= TH) mine = block_sort<TH>(mine, n, lds->list);
     return n;
   }
 
@@ -394,14 +390,9 @@ struct Row {
   // A value that at least k tokens (at most TH) reach, if there are as many: in each wave as many lanes as make k of
   // all waves have a token of that size, own: each lane's largest.
   __device__ __forceinline__ float reached(float own, int k) const {
-    const int t = threadIdx.x & 63;
-    for (int s = 2; s <= 64; s <<= 1)
-      for (int d = s >> 1; d; d >>= 1) {
-        const float o = __shfl_xor(own, d);
-        own = ((t & s) == 0) == ((t & d) == 0) ? fmaxf(own, o) : fminf(own, o);
-      }
     constexpr int W = TH / 64;
-    own = __shfl(own, (k + W - 1) / W - 1);
+    const int place = (k + W - 1) / W - 1;
+    own = read_lane(wave_sort(own, true), place);
     return block_reduce<TH>(own, reinterpret_cast<float*>(lds->part), [](float p, float q) { return fminf(p, q); });
   }
   // Largest and smallest of the tokens that are there, and a thread's own largest.
