@@ -46,7 +46,7 @@ constexpr int kBins = TH == 64 ? 256 : TH == 256 ? 1024 : 2048;
 
 template <int TH>
 struct SelectLds {
-  uint64_t hist[kBins<TH>];
+  uint64_t hist[kBins<TH> + 64];   // the last ones take what counts nothing
   uint64_t list[TH];
   uint64_t part[TH / 64];
   uint64_t at, base;
@@ -59,10 +59,10 @@ struct SelectLds {
 __constant__ double kExp2[9] = {0x1.62e42fefa08dcp-1,  0x1.ebfbdff823df0p-3,  0x1.c6b08d7a95072p-5,
                                 0x1.3b2ab717fb0b6p-7,  0x1.5d87ebe42d79dp-10, 0x1.4308acc67a164p-13,
                                 0x1.fffd75179b1a0p-17, 0x1.63d0ec28f10f2p-20, 0x1.89c489e9e3ae4p-24};
-__device__ __forceinline__ double exp2_small(double f) {
-  double p = kExp2[8];
+__device__ __forceinline__ double exp2_small(double f, double lead) {
+  double p = fma(lead, f, kExp2[7]);
 #pragma unroll
-  for (int i = 7; i >= 0; --i) p = fma(p, f, kExp2[i]);
+  for (int i = 6; i >= 0; --i) p = fma(p, f, kExp2[i]);
   return fma(p, f, 1.0);
 }
 
@@ -73,6 +73,8 @@ struct Row {
   using T = typename TabType<DT>::t;
   static constexpr int VU = 16 / (int)sizeof(T);
   static constexpr int BINS = kBins<TH>;
+  static constexpr int SUB = VU == 4 ? 4 : 2;
+  static constexpr int AT_A_TIME = 2;   // tokens whose masses are computed side by side
   static constexpr bool MORE = NV == 0 || NV == 8;   // rows may be longer than the registers hold
   using E = std::conditional_t<DT == kTabBf16, __bf16, T>;
   typedef E Vec __attribute__((ext_vector_type(VU), aligned(sizeof(T))));
@@ -85,6 +87,7 @@ struct Row {
   mutable Vec r[NV ? NV : 1];
   bool infinite;
   float top, cut, bin_scale, bin_base;   // under `cut` masses are 0
+  double lead;   // kExp2's last, in vector registers: an instruction reads one scalar operand
   double top64, slope, shifter, lowest, least;   // slope: log2 e / T; masses under `least` count nothing
   int F;
   uint64_t from;   // tokens whose place number is under it count nothing
@@ -95,6 +98,8 @@ struct Row {
     infinite = false;
     from = 0;
     least = 0.0;
+    lead = kExp2[8];
+    asm volatile("" : "+v"(lead));
     if constexpr (NV > 0) {
       const int own = (int)threadIdx.x * VU;
 #pragma unroll
@@ -140,7 +145,7 @@ struct Row {
 #pragma unroll
     for (int u = 0; u < VU; ++u) x[u] = b + u >= i && b + u < V ? x[u] : absent();
   }
-  // f(x, token) of all tokens, absent ones (-inf, NaN) among them, and NaN past the row.
+  // f(values, first token) of all groups, absent tokens (-inf, NaN) among them, and NaN past the row.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
 #pragma unroll
@@ -149,12 +154,7 @@ struct Row {
       // kept, does not fit the registers beside them
       int t = threadIdx.x;
       asm volatile("" : "+v"(r[j]), "+v"(t));
-      const int i = base((j * TH + t) * VU);
-#pragma unroll
-      for (int u = 0; u < VU; ++u) {
-        f((float)r[j][u], i + u);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      give(f, r[j], base((j * TH + t) * VU));
     }
     if constexpr (MORE) each_again<NV, NV == 0 ? 1 : VU == 4 ? 4 : 2>(f);
   }
@@ -170,17 +170,41 @@ struct Row {
       for (int k = 0; k < AT_ONCE; ++k) x[k] = read(own + k * TH * VU);
 #pragma unroll
       for (int k = 0; k < AT_ONCE; ++k) {
-        const int i = own + k * TH * VU, b = base(i);
+        const int i = own + k * TH * VU;
         if (infinite) only_infinite(x[k]);
         if (allowed) forbid(x[k], bytes(i));
         if (g + (k + 1) * TH * VU > V) bound(x[k], i);
-#pragma unroll
-        for (int u = 0; u < VU; ++u) {
-          f((float)x[k][u], b + u);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        give(f, x[k], base(i));
       }
     }
+  }
+  template <class F>
+  static __device__ __forceinline__ void give(F f, const Vec& x, int i) {
+    float v[VU];
+#pragma unroll
+    for (int u = 0; u < VU; ++u) v[u] = (float)x[u];
+    f(v, i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // f(x, token) of the tokens for which in(x) holds; a branch for SUB of them, and for each where one does.
+  template <bool AGAIN, class P, class F>
+  __device__ __forceinline__ void each_in(P in, F f) const {
+    const auto some = [&](const float (&x)[VU], int i) {
+#pragma unroll
+      for (int s = 0; s < VU; s += SUB) {
+        bool any = false;
+#pragma unroll
+        for (int u = s; u < s + SUB; ++u) any |= in(x[u]);
+        if (SUB == 1 ? any : __ballot(any) != 0) {
+#pragma unroll
+          for (int u = s; u < s + SUB; ++u)
+            if (SUB == 1 || in(x[u])) f(x[u], i + u);
+        }
+        if (SUB < VU) __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    if constexpr (AGAIN) each_again<0>(some);
+    else each(some);
   }
   // The largest is +inf: those that are count as 0, the others are absent.
   static __device__ __forceinline__ void only_infinite(Vec& x) {
@@ -201,10 +225,10 @@ struct Row {
   __device__ __forceinline__ void masses(float max, float min, double t) {
     top = max;
     top64 = uniform((double)max);
-    slope = uniform(fmin(1.4426950408889634 / t, 1e300));
+    slope = uniform(fmax(fmin(1.4426950408889634 / t, 1e300), 1e-300));
     F = bits > 12 ? 62 - bits : 50;
     shifter = uniform(0x1.8p52 + (double)F);
-    lowest = fmax(-100.0 / slope, -1e308);   // far enough down for a mass of 0
+    lowest = uniform(-100.0 / slope);   // far enough down for a mass of 0
     // bins end where masses fall under 2^-(F+2), or where the row does
     const float reach = (float)((F + 2) * 0.6931472 * t), range = fmaxf(fminf(reach, max - min), 1e-30f);
     cut = uniform(fmaxf(min, max - reach));
@@ -217,7 +241,7 @@ struct Row {
   // the same tokens have to be the same.
   __device__ __forceinline__ uint64_t mass_at(double d) const {
     // where 1.5 2^52 is added the sum's low bits are the nearest whole number, here of log2 plus F
-    const double z = fma(d, slope, shifter), p = exp2_small(fma(d, slope, shifter - z));
+    const double z = fma(d, slope, shifter), p = exp2_small(fma(d, slope, shifter - z), lead);
     const double e = __hiloint2double(__double2hiint(p) + (__double2loint(z) << 20), __double2loint(p));
     // at most 2^50: rounded to a whole number where 2^52 is added, whose bits it then leaves
     const double w = e + 0x1p52;
@@ -273,32 +297,43 @@ struct Row {
   template <bool AGAIN>
   __device__ __forceinline__ Prefix histogram() const {
     clear();
-    const auto add = [&](float x, int i) {
-      if (x >= cut && (!AGAIN || comp(x, i) >= from)) {
-        const uint64_t w = AGAIN ? mass(x) : mass_at((double)x - top64);
-        atomicAdd((unsigned long long*)&lds->hist[bin(x)], (unsigned long long)w);
-      }
-    };
-    if constexpr (AGAIN) each_again<0>(add);
-    else each(add);
+    if constexpr (AGAIN) {
+      each_in<true>([&](float x) { return x >= cut; }, [&](float x, int i) {
+        if (comp(x, i) >= from) atomicAdd((unsigned long long*)&lds->hist[bin(x)], (unsigned long long)mass(x));
+      });
+    } else {
+      // no branch for a token: those under the cut, or absent, add 0, past the bins to a place of their own lane's
+      const uint32_t last = BINS + (threadIdx.x & 63);
+      each([&](const float (&x)[VU], int) {
+#pragma unroll
+        for (int u = 0; u < VU; ++u) {
+          const float v = x[u] >= cut ? x[u] : -INFINITY;
+          const uint64_t w = mass_at(fmax((double)v - top64, lowest));
+          uint32_t b;
+          asm("v_cvt_u32_f32 %0, %1" : "=v"(b) : "v"(bin_at(v)));   // 0 for a NaN and under 0, the largest past it
+          atomicAdd((unsigned long long*)&lds->hist[min(b, last)], (unsigned long long)w);
+          if (u % AT_A_TIME == AT_A_TIME - 1) __builtin_amdgcn_sched_barrier(0);
+        }
+      });
+    }
     __syncthreads();
     return prefix();
   }
 
-  // The tokens for which in(x, i) holds, in falling order, one a thread (0: none), if there are at most TH; how many.
+  // The tokens for which in(x) holds, in falling order, one a thread (0: none), if there are at most TH; how many. AGAIN:
+  // from memory, of those with place numbers in [lo, hi].
   template <bool AGAIN, class P>
-  __device__ __forceinline__ int collect(P in, uint64_t& mine) const {
+  __device__ __forceinline__ int collect(P in, uint64_t& mine, uint64_t lo = 0, uint64_t hi = ~0ull) const {
     if (threadIdx.x == 0) lds->n = 0;
     lds->list[threadIdx.x] = 0;
     __syncthreads();
-    const auto take = [&](float x, int i) {
-      if (in(x, i)) {
+    each_in<AGAIN>(in, [&](float x, int i) {
+      const uint64_t c = comp(x, i);
+      if (!AGAIN || (c >= lo && c <= hi)) {
         const int at = atomicAdd(&lds->n, 1);
-        if (at < TH) lds->list[at] = comp(x, i);
+        if (at < TH) lds->list[at] = c;
       }
-    };
-    if constexpr (AGAIN) each_again<0>(take);
-    else each(take);
+    });
     __syncthreads();
     const int n = uniform(lds->n);
     mine = lds->list[threadIdx.x];
@@ -311,15 +346,16 @@ struct Row {
   // passes `target`, and the sum before it. By bins of the place numbers until a thread can hold each token of one.
   template <class W>
   __device__ __forceinline__ uint64_t descend(uint64_t lo, uint64_t hi, uint64_t target, uint64_t& before, W weight) const {
+    const auto there = [](float x) { return x > -INFINITY; };
     uint64_t mine;
     int n = TH + 1;
     for (int round = 0; round < 16 && n > TH; ++round) {   // each cuts the numbers' range to a 128th at most, or to one number
       int shift = 0;
       while (((hi - lo) >> shift) >= (uint64_t)BINS) ++shift;
       clear();
-      each_again<0>([&](float x, int i) {
+      each_in<true>(there, [&](float x, int i) {
         const uint64_t c = comp(x, i);
-        if (!(x > -INFINITY) || c < lo || c > hi) return;
+        if (c < lo || c > hi) return;
         const uint64_t w = weight(x);
         if (w) atomicAdd((unsigned long long*)&lds->hist[(hi - c) >> shift], (unsigned long long)w);
       });
@@ -330,7 +366,7 @@ struct Row {
       hi -= d << shift;
       const uint64_t width = (1ull << shift) - 1;
       if (hi - lo > width) lo = hi - width;
-      n = collect<true>([&](float x, int i) { return x > -INFINITY && comp(x, i) >= lo && comp(x, i) <= hi; }, mine);
+      n = collect<true>(there, mine, lo, hi);
     }
     return among(mine, target, before, weight);
   }
@@ -356,24 +392,23 @@ struct Row {
   template <bool AGAIN>
   __device__ __forceinline__ bool within(int b, uint64_t target, uint64_t& before, uint64_t& c) const {
     const float lo = b ? (float)b : -INFINITY, hi = b < BINS - 1 ? (float)(b + 1) : bin_at(cut) + 1.0f;
-    const auto in = [&](float x, int i) {
+    const auto in = [&](float x) {
       const float at = bin_at(x);
-      return at >= lo && at < hi && (!AGAIN || comp(x, i) >= from);
+      return at >= lo && at < hi;
     };
     const auto weight = [&](float x) { return mass(x); };
     uint64_t mine;
-    if (collect<AGAIN>(in, mine) <= TH) {
+    if (collect<AGAIN>(in, mine, from) <= TH) {
       c = among(mine, target, before, weight);
       return true;
     }
     if constexpr (AGAIN) {
       uint64_t first = ~0ull, last = 0;
-      each_again<0>([&](float x, int i) {
-        if (in(x, i)) {
-          const uint64_t at = comp(x, i);
-          first = at < first ? at : first;
-          last = at > last ? at : last;
-        }
+      each_in<true>(in, [&](float x, int i) {
+        const uint64_t at = comp(x, i);
+        if (at < from) return;
+        first = at < first ? at : first;
+        last = at > last ? at : last;
       });
       first = block_reduce<TH>(first, lds->part, [](uint64_t p, uint64_t q) { return p < q ? p : q; });
       last = block_reduce<TH>(last, lds->part, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
@@ -399,16 +434,19 @@ struct Row {
   __device__ __forceinline__ void extremes(float& max, float& min, float& own) const {
     own = -INFINITY;
     min = INFINITY;
-    each([&](float x, int) {   // both pass over a NaN
-      own = fmaxf(own, x);
-      min = fminf(min, x);
+    each([&](const float (&x)[VU], int) {   // both pass over a NaN
+#pragma unroll
+      for (int u = 0; u < VU; ++u) {
+        own = fmaxf(own, x[u]);
+        min = fminf(min, x[u]);
+      }
     });
     const auto smaller = [](float p, float q) { return fminf(p, q); };
     max = block_reduce<TH>(own, reinterpret_cast<float*>(lds->part), [](float p, float q) { return fmaxf(p, q); });
     min = block_reduce<TH>(min, reinterpret_cast<float*>(lds->part), smaller);
     if (min == -INFINITY) {
       min = INFINITY;
-      each_again<0>([&](float x, int) { min = x > -INFINITY ? fminf(min, x) : min; });
+      each_in<true>([](float x) { return x > -INFINITY; }, [&](float x, int) { min = fminf(min, x); });
       min = block_reduce<TH>(min, reinterpret_cast<float*>(lds->part), smaller);
     }
   }
@@ -423,14 +461,15 @@ top_logits_kernel(const typename TabType<DT>::t* logits, int64_t ld, int V, int 
   float least = -FLT_MAX;
   if (V > TH) {
     float own = -FLT_MAX;
-    r.each([&](float x, int) { own = fmaxf(own, x); });
+    r.each([&](const auto& x, int) {
+#pragma unroll
+      for (int u = 0; u < Row<DT, TH, NV>::VU; ++u) own = fmaxf(own, x[u]);
+    });
     least = r.reached(own, K);
   }
   uint64_t mine;
-  if (r.template collect<false>([&](float x, int) { return x >= least; }, mine) > TH) {
-    const uint64_t c = r.kth(K, least);
-    r.template collect<true>([&](float x, int i) { return x >= least && r.comp(x, i) >= c; }, mine);
-  }
+  const auto listed = [&](float x) { return x >= least; };
+  if (r.template collect<false>(listed, mine) > TH) r.template collect<true>(listed, mine, r.kth(K, least));
   if (threadIdx.x < K) {
     values[n * K + threadIdx.x] = tab_put<DT>(mine ? r.of(mine) : -INFINITY);
     ids[n * K + threadIdx.x] = mine ? r.id_of(mine) : -1;
@@ -469,7 +508,7 @@ sample_kernel(const typename TabType<DT>::t* logits, int64_t ld, int V, const ui
   r.extremes(max, min, own);
   if (max == -INFINITY || !(t > 0.0)) {
     int first = V;
-    r.template each_again<0>([&](float x, int i) { first = x == max && max > -INFINITY && i < first ? i : first; });
+    r.template each_in<true>([&](float x) { return x == max && max > -INFINITY; }, [&](float, int i) { first = i < first ? i : first; });
     first = block_reduce<TH>(first, reinterpret_cast<int*>(lds.part), [](int a, int b) { return a < b ? a : b; });
     if (threadIdx.x == 0) ids[n] = first < V ? first : -1;
     return;
@@ -492,7 +531,7 @@ sample_kernel(const typename TabType<DT>::t* logits, int64_t ld, int V, const ui
   uint64_t mine = 0, total;
   int many = TH + 1;
   if (V <= TH || (by_k && k <= TH) || (by_m && !by_p))
-    many = r.template collect<false>([&](float x, int) { return x >= lower; }, mine);
+    many = r.template collect<false>([&](float x) { return x >= lower; }, mine);
   if (many <= TH) {   // a token a thread, in order
     if (by_k && threadIdx.x >= k) mine = 0;
     uint64_t w = mine ? r.mass(r.of(mine)) : 0;
@@ -510,7 +549,7 @@ sample_kernel(const typename TabType<DT>::t* logits, int64_t ld, int V, const ui
   if (by_k && many > TH) {
     // without a threshold the kth may not be there
     int there = 0;
-    r.template each_again<0>([&](float x, int) { there += x > -INFINITY; });
+    r.template each_in<true>([](float x) { return x > -INFINITY; }, [&](float, int) { ++there; });
     there = block_reduce<TH>(there, reinterpret_cast<int*>(lds.part), [](int a, int b) { return a + b; });
     if (there > k) r.from = r.kth(k, k <= TH && V > TH ? lower : min);
   }
