@@ -112,12 +112,18 @@ def _distill(what, logits, values, ids, labels, temperature, alpha, reduction):
         if labels.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"{what}: labels of {labels.dtype} (int32 or int64)")
         _shape(what, "labels", labels, lead)
-        labels = labels.reshape(-1).contiguous()
-    K = values.shape[-1]
-    ops.require_gpu(rows, values, ids, labels)
-    ops.same_device(what, rows, values, ids, labels)
-    return (rows, values.detach().reshape(-1, K).contiguous(), ids.reshape(-1, K).contiguous(), labels,
-            float(temperature), float(alpha), ops.REDUCTIONS[reduction])
+        if labels.dim() != 1:
+            labels = labels.reshape(-1)
+        labels = labels.contiguous()
+    if values.dim() != 2:
+        values, ids = values.reshape(-1, values.shape[-1]), ids.reshape(-1, values.shape[-1])
+    d = rows.get_device()
+    # all in order (the usual call), or the check that says what is not
+    if not (d >= 0 and values.get_device() == d and ids.get_device() == d and (labels is None or labels.get_device() == d)):
+        ops.require_gpu(rows, values, ids, labels)
+        ops.same_device(what, rows, values, ids, labels)
+    return (rows, values.contiguous(), ids.contiguous(), labels, float(temperature), float(alpha),
+            ops.REDUCTIONS[reduction])
 
 
 class _DistillFn(torch.autograd.Function):
