@@ -10,6 +10,14 @@
 
 namespace slg {
 
+// A launch takes fewer than 2^32 threads along x: workgroups past the first kGridX go along y, and those past the last
+// end at once.
+constexpr uint32_t kGridX = 1u << 20;
+inline dim3 grid_of(int64_t blocks) {
+  return blocks <= kGridX ? dim3((unsigned)blocks) : dim3(kGridX, (unsigned)cdiv(blocks, kGridX));
+}
+__device__ __forceinline__ uint32_t block_id() { return blockIdx.y * kGridX + blockIdx.x; }   // blocks: at most 2^31
+
 template <typename T, class F>
 __device__ __forceinline__ T by_words(T v, F f) {
   static_assert(sizeof(T) % 4 == 0, "");

@@ -25,6 +25,7 @@ constexpr float kLog2e = 1.44269504f;
 constexpr int kMaxEntries = 1024;
 constexpr int kKept = 8;      // floats kept of a row: m, 1/Z, 1/Z1, the teacher's maximum and 1/sum, a_s T, a_h, counted
 constexpr int kCounts = 256;  // workgroups that count the rows of a mean
+constexpr int kManyRows = 16384;  // more rows than these are summed by kCounts workgroups before the last one
 constexpr int kParts = 1024;  // parts of rows that the loss's first pass is cut into where there are fewer rows
 
 struct Distill {
@@ -225,7 +226,9 @@ __global__ void __launch_bounds__(256) distill_fwd_kernel(Distill a, int parts, 
   __shared__ Sums part[4];
   __shared__ int id[kMaxEntries];
   __shared__ float q[kMaxEntries], lq[kMaxEntries];
-  const int64_t n = blockIdx.x / parts, p = blockIdx.x % parts;
+  const uint32_t b = block_id();
+  const int64_t n = b / (uint32_t)parts, p = b % (uint32_t)parts;
+  if (n >= a.N) return;
   const auto* row = static_cast<const typename TabType<DT>::t*>(a.logits) + n * a.ld;
   const float c = a.inv_t * kLog2e;
   Sums s = sums_of<DT, 256, FORM>(row, p * per, min(a.V, (p + 1) * per), c);
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(256) distill_fwd_kernel(Distill a, int parts, 
   s = block_sums<256>(s, c, part);
   if (FORM == kOne) s.z1 = s.z;
   if (parts > 1) {
-    if (threadIdx.x == 0) part_sums[blockIdx.x] = s;
+    if (threadIdx.x == 0) part_sums[b] = s;
   } else if (threadIdx.x < 64) {
     finish_row<DT>(a, n, s, t, id, q, lq, loss, kept);
   }
@@ -252,31 +255,67 @@ __global__ void __launch_bounds__(64) distill_join_kernel(Distill a, int parts, 
   finish_row<DT>(a, n, s, t, id, q, lq, loss, kept);
 }
 
-// Rows with an entry or a label, counted by kCounts workgroups of four waves.
+// Rows with an entry or a label, counted by kCounts workgroups of four waves: a lane a row while the label or the first
+// entry is there, a wave a row where not.
 __global__ void __launch_bounds__(256) distill_count_kernel(Distill a, int* counts) {
   __shared__ int part[4];
+  constexpr int64_t kWaves = kCounts * 4;
+  const int lane = threadIdx.x & 63;
+  const int64_t per = min((int64_t)64, (a.N + kWaves - 1) / kWaves);
   int c = 0;
-  for (int64_t n = blockIdx.x * 4 + (threadIdx.x >> 6); n < a.N; n += (int64_t)gridDim.x * 4) {
-    bool any = label_of(a, n) >= 0;
-    for (int j = threadIdx.x & 63; !__ballot(any) && j - (int)(threadIdx.x & 63) < a.K; j += 64) {
+  for (int64_t first = ((int64_t)blockIdx.x * 4 + wave_id()) * per; first < a.N; first += kWaves * per) {
+    const int64_t n = first + lane;
+    const bool own = lane < per && n < a.N;
+    bool any = false;
+    if (own) {
       float t;
-      any = j < a.K && entry(a, n, j, t) >= 0;
+      const bool hard = label_of(a, n) >= 0, soft = entry(a, n, 0, t) >= 0;
+      any = hard || soft;
     }
-    c += __ballot(any) != 0;
+    c += __popcll(__ballot(any));
+    for (uint64_t left = __ballot(own && !any); left; left &= left - 1) {
+      const int64_t row = first + __builtin_ctzll(left);
+      bool some = false;
+      for (int j = lane; !__ballot(some) && j - lane < a.K; j += 64) {
+        float t;
+        some = j < a.K && entry(a, row, j, t) >= 0;
+      }
+      c += __ballot(some) != 0;
+    }
   }
-  c = block_reduce<256>((threadIdx.x & 63) == 0 ? c : 0, part, [](int x, int y) { return x + y; });
+  c = block_reduce<256>(lane == 0 ? c : 0, part, [](int x, int y) { return x + y; });
   if (threadIdx.x == 0) counts[blockIdx.x] = c;
 }
 
-// Sum of the rows' losses, or their mean over the rows that count (by `counted`, or where that is null by what is
-// kept of the rows), and what an upstream gradient is multiplied by.
-__global__ void __launch_bounds__(1024) distill_mean_kernel(const float* loss, const float* kept, const int* counts, int64_t N, int mean,
-                                                            float* out, float* factor) {
-  __shared__ double part[16];
+// Sum of the rows' losses, or their mean over the rows that count (by `counts`, or where that is null by what is
+// kept of the rows), and what an upstream gradient is multiplied by. One workgroup, behind another kernel that sums the
+// rows in kCounts runs where there are many.
+__global__ void __launch_bounds__(256) distill_sum_kernel(const float* loss, const float* kept, int64_t N, double2* sums) {
+  __shared__ double part[4];
+  const int64_t per = (N + kCounts - 1) / kCounts, from = blockIdx.x * per, to = min(N, from + per);
   double s = 0.0, c = 0.0;
-  for (int64_t n = threadIdx.x; n < N; n += 1024) {
+#pragma unroll 4
+  for (int64_t n = from + threadIdx.x; n < to; n += 256) {
     s += (double)loss[n];
     if (kept) c += (double)kept[n * kKept + 7];
+  }
+  const auto add = [](double x, double y) { return x + y; };
+  s = block_reduce<256>(s, part, add);
+  c = block_reduce<256>(c, part, add);
+  if (threadIdx.x == 0) sums[blockIdx.x] = {s, c};
+}
+__global__ void __launch_bounds__(1024) distill_mean_kernel(const float* loss, const float* kept, const double2* sums, const int* counts,
+                                                            int64_t N, int mean, float* out, float* factor) {
+  __shared__ double part[16];
+  double s = 0.0, c = 0.0;
+  if (sums) {
+    if (threadIdx.x < kCounts) s = sums[threadIdx.x].x, c = sums[threadIdx.x].y;
+  } else {
+#pragma unroll 4
+    for (int64_t n = threadIdx.x; n < N; n += 1024) {
+      s += (double)loss[n];
+      if (kept) c += (double)kept[n * kKept + 7];
+    }
   }
   if (counts && threadIdx.x < kCounts) c = (double)counts[threadIdx.x];
   const auto add = [](double x, double y) { return x + y; };
@@ -354,7 +393,9 @@ distill_bwd_kernel(Distill a, const float* kept, const float* upstream, int per_
   using T = typename TabType<DT>::t;
   __shared__ int id[kMaxEntries + 1];
   __shared__ float share[kMaxEntries + 1];
-  const int64_t n = blockIdx.x / chunks, from = (blockIdx.x % chunks) * chunk, to = min(a.V, from + chunk);
+  const uint32_t b = block_id();
+  const int64_t n = b / (uint32_t)chunks, from = b % (uint32_t)chunks * chunk, to = min(a.V, from + chunk);
+  if (n >= a.N) return;
   const T* row = static_cast<const T*>(a.logits) + n * a.ld;
   T* out = static_cast<T*>(grad) + n * a.V;
   const float4* k = reinterpret_cast<const float4*>(kept + n * kKept);
@@ -418,7 +459,8 @@ distill_both_kernel(Distill a, const int* counts, float scale, float* loss, void
   __shared__ float lq[kMaxEntries], part[2][TH / 64];
   __shared__ int ipart[TH / 64];
   __shared__ Teacher told;
-  const int64_t n = blockIdx.x;
+  const int64_t n = block_id();
+  if (n >= a.N) return;
   const T* row = static_cast<const T*>(a.logits) + n * a.ld;
   T* out = static_cast<T*>(grad) + n * a.V;
   const int V = (int)a.V, groups = V / U;   // whole ones; the row's last V % U values are one thread's
@@ -569,10 +611,19 @@ struct Kept {
   float *rows, *loss, *factor;
   int* counts;
   Sums* parts;
+  double2* sums;   // in the parts' place, of which there are none where rows are many
 };
 Kept layout(float* kept, int64_t N) {
-  float *loss = kept + N * kKept + 4, *counts = loss + N;
-  return {kept, loss, kept + N * kKept, reinterpret_cast<int*>(counts), reinterpret_cast<Sums*>(counts + kCounts)};
+  float *loss = kept + N * kKept + 4, *counts = loss + N, *parts = counts + kCounts;
+  return {kept, loss, kept + N * kKept, reinterpret_cast<int*>(counts), reinterpret_cast<Sums*>(parts),
+          reinterpret_cast<double2*>(kept + cdiv(parts - kept, 4) * 4)};
+}
+
+// The loss of all rows.
+void sum_rows(const float* rows, const float* kept, const int* counts, int64_t N, bool mean, float* loss, const Kept& k, hipStream_t st) {
+  double2* sums = N > kManyRows ? k.sums : nullptr;
+  if (sums) hipLaunchKernelGGL(distill_sum_kernel, dim3(kCounts), dim3(256), 0, st, rows, mean ? kept : nullptr, N, sums);
+  hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, st, rows, kept, sums, counts, N, mean, loss, k.factor);
 }
 // Parts of a row: one where there are rows for every compute unit, else as many as fill them, of 2048 values at least.
 int64_t parts_of(int64_t N, int64_t V) { return N >= kParts / 2 ? 1 : std::max<int64_t>(1, std::min<int64_t>(kParts / N, V / 2048)); }
@@ -601,13 +652,13 @@ int slg_distill_fwd(const void* logits, int32_t dtype, int64_t N, int64_t V, int
     const int64_t parts = parts_of(N, V), per = cdiv(cdiv(V, parts), 8) * 8;
     by_form(a, dtype, [&](auto dt, auto form) {
       constexpr int DT = decltype(dt)::value;
-      hipLaunchKernelGGL((distill_fwd_kernel<DT, decltype(form)::value>), dim3((unsigned)(N * parts)), dim3(256), 0, st, a, (int)parts,
+      hipLaunchKernelGGL((distill_fwd_kernel<DT, decltype(form)::value>), grid_of(N * parts), dim3(256), 0, st, a, (int)parts,
                          per, k.parts, rows, k.rows);
       if (parts > 1) hipLaunchKernelGGL(distill_join_kernel<DT>, dim3((unsigned)N), dim3(64), 0, st, a, (int)parts, k.parts, rows, k.rows);
     });
   }
   if (reduction)
-    hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, st, rows, k.rows, nullptr, N, reduction == 2, loss, k.factor);
+    sum_rows(rows, k.rows, nullptr, N, reduction == 2, loss, k, st);
   SLG_LAUNCH_CHECK("distill_fwd");
   return 0;
 }
@@ -624,7 +675,7 @@ int slg_distill_bwd(const void* logits, int32_t dtype, int64_t N, int64_t V, int
   // whole rows where there are enough of them, else chunks that make 2048 workgroups, of 2048 values at least
   const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>(cdiv(2048, N), V / 2048)), chunk = cdiv(cdiv(V, chunks), 8) * 8;
   by_type(dtype, [&](auto dt) {
-    hipLaunchKernelGGL((distill_bwd_kernel<decltype(dt)::value>), dim3((unsigned)(N * chunks)), dim3(256), 0, as_stream(stream), a,
+    hipLaunchKernelGGL((distill_bwd_kernel<decltype(dt)::value>), grid_of(N * chunks), dim3(256), 0, as_stream(stream), a,
                        kept, upstream, reduction == 0, reduction ? layout(const_cast<float*>(kept), N).factor : nullptr, scale, chunk,
                        (int)chunks, grad);
   });
@@ -656,14 +707,14 @@ int slg_distill_loss_grad(const void* logits, int32_t dtype, int64_t N, int64_t 
   by_form(a, dtype, [&](auto dt, auto form) {
     constexpr int DT = decltype(dt)::value, U = Group<DT>::U;
     constexpr Form FORM = decltype(form)::value;
-    const auto go = [&](auto kern, int th) { hipLaunchKernelGGL(kern, dim3((unsigned)N), dim3(th), 0, st, a, counts, scale, rows, grad); };
+    const auto go = [&](auto kern, int th) { hipLaunchKernelGGL(kern, grid_of(N), dim3(th), 0, st, a, counts, scale, rows, grad); };
     if (V <= 64 * 4 * U) go(distill_both_kernel<DT, 64, 4, FORM>, 64);
     else if (V <= 256 * 4 * U) go(distill_both_kernel<DT, 256, 4, FORM>, 256);
     else if (DT != kTabF32 || V <= 512 * 8 * U) go(distill_both_kernel<DT, 512, 8, FORM>, 512);
     else if constexpr (DT == kTabF32) go(distill_both_kernel<DT, 1024, 8, FORM>, 1024);
   });
   if (reduction)
-    hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, st, rows, nullptr, counts, N, reduction == 2, loss, k.factor);
+    sum_rows(rows, nullptr, counts, N, reduction == 2, loss, k, st);
   SLG_LAUNCH_CHECK("distill_loss_grad");
   return 0;
 }

@@ -454,9 +454,11 @@ struct Row {
 
 template <int DT, int TH, int NV>
 __global__ void __launch_bounds__(TH)
-top_logits_kernel(const typename TabType<DT>::t* logits, int64_t ld, int V, int K, typename TabType<DT>::t* values, int64_t* ids) {
+top_logits_kernel(const typename TabType<DT>::t* logits, int64_t N, int64_t ld, int V, int K, typename TabType<DT>::t* values,
+                  int64_t* ids) {
   __shared__ SelectLds<TH> lds;
-  const int64_t n = blockIdx.x;
+  const int64_t n = block_id();
+  if (n >= N) return;
   Row<DT, TH, NV> r(logits + n * ld, nullptr, V, &lds);
   float least = -FLT_MAX;
   if (V > TH) {
@@ -496,10 +498,11 @@ __device__ inline uint64_t target_of(float u, uint64_t total) {
 
 template <int DT, int TH, int NV>
 __global__ void __launch_bounds__(TH, 4)
-sample_kernel(const typename TabType<DT>::t* logits, int64_t ld, int V, const uint8_t* allowed, int64_t allowed_ld, const float* us,
-              Limits lim, int64_t* ids) {
+sample_kernel(const typename TabType<DT>::t* logits, int64_t N, int64_t ld, int V, const uint8_t* allowed, int64_t allowed_ld,
+              const float* us, Limits lim, int64_t* ids) {
   __shared__ SelectLds<TH> lds;
-  const int64_t n = blockIdx.x;
+  const int64_t n = block_id();
+  if (n >= N) return;
   Row<DT, TH, NV> r(logits + n * ld, allowed ? allowed + n * allowed_ld : nullptr, V, &lds);
   const double t = lim.ts ? lim.ts[n] : lim.t, p = lim.ps ? lim.ps[n] : lim.p, m = lim.ms ? lim.ms[n] : lim.m;
   const int64_t k = lim.ks ? lim.ks[n] : lim.k;
@@ -641,8 +644,8 @@ int slg_top_logits(const void* logits, int32_t dtype, int64_t N, int64_t V, int6
   if (N == 0) return 0;
   dispatch<true>(dtype, V, K, [&](auto dt, auto th, auto nv) {
     using T = typename TabType<decltype(dt)::value>::t;
-    hipLaunchKernelGGL((top_logits_kernel<decltype(dt)::value, decltype(th)::value, decltype(nv)::value>), dim3((unsigned)N), dim3(decltype(th)::value), 0,
-                       as_stream(stream), static_cast<const T*>(logits), ld, (int)V, (int)K, static_cast<T*>(values), ids);
+    hipLaunchKernelGGL((top_logits_kernel<decltype(dt)::value, decltype(th)::value, decltype(nv)::value>), grid_of(N), dim3(decltype(th)::value), 0,
+                       as_stream(stream), static_cast<const T*>(logits), N, ld, (int)V, (int)K, static_cast<T*>(values), ids);
   });
   SLG_LAUNCH_CHECK("top_logits");
   return 0;
@@ -662,8 +665,8 @@ int slg_sample_logits(const void* logits, int32_t dtype, int64_t N, int64_t V, i
   const Limits lim{temperature, top_p, min_p, top_k, temperatures, top_ps, min_ps, top_ks};
   dispatch<false>(dtype, V, 1, [&](auto dt, auto th, auto nv) {
     using T = typename TabType<decltype(dt)::value>::t;
-    hipLaunchKernelGGL((sample_kernel<decltype(dt)::value, decltype(th)::value, decltype(nv)::value>), dim3((unsigned)N), dim3(decltype(th)::value), 0,
-                       as_stream(stream), static_cast<const T*>(logits), ld, (int)V, allowed, allowed_ld, u, lim, ids);
+    hipLaunchKernelGGL((sample_kernel<decltype(dt)::value, decltype(th)::value, decltype(nv)::value>), grid_of(N), dim3(decltype(th)::value), 0,
+                       as_stream(stream), static_cast<const T*>(logits), N, ld, (int)V, allowed, allowed_ld, u, lim, ids);
   });
   SLG_LAUNCH_CHECK("sample_logits");
   return 0;

@@ -56,7 +56,7 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
     token, and limits out of their range act as their nearest bound). ``mask`` (bool, ``[V]`` to ``[..., V]``) is True for
     tokens that are allowed. A NaN or -inf is no token; a row without one gives -1.
 
-    Masses are held as whole numbers of 2^-F of the largest, F = min(52, 62 - bits of V), so that their sums are exact
+    Masses are held as whole numbers of 2^-F of the largest, F = min(50, 62 - bits of V), so that their sums are exact
     and the same draw comes from the same inputs on every call. A ``u`` outside [0, 1) acts as its nearest bound."""
     lead = logits.shape[:-1]
     rows = ops.check_logits("sample_logits", logits.detach())

@@ -1,0 +1,81 @@
+"""The operators on logits with more rows than one dimension of a launch takes (2^32 threads), and sums over many
+rows."""
+import pytest
+import torch
+
+import silogic_amd as sl
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+ROWS = (1 << 26) + 1000   # of workgroups of 64 threads and more
+
+
+def test_rows_past_a_launch_dimension_are_listed_and_drawn():
+    """The largest token, which k = 1, temperature 0 and u = 0 all give, of each of 2^26 rows and some."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(ROWS, 4, device=DEV, generator=g)
+    best = x.max(1).values
+    values, ids = sl.top_logits(x, 1)
+    assert torch.equal(values[:, 0], best) and torch.equal(x.gather(1, ids)[:, 0], best)
+    u = torch.zeros(ROWS, device=DEV)
+    for t in (0.0, 1.0):
+        ids = sl.sample_logits(x, u, temperature=t)
+        assert torch.equal(x.gather(1, ids[:, None])[:, 0], best)
+
+
+def test_rows_past_a_launch_dimension_have_losses_and_gradients():
+    """Two logits and one entry: -log p of it, and p less 1 there. In units of 2^-24: the difference d of the logits is
+    rounded (|d|), so are the exponential's argument (|d| e^-|d| each for log2 e and the product, under 1 together) and
+    itself (2), the sum (1 of at most 2), its logarithm (2 of at most 0.7) and the loss's two additions (|loss| each): under
+    8 + 3 |loss|. A probability takes the exponential's and the sum's errors: under 16, and half a step of 1."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.randn(ROWS, 2, device=DEV, generator=g)
+    ids = torch.randint(0, 2, (ROWS, 1), device=DEV, generator=g, dtype=torch.int32)
+    values = torch.zeros(ROWS, 1, device=DEV)
+    p = torch.softmax(x.double(), 1)
+    want = -p.gather(1, ids.long())[:, 0].log()
+    tol = 2.0 ** -24 * (8 + 3 * want)
+    p.scatter_add_(1, ids.long(), torch.full_like(p[:, :1], -1.0))
+    loss, grad = sl.distill_loss_and_grad(x, values, ids, reduction="none")
+    assert bool(((loss.double() - want).abs() <= tol).all())
+    assert float((grad.double() - p).abs().max()) <= 17 * 2.0 ** -24
+    del grad
+    x.requires_grad_()
+    mean = sl.distill_loss(x, values, ids)
+    mean.backward()
+    mean = mean.detach()
+    # the mean's own rounding beside its terms'
+    assert abs(float(mean) - float(want.mean())) <= float(tol.mean()) + 2.0 ** -24 * float(want.mean())
+    # the share of a row (1 / N, twice rounded) before the probabilities', in units of it
+    assert float((x.grad.double() * ROWS - p).abs().max()) <= 20 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("N", [1, 1023, 1025, 16384, 16385, 70001])
+@pytest.mark.parametrize("first", [True, False])
+def test_means_over_many_rows_count_the_rows(N, first):
+    """Equal logits, where every row that counts has a loss of log 8 at one entry: the mean is that, whichever rows
+    have nothing, and the gradient's sum of absolute values over a row is 2 (1 - 1/8) over the count. `first`: the
+    entry is the first one or the last of 70."""
+    g = torch.Generator(device=DEV).manual_seed(N)
+    x = torch.zeros(N, 8, device=DEV, requires_grad=True)
+    ids = torch.full((N, 70), -1, device=DEV)
+    some = torch.rand(N, device=DEV, generator=g) < 0.6
+    some[N // 2] = True
+    ids[some, 0 if first else 69] = 3
+    values = torch.zeros(N, 70, device=DEV)
+    labels = torch.full((N,), -100, device=DEV)
+    labels[::5] = 3   # of rows with and without entries
+    count = int((some | (labels == 3)).sum())
+    loss = sl.distill_loss(x, values, ids, labels, alpha=0.5)
+    loss.backward()
+    terms = (some.double() + (labels == 3).double()).sum().item() * 0.5
+    want = terms * 2.0794415416798357 / count
+    # log 8 takes the logarithm of an exact sum (2 units of 2^-24), its half is exact, a row adds two, the mean one
+    tol = 5 * 2.0 ** -24 * max(want, 1.0) * 2.1
+    assert abs(float(loss) - want) <= tol
+    both, grad = sl.distill_loss_and_grad(x, values, ids, labels, alpha=0.5)
+    assert abs(float(both) - want) <= tol
+    rows = (some.double() + (labels == 3).double()) * 0.5 * 1.75 / count
+    for got in (x.grad, grad):
+        # 1/8 is exact; the share 1 / count and its products round three times, the two tokens' sums once each
+        assert bool(((got.double().abs().sum(1) - rows).abs() <= 8 * 2.0 ** -24 * rows).all())
