@@ -162,6 +162,18 @@ __device__ __forceinline__ Sums block_sums(Sums v, float c, Sums* part) {
   return v;
 }
 
+// A row's entries in LDS, sized by K: their tokens and their shares, and behind them the label's, and their logs.
+struct Entries {
+  int* id;
+  float *share, *log;
+  __device__ __forceinline__ explicit Entries(int K) {
+    extern __shared__ float entries[];
+    id = reinterpret_cast<int*>(entries);
+    share = entries + K + 1;
+    log = share + K + 1;
+  }
+};
+
 struct Teacher {   // maximum and sum of its entries, and whether there are any
   float top, total;
   bool some;
@@ -221,38 +233,36 @@ __device__ __forceinline__ void finish_row(const Distill& a, int64_t n, const Su
 }
 
 // The loss of a row, a workgroup each; with parts > 1 the sums of a part of a row, joined by the next kernel.
-template <int DT, Form FORM>
-__global__ void __launch_bounds__(256) distill_fwd_kernel(Distill a, int parts, int64_t per, Sums* part_sums, float* loss, float* kept) {
-  __shared__ Sums part[4];
-  __shared__ int id[kMaxEntries];
-  __shared__ float q[kMaxEntries], lq[kMaxEntries];
+template <int DT, int TH, Form FORM>
+__global__ void __launch_bounds__(TH) distill_fwd_kernel(Distill a, int parts, int64_t per, Sums* part_sums, float* loss, float* kept) {
+  __shared__ Sums part[TH / 64];
+  const Entries e(a.K);
   const uint32_t b = block_id();
   const int64_t n = b / (uint32_t)parts, p = b % (uint32_t)parts;
   if (n >= a.N) return;
   const auto* row = static_cast<const typename TabType<DT>::t*>(a.logits) + n * a.ld;
   const float c = a.inv_t * kLog2e;
-  Sums s = sums_of<DT, 256, FORM>(row, p * per, min(a.V, (p + 1) * per), c);
+  Sums s = sums_of<DT, TH, FORM>(row, p * per, min(a.V, (p + 1) * per), c);
   Teacher t{};
-  if (parts == 1 && threadIdx.x < 64) t = teacher_of(a, n, id, q, lq);
-  s = block_sums<256>(s, c, part);
+  if (parts == 1 && threadIdx.x < 64) t = teacher_of(a, n, e.id, e.share, e.log);
+  s = block_sums<TH>(s, c, part);
   if (FORM == kOne) s.z1 = s.z;
   if (parts > 1) {
     if (threadIdx.x == 0) part_sums[b] = s;
   } else if (threadIdx.x < 64) {
-    finish_row<DT>(a, n, s, t, id, q, lq, loss, kept);
+    finish_row<DT>(a, n, s, t, e.id, e.share, e.log, loss, kept);
   }
 }
 template <int DT>
 __global__ void __launch_bounds__(64) distill_join_kernel(Distill a, int parts, const Sums* part_sums, float* loss, float* kept) {
-  __shared__ int id[kMaxEntries];
-  __shared__ float q[kMaxEntries], lq[kMaxEntries];
+  const Entries e(a.K);
   const int64_t n = blockIdx.x;
   const float c = a.inv_t * kLog2e;
   Sums s{-INFINITY, 0.0f, 0.0f};
   for (int p = threadIdx.x; p < parts; p += 64) s = join(s, part_sums[n * parts + p], c);
-  const Teacher t = teacher_of(a, n, id, q, lq);
+  const Teacher t = teacher_of(a, n, e.id, e.share, e.log);
   s = block_sums<64>(s, c, nullptr);
-  finish_row<DT>(a, n, s, t, id, q, lq, loss, kept);
+  finish_row<DT>(a, n, s, t, e.id, e.share, e.log, loss, kept);
 }
 
 // Rows with an entry or a label, counted by kCounts workgroups of four waves: a lane a row while the label or the first
@@ -375,24 +385,27 @@ __device__ __forceinline__ void name_tokens(const typename TabType<DT>::t* row, 
     if (i < from || i >= to) continue;
     float q = 0.0f;
     bool first = true;
-    for (int o = 0; o <= K; ++o) {
-      if (id[o] != i) continue;
-      first &= o >= j;
-      q += o < K ? weight * share[o] : share[o];
+#pragma unroll 8
+    for (int o = 0; o < K; ++o) {   // no branch: the reads are in flight together
+      const bool same = id[o] == i;
+      first &= !same || o >= j;
+      q += same ? weight * share[o] : 0.0f;
     }
+    if (id[K] == i) q += share[K];
     if (first) out[i] = Group<DT>::round(slope.at<FORM>(tab_get<DT>(row[i])) - q);
   }
 }
 
 // Gradient of `chunk` logits of a row: all of them from their probabilities, then those that are named.
-template <int DT>
-__global__ void __launch_bounds__(256)
+template <int DT, int TH>
+__global__ void __launch_bounds__(TH)
 distill_bwd_kernel(Distill a, const float* kept, const float* upstream, int per_row, const float* factor, float scale, int64_t chunk,
                    int chunks, void* grad) {
   using G = Group<DT>;
   using T = typename TabType<DT>::t;
-  __shared__ int id[kMaxEntries + 1];
-  __shared__ float share[kMaxEntries + 1];
+  const Entries entries(a.K);
+  int* id = entries.id;
+  float* share = entries.share;
   const uint32_t b = block_id();
   const int64_t n = b / (uint32_t)chunks, from = b % (uint32_t)chunks * chunk, to = min(a.V, from + chunk);
   if (n >= a.N) return;
@@ -404,7 +417,7 @@ distill_bwd_kernel(Distill a, const float* kept, const float* upstream, int per_
   if (upstream) g *= upstream[per_row ? n : 0];
   if (factor) g *= *factor;
   const float a_s = k1.y, a_h = k1.z;
-  constexpr int64_t kStep = 256 * G::U;
+  constexpr int64_t kStep = TH * G::U;
   int64_t i = from + (int64_t)threadIdx.x * G::U;
   if (g == 0.0f || (a_s == 0.0f && a_h == 0.0f)) {
     const float v[G::U] = {};
@@ -414,7 +427,7 @@ distill_bwd_kernel(Distill a, const float* kept, const float* upstream, int per_
   }
   Form form;
   const Slope slope = slope_of(a, k0.x, k0.y, k0.z, g * a_s, g * a_h, form);
-  for (int j = threadIdx.x; j < a.K; j += 256) {
+  for (int j = threadIdx.x; j < a.K; j += TH) {
     float t;
     const int e = a_s != 0.0f ? entry(a, n, j, t) : -1;
     id[j] = e;
@@ -443,7 +456,7 @@ distill_bwd_kernel(Distill a, const float* kept, const float* upstream, int per_
     }
     for (; i < to; ++i) out[i] = G::round(slope.at<FORM>(tab_get<DT>(row[i])));
     written();
-    name_tokens<DT, FORM>(row, out, a.K, id, share, 1.0f, from, to, slope, threadIdx.x, 256);
+    name_tokens<DT, FORM>(row, out, a.K, id, share, 1.0f, from, to, slope, threadIdx.x, TH);
   });
 }
 
@@ -454,9 +467,10 @@ distill_both_kernel(Distill a, const int* counts, float scale, float* loss, void
   using G = Group<DT>;
   using T = typename TabType<DT>::t;
   constexpr int U = G::U, kHeld = NV * TH * U;
-  __shared__ int id[kMaxEntries + 1];
-  __shared__ float share[kMaxEntries + 1];
-  __shared__ float lq[kMaxEntries], part[2][TH / 64];
+  const Entries entries(a.K);
+  int* id = entries.id;
+  float *share = entries.share, *lq = entries.log;
+  __shared__ float part[2][TH / 64];
   __shared__ int ipart[TH / 64];
   __shared__ Teacher told;
   const int64_t n = block_id();
@@ -628,6 +642,12 @@ void sum_rows(const float* rows, const float* kept, const int* counts, int64_t N
 // Parts of a row: one where there are rows for every compute unit, else as many as fill them, of 2048 values at least.
 int64_t parts_of(int64_t N, int64_t V) { return N >= kParts / 2 ? 1 : std::max<int64_t>(1, std::min<int64_t>(kParts / N, V / 2048)); }
 
+int entry_bytes(const Distill& a) { return (3 * a.K + 2) * 4; }
+// A wave a row of few values: with 256 threads the loss of 65536 x 49 fp32 takes 117 us instead of 47, of 65536 x 2000
+// 155 instead of 111, the gradient of 65536 x 1000 143 instead of 107, but of 65536 x 2000 199 where one wave takes 218.
+bool loss_by_wave(const Distill& a) { return a.V <= 2048; }
+bool grad_by_wave(const Distill& a) { return a.V <= 1024; }
+
 }  // namespace
 
 extern "C" {
@@ -652,9 +672,15 @@ int slg_distill_fwd(const void* logits, int32_t dtype, int64_t N, int64_t V, int
     const int64_t parts = parts_of(N, V), per = cdiv(cdiv(V, parts), 8) * 8;
     by_form(a, dtype, [&](auto dt, auto form) {
       constexpr int DT = decltype(dt)::value;
-      hipLaunchKernelGGL((distill_fwd_kernel<DT, decltype(form)::value>), grid_of(N * parts), dim3(256), 0, st, a, (int)parts,
-                         per, k.parts, rows, k.rows);
-      if (parts > 1) hipLaunchKernelGGL(distill_join_kernel<DT>, dim3((unsigned)N), dim3(64), 0, st, a, (int)parts, k.parts, rows, k.rows);
+      constexpr Form FORM = decltype(form)::value;
+      const int lds = entry_bytes(a);
+      if (parts == 1 && loss_by_wave(a))
+        hipLaunchKernelGGL((distill_fwd_kernel<DT, 64, FORM>), grid_of(N), dim3(64), lds, st, a, 1, per, k.parts, rows, k.rows);
+      else
+        hipLaunchKernelGGL((distill_fwd_kernel<DT, 256, FORM>), grid_of(N * parts), dim3(256), lds, st, a, (int)parts, per, k.parts, rows,
+                           k.rows);
+      if (parts > 1)
+        hipLaunchKernelGGL(distill_join_kernel<DT>, dim3((unsigned)N), dim3(64), lds, st, a, (int)parts, k.parts, rows, k.rows);
     });
   }
   if (reduction)
@@ -675,9 +701,13 @@ int slg_distill_bwd(const void* logits, int32_t dtype, int64_t N, int64_t V, int
   // whole rows where there are enough of them, else chunks that make 2048 workgroups, of 2048 values at least
   const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>(cdiv(2048, N), V / 2048)), chunk = cdiv(cdiv(V, chunks), 8) * 8;
   by_type(dtype, [&](auto dt) {
-    hipLaunchKernelGGL((distill_bwd_kernel<decltype(dt)::value>), grid_of(N * chunks), dim3(256), 0, as_stream(stream), a,
-                       kept, upstream, reduction == 0, reduction ? layout(const_cast<float*>(kept), N).factor : nullptr, scale, chunk,
-                       (int)chunks, grad);
+    constexpr int DT = decltype(dt)::value;
+    const auto go = [&](auto kern, int th) {
+      hipLaunchKernelGGL(kern, grid_of(N * chunks), dim3(th), entry_bytes(a), as_stream(stream), a, kept, upstream, reduction == 0,
+                         reduction ? layout(const_cast<float*>(kept), N).factor : nullptr, scale, chunk, (int)chunks, grad);
+    };
+    if (grad_by_wave(a)) go(distill_bwd_kernel<DT, 64>, 64);
+    else go(distill_bwd_kernel<DT, 256>, 256);
   });
   SLG_LAUNCH_CHECK("distill_bwd");
   return 0;
@@ -707,7 +737,7 @@ int slg_distill_loss_grad(const void* logits, int32_t dtype, int64_t N, int64_t 
   by_form(a, dtype, [&](auto dt, auto form) {
     constexpr int DT = decltype(dt)::value, U = Group<DT>::U;
     constexpr Form FORM = decltype(form)::value;
-    const auto go = [&](auto kern, int th) { hipLaunchKernelGGL(kern, grid_of(N), dim3(th), 0, st, a, counts, scale, rows, grad); };
+    const auto go = [&](auto kern, int th) { hipLaunchKernelGGL(kern, grid_of(N), dim3(th), entry_bytes(a), st, a, counts, scale, rows, grad); };
     if (V <= 64 * 4 * U) go(distill_both_kernel<DT, 64, 4, FORM>, 64);
     else if (V <= 256 * 4 * U) go(distill_both_kernel<DT, 256, 4, FORM>, 256);
     else if (DT != kTabF32 || V <= 512 * 8 * U) go(distill_both_kernel<DT, 512, 8, FORM>, 512);
