@@ -3,7 +3,8 @@
 // the same in all threads comes back in scalar registers.
 //
 // Lanes exchange by DPP moves and swizzles, whose pattern is in the instruction: a shuffle by a lane's number takes
-// four more instructions for the address and goes through LDS (64 largest of 4096 rows of 32000: 73 us with those).
+// four more instructions for the address and goes through LDS (64 largest of 4096 rows of 32000 bf16: 73 us with those,
+// 53 without).
 #pragma once
 
 #include "slg_common.h"

@@ -10,9 +10,10 @@
 //
 // Both softmaxes share their maximum m: what is kept of a row is m, 1/Z and 1/Z1 (and the teacher's own), so that a
 // probability is exp((s - m) / T) / Z with the difference exact where it matters. Sums are fp32, those over rows 64
-// bits; the gradient is rounded once. All kernels are bound by the logits' bytes: one pass for the loss (the running
-// maximum and sums of each thread joined at the end), another with the write for the gradient. Both from one call
-// hold the row in registers between them.
+// bits; the gradient is rounded once. With long rows all kernels are bound by the logits' bytes: one pass for the loss
+// (the running maximum and sums of each thread joined at the end), another with the write for the gradient. Both from
+// one call hold the row in registers between them. Times below are of 4096 x 32000 and 64 entries, on a card whose
+// copies reach 5.0 to 5.4 TB/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -162,15 +163,46 @@ __device__ __forceinline__ Sums block_sums(Sums v, float c, Sums* part) {
   return v;
 }
 
-// A row's entries in LDS, sized by K: their tokens and their shares, and behind them the label's, and their logs.
+// A row's entries in LDS, sized by K: their tokens, shares and the shares' logs, and for the gradient a table of the
+// tokens that are named: open addressing, at most half full. Of a token's entries the first one writes its gradient.
+// (Each entry compared with each other: 256 entries of 8192 x 500 bf16 took 167 us with the loss, 195 by itself, where
+// the table takes 36 and 20; at one entry both take the same.)
 struct Entries {
+  static constexpr int kNone = 0x7fffffff;   // no token
+  int K, mask;
   int* id;
   float *share, *log;
-  __device__ __forceinline__ explicit Entries(int K) {
+  int *slot, *key, *first;   // of an entry, or -1; of a slot: its token, negative (by 2^31) if several entries name it
+  __device__ __forceinline__ Entries(int k, int slots) : K(k), mask(slots - 1) {
     extern __shared__ float entries[];
     id = reinterpret_cast<int*>(entries);
-    share = entries + K + 1;
-    log = share + K + 1;
+    share = entries + K;
+    log = share + K;
+    slot = reinterpret_cast<int*>(log + K);
+    key = slot + K;
+    first = key + slots;
+  }
+  // By `threads` threads, of which this is the `own`th; then a barrier, where it is not one wave.
+  __device__ __forceinline__ void clear(int own, int threads) const {
+    for (int i = own; i <= mask; i += threads) key[i] = kNone, first[i] = kNone;
+  }
+  __device__ __forceinline__ int place(int token) const { return (int)((uint32_t)token * 0x9e3779b1u >> 7) & mask; }
+  // Entry j names `token` (-1: none). At the next barrier the table knows.
+  __device__ __forceinline__ void name(int j, int token) const {
+    int at = token < 0 ? -1 : place(token);
+    if (token >= 0) {
+      for (;; at = (at + 1) & mask) {
+        const int was = atomicCAS(&key[at], kNone, token);
+        if (was == kNone || (was & kNone) == token) break;
+      }
+      if (atomicMin(&first[at], j) != kNone) atomicOr(&key[at], ~kNone);
+    }
+    slot[j] = at;
+  }
+  __device__ __forceinline__ bool named(int token) const {
+    for (int at = place(token); key[at] != kNone; at = (at + 1) & mask)
+      if ((key[at] & kNone) == token) return true;
+    return false;
   }
 };
 
@@ -232,11 +264,13 @@ __device__ __forceinline__ void finish_row(const Distill& a, int64_t n, const Su
   }
 }
 
-// The loss of a row, a workgroup each; with parts > 1 the sums of a part of a row, joined by the next kernel.
+// The loss of a row, a workgroup each; with parts > 1 the sums of a part of a row, joined by the next kernel. 100 to 108
+// us in fp32, 4.9 to 5.2 TB/s: memory; the vector instructions take about a third of their issue. Of 16 x 131071
+// fp16 logits in 63 parts 4.8 us, and 4.1 for the join: latency.
 template <int DT, int TH, Form FORM>
 __global__ void __launch_bounds__(TH) distill_fwd_kernel(Distill a, int parts, int64_t per, Sums* part_sums, float* loss, float* kept) {
   __shared__ Sums part[TH / 64];
-  const Entries e(a.K);
+  const Entries e(a.K, 1);
   const uint32_t b = block_id();
   const int64_t n = b / (uint32_t)parts, p = b % (uint32_t)parts;
   if (n >= a.N) return;
@@ -255,7 +289,7 @@ __global__ void __launch_bounds__(TH) distill_fwd_kernel(Distill a, int parts, i
 }
 template <int DT>
 __global__ void __launch_bounds__(64) distill_join_kernel(Distill a, int parts, const Sums* part_sums, float* loss, float* kept) {
-  const Entries e(a.K);
+  const Entries e(a.K, 1);
   const int64_t n = blockIdx.x;
   const float c = a.inv_t * kLog2e;
   Sums s{-INFINITY, 0.0f, 0.0f};
@@ -373,39 +407,35 @@ __device__ __forceinline__ void written() {
   __syncthreads();
 }
 
-// The tokens of [from, to) that entries name, written again with their shares taken off, each by the first entry that
-// names it; by `threads` threads, of which this is the `own`th. weight * share[j] of entries 0..K-1, share[K] of the
-// label.
+// The tokens of [from, to) that entries or the label name, written again with their shares taken off; by `threads`
+// threads, of which this is the `own`th. weight * share of an entry, label_share of the label (-1: none).
 template <int DT, Form FORM>
-__device__ __forceinline__ void name_tokens(const typename TabType<DT>::t* row, typename TabType<DT>::t* out, int K, const int* id,
-                                            const float* share, float weight, int64_t from, int64_t to, const Slope& slope, int own,
+__device__ __forceinline__ void name_tokens(const typename TabType<DT>::t* row, typename TabType<DT>::t* out, const Entries& e, float weight,
+                                            int label, float label_share, int64_t from, int64_t to, const Slope& slope, int own,
                                             int threads) {
-  for (int j = own; j <= K; j += threads) {
-    const int i = id[j];
-    if (i < from || i >= to) continue;
-    float q = 0.0f;
-    bool first = true;
-#pragma unroll 8
-    for (int o = 0; o < K; ++o) {   // no branch: the reads are in flight together
-      const bool same = id[o] == i;
-      first &= !same || o >= j;
-      q += same ? weight * share[o] : 0.0f;
-    }
-    if (id[K] == i) q += share[K];
-    if (first) out[i] = Group<DT>::round(slope.at<FORM>(tab_get<DT>(row[i])) - q);
+  const auto write = [&](int i, float q) { out[i] = Group<DT>::round(slope.at<FORM>(tab_get<DT>(row[i])) - q); };
+  for (int j = own; j < e.K; j += threads) {
+    const int at = e.slot[j];
+    if (at < 0 || e.first[at] != j) continue;
+    const int i = e.key[at] & Entries::kNone;
+    float q = weight * e.share[j];
+    if (e.key[at] < 0)
+      for (int o = j + 1; o < e.K; ++o) q += e.slot[o] == at ? weight * e.share[o] : 0.0f;
+    write(i, i == label ? q + label_share : q);
   }
+  if (own == threads - 1 && label >= from && label < to && !e.named(label)) write(label, label_share);
 }
 
-// Gradient of `chunk` logits of a row: all of them from their probabilities, then those that are named.
+// Gradient of `chunk` logits of a row: all of them from their probabilities, then those that are named. 208 us in fp32,
+// 5.0 TB/s of reads and writes: memory. The second write of the few named tokens takes the place of a look at the
+// entries by every token.
 template <int DT, int TH>
 __global__ void __launch_bounds__(TH)
-distill_bwd_kernel(Distill a, const float* kept, const float* upstream, int per_row, const float* factor, float scale, int64_t chunk,
-                   int chunks, void* grad) {
+distill_bwd_kernel(Distill a, int slots, const float* kept, const float* upstream, int per_row, const float* factor, float scale,
+                   int64_t chunk, int chunks, void* grad) {
   using G = Group<DT>;
   using T = typename TabType<DT>::t;
-  const Entries entries(a.K);
-  int* id = entries.id;
-  float* share = entries.share;
+  const Entries e(a.K, slots);
   const uint32_t b = block_id();
   const int64_t n = b / (uint32_t)chunks, from = b % (uint32_t)chunks * chunk, to = min(a.V, from + chunk);
   if (n >= a.N) return;
@@ -427,13 +457,15 @@ distill_bwd_kernel(Distill a, const float* kept, const float* upstream, int per_
   }
   Form form;
   const Slope slope = slope_of(a, k0.x, k0.y, k0.z, g * a_s, g * a_h, form);
+  e.clear(threadIdx.x, TH);
+  __syncthreads();
   for (int j = threadIdx.x; j < a.K; j += TH) {
-    float t;
-    const int e = a_s != 0.0f ? entry(a, n, j, t) : -1;
-    id[j] = e;
-    share[j] = e < 0 ? 0.0f : g * a_s * expf((t - k0.w) * a.inv_t) * k1.x;
+    float t = -INFINITY;
+    const int token = a_s != 0.0f ? entry(a, n, j, t) : -1;
+    e.share[j] = g * a_s * expf((t - k0.w) * a.inv_t) * k1.x;
+    e.name(j, token >= from && token < to ? token : -1);
   }
-  if (threadIdx.x == 0) id[a.K] = a_h != 0.0f ? label_of(a, n) : -1, share[a.K] = g * a_h;
+  const int label = a_h != 0.0f ? label_of(a, n) : -1;
   by_row_form(form, [&](auto row_form) {
     constexpr Form FORM = decltype(row_form)::value;
     for (; i + 3 * kStep + G::U <= to; i += 4 * kStep) {
@@ -456,20 +488,21 @@ distill_bwd_kernel(Distill a, const float* kept, const float* upstream, int per_
     }
     for (; i < to; ++i) out[i] = G::round(slope.at<FORM>(tab_get<DT>(row[i])));
     written();
-    name_tokens<DT, FORM>(row, out, a.K, id, share, 1.0f, from, to, slope, threadIdx.x, TH);
+    name_tokens<DT, FORM>(row, out, e, 1.0f, label, g * a_h, from, to, slope, threadIdx.x, TH);
   });
 }
 
-// Loss and gradient of a row, a workgroup each, the row's first NV groups of each thread in registers between them.
+// Loss and gradient of a row, a workgroup each, the row's first NV groups of each thread in registers between them. In
+// bf16 with labels at T = 2 105 us, 5.0 TB/s: memory, with the vector instructions at some 75% of their issue (two
+// passes over the row, an exponential in each). With two workgroups a compute unit one row is read while another is
+// summed.
 template <int DT, int TH, int NV, Form FORM>
 __global__ void __launch_bounds__(TH, TH == 1024 ? 8 : 1)
-distill_both_kernel(Distill a, const int* counts, float scale, float* loss, void* grad) {
+distill_both_kernel(Distill a, int slots, const int* counts, float scale, float* loss, void* grad) {
   using G = Group<DT>;
   using T = typename TabType<DT>::t;
   constexpr int U = G::U, kHeld = NV * TH * U;
-  const Entries entries(a.K);
-  int* id = entries.id;
-  float *share = entries.share, *lq = entries.log;
+  const Entries e(a.K, slots);
   __shared__ float part[2][TH / 64];
   __shared__ int ipart[TH / 64];
   __shared__ Teacher told;
@@ -487,8 +520,10 @@ distill_both_kernel(Distill a, const int* counts, float scale, float* loss, void
   }
   const int y = label_of(a, n);
   if (threadIdx.x < 64) {
-    const Teacher t = teacher_of(a, n, id, share, lq);
+    e.clear(threadIdx.x, 64);
+    const Teacher t = teacher_of(a, n, e.id, e.share, e.log);
     if (threadIdx.x == 0) told = t;
+    for (int j = threadIdx.x; j < a.K; j += 64) e.name(j, e.id[j]);
   }
   // f(values, first token) of the thread's groups
   const auto each = [&](auto f) {
@@ -565,16 +600,12 @@ distill_both_kernel(Distill a, const int* counts, float scale, float* loss, void
       rest([&](float x, int i) { out[i] = G::round(slope.at<decltype(row_form)::value>(x)); });
     });
   }
-  if (threadIdx.x == 0) {
-    id[a.K] = hard ? y : -1;
-    share[a.K] = scale * a_h;
-  }
   written();
   // the first wave sums the loss while the others write the tokens that are named
-  if (threadIdx.x < 64) finish_row<DT>(a, n, Sums{m, z, z1}, t, id, share, lq, loss, nullptr);
+  if (threadIdx.x < 64) finish_row<DT>(a, n, Sums{m, z, z1}, t, e.id, e.share, e.log, loss, nullptr);
   if (!dead && (TH == 64 || threadIdx.x >= 64))
     by_form_here([&](auto row_form) {
-      name_tokens<DT, decltype(row_form)::value>(row, out, a.K, id, share, scale * a_s / t.total, 0, V, slope,
+      name_tokens<DT, decltype(row_form)::value>(row, out, e, scale * a_s / t.total, hard ? y : -1, scale * a_h, 0, V, slope,
                                                  TH == 64 ? threadIdx.x : threadIdx.x - 64, TH == 64 ? 64 : TH - 64);
     });
 }
@@ -642,7 +673,13 @@ void sum_rows(const float* rows, const float* kept, const int* counts, int64_t N
 // Parts of a row: one where there are rows for every compute unit, else as many as fill them, of 2048 values at least.
 int64_t parts_of(int64_t N, int64_t V) { return N >= kParts / 2 ? 1 : std::max<int64_t>(1, std::min<int64_t>(kParts / N, V / 2048)); }
 
-int entry_bytes(const Distill& a) { return (3 * a.K + 2) * 4; }
+// Slots for the tokens that K entries name, and LDS of the entries with them (0: without).
+int slots_of(const Distill& a) {
+  int s = 2;
+  while (s < 2 * a.K) s *= 2;
+  return s;
+}
+int entry_bytes(const Distill& a, int slots) { return (slots ? 4 * a.K + 2 * slots : 3 * a.K) * 4; }
 // A wave a row of few values: with 256 threads the loss of 65536 x 49 fp32 takes 117 us instead of 47, of 65536 x 2000
 // 155 instead of 111, the gradient of 65536 x 1000 143 instead of 107, but of 65536 x 2000 199 where one wave takes 218.
 bool loss_by_wave(const Distill& a) { return a.V <= 2048; }
@@ -673,7 +710,7 @@ int slg_distill_fwd(const void* logits, int32_t dtype, int64_t N, int64_t V, int
     by_form(a, dtype, [&](auto dt, auto form) {
       constexpr int DT = decltype(dt)::value;
       constexpr Form FORM = decltype(form)::value;
-      const int lds = entry_bytes(a);
+      const int lds = entry_bytes(a, 0);
       if (parts == 1 && loss_by_wave(a))
         hipLaunchKernelGGL((distill_fwd_kernel<DT, 64, FORM>), grid_of(N), dim3(64), lds, st, a, 1, per, k.parts, rows, k.rows);
       else
@@ -700,10 +737,11 @@ int slg_distill_bwd(const void* logits, int32_t dtype, int64_t N, int64_t V, int
   if (N == 0) return 0;
   // whole rows where there are enough of them, else chunks that make 2048 workgroups, of 2048 values at least
   const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>(cdiv(2048, N), V / 2048)), chunk = cdiv(cdiv(V, chunks), 8) * 8;
+  const int slots = slots_of(a);
   by_type(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const auto go = [&](auto kern, int th) {
-      hipLaunchKernelGGL(kern, grid_of(N * chunks), dim3(th), entry_bytes(a), as_stream(stream), a, kept, upstream, reduction == 0,
+      hipLaunchKernelGGL(kern, grid_of(N * chunks), dim3(th), entry_bytes(a, slots), as_stream(stream), a, slots, kept, upstream, reduction == 0,
                          reduction ? layout(const_cast<float*>(kept), N).factor : nullptr, scale, chunk, (int)chunks, grad);
     };
     if (grad_by_wave(a)) go(distill_bwd_kernel<DT, 64>, 64);
@@ -733,11 +771,12 @@ int slg_distill_loss_grad(const void* logits, int32_t dtype, int64_t N, int64_t 
   const Kept k = layout(kept, N);
   float* rows = reduction ? k.loss : loss;
   int* counts = reduction == 2 ? k.counts : nullptr;
+  const int slots = slots_of(a);
   if (counts) hipLaunchKernelGGL(distill_count_kernel, dim3(kCounts), dim3(256), 0, st, a, counts);
   by_form(a, dtype, [&](auto dt, auto form) {
     constexpr int DT = decltype(dt)::value, U = Group<DT>::U;
     constexpr Form FORM = decltype(form)::value;
-    const auto go = [&](auto kern, int th) { hipLaunchKernelGGL(kern, grid_of(N), dim3(th), entry_bytes(a), st, a, counts, scale, rows, grad); };
+    const auto go = [&](auto kern, int th) { hipLaunchKernelGGL(kern, grid_of(N), dim3(th), entry_bytes(a, slots), st, a, slots, counts, scale, rows, grad); };
     if (V <= 64 * 4 * U) go(distill_both_kernel<DT, 64, 4, FORM>, 64);
     else if (V <= 256 * 4 * U) go(distill_both_kernel<DT, 256, 4, FORM>, 256);
     else if (DT != kTabF32 || V <= 512 * 8 * U) go(distill_both_kernel<DT, 512, 8, FORM>, 512);

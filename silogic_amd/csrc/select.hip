@@ -452,6 +452,9 @@ struct Row {
   }
 };
 
+// The K largest of a row, a workgroup each. 64 of 4096 x 32000 bf16: 52 us, 5.0 TB/s, where 512 threads hold the row in
+// 64 registers each and two passes look at it (lanes' maxima, then what is past the threshold, some 190 tokens): memory,
+// with the vector instructions at 80% of their issue. 100 of 33 x 131071 fp32: 17 to 19 us, on 33 compute units.
 template <int DT, int TH, int NV>
 __global__ void __launch_bounds__(TH)
 top_logits_kernel(const typename TabType<DT>::t* logits, int64_t N, int64_t ld, int V, int K, typename TabType<DT>::t* values,
@@ -496,6 +499,12 @@ __device__ inline uint64_t target_of(float u, uint64_t total) {
   return t < total ? t : total - 1;
 }
 
+// A token of a row, a workgroup each. 4096 x 32000 fp32: 110 us by min_p, 126 by the first 50, 203 without a limit and 233
+// by top_p, where each token's mass (24 vector instructions, most in 64 bits) and its place in a histogram (an LDS
+// atomic of 64 bits, 15 cycles a wave) are what bounds it: vector instructions 73% of their issue. Half of such a row
+// fits the registers at two workgroups a compute unit; a form of 1024 threads or 16 groups a thread, which hold all of it
+// with one, was slower, as was one of 256 threads for short lists (64 rows of 32000: 28 us instead of 21). Masses of 32
+// bits for the histogram, with exact ones where a border is near, came to 185 us without a limit but 252 by top_p.
 template <int DT, int TH, int NV>
 __global__ void __launch_bounds__(TH, 4)
 sample_kernel(const typename TabType<DT>::t* logits, int64_t N, int64_t ld, int V, const uint8_t* allowed, int64_t allowed_ld,

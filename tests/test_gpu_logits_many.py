@@ -1,8 +1,9 @@
-"""The operators on logits with more rows than one dimension of a launch takes (2^32 threads), and sums over many
-rows."""
+"""The operators on logits with more rows than one dimension of a launch takes (2^32 threads), sums over many rows, and
+many entries of a row that name few tokens."""
 import pytest
 import torch
 
+import logits_oracle as orc
 import silogic_amd as sl
 
 pytestmark = pytest.mark.gpu
@@ -68,6 +69,7 @@ def test_means_over_many_rows_count_the_rows(N, first):
     count = int((some | (labels == 3)).sum())
     loss = sl.distill_loss(x, values, ids, labels, alpha=0.5)
     loss.backward()
+    loss = loss.detach()
     terms = (some.double() + (labels == 3).double()).sum().item() * 0.5
     want = terms * 2.0794415416798357 / count
     # log 8 takes the logarithm of an exact sum (2 units of 2^-24), its half is exact, a row adds two, the mean one
@@ -79,3 +81,29 @@ def test_means_over_many_rows_count_the_rows(N, first):
     for got in (x.grad, grad):
         # 1/8 is exact; the share 1 / count and its products round three times, the two tokens' sums once each
         assert bool(((got.double().abs().sum(1) - rows).abs() <= 8 * 2.0 ** -24 * rows).all())
+
+
+@pytest.mark.parametrize("K", [1, 2, 3, 16, 33, 64, 255, 256, 1000, 1024])
+@pytest.mark.parametrize("N,V", [(3, 2000), (600, 90), (600, 1500), (520, 5003), (2, 9000)])
+def test_entries_that_name_the_same_tokens(N, V, K):
+    """Tokens named by many entries, by all of them, by two far apart, some by the label too: each has the sum of its
+    entries' probabilities. Ids are int32 for odd K."""
+    g = torch.Generator(device=DEV).manual_seed(K)
+    x = 2 * torch.randn(N, V, device=DEV, generator=g)
+    values = torch.randn(N, K, device=DEV, generator=g)
+    few = torch.randint(0, V, (N, 1), device=DEV, generator=g)
+    ids = torch.randint(0, V, (N, K), device=DEV, generator=g)
+    ids[::4] = (few + 7 * torch.randint(0, 5, (N, K), device=DEV, generator=g))[::4] % V   # of five tokens
+    ids[1::4] = few[1::4]                                                                   # of one
+    ids[2::4, -1] = ids[2::4, 0]
+    ids[:, K // 2] = torch.where(torch.rand(N, device=DEV, generator=g) < 0.3, -1, ids[:, K // 2])
+    labels = torch.where(torch.rand(N, device=DEV, generator=g) < 0.5, ids[:, 0], few[:, 0])
+    if K % 2:
+        ids = ids.int()
+    for lab in (None, labels):
+        want = orc.distill(x, values, ids, lab, 2.0, 0.5, "sum")
+        orc.check_distill(*sl.distill_loss_and_grad(x, values, ids, lab, temperature=2.0, reduction="sum"), want)
+        xg = x.clone().requires_grad_()
+        loss = sl.distill_loss(xg, values, ids, lab, temperature=2.0, reduction="sum")
+        loss.backward()
+        orc.check_distill(loss.detach(), xg.grad, want)
