@@ -42,7 +42,7 @@ __device__ inline float value_of(uint32_t key) {
 // Bins of a histogram: enough that a long row's fullest bin seldom holds more tokens than threads, few enough to
 // clear and scan.
 template <int TH>
-constexpr int kBins = TH == 64 ? 256 : TH == 256 ? 1024 : 2048;
+constexpr int kBins = TH <= 256 ? 4 * TH : 2048;
 
 template <int TH>
 struct SelectLds {
@@ -610,10 +610,10 @@ using namespace slg;
 
 namespace {
 
-// f with the type, the threads and the groups of 16 bytes a thread of a row of V logits. Listing up to k tokens takes
+// f with the type, the threads and the groups of 16 bytes a thread of N rows of V logits. Listing up to k tokens takes
 // as many threads.
 template <bool LIST, class F>
-void dispatch(int dtype, int64_t V, int64_t k, F f) {
+void dispatch(int dtype, int64_t N, int64_t V, int64_t k, F f) {
   using std::integral_constant;
   const auto by_size = [&](auto dt) {
     constexpr int VU = 16 / (int)sizeof(typename TabType<decltype(dt)::value>::t);
@@ -621,16 +621,23 @@ void dispatch(int dtype, int64_t V, int64_t k, F f) {
     const int64_t groups = cdiv(V, VU);
     // a row that fills no group is read token by token
     if (V < VU) return go(integral_constant<int, 64>{}, integral_constant<int, 0>{});
+    // as few threads as hold the row: more rows are under way side by side, and their barriers are of fewer waves (8192
+    // rows of 2000 fp32 by top_p take 42 us with 128 threads, 69 with 512; of 8000 106 with 256, 170 with 512); but about
+    // three times k tokens reach a list's threshold, and 40 of 64 rows of 2000 take 12 us with 128 threads, 27 with 64
     if (groups <= 128 && k <= 24) return go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-    if (groups <= 1024 && k <= 96) return go(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    if (groups <= 256 && k <= 48) return go(integral_constant<int, 128>{}, integral_constant<int, 2>{});
+    if (groups <= 512 && k <= 48) return go(integral_constant<int, 128>{}, integral_constant<int, 4>{});
+    if (groups <= 1024 && k <= 48) return go(integral_constant<int, 128>{}, integral_constant<int, 8>{});
+    if (groups <= 2048 && k <= 96) return go(integral_constant<int, 256>{}, integral_constant<int, 8>{});
     if constexpr (LIST) {
-      // about three times k tokens reach the threshold
-      if (groups <= 4096 && k <= 160) go(integral_constant<int, 512>{}, integral_constant<int, 8>{});
-      else if (groups <= 4096) go(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
-      else go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
+      if (groups <= 4096 && k <= 160) return go(integral_constant<int, 512>{}, integral_constant<int, 8>{});
+      if (groups <= 4096) return go(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
+      go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
     } else {
-      if (groups <= 2048) go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
-      else go(integral_constant<int, 512>{}, integral_constant<int, 8>{});
+      // a compute unit holds one workgroup of 1024 threads, or two of 512: fp32 by top_p, 64 rows of 130000 take 48 us with
+      // the former and 60 with the latter, 300 of 50257 61 and 51, 4096 of 32000 307 and 214
+      if (groups > 4096 && N <= 256) return go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
+      go(integral_constant<int, 512>{}, integral_constant<int, 8>{});
     }
   };
   if (dtype == kTabF32) by_size(integral_constant<int, kTabF32>{});
@@ -651,7 +658,7 @@ int slg_top_logits(const void* logits, int32_t dtype, int64_t N, int64_t V, int6
   SLG_REQUIRE(sizes(N, V, ld) && K >= 1 && K <= V && K <= kMaxTop, SLG_E_SHAPE, "top_logits: N %lld, V %lld, K %lld", (long long)N,
               (long long)V, (long long)K);
   if (N == 0) return 0;
-  dispatch<true>(dtype, V, K, [&](auto dt, auto th, auto nv) {
+  dispatch<true>(dtype, N, V, K, [&](auto dt, auto th, auto nv) {
     using T = typename TabType<decltype(dt)::value>::t;
     hipLaunchKernelGGL((top_logits_kernel<decltype(dt)::value, decltype(th)::value, decltype(nv)::value>), grid_of(N), dim3(decltype(th)::value), 0,
                        as_stream(stream), static_cast<const T*>(logits), N, ld, (int)V, (int)K, static_cast<T*>(values), ids);
@@ -672,7 +679,7 @@ int slg_sample_logits(const void* logits, int32_t dtype, int64_t N, int64_t V, i
   SLG_REQUIRE(min_ps || (min_p >= 0.0 && min_p <= 1.0), SLG_E_ARG, "sample_logits: min_p %g outside [0, 1]", min_p);
   if (N == 0) return 0;
   const Limits lim{temperature, top_p, min_p, top_k, temperatures, top_ps, min_ps, top_ks};
-  dispatch<false>(dtype, V, 1, [&](auto dt, auto th, auto nv) {
+  dispatch<false>(dtype, N, V, 1, [&](auto dt, auto th, auto nv) {
     using T = typename TabType<decltype(dt)::value>::t;
     hipLaunchKernelGGL((sample_kernel<decltype(dt)::value, decltype(th)::value, decltype(nv)::value>), grid_of(N), dim3(decltype(th)::value), 0,
                        as_stream(stream), static_cast<const T*>(logits), N, ld, (int)V, allowed, allowed_ld, u, lim, ids);
