@@ -26,7 +26,9 @@ constexpr float kLog2e = 1.44269504f;
 constexpr int kMaxEntries = 1024;
 constexpr int kKept = 8;      // floats kept of a row: m, 1/Z, 1/Z1, the teacher's maximum and 1/sum, a_s T, a_h, counted
 constexpr int kCounts = 256;  // workgroups that count the rows of a mean
-constexpr int kManyRows = 16384;  // more rows than these are summed by kCounts workgroups before the last one
+// More rows than these are summed by kCounts workgroups before the last one: the loss of 32768 x 49 took 62 us so, 74
+// without, of 16384 x 49 41 both ways.
+constexpr int kManyRows = 16384;
 constexpr int kParts = 1024;  // parts of rows that the loss's first pass is cut into where there are fewer rows
 
 struct Distill {

@@ -1,5 +1,7 @@
 """The operators on logits with more rows than one dimension of a launch takes (2^32 threads), sums over many rows, and
 many entries of a row that name few tokens."""
+import threading
+
 import pytest
 import torch
 
@@ -107,3 +109,63 @@ def test_entries_that_name_the_same_tokens(N, V, K):
         loss = sl.distill_loss(xg, values, ids, lab, temperature=2.0, reduction="sum")
         loss.backward()
         orc.check_distill(loss.detach(), xg.grad, want)
+
+
+@pytest.mark.parametrize("groups", [128, 256, 512, 1024, 2048, 4096])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_rows_at_the_sizes_where_threads_change(groups, dtype):
+    """Rows that fill a form's registers, and one logit more or less: listed and drawn as the definitions do, and the same
+    among many rows, which other forms may take."""
+    unit = 16 // torch.tensor([], dtype=dtype).element_size()
+    g = torch.Generator(device=DEV).manual_seed(groups)
+    for V in (groups * unit - 1, groups * unit, groups * unit + 1):
+        x = (3 * torch.randn(300, V, device=DEV, generator=g)).to(dtype)
+        x[0] = x[0].round()
+        x[1, V // 3:] = -float("inf")
+        few = x[:8]
+        for k in (1, 24, 25, 48, 49, 96, 97, 160, 161):
+            values, ids = sl.top_logits(x, k)
+            v, i = orc.top(few, k)
+            assert torch.equal(values[:8].cpu().to(orc.F64), v) and torch.equal(ids[:8].cpu(), i), (V, k)
+        u = torch.rand(300, device=DEV, generator=g)
+        for limits in ((1.0, 0, 1.0, 0.0), (0.7, 40, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (1.3, 70, 0.8, 0.01), (1.0, 0, 1.0, 0.05),
+                       (1.0, 300, 0.95, 0.0)):
+            got = sl.sample_logits(few, u[:8], *limits)
+            assert torch.equal(got.cpu(), orc.sample(few, u[:8].cpu(), *limits)), (V, limits)
+            all_rows = sl.sample_logits(x, u, *limits)
+            parts = [sl.sample_logits(x[a:a + 60], u[a:a + 60], *limits) for a in range(0, 300, 60)]
+            assert torch.equal(all_rows, torch.cat(parts)) and torch.equal(all_rows[:8], got), (V, limits)
+
+
+def test_calls_of_two_threads_at_once():
+    """Two host threads, a stream each, call everything on inputs of their own; each has what one thread alone gets."""
+    def work(seed):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        out = []
+        for N, V in ((700, 300), (9, 40000), (600, 5000)):
+            x = torch.randn(N, V, device=DEV, generator=g)
+            values, ids = sl.top_logits(x, 20)
+            xg = x.flip(0).requires_grad_()
+            loss = sl.distill_loss(xg, values, ids, temperature=2.0)
+            loss.backward()
+            out += [values, ids, loss.detach(), xg.grad, *sl.distill_loss_and_grad(x, values, ids, ids[:, 0]),
+                    sl.sample_logits(x, torch.rand(N, device=DEV, generator=g), top_p=0.9)]
+        return out
+
+    def on_a_stream(seed, results):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            results[seed] = [work(seed) for _ in range(5)]
+        stream.synchronize()
+
+    alone, together = {}, {}
+    for seed in (1, 2):
+        on_a_stream(seed, alone)
+    threads = [threading.Thread(target=on_a_stream, args=(seed, together)) for seed in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for seed in (1, 2):
+        for got in together[seed]:
+            assert all(torch.equal(a, b) for a, b in zip(got, alone[seed][0]))
