@@ -15,15 +15,25 @@ def _shape(what, name, t, shape):
         raise ValueError(f"{what}: {name} {tuple(t.shape)}, {tuple(shape)} expected")
 
 
+def _plain(t):
+    return t.detach() if t.requires_grad else t
+
+
+def _flat(t, dtype):
+    t = _plain(t)
+    return ops._c(t if t.dim() == 1 else t.reshape(-1), dtype)
+
+
 def top_logits(logits, k):
     """The ``k`` largest logits of each row and their ids, ``(values, ids)`` ``[..., k]`` in the logits' type and
     int64: by value, equal values by the lower id. What a student keeps of its teacher (:func:`distill_loss`). A NaN
     or -inf is no token; past the tokens that are there values are -inf and ids -1. ``k`` is at most 1024, ``V``
     2^24. No gradient flows through it."""
-    rows = ops.check_logits("top_logits", logits.detach())
+    rows = ops.check_logits("top_logits", _plain(logits))
     if not 1 <= k <= min(rows.shape[1], 1024):
         raise ValueError(f"top_logits: {k} of {rows.shape[1]} logits (1 to 1024, and no more than there are)")
-    ops.require_gpu(rows)
+    if rows.get_device() < 0:
+        ops.require_gpu(rows)
     if torch.compiler.is_compiling():
         values, ids = torch.ops.silogic_hip.top_logits(rows, k)
     else:
@@ -39,9 +49,13 @@ def _limit(name, v, lead, dtype, least, most):
         if v.dtype.is_floating_point != dtype.is_floating_point or v.dtype in (torch.bool, torch.complex64, torch.complex128):
             raise TypeError(f"sample_logits: {name} of {v.dtype}")
         _shape("sample_logits", name, v, lead)
-        return ops._c(v.detach().reshape(-1), dtype)
+        return _flat(v, dtype)
     if not least <= v <= most:
         raise ValueError(f"sample_logits: {name} {v} outside [{least}, {most}]")
+    if not isinstance(v, int if dtype == torch.int64 else (int, float)):   # another library's number
+        if dtype == torch.int64 and v != int(v):
+            raise TypeError(f"sample_logits: {name} {v} is no whole number")
+        v = int(v) if dtype == torch.int64 else float(v)
     return v
 
 
@@ -59,14 +73,14 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
     Masses are held as whole numbers of 2^-F of the largest, F = min(50, 62 - bits of V), so that their sums are exact
     and the same draw comes from the same inputs on every call. A ``u`` outside [0, 1) acts as its nearest bound."""
     lead = logits.shape[:-1]
-    rows = ops.check_logits("sample_logits", logits.detach())
+    rows = ops.check_logits("sample_logits", _plain(logits))
     if rows.shape[1] > 1 << 24:
         raise ValueError(f"sample_logits: {rows.shape[1]} logits a row (at most 2^24)")
     if not u.dtype.is_floating_point:
         raise TypeError(f"sample_logits: u of {u.dtype}")
     _shape("sample_logits", "u", u, lead)
     f32 = torch.float32
-    u = ops._c(u.detach().reshape(-1), f32)
+    u = _flat(u, f32)
     t = _limit("temperature", temperature, lead, f32, 0.0, math.inf)
     k = _limit("top_k", top_k, lead, torch.int64, 0, (1 << 63) - 1)
     p = _limit("top_p", top_p, lead, f32, 0.0, 1.0)
@@ -74,15 +88,19 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
     if mask is not None:
         if mask.dtype != torch.bool:
             raise TypeError(f"sample_logits: mask of {mask.dtype} (bool)")
-        try:
-            mask = mask.expand(logits.shape)
-        except RuntimeError:
-            raise ValueError(f"sample_logits: mask {tuple(mask.shape)} for logits {tuple(logits.shape)}") from None
+        if mask.shape != logits.shape:
+            try:
+                mask = mask.expand(logits.shape)
+            except RuntimeError:
+                raise ValueError(f"sample_logits: mask {tuple(mask.shape)} for logits {tuple(logits.shape)}") from None
         mask = mask.reshape(-1, rows.shape[1]) if mask.dim() != 2 else mask
         mask = mask if mask.stride(1) == 1 or mask.shape[1] == 1 else mask.contiguous()
-    each = [v for v in (t, k, p, m) if isinstance(v, torch.Tensor)]
-    ops.require_gpu(rows, u, mask, *each)
-    ops.same_device("sample_logits", rows, u, mask, *each)
+    d = rows.get_device()
+    # all in order (the usual call), or the check that says what is not
+    if not (d >= 0 and all(v is None or v.get_device() == d for v in (u, mask, t, k, p, m) if not isinstance(v, (int, float)))):
+        each = [v for v in (t, k, p, m) if isinstance(v, torch.Tensor)]
+        ops.require_gpu(rows, u, mask, *each)
+        ops.same_device("sample_logits", rows, u, mask, *each)
     if torch.compiler.is_compiling():
         number = [0 if isinstance(v, torch.Tensor) else v for v in (t, k, p, m)]
         ids = torch.ops.silogic_hip.sample_logits(rows, u, *(kind(v) for kind, v in zip((float, int, float, float), number)),

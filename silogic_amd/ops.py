@@ -612,8 +612,10 @@ def sample_logits(logits, u, t, k, p, m, mask):
     None or bool ``[N, V]`` (``slg_sample_logits``)."""
     N, V = logits.shape
     ids = logits.new_empty((N,), dtype=torch.int64)
-    number = [0 if isinstance(v, torch.Tensor) else v for v in (t, k, p, m)]
-    each = [v.data_ptr() if isinstance(v, torch.Tensor) else None for v in (t, k, p, m)]
+    number, each = [t, k, p, m], [None] * 4
+    for i, v in enumerate(number):
+        if isinstance(v, torch.Tensor):
+            number[i], each[i] = 0, v.data_ptr()
     call_on(logits, "slg_sample_logits", logits.data_ptr(), TABLE_DTYPES[logits.dtype], N, V, logits.stride(0),
             None if mask is None else mask.data_ptr(), 0 if mask is None else mask.stride(0), u.data_ptr(),
             *number, *each, ids.data_ptr())

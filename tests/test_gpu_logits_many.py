@@ -2,6 +2,7 @@
 many entries of a row that name few tokens."""
 import threading
 
+import numpy as np
 import pytest
 import torch
 
@@ -169,3 +170,13 @@ def test_calls_of_two_threads_at_once():
     for seed in (1, 2):
         for got in together[seed]:
             assert all(torch.equal(a, b) for a, b in zip(got, alone[seed][0]))
+
+
+def test_limits_as_numbers_of_any_library():
+    x = torch.randn(5, 300, device=DEV)
+    u = torch.rand(5, device=DEV)
+    want = sl.sample_logits(x, u, temperature=2, top_k=40, top_p=0.5, min_p=0.25)
+    assert torch.equal(want.cpu(), orc.sample(x, u.cpu(), 2.0, 40, 0.5, 0.25))
+    for number in (np.float32, np.float64):
+        assert torch.equal(sl.sample_logits(x, u, number(2), np.int32(40), number(0.5), number(0.25)), want)
+    assert torch.equal(sl.sample_logits(x, u, np.int64(2), 40.0, 0.5, 0.25), want)

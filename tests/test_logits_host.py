@@ -2,6 +2,7 @@
 import ctypes as C
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -122,3 +123,13 @@ def test_the_scale_is_finite():
     for scale in (NAN, math.inf):
         with pytest.raises(ValueError):
             sl.distill_loss_and_grad(x, v, i, scale=scale)
+
+
+def test_limits_are_numbers_of_any_library():
+    """Those of numpy are taken as Python's are; a top_k that is no whole number is refused before anything runs."""
+    x, u = torch.randn(3, 20), torch.rand(3)
+    for limits in (dict(top_k=np.int64(4)), dict(top_k=4.0), dict(top_p=np.float32(0.5)), dict(temperature=np.int32(1))):
+        with pytest.raises(RuntimeError, match="GPU"):
+            sl.sample_logits(x, u, **limits)
+    with pytest.raises(TypeError, match="whole"):
+        sl.sample_logits(x, u, top_k=4.5)
