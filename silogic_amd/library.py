@@ -496,7 +496,7 @@ token_encode.register_autograd(_token_backward, setup_context=_token_setup)
 
 
 # ---------------------------------------------------------------------------
-# A network's logits: what torch.compile traces (rows [N, V] as ops takes them)
+# A network's logits: what torch.compile and other tracers see (rows [N, V] as ops takes them)
 # ---------------------------------------------------------------------------
 @torch.library.custom_op(f"{_NS}::top_logits", mutates_args=())
 def top_logits(logits: Tensor, k: int) -> Tuple[Tensor, Tensor]:
@@ -516,7 +516,8 @@ def sample_logits(logits: Tensor, u: Tensor, temperature: float, top_k: int, top
     from . import logits as lg
     limits = [v if each is None else each for v, each in
               ((temperature, temperatures), (top_k, top_ks), (top_p, top_ps), (min_p, min_ps))]
-    return lg.sample_logits(logits, u, *limits, mask)
+    rows, u, limits, mask = lg._sample(logits, u, *limits, mask)
+    return ops.sample_logits(rows, u, *limits, mask)
 
 
 @sample_logits.register_fake

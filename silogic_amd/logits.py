@@ -6,6 +6,7 @@ others first. Everything is computed in 32 bits or more."""
 import math
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import ops
 
@@ -29,12 +30,13 @@ def top_logits(logits, k):
     int64: by value, equal values by the lower id. What a student keeps of its teacher (:func:`distill_loss`). A NaN
     or -inf is no token; past the tokens that are there values are -inf and ids -1. ``k`` is at most 1024, ``V``
     2^24. No gradient flows through it."""
+    whole = ops.one_op("top_logits", logits)
     rows = ops.check_logits("top_logits", _plain(logits))
     if not 1 <= k <= min(rows.shape[1], 1024):
         raise ValueError(f"top_logits: {k} of {rows.shape[1]} logits (1 to 1024, and no more than there are)")
     if rows.get_device() < 0:
         ops.require_gpu(rows)
-    if torch.compiler.is_compiling():
+    if whole:
         values, ids = torch.ops.silogic_hip.top_logits(rows, k)
     else:
         values, ids = ops.top_logits(rows, k)
@@ -59,19 +61,8 @@ def _limit(name, v, lead, dtype, least, most):
     return v
 
 
-def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):
-    """A token id (int64) of each row of ``logits [..., V]`` from a random number ``u [...]`` in [0, 1).
-
-    Tokens are taken by value, equal values by the lower id, with masses ``exp((logit - largest) / temperature)``.
-    Kept are the first ``top_k`` (0: all); of these those before which lies less than ``top_p`` of their mass; of
-    these those with a mass of at least ``min_p`` times the largest. The token drawn is the first whose running sum
-    of kept masses passes ``u`` times their sum. ``temperature`` 0 takes the first token. Each limit is a number, or
-    a tensor ``[...]`` with one of each row (in fp32; there a temperature that is not over 0 takes the first
-    token, and limits out of their range act as their nearest bound). ``mask`` (bool, ``[V]`` to ``[..., V]``) is True for
-    tokens that are allowed. A NaN or -inf is no token; a row without one gives -1.
-
-    Masses are held as whole numbers of 2^-F of the largest, F = min(50, 62 - bits of V), so that their sums are exact
-    and the same draw comes from the same inputs on every call. A ``u`` outside [0, 1) acts as its nearest bound."""
+def _sample(logits, u, temperature, top_k, top_p, min_p, mask):
+    """The arguments as the kernel reads them."""
     lead = logits.shape[:-1]
     rows = ops.check_logits("sample_logits", _plain(logits))
     if rows.shape[1] > 1 << 24:
@@ -101,13 +92,31 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
         each = [v for v in (t, k, p, m) if isinstance(v, torch.Tensor)]
         ops.require_gpu(rows, u, mask, *each)
         ops.same_device("sample_logits", rows, u, mask, *each)
-    if torch.compiler.is_compiling():
-        number = [0 if isinstance(v, torch.Tensor) else v for v in (t, k, p, m)]
+    return rows, u, (t, k, p, m), mask
+
+
+def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):
+    """A token id (int64) of each row of ``logits [..., V]`` from a random number ``u [...]`` in [0, 1).
+
+    Tokens are taken by value, equal values by the lower id, with masses ``exp((logit - largest) / temperature)``.
+    Kept are the first ``top_k`` (0: all); of these those before which lies less than ``top_p`` of their mass; of
+    these those with a mass of at least ``min_p`` times the largest. The token drawn is the first whose running sum
+    of kept masses passes ``u`` times their sum. ``temperature`` 0 takes the first token. Each limit is a number, or
+    a tensor ``[...]`` with one of each row (in fp32; there a temperature that is not over 0 takes the first
+    token, and limits out of their range act as their nearest bound). ``mask`` (bool, ``[V]`` to ``[..., V]``) is True for
+    tokens that are allowed. A NaN or -inf is no token; a row without one gives -1.
+
+    Masses are held as whole numbers of 2^-F of the largest, F = min(50, 62 - bits of V), so that their sums are exact
+    and the same draw comes from the same inputs on every call. A ``u`` outside [0, 1) acts as its nearest bound."""
+    whole = ops.one_op("sample_logits", logits, u, temperature, top_k, top_p, min_p, mask)
+    rows, u, limits, mask = _sample(logits, u, temperature, top_k, top_p, min_p, mask)
+    if whole:
+        number = [0 if isinstance(v, torch.Tensor) else v for v in limits]
         ids = torch.ops.silogic_hip.sample_logits(rows, u, *(kind(v) for kind, v in zip((float, int, float, float), number)),
-                                                  *(v if isinstance(v, torch.Tensor) else None for v in (t, k, p, m)), mask)
+                                                  *(v if isinstance(v, torch.Tensor) else None for v in limits), mask)
     else:
-        ids = ops.sample_logits(rows, u, t, k, p, m, mask)
-    return ids if logits.dim() == 2 else ids.view(lead)
+        ids = ops.sample_logits(rows, u, *limits, mask)
+    return ids if logits.dim() == 2 else ids.view(logits.shape[:-1])
 
 
 def _distill(what, logits, values, ids, labels, temperature, alpha, reduction):
@@ -169,9 +178,12 @@ def distill_loss(logits, values, ids, labels=None, temperature=1.0, alpha=0.5, r
     themselves. An entry with an id outside 0..V-1 or a value of -inf is absent, so is a label outside 0..V-1. A term
     without an entry or a label counts 0, as does a row of -inf alone; ``mean`` is over the rows with an entry or a
     label. Losses are fp32; the logits' gradient is in their type, rounded once, and the same bits on every call. The
-    teacher gets no gradient, and there is no second derivative."""
+    teacher gets no gradient, and there is no second derivative, none in forward mode and no ``torch.func`` transform."""
+    whole = ops.one_op("distill_loss", logits, values, ids, labels)
+    if not torch.compiler.is_compiling() and forward_ad.unpack_dual(logits).tangent is not None:
+        raise NotImplementedError("distill_loss: no derivative in forward mode")
     args = _distill("distill_loss", logits, values, ids, labels, temperature, alpha, reduction)
-    if torch.compiler.is_compiling():
+    if whole:
         loss = torch.ops.silogic_hip.distill_loss(*args)[0]
     elif ops._grad_path(logits):
         loss = _DistillFn.apply(*args)
@@ -186,8 +198,9 @@ def distill_loss_and_grad(logits, values, ids, labels=None, temperature=1.0, alp
     batches that are accumulated). The logits are read once where a row fits a workgroup's registers."""
     if not math.isfinite(scale):
         raise ValueError(f"distill_loss_and_grad: scale {scale}")
+    whole = ops.one_op("distill_loss_and_grad", logits, values, ids, labels)
     args = _distill("distill_loss_and_grad", logits.detach(), values, ids, labels, temperature, alpha, reduction)
-    if torch.compiler.is_compiling():
+    if whole:
         loss, grad = torch.ops.silogic_hip.distill_loss_grad(*args, float(scale))
     else:
         loss, grad = ops.distill_loss_grad(*args, float(scale))
