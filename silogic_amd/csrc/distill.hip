@@ -29,6 +29,9 @@ constexpr int kCounts = 256;  // workgroups that count the rows of a mean
 // More rows than these are summed by kCounts workgroups before the last one: the loss of 32768 x 49 took 62 us so, 74
 // without, of 16384 x 49 41 both ways.
 constexpr int kManyRows = 16384;
+// Past this temperature a small soft loss is summed without cancellation (close_loss): the factor T^2 would bring the
+// roundings of the logarithms, some 2^-20, to the loss's own size at T = 1000. Up to it they come to 2^-16 at most.
+constexpr float kFarT = 4.0f;
 constexpr int kParts = 1024;  // parts of rows that the loss's first pass is cut into where there are fewer rows
 
 struct Distill {
@@ -237,6 +240,48 @@ __device__ __forceinline__ Teacher teacher_of(const Distill& a, int64_t n, int* 
   return {top, total, __ballot(any) != 0};
 }
 
+// e^r - 1 - r, which is not negative; by its series where the exponential's rounding would be left of it.
+__device__ __forceinline__ float past_tangent(float r) {
+  if (!(fabsf(r) < 0.5f)) return expf(r) - 1.0f - r;
+  float p = 1.0f / 362880.0f;
+  p = fmaf(p, r, 1.0f / 40320.0f);
+  p = fmaf(p, r, 1.0f / 5040.0f);
+  p = fmaf(p, r, 1.0f / 720.0f);
+  p = fmaf(p, r, 1.0f / 120.0f);
+  p = fmaf(p, r, 1.0f / 24.0f);
+  p = fmaf(p, r, 1.0f / 6.0f);
+  return r * r * fmaf(p, r, 0.5f);
+}
+
+// One wave: sum_j q_j (log q_j - log p[i_j]) where that is small beside its terms. With r_j = log(p[i_j] / q_j) it is
+//   sum_j q_j (e^(r_j) - 1 - r_j) + 1 - sum_j p[i_j]:
+// no term of the sum is negative, and the rest is what the tokens that no entry names have, here summed in 64 bits of
+// the same exponentials as the named ones' (0 where all are named once). An error of both softmaxes' sums then counts by
+// its square. False, and nothing, where the entries name half of p or less: the loss is log 2 at least, and its terms'
+// own roundings are small beside it.
+template <int DT>
+__device__ __forceinline__ bool close_loss(const Distill& a, const typename TabType<DT>::t* row, const Sums& s, float rtot, const int* id,
+                                           const float* q, const float* lq, float& loss) {
+  const int lane = threadIdx.x & 63;
+  const auto add = [](double x, double y) { return x + y; };
+  const auto mass = [&](int64_t i) { return (double)exp2_fast((tab_get<DT>(row[i]) - s.m) * (a.inv_t * kLog2e)); };
+  double named = 0.0, total = 0.0, all = 0.0;
+  for (int j = lane; j < a.K; j += 64)
+    if (q[j] != 0.0f) named += mass(id[j]), total += (double)q[j];
+  named = wave_reduce(named, add);
+  if (!(named > 0.5 * (double)s.z)) return false;
+  total = wave_reduce(total, add);
+  for (int64_t i = lane; i < a.V; i += 64) all += mass(i);
+  all = wave_reduce(all, add);
+  const float shift = (float)log(all / total);
+  float l = 0.0f;
+  for (int j = lane; j < a.K; j += 64)
+    if (q[j] != 0.0f) l += q[j] * rtot * past_tangent((tab_get<DT>(row[id[j]]) - s.m) * a.inv_t - lq[j] - shift);
+  l = wave_reduce(l, [](float x, float y) { return x + y; });
+  loss = l + (float)((all - named) / all);
+  return true;
+}
+
 // One wave: the row's loss from its sums, and what is kept of it.
 template <int DT>
 __device__ __forceinline__ void finish_row(const Distill& a, int64_t n, const Sums& s, const Teacher& t, const int* id, const float* q,
@@ -247,12 +292,13 @@ __device__ __forceinline__ void finish_row(const Distill& a, int64_t n, const Su
   const bool soft = t.some && alive, hard = y >= 0 && alive;
   const float rtot = 1.0f / t.total, logs = logf(s.z) - logf(t.total);
   float l = 0.0f;
-  if (soft)
+  if (soft && !(a.T > kFarT && close_loss<DT>(a, row, s, rtot, id, q, lq, l))) {
     for (int j = lane; j < a.K; j += 64) {
       const float e = q[j];
       if (e != 0.0f) l += e * rtot * (lq[j] - (tab_get<DT>(row[id[j]]) - s.m) * a.inv_t + logs);
     }
-  l = wave_reduce(l, [](float x, float y) { return x + y; });
+    l = wave_reduce(l, [](float x, float y) { return x + y; });
+  }
   const float share = a.labels ? 1.0f - a.alpha : 1.0f;
   if (lane == 0) {
     float v = soft ? share * a.T * a.T * l : 0.0f;
