@@ -5,10 +5,13 @@
 //
 // Drawing (temperature T, limits k, p and m, a random number u in [0, 1)): masses w = exp((s - max) / T), of which
 // the first k tokens stay, of these those before which lies less than p of their mass, of these those with w >= m;
-// drawn is the first whose running sum passes u times theirs. Masses are held as whole numbers of 2^-F, F = 62 -
-// log2 V and at most 50 (47 bits at 32000 tokens), from an exponential that is off by 2^-43 of itself: their sums are
-// exact, the same in any order, so LDS atomics may make them, and a border between two tokens is where 64-bit sums
-// have it up to about 2^-43 of the sum.
+// drawn is the first whose running sum passes u times theirs. Masses are held as whole numbers of 2^-F from an
+// exponential that is off by 2^-43 of itself, F at most 50 and such that the sum of a row stays under 2^63: 62 - log2 V
+// (47 at 32000 tokens), or from 2^18 tokens on 62 less the log of the row's own sum. Their sums are exact, the same in
+// any order, so LDS atomics may make them. A mass is off by half a 2^-F, V of them by V 2^-(F+1): a border between two
+// tokens is where sums without rounding have it up to 2^-33 of the sum at 32000 tokens and 2^-27 at most, an eighth of
+// the steps that u has near 1. (By V alone the 2^24 tokens of a row would be off by 2^-14: a flat tail of masses under
+// 2^-38 that hold 6e-5 together would come to 0.)
 //
 // A workgroup takes a row, in registers where it fits (the only read of it). What the limits keep is found by value
 // first: k tokens are at least as large as a threshold that k lanes' own maxima reach, min_p is a threshold by
@@ -227,6 +230,9 @@ struct Row {
     top64 = uniform((double)max);
     slope = uniform(fmax(fmin(1.4426950408889634 / t, 1e300), 1e-300));
     F = bits > 12 ? 62 - bits : 50;
+    if constexpr (NV == 8 && TH >= 512) {
+      if (bits > 18) F = bits_of_mass();
+    }
     shifter = uniform(0x1.8p52 + (double)F);
     lowest = uniform(-100.0 / slope);   // far enough down for a mass of 0
     // bins end where masses fall under 2^-(F+2), or where the row does
@@ -236,6 +242,19 @@ struct Row {
     const float scale = ((float)BINS - 1.0f) / range;
     bin_scale = uniform(fabsf(max) * scale < 4194304.0f ? scale : 0.0f);
     bin_base = uniform(max * bin_scale);
+  }
+  // F of a long row: by its sum in 32 bits, which chains of at most 2^16 additions leave within 2^-8 of itself.
+  __device__ __forceinline__ int bits_of_mass() const {
+    float sum = 0.0f;
+    each([&](const float (&x)[VU], int) {
+#pragma unroll
+      for (int u = 0; u < VU; ++u) {
+        const float z = (float)(fmax((double)x[u] - top64, -100.0 / slope) * slope);
+        sum += x[u] > -INFINITY ? __builtin_amdgcn_exp2f(z) : 0.0f;
+      }
+    });
+    sum = block_reduce<TH>(sum, reinterpret_cast<float*>(lds->part), [](float p, float q) { return p + q; });
+    return min(50, 62 - __builtin_amdgcn_frexp_expf(sum));   // the sum is 1 at least
   }
   // 2^F exp(d / T) to a whole number. The products are of single roundings in every place that this comes to: sums over
   // the same tokens have to be the same.
