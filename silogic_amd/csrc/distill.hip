@@ -4,8 +4,8 @@
 //   p    = softmax(s / T),  p1 = softmax(s)
 //   loss = a_s T^2 sum_j q_j (log q_j - log p[i_j]) - a_h log p1[label]
 //   grad = a_s T (p - sum of q_j with i_j = .) + a_h (p1 - [. = label])
-// a_s = 1 - alpha and a_h = alpha with labels, else 1 and 0. A term whose entries or label are missing counts 0, and
-// so does a row of logits that are all -inf; "mean" is over the rows that have an entry or a label. A token named
+// a_s = 1 - alpha and a_h = alpha with labels, else 1 and 0. A term whose entries or label are missing, or whose share
+// is 0, counts 0 whatever its values are, and so does a row of logits that are all -inf; "mean" is over the rows that have an entry or a label. A token named
 // twice gets both entries' probabilities.
 //
 // Both softmaxes share their maximum m: what is kept of a row is m, 1/Z and 1/Z1 (and the teacher's own), so that a
@@ -65,6 +65,9 @@ __device__ __forceinline__ int label_of(const Distill& a, int64_t n) {
   const int64_t y = load_id(a.labels, a.label_bytes, n);
   return y >= 0 && y < a.V ? (int)y : -1;
 }
+
+// The soft term's share of the loss.
+__device__ __forceinline__ float soft_share(const Distill& a) { return a.labels ? 1.0f - a.alpha : 1.0f; }
 
 // Under 2^-126 it is 0.
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -289,7 +292,8 @@ __device__ __forceinline__ void finish_row(const Distill& a, int64_t n, const Su
   const auto* row = static_cast<const typename TabType<DT>::t*>(a.logits) + n * a.ld;
   const int lane = threadIdx.x & 63, y = label_of(a, n);
   const bool alive = s.z != 0.0f;   // a NaN stays
-  const bool soft = t.some && alive, hard = y >= 0 && alive;
+  const float share = soft_share(a);
+  const bool soft = t.some && alive && share != 0.0f, hard = y >= 0 && alive && a.alpha != 0.0f;
   const float rtot = 1.0f / t.total, logs = logf(s.z) - logf(t.total);
   float l = 0.0f;
   if (soft && !(a.T > kFarT && close_loss<DT>(a, row, s, rtot, id, q, lq, l))) {
@@ -299,7 +303,6 @@ __device__ __forceinline__ void finish_row(const Distill& a, int64_t n, const Su
     }
     l = wave_reduce(l, [](float x, float y) { return x + y; });
   }
-  const float share = a.labels ? 1.0f - a.alpha : 1.0f;
   if (lane == 0) {
     float v = soft ? share * a.T * a.T * l : 0.0f;
     if (hard) v += a.alpha * (logf(s.z1) - (tab_get<DT>(row[y]) - s.m));
@@ -571,7 +574,7 @@ distill_both_kernel(Distill a, int slots, const int* counts, float scale, float*
     e.clear(threadIdx.x, 64);
     const Teacher t = teacher_of(a, n, e.id, e.share, e.log);
     if (threadIdx.x == 0) told = t;
-    for (int j = threadIdx.x; j < a.K; j += 64) e.name(j, e.id[j]);
+    for (int j = threadIdx.x; j < a.K; j += 64) e.name(j, soft_share(a) != 0.0f ? e.id[j] : -1);
   }
   // f(values, first token) of the thread's groups
   const auto each = [&](auto f) {
@@ -622,7 +625,7 @@ distill_both_kernel(Distill a, int slots, const int* counts, float scale, float*
   if constexpr (TH == 64) __syncthreads();
   const Teacher t = told;
   const bool soft = t.some && z != 0.0f, hard = y >= 0 && z != 0.0f;   // as in finish_row
-  const float a_s = soft ? (a.labels ? 1.0f - a.alpha : 1.0f) * a.T : 0.0f, a_h = hard ? a.alpha : 0.0f;
+  const float a_s = soft ? soft_share(a) * a.T : 0.0f, a_h = hard ? a.alpha : 0.0f;
   const bool dead = scale == 0.0f || (a_s == 0.0f && a_h == 0.0f);
   Form form;
   const Slope slope = slope_of(a, m, 1.0f / z, 1.0f / z1, scale * a_s, scale * a_h, form);
