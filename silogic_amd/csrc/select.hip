@@ -198,10 +198,10 @@ struct Row {
         bool any = false;
 #pragma unroll
         for (int u = s; u < s + SUB; ++u) any |= in(x[u]);
-        if (SUB == 1 ? any : __ballot(any) != 0) {
+        if (__ballot(any) != 0) {
 #pragma unroll
           for (int u = s; u < s + SUB; ++u)
-            if (SUB == 1 || in(x[u])) f(x[u], i + u);
+            if (in(x[u])) f(x[u], i + u);
         }
         if (SUB < VU) __builtin_amdgcn_sched_barrier(0);
       }
@@ -577,7 +577,7 @@ sample_kernel(const typename TabType<DT>::t* logits, int64_t N, int64_t ld, int 
     if (w && target >= run && target - run < w) ids[n] = r.id_of(mine);
     return;
   }
-  if (by_k && many > TH) {
+  if (by_k) {
     // without a threshold the kth may not be there
     int there = 0;
     r.template each_in<true>([](float x) { return x > -INFINITY; }, [&](float, int) { ++there; });
