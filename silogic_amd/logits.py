@@ -86,13 +86,17 @@ def _sample(logits, u, temperature, top_k, top_p, min_p, mask):
                 raise ValueError(f"sample_logits: mask {tuple(mask.shape)} for logits {tuple(logits.shape)}") from None
         mask = mask.reshape(-1, rows.shape[1]) if mask.dim() != 2 else mask
         mask = mask if mask.stride(1) == 1 or mask.shape[1] == 1 else mask.contiguous()
+    limits = (t, k, p, m)
     d = rows.get_device()
     # all in order (the usual call), or the check that says what is not
-    if not (d >= 0 and all(v is None or v.get_device() == d for v in (u, mask, t, k, p, m) if not isinstance(v, (int, float)))):
-        each = [v for v in (t, k, p, m) if isinstance(v, torch.Tensor)]
+    there = d >= 0 and u.get_device() == d and (mask is None or mask.get_device() == d)
+    for v in limits:
+        there &= isinstance(v, (int, float)) or v.get_device() == d
+    if not there:
+        each = [v for v in limits if isinstance(v, torch.Tensor)]
         ops.require_gpu(rows, u, mask, *each)
         ops.same_device("sample_logits", rows, u, mask, *each)
-    return rows, u, (t, k, p, m), mask
+    return rows, u, limits, mask
 
 
 def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):

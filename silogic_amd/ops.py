@@ -57,25 +57,26 @@ def _grad_path(*ts):
 
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
+_modes = torch._C._len_torch_dispatch_stack
+_transforms = torch._C._functorch.peek_interpreter_stack
 
 
-def one_op(what, *ts):
-    """True when a call on ``ts`` must run as one custom operator, because
-    something looks at the operators that it is made of and a launch is none:
+def one_op(what, logits, *others):
+    """True when a call must run as one custom operator, because something
+    looks at the operators that it is made of and a launch is none:
     ``torch.compile``, another tracer or mode (``make_fx``, fake tensors), a
     tensor subclass. Raises under ``vmap`` and the derivatives of
     ``torch.func``, which an operator would not take either (``jvp`` would give
     it tangents of zero)."""
     if torch.compiler.is_compiling():
         return True
-    if torch._C._functorch.peek_interpreter_stack() is not None:
-        if any(torch._C._functorch.is_gradtrackingtensor(t) or torch._C._functorch.is_batchedtensor(t) for t in ts
-               if isinstance(t, torch.Tensor)):
+    if _transforms() is not None:
+        if any(torch._C._functorch.is_gradtrackingtensor(t) or torch._C._functorch.is_batchedtensor(t)
+               for t in (logits, *others) if isinstance(t, torch.Tensor)):
             raise NotImplementedError(f"{what}: no torch.func transform of it (vmap: call it on [..., V]; gradients: "
                                       "torch.autograd)")
         return True
-    return torch._C._len_torch_dispatch_stack() > 0 or any(isinstance(t, torch.Tensor) and type(t) not in _PLAIN
-                                                           for t in ts)
+    return _modes() > 0 or type(logits) not in _PLAIN
 
 
 def _c(t, dtype=None):
