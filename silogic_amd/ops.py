@@ -64,8 +64,8 @@ _transforms = torch._C._functorch.peek_interpreter_stack
 def one_op(what, logits, *others):
     """True when a call must run as one custom operator, because something
     looks at the operators that it is made of and a launch is none:
-    ``torch.compile``, another tracer or mode (``make_fx``, fake tensors), a
-    tensor subclass. Raises under ``vmap`` and the derivatives of
+    ``torch.compile``, another tracer or mode (``make_fx``, fake tensors,
+    ``torch.jit.trace``), a tensor subclass. Raises under ``vmap`` and the derivatives of
     ``torch.func``, which an operator would not take either (``jvp`` would give
     it tangents of zero)."""
     if torch.compiler.is_compiling():
@@ -76,7 +76,7 @@ def one_op(what, logits, *others):
             raise NotImplementedError(f"{what}: no torch.func transform of it (vmap: call it on [..., V]; gradients: "
                                       "torch.autograd)")
         return True
-    return _modes() > 0 or type(logits) not in _PLAIN
+    return _modes() > 0 or torch._C._is_tracing() or type(logits) not in _PLAIN
 
 
 def _c(t, dtype=None):

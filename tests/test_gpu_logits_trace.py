@@ -54,3 +54,13 @@ def test_the_loss_by_functionalized_code():
     given = _inputs(9, 50, 4)
     call = lambda x, v, i, y, u: sl.distill_loss_and_grad(x, v, i, y)[1]  # noqa: E731
     assert torch.equal(torch.func.functionalize(call)(*given), call(*given))
+
+
+def test_a_recorded_call_runs_on_new_inputs():
+    """torch.jit.trace records operators, too."""
+    call = lambda x, u: (sl.sample_logits(x, u, top_p=0.9), *sl.top_logits(x, 4))  # noqa: E731
+    x, _, _, _, u = _inputs(9, 50, 5)
+    recorded = torch.jit.trace(call, (x, u))
+    x, _, _, _, u = _inputs(9, 50, 6)
+    for got, want in zip(recorded(x, u), call(x, u)):
+        assert torch.equal(got, want)
