@@ -267,14 +267,27 @@ __device__ __forceinline__ bool close_loss(const Distill& a, const typename TabT
                                            const float* q, const float* lq, float& loss) {
   const int lane = threadIdx.x & 63;
   const auto add = [](double x, double y) { return x + y; };
-  const auto mass = [&](int64_t i) { return (double)exp2_fast((tab_get<DT>(row[i]) - s.m) * (a.inv_t * kLog2e)); };
+  const auto mass_of = [&](float x) { return (double)exp2_fast((x - s.m) * (a.inv_t * kLog2e)); };
+  const auto mass = [&](int64_t i) { return mass_of(tab_get<DT>(row[i])); };
   double named = 0.0, total = 0.0, all = 0.0;
   for (int j = lane; j < a.K; j += 64)
     if (q[j] != 0.0f) named += mass(id[j]), total += (double)q[j];
   named = wave_reduce(named, add);
   if (!(named > 0.5 * (double)s.z)) return false;
   total = wave_reduce(total, add);
-  for (int64_t i = lane; i < a.V; i += 64) all += mass(i);
+  int64_t i = lane;
+  // two loads in flight: with four the forms of 512 threads lose a workgroup a compute unit to registers
+  for (; i + 64 < a.V; i += 2 * 64) {
+    float v[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) v[k] = tab_get<DT>(row[i + k * 64]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      __builtin_amdgcn_sched_barrier(0);
+      all += mass_of(v[k]);
+    }
+  }
+  for (; i < a.V; i += 64) all += mass(i);
   all = wave_reduce(all, add);
   const float shift = (float)log(all / total);
   float l = 0.0f;
