@@ -323,7 +323,8 @@ int slg_token_encode_hard(const void* ids, int32_t id_bytes, int64_t B, int64_t 
  *                          -inf), and labels [N] (NULL: none; absent: outside
  *                          0..V-1): (1 - alpha) T^2 KL(softmax(values / T) ||
  *                          softmax(logits / T)) + alpha * cross entropy, the KL
- *                          alone without labels. A term without entries or label,
+ *                          alone without labels, summed by entry (a token named
+ *                          twice has two terms). A term without entries or label,
  *                          or with a factor of 0, counts 0. reduction 0: loss
  *                          [N], 1: their sum, 2: the mean over rows with an entry
  *                          or a label. 1e-4 <= T <= 1e4. kept:

@@ -4,16 +4,21 @@
 //   p    = softmax(s / T),  p1 = softmax(s)
 //   loss = a_s T^2 sum_j q_j (log q_j - log p[i_j]) - a_h log p1[label]
 //   grad = a_s T (p - sum of q_j with i_j = .) + a_h (p1 - [. = label])
-// a_s = 1 - alpha and a_h = alpha with labels, else 1 and 0. A term whose entries or label are missing, or whose share
-// is 0, counts 0 whatever its values are, and so does a row of logits that are all -inf; "mean" is over the rows that have an entry or a label. A token named
-// twice gets both entries' probabilities.
+// a_s = 1 - alpha and a_h = alpha with labels, else 1 and 0. A term whose entries or label are missing, or whose
+// share is 0, counts 0 whatever its values are, and so does a row of logits that are all -inf; "mean" is over the
+// rows that have an entry or a label. A token named twice gets both entries' probabilities, and the loss both terms
+// of the sum over entries.
 //
 // Both softmaxes share their maximum m: what is kept of a row is m, 1/Z and 1/Z1 (and the teacher's own), so that a
 // probability is exp((s - m) / T) / Z with the difference exact where it matters. Sums are fp32, those over rows 64
-// bits; the gradient is rounded once. With long rows all kernels are bound by the logits' bytes: one pass for the loss
-// (the running maximum and sums of each thread joined at the end), another with the write for the gradient. Both from
-// one call hold the row in registers between them. Times below are of 4096 x 32000 and 64 entries, on a card whose
-// copies reach 5.0 to 5.4 TB/s.
+// bits; the gradient is rounded once. With long rows all kernels are bound by the logits' bytes: one pass for the
+// loss (the running maximum and sums of each thread joined at the end), another with the write for the gradient. Both
+// from one call hold the row in registers between them. Times below are of 4096 x 32000 and 64 entries, on a card
+// whose copies reach 5.0 to 5.4 TB/s.
+//
+// Roundings: an exponential's argument (s - m) log2 e / T takes four (the difference, 1 / T, the factor, the product) and
+// the exponential one, so that a probability is off by some 2^-22 of itself times 1 + (m - s) / T, and by its row's sum,
+// which chains of V / threads additions and as many rescaled maxima make. Under 2^-126 of the largest it is 0.
 #include <algorithm>
 #include <type_traits>
 
@@ -26,8 +31,8 @@ constexpr float kLog2e = 1.44269504f;
 constexpr int kMaxEntries = 1024;
 constexpr int kKept = 8;      // floats kept of a row: m, 1/Z, 1/Z1, the teacher's maximum and 1/sum, a_s T, a_h, counted
 constexpr int kCounts = 256;  // workgroups that count the rows of a mean
-// More rows than these are summed by kCounts workgroups before the last one: the loss of 32768 x 49 took 62 us so, 74
-// without, of 16384 x 49 41 both ways.
+// More rows than these are summed by kCounts workgroups before the last one: the loss of 32768 x 49 takes 25 us so and 38
+// without, of 16384 x 49 17 and 22, of 250 x 257 9 and 7.
 constexpr int kManyRows = 16384;
 // Past this temperature a small soft loss is summed without cancellation (close_loss): the factor T^2 would bring the
 // roundings of the logarithms, some 2^-20, to the loss's own size at T = 1000. Up to it they come to 2^-16 at most.
@@ -328,9 +333,9 @@ __device__ __forceinline__ void finish_row(const Distill& a, int64_t n, const Su
   }
 }
 
-// The loss of a row, a workgroup each; with parts > 1 the sums of a part of a row, joined by the next kernel. 100 to 108
-// us in fp32, 4.9 to 5.2 TB/s: memory; the vector instructions take about a third of their issue. Of 16 x 131071
-// fp16 logits in 63 parts 4.8 us, and 4.1 for the join: latency.
+// The loss of a row, a workgroup each; with parts > 1 the sums of a part of a row, joined by the next kernel. 108 us
+// in fp32, 4.9 TB/s, 65 in bf16 with labels: memory; the vector instructions take about a third of their issue. Of 16
+// x 131071 fp16 logits in 63 parts 4.8 us, and 4.1 for the join: latency.
 template <int DT, int TH, Form FORM>
 __global__ void __launch_bounds__(TH) distill_fwd_kernel(Distill a, int parts, int64_t per, Sums* part_sums, float* loss, float* kept) {
   __shared__ Sums part[TH / 64];
@@ -490,9 +495,9 @@ __device__ __forceinline__ void name_tokens(const typename TabType<DT>::t* row, 
   if (own == threads - 1 && label >= from && label < to && !e.named(label)) write(label, label_share);
 }
 
-// Gradient of `chunk` logits of a row: all of them from their probabilities, then those that are named. 204 us in fp32,
-// 5.1 TB/s of reads and writes: memory; 16 x 131071 fp16 in 63 parts 6 us. The second write of the few named tokens takes the place of a look at the
-// entries by every token.
+// Gradient of `chunk` logits of a row: all of them from their probabilities, then those that are named. 204 to 217 us
+// in fp32, 4.8 to 5.1 TB/s of reads and writes, 113 in bf16 with labels: memory; 16 x 131071 fp16 in 63 parts 6 us.
+// The second write of the few named tokens takes the place of a look at the entries by every token.
 template <int DT, int TH>
 __global__ void __launch_bounds__(TH)
 distill_bwd_kernel(Distill a, int slots, const float* kept, const float* upstream, int per_row, const float* factor, float scale,
@@ -556,10 +561,10 @@ distill_bwd_kernel(Distill a, int slots, const float* kept, const float* upstrea
   });
 }
 
-// Loss and gradient of a row, a workgroup each, the row's first NV groups of each thread in registers between them. In
-// bf16 with labels at T = 2 105 us, 5.0 TB/s: memory, with the vector instructions at some 75% of their issue (two
-// passes over the row, an exponential in each). With two workgroups a compute unit one row is read while another is
-// summed.
+// Loss and gradient of a row, a workgroup each, the row's first NV groups of each thread in registers between them.
+// In bf16 with labels at T = 2 105 us of a call's 115, 5.0 TB/s: memory, with the vector instructions at some 75% of
+// their issue (two passes over the row, an exponential in each). With two workgroups a compute unit one row is read
+// while another is summed.
 template <int DT, int TH, int NV, Form FORM>
 __global__ void __launch_bounds__(TH, TH == 1024 ? 8 : 1)
 distill_both_kernel(Distill a, int slots, const int* counts, float scale, float* loss, void* grad) {
@@ -687,7 +692,7 @@ void by_type(int dtype, F f) {
   else f(std::integral_constant<int, kTabF16>{});
 }
 // f with the type and the form of the sums. At temperature 2 the second softmax is the first one's square (loss and
-// gradient of 4096 x 32000 bf16 with labels in one kernel: 119 us, with two exponentials 138).
+// gradient of 4096 x 32000 bf16 with labels by one call: 115 us, with two exponentials 125, as at T = 3 and 4).
 template <class F>
 void by_form(const Distill& a, int dtype, F f) {
   by_type(dtype, [&](auto dt) {
@@ -744,8 +749,9 @@ int slots_of(const Distill& a) {
   return s;
 }
 int entry_bytes(const Distill& a, int slots) { return (slots ? 4 * a.K + 2 * slots : 3 * a.K) * 4; }
-// A wave a row of few values: with 256 threads the loss of 65536 x 49 fp32 takes 117 us instead of 47, of 65536 x 2000
-// 155 instead of 111, the gradient of 65536 x 1000 143 instead of 107, but of 65536 x 2000 199 where one wave takes 218.
+// A wave a row of few values: with 256 threads the loss of 65536 x 49 fp32 takes 109 us instead of 41, of 65536 x 2000
+// 159 instead of 116, the gradient of 65536 x 49 98 instead of 35, of 65536 x 1000 146 instead of 141, but of 65536 x 2000
+// 211 where one wave takes 235.
 bool loss_by_wave(const Distill& a) { return a.V <= 2048; }
 bool grad_by_wave(const Distill& a) { return a.V <= 1024; }
 
@@ -841,6 +847,8 @@ int slg_distill_loss_grad(const void* logits, int32_t dtype, int64_t N, int64_t 
     constexpr int DT = decltype(dt)::value, U = Group<DT>::U;
     constexpr Form FORM = decltype(form)::value;
     const auto go = [&](auto kern, int th) { hipLaunchKernelGGL(kern, grid_of(N), dim3(th), entry_bytes(a, slots), st, a, slots, counts, scale, rows, grad); };
+    // the row in as few threads' registers as hold it; 512 threads read what is past 32768 values of 16 bits again (4096 x
+    // 50257 bf16 with labels 231 us, x 65536 269; 1024 threads, which would hold it, 218 and 236: not built)
     if (V <= 64 * 4 * U) go(distill_both_kernel<DT, 64, 4, FORM>, 64);
     else if (V <= 256 * 4 * U) go(distill_both_kernel<DT, 256, 4, FORM>, 256);
     else if (DT != kTabF32 || V <= 512 * 8 * U) go(distill_both_kernel<DT, 512, 8, FORM>, 512);

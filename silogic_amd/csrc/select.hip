@@ -471,9 +471,10 @@ struct Row {
   }
 };
 
-// The K largest of a row, a workgroup each. 64 of 4096 x 32000 bf16: 52 us, 5.0 TB/s, where 512 threads hold the row in
-// 64 registers each and two passes look at it (lanes' maxima, then what is past the threshold, some 190 tokens): memory,
-// with the vector instructions at 80% of their issue. 100 of 33 x 131071 fp32: 17 to 19 us, on 33 compute units.
+// The K largest of a row, a workgroup each. 64 of 4096 x 32000 bf16: 52 to 55 us, 4.8 to 5.0 TB/s, where 512 threads
+// hold the row in 64 registers each and two passes look at it (lanes' maxima, then what is past the threshold, some
+// 190 tokens): memory, with the vector instructions at 80% of their issue; in fp32 96 us, 5.5 TB/s. 100 of 33 x
+// 131071 fp32: 18 to 20 us, on 33 compute units.
 template <int DT, int TH, int NV>
 __global__ void __launch_bounds__(TH)
 top_logits_kernel(const typename TabType<DT>::t* logits, int64_t N, int64_t ld, int V, int K, typename TabType<DT>::t* values,
@@ -518,12 +519,13 @@ __device__ inline uint64_t target_of(float u, uint64_t total) {
   return t < total ? t : total - 1;
 }
 
-// A token of a row, a workgroup each. 4096 x 32000 fp32: 110 us by min_p, 126 by the first 50, 203 without a limit and 233
-// by top_p, where each token's mass (24 vector instructions, most in 64 bits) and its place in a histogram (an LDS
-// atomic of 64 bits, 15 cycles a wave) are what bounds it: vector instructions 73% of their issue. Half of such a row
-// fits the registers at two workgroups a compute unit; a form of 1024 threads or 16 groups a thread, which hold all of it
-// with one, was slower, as was one of 256 threads for short lists (64 rows of 32000: 28 us instead of 21). Masses of 32
-// bits for the histogram, with exact ones where a border is near, came to 185 us without a limit but 252 by top_p.
+// A token of a row, a workgroup each. 4096 x 32000 fp32, in a captured graph over three sets of inputs: 113 us by
+// min_p, 125 by the first 40, 203 without a limit and 219 by top_p, where each token's mass (24 vector instructions,
+// most in 64 bits) and its place in a histogram (an LDS atomic of 64 bits, 15 cycles a wave) are what bounds it:
+// vector instructions 73% of their issue. Half of such a row fits the registers at two workgroups a compute unit; a
+// form of 1024 threads or 16 groups a thread, which hold all of it with one, was slower, as was one of 256 threads
+// for short lists (64 rows of 32000: 28 us instead of 21). Masses of 32 bits for the histogram, with exact ones where
+// a border is near, came to 185 us without a limit (exact ones alone then to 202) but 252 by top_p (234).
 template <int DT, int TH, int NV>
 __global__ void __launch_bounds__(TH, 4)
 sample_kernel(const typename TabType<DT>::t* logits, int64_t N, int64_t ld, int V, const uint8_t* allowed, int64_t allowed_ld,
@@ -630,7 +632,9 @@ using namespace slg;
 namespace {
 
 // f with the type, the threads and the groups of 16 bytes a thread of N rows of V logits. Listing up to k tokens takes
-// as many threads.
+// as many threads. (Draws pass k = 1 whatever their limit, which may be each row's own: where fewer lanes hold tokens
+// than their top_k asks for, there is no threshold, and the list overflows into the histograms. 4096 x 257 by the first
+// 50 take 17 us in fp32 and 24 in bf16, by top_p 12 and 14.)
 template <bool LIST, class F>
 void dispatch(int dtype, int64_t N, int64_t V, int64_t k, F f) {
   using std::integral_constant;
@@ -641,8 +645,9 @@ void dispatch(int dtype, int64_t N, int64_t V, int64_t k, F f) {
     // a row that fills no group is read token by token
     if (V < VU) return go(integral_constant<int, 64>{}, integral_constant<int, 0>{});
     // as few threads as hold the row: more rows are under way side by side, and their barriers are of fewer waves (8192
-    // rows of 2000 fp32 by top_p take 42 us with 128 threads, 69 with 512; of 8000 106 with 256, 170 with 512); but about
-    // three times k tokens reach a list's threshold, and 40 of 64 rows of 2000 take 12 us with 128 threads, 27 with 64
+    // rows of 2000 fp32 by top_p take 42 us with 128 threads, 214 with 512 of eight groups; of 8000 113 with 256, 223 with
+    // 512); but about three times k tokens reach a list's threshold where the row fills the lanes, and 40 of 64 rows of 500
+    // take 5 us with 128 threads, 11 with 64
     if (groups <= 128 && k <= 24) return go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
     if (groups <= 256 && k <= 48) return go(integral_constant<int, 128>{}, integral_constant<int, 2>{});
     if (groups <= 512 && k <= 48) return go(integral_constant<int, 128>{}, integral_constant<int, 4>{});
@@ -653,8 +658,8 @@ void dispatch(int dtype, int64_t N, int64_t V, int64_t k, F f) {
       if (groups <= 4096) return go(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
       go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
     } else {
-      // a compute unit holds one workgroup of 1024 threads, or two of 512: fp32 by top_p, 64 rows of 130000 take 48 us with
-      // the former and 60 with the latter, 300 of 50257 61 and 51, 4096 of 32000 307 and 214
+      // a compute unit holds one workgroup of 1024 threads, or two of 512: fp32 by top_p, 64 rows of 130000 take 53 us with
+      // the former and 65 with the latter, 300 of 50257 62 and 53, 4096 of 32000 307 and 219
       if (groups > 4096 && N <= 256) return go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
       go(integral_constant<int, 512>{}, integral_constant<int, 8>{});
     }

@@ -179,14 +179,17 @@ def distill_loss(logits, values, ids, labels=None, temperature=1.0, alpha=0.5, r
 
         (1 - alpha) T^2 KL(softmax(values / T) || softmax(logits / T)) + alpha cross_entropy(logits, labels)
 
-    (the first term alone, without its factor, where not). The teacher's probabilities are those of its entries among
-    themselves. An entry with an id outside 0..V-1 or a value of -inf is absent, so is a label outside 0..V-1. A term
-    without an entry or a label, or with a factor of 0, counts 0, as does a row of -inf alone; ``mean`` is over the rows
-    with an entry or a label. ``temperature`` lies in 1e-4 to 1e4. Over 4 a small first term is summed without
-    cancellation; up to 4, and in the gradient, two 32-bit numbers are subtracted (the loss is off by some T^2 2^-21 then,
-    a gradient by some T 2^-22 of the probabilities). Losses are fp32; the logits' gradient is in their type, rounded
-    once, and the same bits on every call. The teacher gets no gradient, and there is no second derivative, none in
-    forward mode and no ``torch.func`` transform."""
+    (the first term alone, without its factor, where not). The teacher's probabilities q are those of its entries
+    among themselves, KL is the sum of q_j (log q_j - log p[ids_j]) over the entries: a token that two of them name
+    gets both their probabilities, each with its own logarithm. An entry with an id outside 0..V-1 or a value of -inf
+    is absent, so is a label outside 0..V-1. A term without an entry or a label, or with a factor of 0, counts 0, as
+    does a row of -inf alone; ``mean`` is over the rows with an entry or a label.
+
+    ``temperature`` lies in 1e-4 to 1e4. Over 4 a small first term is summed without cancellation; up to 4, and in the
+    gradient, two 32-bit numbers are subtracted (the loss is off by some T^2 2^-21 then, a gradient by some T 2^-22 of
+    the probabilities). Losses are fp32; the logits' gradient is in their type, rounded once, and the same bits on
+    every call. The teacher gets no gradient, and there is no second derivative, none in forward mode and no
+    ``torch.func`` transform."""
     whole = ops.one_op("distill_loss", logits, values, ids, labels)
     if not torch.compiler.is_compiling() and forward_ad.unpack_dual(logits).tangent is not None:
         raise NotImplementedError("distill_loss: no derivative in forward mode")
