@@ -110,9 +110,10 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
     token, and limits out of their range act as their nearest bound). ``mask`` (bool, ``[V]`` to ``[..., V]``) is True for
     tokens that are allowed. A NaN or -inf is no token; a row without one gives -1.
 
-    Masses are held as whole numbers of 2^-F of the largest, so that their sums are exact and the same draw comes from the
-    same inputs on every call. F is at most 50 and 62 less the bits of V, or from 2^18 logits on of the row's own sum: a
-    border between tokens is off by 2^-43 and V 2^-(F+1) largest masses, together 2^-27 of the sum at most. A ``u`` outside [0, 1) acts as its nearest bound."""
+    Masses are held as whole numbers of 2^-F of the largest, so that their sums are exact and the same draw comes from
+    the same inputs on every call. F is at most 50 and 62 less the bits of V, or from 2^18 logits on of the row's own
+    sum: a border between tokens is off by 2^-43 and V 2^-(F+1) largest masses, together 2^-27 of the sum at most. A
+    ``u`` outside [0, 1) acts as its nearest bound."""
     whole = ops.one_op("sample_logits", logits, u, temperature, top_k, top_p, min_p, mask)
     rows, u, limits, mask = _sample(logits, u, temperature, top_k, top_p, min_p, mask)
     if whole:
